@@ -227,6 +227,49 @@ int qimg_sage_attention(const uint16_t* q_f16, const uint16_t* k_f16, const uint
                         void* out, int out_dtype, float sm_scale, int BH, int S, int D,
                         int causal, void* scratch, int64_t scratch_bytes, void* stream);
 
+/* ---- prompts: packed attention ----------------------------------------- */
+
+/* Attention over `batch` sequences that lie one behind the other. No
+ * counterpart in the reference, whose unquantized attention
+ * (cuda_kernels.cu:2019-2112) takes one sequence and equal head counts.
+ *   q [total_q, n_heads, head_dim], k and v [total_k, n_kv_heads, head_dim],
+ *   out as q, all `dtype` (QIMG_BF16 or QIMG_FP16); *_stride_t and *_stride_h
+ *   are the strides in elements between tokens and between heads (a packed
+ *   [T, (Hq + 2 Hk) D] projection or head-major [H, T, D] tensors are read in
+ *   place), multiples of 8, of tokens at most 2^24.
+ *   n_heads a multiple of n_kv_heads (head h reads kv head
+ *   h / (n_heads / n_kv_heads)); head_dim 64 or 128.
+ *   cu_seqlens_q, cu_seqlens_k: int32 [batch + 1] on the device, rising from 0;
+ *   sequence b has queries cu_seqlens_q[b] .. cu_seqlens_q[b + 1] and keys
+ *   cu_seqlens_k[b] .. cu_seqlens_k[b + 1], of which the first k_lens[b]
+ *   (int32 [batch] on the device) are in use, all with k_lens NULL (a cache with room behind its last
+ *   key). Lengths may be 0. Offsets outside the tensors are clamped to them.
+ *   causal: key j is visible to query i when j <= i + keys - queries.
+ * out[i] = sum_j p_ij v_j over the visible keys, p = softmax(sm_scale q.k); a
+ * query that sees no key gives zeros. Rows of no sequence are not written.
+ * What lies behind a sequence's last key or is hidden from a row does not
+ * reach that row, NaN and infinities included. sm_scale > 0, finite. out
+ * overlaps none of q, k, v.
+ * scratch: qimg_attention_varlen_scratch_bytes(...) bytes (may be 0: NULL).
+ * One scratch buffer serves one call at a time. */
+typedef struct {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* out;
+    int dtype;
+    int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h, out_stride_t, out_stride_h;
+    const int32_t* cu_seqlens_q;
+    const int32_t* cu_seqlens_k;
+    const int32_t* k_lens;
+    int batch, total_q, total_k, n_heads, n_kv_heads, head_dim;
+    float sm_scale;
+    int causal;
+} qimg_attn_varlen;
+int64_t qimg_attention_varlen_scratch_bytes(int total_q, int total_k, int batch, int n_heads, int n_kv_heads,
+                                            int head_dim);
+int qimg_attention_varlen(const qimg_attn_varlen* args, void* scratch, int64_t scratch_bytes, void* stream);
+
 /* ---- MMDiT joint block: the operations around the hot path ------------ */
 
 /* silu_fp32 (cuda_kernels.cu:1881-1893): out[i] = x[i] / (1 + exp(-x[i])). */

@@ -47,7 +47,11 @@ HIP_FLAGS = [
 ]
 
 SOURCES = ["hadamard_quant.hip", "gemm_w8a8.hip", "gemm_small_m.hip", "gemm_bf16.hip", "sage_attention.hip", "block_ops.hip",
-           "mmdit_block.hip", "capi.hip", "linear_noalloc.hip", "int4.hip", "capi_int4.hip"]
+           "mmdit_block.hip", "capi.hip", "linear_noalloc.hip", "int4.hip", "capi_int4.hip",
+           "attention_varlen.hip", "capi_prompt.hip"]
+# MFMA results in vector registers: with the accumulators in AGPRs the compiler
+# copies them back and forth around every rescale of the online softmax.
+SOURCE_FLAGS = {"attention_varlen.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form=1")}
 HOST_SOURCES = ["kernels.cpp", "checkpoint.cpp"]
 PROBE_SOURCE = "mfma_probe.hip"
 
@@ -73,7 +77,7 @@ def build(jobs: int = 4, verbose: bool = True) -> str:
         futs = []
         for s in SOURCES:
             o = os.path.join(OBJ, os.path.splitext(s)[0] + ".o")
-            futs.append(ex.submit(_compile, os.path.join(CSRC, s), o))
+            futs.append(ex.submit(_compile, os.path.join(CSRC, s), o, SOURCE_FLAGS.get(s, ())))
             hot_objs.append(o)
         for s in HOST_SOURCES:
             o = os.path.join(OBJ, "host_" + os.path.splitext(s)[0] + ".o")

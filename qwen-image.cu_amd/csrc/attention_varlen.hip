@@ -1,0 +1,846 @@
+// attention_varlen.hip — unquantized attention over packed sequences:
+//   s_ij = sm_scale * q_i . k_j             (j visible to i)
+//   o_i  = sum_j e^(s_ij - m_i) v_j / sum_j e^(s_ij - m_i)
+// for sequences of different lengths that lie one behind the other, grouped
+// heads (Hq a multiple of Hk, query head h reads kv head h / (Hq / Hk)), bf16
+// or fp16. Key j of a sequence with lq queries and lk keys is visible to
+// query i when j < lk and, if causal, j <= i + lk - lq (the last query sees
+// the last key). A query that sees no key gives zeros.
+//
+// Rows: a tile's rows are (token, head of the group) pairs of one sequence
+// and one kv head, row = token * group + head, so the heads of a group share
+// the K and V they read (one token of 7 heads is 7 rows of a tile, not 7
+// tiles), and a causal tile spans few tokens.
+//
+// Arithmetic: v_mfma_f32_32x32x16 on both products, fp32 accumulation, base-2
+// online softmax with the running maximum and sum in fp32. Scores are computed
+// transposed (S^T = K Q^T), so a lane holds one query row's scores and the P
+// registers are the second product's operand as they are: with O^T = V^T P^T
+// element e of lane half h stands for key 16 t + 8 (e / 4) + 4 h + e % 4 of a
+// 16-key group t, and V^T comes from row-major V in LDS through
+// ds_read_b64_tr_b16, whose four values are 4 consecutive keys of one channel.
+// P is rounded to the inputs' type for the second product (relative error at
+// most 2^-8 a term in bf16 as in the result itself; the row sum adds the
+// rounded values, so a constant V is returned exactly). The maximum moves, and
+// O and the sum are rescaled, only when a tile exceeds it by more than
+// kSlack (log2 units): P then reaches 2^kSlack, which changes no relative
+// rounding. fp16 P carries a further factor 2^kBias16 (at most 2^15 in all),
+// so that a value leaves the type's range only below 2^-31 of the maximum.
+//
+// K and V tiles go to LDS by buffer loads whose descriptor ends at the
+// sequence's last key: rows behind it arrive as zeros, so nothing that lies
+// there (another sequence, an unused part of a cache) reaches the result, NaN
+// included. Every tile has a descriptor of its own (64-bit base), so offsets
+// inside one stay small however long the cache is.
+#include <type_traits>
+
+#include "qimg_device.h"
+#include "qimg_internal.h"
+
+namespace qimg {
+
+namespace {
+
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef short v8s __attribute__((ext_vector_type(8)));
+
+constexpr float kNegInf = -__builtin_inff();
+constexpr float kSlack = 8.0f;   // lazy-rescale threshold of the running maximum (log2 units)
+constexpr float kBias16 = 7.0f;  // log2 of the factor on fp16 P
+constexpr int kRsrcWord3 = 0x00020000;  // raw unswizzled buffer (gfx9 family)
+
+// element type: fragment vector, MFMA, P pair packing and its row sum, and
+// the mask of a value's exponent bits (all ones: infinity or NaN)
+struct Bf16 {
+    using frag = v8bf;
+    static constexpr float kPBias = 0.0f;
+    static constexpr uint32_t kExp = 0x7f80u, kMant = 0x007fu;
+    __device__ static __forceinline__ v16f mma(frag a, frag b, v16f c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+    __device__ static __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
+    __device__ static __forceinline__ float add2(uint32_t p, float s) {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, p), __builtin_bit_cast(b2, 0x3f803f80u), s,
+                                               false);
+    }
+    __device__ static __forceinline__ uint16_t round(float v) { return f32_to_bf16(v); }
+};
+struct Fp16 {
+    using frag = v8h;
+    static constexpr float kPBias = kBias16;
+    static constexpr uint32_t kExp = 0x7c00u, kMant = 0x03ffu;
+    __device__ static __forceinline__ v16f mma(frag a, frag b, v16f c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+    __device__ static __forceinline__ uint32_t pack(float a, float b) {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        typedef float f2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, h2));
+    }
+    __device__ static __forceinline__ float add2(uint32_t p, float s) {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, p), __builtin_bit_cast(h2, 0x3c003c00u), s, false);
+    }
+    __device__ static __forceinline__ uint16_t round(float v) { return f32_to_f16(v); }
+};
+
+// max of the two lane halves' values (lanes l and l ^ 32)
+__device__ __forceinline__ float half_max(float v) {
+    const unsigned u = __float_as_uint(v);
+    const auto sw = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+    const unsigned u = __float_as_uint(v);
+    const auto sw = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+}
+
+// LDS tiles of ROWS keys x D channels, rows unpadded, 16-byte chunks swizzled
+// by row: a K fragment read takes one logical chunk of 16 consecutive rows
+// (ds_read_b128, 16 lanes a cycle over 256 bytes of banks), so those need 16
+// different bank groups; a transposing V read takes 64 bytes of each of 4
+// consecutive rows per half wave, which need 4 different quarters of the
+// banks.
+template <int D>
+__device__ __forceinline__ int swz_k(int row, int c) {
+    return D == 128 ? c ^ (row & 15) : c ^ ((row >> 1) & 7);
+}
+template <int D>
+__device__ __forceinline__ int swz_v(int row, int c) {
+    return D == 128 ? c ^ (4 * (row & 3)) : c ^ (4 * ((row >> 1) & 1));
+}
+
+// One sequence's tile of rows.
+struct RowTile {
+    int q0, lq, k0, lk;  // first query and key row, their numbers
+    int row0;            // first (token, head) row of the tile in the sequence
+    bool found;
+};
+
+// Tile `idx` of the launch: the sequences' tiles of `rows` rows in order,
+// inside a causal sequence the last (longest) tile first. Offsets outside
+// [0, total] or falling ones are clamped, so no tile reaches past the tensors.
+// Each lane takes one sequence; a wave scans 64 of them at a time.
+__device__ __forceinline__ RowTile find_tile(const AttnVarlenArgs& a, int idx, int rows) {
+    const int lane = threadIdx.x & 63;
+    RowTile t;
+    t.found = false;
+    t.q0 = t.lq = t.k0 = t.lk = t.row0 = 0;
+    int before = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+        const int b = b0 + lane;
+        int qs = 0, qe = 0;
+        if (b < a.batch) {
+            qs = min(max(a.cu_q[b], 0), a.total_q);
+            qe = min(max(a.cu_q[b + 1], qs), a.total_q);
+        }
+        const int n = static_cast<int>((static_cast<int64_t>(qe - qs) * a.group + rows - 1) / rows);
+        int incl = n;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int v = __shfl_up(incl, off, 64);
+            if (lane >= off) incl += v;
+        }
+        const int total = __builtin_amdgcn_readlane(incl, 63);
+        if (idx < before + total) {
+            const uint64_t hit = __ballot(before + incl > idx);
+            const int src = __builtin_ctzll(hit);
+            const int sb = b0 + src;
+            t.q0 = __builtin_amdgcn_readlane(qs, src);
+            t.lq = __builtin_amdgcn_readlane(qe, src) - t.q0;
+            const int cnt = __builtin_amdgcn_readlane(n, src);
+            const int first = before + __builtin_amdgcn_readlane(incl, src) - cnt;
+            const int ks = min(max(__builtin_amdgcn_readfirstlane(a.cu_k[sb]), 0), a.total_k);
+            const int ke = min(max(__builtin_amdgcn_readfirstlane(a.cu_k[sb + 1]), ks), a.total_k);
+            t.k0 = ks;
+            t.lk = ke - ks;
+            if (a.k_lens != nullptr) t.lk = min(t.lk, max(__builtin_amdgcn_readfirstlane(a.k_lens[sb]), 0));
+            const int i = idx - first;
+            t.row0 = (a.causal ? cnt - 1 - i : i) * rows;
+            t.found = true;
+            return t;
+        }
+        before += total;
+    }
+    return t;
+}
+
+// number of keys that the query of `token` sees
+__device__ __forceinline__ int visible(const AttnVarlenArgs& a, const RowTile& t, int token) {
+    if (!a.causal) return t.lk;
+    return min(max(token + 1 + t.lk - t.lq, 0), t.lk);
+}
+
+// DMA of keys [key, key + ROWS) of one kv head to LDS: instruction j brings
+// 1 KB = 512 / D rows, instructions w, w + nw, .. here. Rows from the
+// sequence's end on are zeros.
+template <int D, int ROWS, bool VTILE>
+__device__ __forceinline__ void dma_tile(const uint16_t* base, int64_t stride, int key, int lk, uint8_t* lds, int w,
+                                         int nw) {
+    constexpr int RPI = 512 / D, CPR = D / 8;
+    const int lane = threadIdx.x & 63;
+    const int left = min(lk - key, ROWS);
+    const int bytes = left > 0 ? static_cast<int>(((left - 1) * stride + D) * 2) : 0;
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint16_t*>(base + static_cast<int64_t>(key) * stride), 0, bytes, kRsrcWord3);
+    const int lr = lane / CPR;
+#pragma unroll
+    for (int i = 0; i < ROWS / RPI; ++i) {
+        if (i * nw >= ROWS / RPI) break;
+        const int j = w + i * nw;
+        const int row = j * RPI + lr;
+        const int c = VTILE ? swz_v<D>(row, lane % CPR) : swz_k<D>(row, lane % CPR);
+        const uint32_t off = static_cast<uint32_t>(row) * static_cast<uint32_t>(stride) * 2u + c * 16;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            r, (__attribute__((address_space(3))) void*)(lds + j * 1024), 16, off, 0, 0, 0);
+    }
+}
+
+// A lane's byte offsets into a V tile for the transposing reads of channel
+// block dt (rows 16 t + 8 e + 4 half + lane % 16 / 4 add (16 t + 8 e) * 2 D)
+template <int D>
+__device__ __forceinline__ int v_lane_off(int dt) {
+    const int lane = threadIdx.x & 63, i = lane & 15;
+    const int row = 4 * (lane >> 5) + (i >> 2);
+    const int chunk = 4 * dt + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+    return row * (2 * D) + swz_v<D>(row, chunk) * 16 + (i & 1) * 8;
+}
+// The V^T fragments of 16-key group t, one per 32 channels: two transposing
+// reads each (4 keys a lane), waited for in the same statement. (Through the
+// builtin the compiler orders the reads behind every load in flight, the next
+// tiles' DMA included.)
+template <class T, int D, int t>
+__device__ __forceinline__ void read_v(const uint8_t* vt, const int (&off)[D / 32], typename T::frag (&f)[D / 32]) {
+    typedef int v2i __attribute__((ext_vector_type(2)));
+    constexpr int O0 = 16 * t * 2 * D, O1 = O0 + 8 * 2 * D;
+    const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+        (__attribute__((address_space(3))) const uint8_t*)vt));
+    v2i r[D / 16];
+    if constexpr (D == 128) {
+        asm volatile(
+            "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+            "ds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+            "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+            "ds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+            "s_waitcnt lgkmcnt(0)"
+            : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+            : "v"(base + off[0]), "v"(base + off[1]), "v"(base + off[2]), "v"(base + off[3]), "n"(O0), "n"(O1)
+            : "memory");
+    } else {
+        asm volatile(
+            "ds_read_b64_tr_b16 %0, %4 offset:%6\n\tds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
+            "ds_read_b64_tr_b16 %2, %5 offset:%6\n\tds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
+            "s_waitcnt lgkmcnt(0)"
+            : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
+            : "v"(base + off[0]), "v"(base + off[1]), "n"(O0), "n"(O1)
+            : "memory");
+    }
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+        f[d] = __builtin_bit_cast(typename T::frag, __builtin_shufflevector(r[2 * d], r[2 * d + 1], 0, 1, 2, 3));
+}
+
+// An infinite or NaN value of V at a key that some row does not see would
+// reach that row as 0 * inf. In a tile with hidden keys the fragments are
+// looked over, such values are taken out of the product (sanitize) and, once
+// the loop is done, added to the rows that see them (add_nonfinite).
+template <class T>
+__device__ __forceinline__ bool has_nonfinite(typename T::frag f) {
+    const v4i w = __builtin_bit_cast(v4i, f);
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t u = static_cast<uint32_t>(w[i]);
+        bad |= (u & T::kExp) == T::kExp;
+        bad |= (u & (T::kExp << 16)) == (T::kExp << 16);
+    }
+    return bad;
+}
+template <class T>
+__device__ __forceinline__ typename T::frag sanitize(typename T::frag f) {
+    v4i w = __builtin_bit_cast(v4i, f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t u = static_cast<uint32_t>(w[i]);
+        u = (u & T::kExp) == T::kExp ? u & 0xffff0000u : u;
+        u = (u & (T::kExp << 16)) == (T::kExp << 16) ? u & 0xffffu : u;
+        w[i] = static_cast<int>(u);
+    }
+    return __builtin_bit_cast(typename T::frag, w);
+}
+// o (channels 32 d + 8 g + 4 half + c of the lane's row) += the infinite and NaN
+// values of keys [key0, kmax)
+template <class T, int DT>
+__device__ __forceinline__ void add_nonfinite(const uint16_t* v, int64_t stride, int key0, int kmax, v16f (&o)[DT]) {
+    const int half = (threadIdx.x & 63) >> 5;
+    for (int key = key0; key < kmax; ++key) {
+        const uint16_t* vr = v + key * stride + 4 * half;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const uint2 u = *reinterpret_cast<const uint2*>(vr + 32 * d + 8 * g);
+                const uint32_t h[4] = {u.x & 0xffffu, u.x >> 16, u.y & 0xffffu, u.y >> 16};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const float inf = (h[c] & 0x8000u) ? -__builtin_inff() : __builtin_inff();
+                    const float bad = (h[c] & T::kMant) ? __builtin_nanf("") : inf;
+                    o[d][4 * g + c] += (h[c] & T::kExp) == T::kExp ? bad : 0.0f;
+                }
+            }
+    }
+}
+
+// ---- few rows: 32 of them, the keys over the waves --------------------------
+// Four waves share a tile of 32 rows and take its 32-key tiles in turn, each
+// with a ring of two K and two V slots of its own (no barrier in the loop; a
+// slot is refilled as soon as its fragments are in registers, so a wave keeps
+// up to four half tiles in flight). Their (O, m, sum) are joined through LDS
+// in wave order. With splits > 1 a sequence's keys are further cut into that
+// many ranges, one workgroup each, whose partial results attn_join_kernel adds
+// in order.
+constexpr int SR = 32, SK = 32, SW = 4;
+
+// Tiles [begin, end) of key range `split`, of `count` ranges in use: a.split_tiles tiles
+// each, more where the launch's a.splits ranges would not reach kend.
+struct KeyRange {
+    int begin, end, count;
+};
+__device__ __forceinline__ KeyRange split_range(const AttnVarlenArgs& a, int kend, int split) {
+    const int n = (kend + SK - 1) / SK;
+    const int per = a.splits == 1 ? n : max(a.split_tiles, (n + a.splits - 1) / a.splits);
+    KeyRange r;
+    r.begin = min(split * per, n);
+    r.end = min(r.begin + per, n);
+    r.count = per > 0 ? (n + per - 1) / per : 0;
+    return r;
+}
+
+// E channels of an output row: acc / tot, zeros where the row sees no key
+template <class T, int E>
+__device__ __forceinline__ void store_row(uint16_t* op, const float (&acc)[E], float tot, bool none) {
+    const float inv = 1.0f / tot;
+#pragma unroll
+    for (int e = 0; e < E; e += 8) {
+        u32x4 st;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) st[c] = none ? 0u : T::pack(acc[e + 2 * c] * inv, acc[e + 2 * c + 1] * inv);
+        *reinterpret_cast<u32x4*>(op + e) = st;
+    }
+}
+
+template <class T, int D>
+__global__ __launch_bounds__(SW * 64, 1) void attn_few_kernel(AttnVarlenArgs a) {
+    using frag = typename T::frag;
+    constexpr int KS = D / 16, DT = D / 32;
+    constexpr int TB = SK * D * 2;  // bytes of a K or V tile
+    constexpr int P = TB / 1024;    // DMA instructions per tile
+    constexpr int PITCH = D + 4;    // floats per row of the joined O
+    // One LDS object: with two, the compiler orders every read of this one
+    // behind all DMA in flight.
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[SW * 4 * TB + SW * SR * 8];
+    float(*ml)[SR][2] = reinterpret_cast<float(*)[SR][2]>(ring + SW * 4 * TB);
+    static_assert(4 * TB >= SR * PITCH * 4, "O takes the place of a wave's ring");
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l32 = lane & 31, half = lane >> 5;
+    const int split = blockIdx.x % a.splits;
+    const int item = blockIdx.x / a.splits;
+    const int hk = item % a.hk;
+    const RowTile t = find_tile(a, item / a.hk, SR);
+    if (!t.found) return;
+
+    const int rows = t.lq * a.group;  // < 2^31: the host bounds total_q * Hq
+    const int row = t.row0 + l32;
+    const bool valid = row < rows;
+    const int token = (valid ? row : rows - 1) / a.group;
+    const int head = hk * a.group + (valid ? row : rows - 1) % a.group;
+    const int kmax = visible(a, t, token);
+    const int row_last = min(t.row0 + SR, rows) - 1;
+    const int kend = visible(a, t, row_last / a.group);
+    const int kfull = visible(a, t, t.row0 / a.group);
+
+    const KeyRange range = split_range(a, kend, split);
+    const int tile0 = range.begin, tile1 = range.end;
+    if (split >= max(range.count, 1)) return;
+
+    frag qf[KS];
+    {
+        const uint16_t* qp = a.q + (static_cast<int64_t>(t.q0) + token) * a.q_t + head * a.q_h + 8 * half;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const frag*>(qp + 16 * s);
+    }
+    const uint16_t* kbase = a.k + static_cast<int64_t>(t.k0) * a.k_t + hk * a.k_h;
+    const uint16_t* vbase = a.v + static_cast<int64_t>(t.k0) * a.v_t + hk * a.v_h;
+    uint8_t* kring = ring + wave * 4 * TB;
+    uint8_t* vring = kring + 2 * TB;
+
+    v16f o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+    float m = kNegInf, sum = 0.0f;
+    int nonfinite = -1;  // first of this wave's tiles whose V was sanitized
+
+    int voff[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) voff[d] = v_lane_off<D>(d);
+
+    auto key_of = [&](int i) { return (tile0 + wave + SW * i) * SK; };
+    auto issue_k = [&](int i) { dma_tile<D, SK, false>(kbase, a.k_t, key_of(i), t.lk, kring + (i & 1) * TB, 0, 1); };
+    auto issue_v = [&](int i) { dma_tile<D, SK, true>(vbase, a.v_t, key_of(i), t.lk, vring + (i & 1) * TB, 0, 1); };
+    const int n = tile1 - tile0 > wave ? (tile1 - tile0 - wave + SW - 1) / SW : 0;
+    if (n > 0) {
+        issue_k(0);
+        issue_v(0);
+        issue_k(1);
+        issue_v(1);
+    }
+    for (int i = 0; i < n; ++i) {
+        const int key0 = key_of(i);
+        __builtin_amdgcn_sched_barrier(0);
+        wait_vmcnt<3 * P>();  // K of tile i
+        __builtin_amdgcn_sched_barrier(0);
+        v16f s;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+        const uint8_t* kt = kring + (i & 1) * TB;
+        frag kf[KS];
+#pragma unroll
+        for (int c = 0; c < KS; ++c)
+            kf[c] = *reinterpret_cast<const frag*>(kt + l32 * (2 * D) + swz_k<D>(l32, 2 * c + half) * 16);
+#pragma unroll
+        for (int c = 0; c < KS; ++c) s = T::mma(kf[c], qf[c], s);
+        __builtin_amdgcn_sched_barrier(0);
+        wait_lgkmcnt0();  // the slot's fragments are in registers
+        __builtin_amdgcn_sched_barrier(0);
+        issue_k(i + 2);
+
+        const bool hidden = key0 + SK > kfull;  // some row does not see some key
+        float p[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) p[r] = s[r] * a.scale_log2;
+        if (hidden) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (key0 + 8 * (r >> 2) + 4 * half + (r & 3) >= kmax) p[r] = kNegInf;
+        }
+        float mt = p[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mt = fmaxf(mt, p[r]);
+        mt = half_max(mt);
+        const bool bump = mt > m + kSlack;
+        const float m_new = bump ? mt : m;
+        if (__ballot(bump)) {
+            const float f = bump ? __builtin_amdgcn_exp2f(m - m_new) : 1.0f;
+            sum *= f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][r] *= f;
+        }
+        m = m_new;
+        const float neg = (m == kNegInf ? 0.0f : -m) + T::kPBias;
+        uint32_t pk[8];
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+            pk[r / 2] = T::pack(__builtin_amdgcn_exp2f(p[r] + neg), __builtin_amdgcn_exp2f(p[r + 1] + neg));
+            sum = T::add2(pk[r / 2], sum);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        wait_vmcnt<3 * P>();  // V of tile i
+        __builtin_amdgcn_sched_barrier(0);
+        const uint8_t* vt = vring + (i & 1) * TB;
+        frag vf[2][DT];
+        read_v<T, D, 0>(vt, voff, vf[0]);
+        read_v<T, D, 1>(vt, voff, vf[1]);
+        __builtin_amdgcn_sched_barrier(0);
+        issue_v(i + 2);
+        if (hidden) {
+            bool bad = false;
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+#pragma unroll
+                for (int d = 0; d < DT; ++d) bad |= has_nonfinite<T>(vf[g][d]);
+            if (__ballot(bad)) {
+                if (nonfinite < 0) nonfinite = i;
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) vf[g][d] = sanitize<T>(vf[g][d]);
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            const frag pf = __builtin_bit_cast(frag, (v4i){static_cast<int>(pk[4 * g]), static_cast<int>(pk[4 * g + 1]),
+                                                           static_cast<int>(pk[4 * g + 2]), static_cast<int>(pk[4 * g + 3])});
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[d] = T::mma(vf[g][d], pf, o[d]);
+        }
+    }
+    wait_vmcnt<0>();  // the loads past the last tile no longer write the ring
+
+    if (nonfinite >= 0)
+        for (int i = nonfinite; i < n; ++i)
+            add_nonfinite<T, DT>(vbase, a.v_t, key_of(i), min(key_of(i) + SK, kmax), o);
+
+    // the waves' shares: O into the wave's own ring, m and sum beside it
+    sum = half_sum(sum);
+    float* osh = reinterpret_cast<float*>(ring + wave * 4 * TB);
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<v4f*>(osh + l32 * PITCH + 32 * d + 8 * g + 4 * half) =
+                (v4f){o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+    if (half == 0) {
+        ml[wave][l32][0] = m;
+        ml[wave][l32][1] = sum;
+    }
+    __syncthreads();
+
+    // thread: row tid / 8, channels (tid % 8) * D / 8 ..
+    const int jr = threadIdx.x >> 3;
+    const int jrow = t.row0 + jr;
+    if (jrow >= rows) return;
+    constexpr int E = D / 8;
+    const int c0 = (threadIdx.x & 7) * E;
+    float mm = ml[0][jr][0];
+#pragma unroll
+    for (int w = 1; w < SW; ++w) mm = fmaxf(mm, ml[w][jr][0]);
+    float tot = 0.0f, acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < SW; ++w) {
+        const float mw = ml[w][jr][0];
+        if (mw == kNegInf) {  // no finite score: a NaN sum still counts
+            tot += ml[w][jr][1];
+            continue;
+        }
+        const float f = __builtin_amdgcn_exp2f(mw - mm);
+        tot += f * ml[w][jr][1];
+        const float* src = reinterpret_cast<const float*>(ring + w * 4 * TB) + jr * PITCH + c0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += f * src[e];
+    }
+    const int jtoken = jrow / a.group, jhead = hk * a.group + jrow % a.group;
+    if (a.splits > 1) {
+        const int64_t at = ((static_cast<int64_t>(t.q0) + jtoken) * a.hq + jhead) * a.splits + split;
+        float* po = a.part_o + at * D + c0;
+#pragma unroll
+        for (int e = 0; e < E; e += 4)
+            *reinterpret_cast<v4f*>(po + e) = (v4f){acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
+        if (c0 == 0) {
+            a.part_ml[2 * at] = mm;
+            a.part_ml[2 * at + 1] = tot;
+        }
+        return;
+    }
+    store_row<T, E>(a.out + (static_cast<int64_t>(t.q0) + jtoken) * a.o_t + jhead * a.o_h + c0, acc, tot,
+                    visible(a, t, jtoken) == 0);
+}
+
+// The key ranges' partial results of a tile of 32 rows, added in range order:
+// thread: row tid / 8, channels (tid % 8) * D / 8 ..
+template <class T, int D>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnVarlenArgs a) {
+    constexpr int E = D / 8;
+    const int hk = blockIdx.x % a.hk;
+    const RowTile t = find_tile(a, blockIdx.x / a.hk, SR);
+    if (!t.found) return;
+    const int row = t.row0 + (threadIdx.x >> 3);
+    if (row >= t.lq * a.group) return;
+    const int c0 = (threadIdx.x & 7) * E;
+    const int64_t token = static_cast<int64_t>(t.q0) + row / a.group;
+    const int head = hk * a.group + row % a.group;
+    const int64_t at = (token * a.hq + head) * a.splits;
+    const int kend = visible(a, t, (min(t.row0 + SR, t.lq * a.group) - 1) / a.group);
+    const int used = split_range(a, kend, 0).count;
+    float mm = kNegInf, tot = 0.0f, acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+    for (int s = 0; s < used; ++s) mm = fmaxf(mm, a.part_ml[2 * (at + s)]);
+    for (int s = 0; s < used; ++s) {
+        const float ms = a.part_ml[2 * (at + s)], ts = a.part_ml[2 * (at + s) + 1];
+        const float f = ms == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(ms - mm);  // -inf: O is zero there
+        tot += f * ts;
+        const float* po = a.part_o + (at + s) * D + c0;
+#pragma unroll
+        for (int e = 0; e < E; e += 4) {
+            const v4f v = *reinterpret_cast<const v4f*>(po + e);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[e + c] += f * v[c];
+        }
+    }
+    store_row<T, E>(a.out + token * a.o_t + head * a.o_h + c0, acc, tot, visible(a, t, row / a.group) == 0);
+}
+
+// ---- many rows: 256 of them, eight waves over one ring -----------------------
+// Wave w owns rows 32 w .. of the tile; 64-key tiles of K and V stream through
+// LDS rings (4 K slots, 5 V slots, three tiles ahead) and serve all eight
+// waves, so a tile's bytes are read once for 256 rows. A step is a softmax
+// phase (VALU, then the next tile's scores) and a PV phase (MFMA); waves 0-3
+// run softmax(kt), PV(kt), waves 4-7 PV(kt - 1), softmax(kt), so that a SIMD's
+// two waves use different units. One barrier a step. A wave skips tiles that
+// none of its rows sees.
+constexpr int MR = 256, MK = 64, MW = 8, MKS = 4, MVS = 5, MAHEAD = 3;
+
+template <class T, int D>
+__global__ __launch_bounds__(MW * 64) void attn_many_kernel(AttnVarlenArgs a, int tiles) {
+    using frag = typename T::frag;
+    constexpr int KS = D / 16, DT = D / 32;
+    constexpr int TB = MK * D * 2;
+    constexpr int PER = 2 * TB / 1024 / MW;  // DMA instructions per wave and tile (K and V)
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[(MKS + MVS) * TB];
+    uint8_t* const vring = ring + MKS * TB;
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l32 = lane & 31, half = lane >> 5;
+    // Causal: the sequences' last, longest tiles first, the heads of one tile
+    // side by side (a head stays on few XCDs as workgroups go round-robin over
+    // them). Otherwise all tiles of a head on one XCD.
+    int hk, idx;
+    if (a.causal) {
+        hk = blockIdx.x % a.hk;
+        idx = blockIdx.x / a.hk;
+    } else {
+        const int logical = xcd_remap(blockIdx.x, tiles * a.hk);
+        hk = logical / tiles;
+        idx = logical % tiles;
+    }
+    const RowTile t = find_tile(a, idx, MR);
+    if (!t.found) return;
+
+    const int rows = t.lq * a.group;
+    const int row = min(t.row0 + 32 * wave + l32, rows - 1);
+    const bool valid = t.row0 + 32 * wave + l32 < rows;
+    const int token = row / a.group;
+    const int head = hk * a.group + row % a.group;
+    const int kmax = visible(a, t, token);
+    const int kend = visible(a, t, (min(t.row0 + MR, rows) - 1) / a.group);  // of the whole tile
+    const int nkt = (kend + MK - 1) / MK;
+    // of this wave's rows: keys that all of them see, and that any of them sees
+    const int wrow0 = t.row0 + 32 * wave;
+    const int wfull = wrow0 < rows ? visible(a, t, wrow0 / a.group) : 0;
+    const int wend = wrow0 < rows ? visible(a, t, (min(wrow0 + 32, rows) - 1) / a.group) : 0;
+
+    frag qf[KS];
+    {
+        const uint16_t* qp = a.q + (static_cast<int64_t>(t.q0) + token) * a.q_t + head * a.q_h + 8 * half;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const frag*>(qp + 16 * s);
+    }
+    const uint16_t* kbase = a.k + static_cast<int64_t>(t.k0) * a.k_t + hk * a.k_h;
+    const uint16_t* vbase = a.v + static_cast<int64_t>(t.k0) * a.v_t + hk * a.v_h;
+    auto issue = [&](int kt) {
+        dma_tile<D, MK, false>(kbase, a.k_t, kt * MK, t.lk, ring + kt % MKS * TB, wave, MW);
+        dma_tile<D, MK, true>(vbase, a.v_t, kt * MK, t.lk, vring + kt % MVS * TB, wave, MW);
+    };
+
+    v16f o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+    float m = kNegInf, sum = 0.0f;
+    int nonfinite = -1;  // first of this wave's tiles whose V was sanitized
+    int voff[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) voff[d] = v_lane_off<D>(d);
+
+#pragma unroll
+    for (int i = 0; i < MAHEAD; ++i) issue(i);
+    wait_vmcnt<PER>();  // tiles 0 and 1
+    __builtin_amdgcn_s_barrier();
+
+    v16f s[2];
+    auto scores = [&](int kt) {
+        const uint8_t* kl = ring + kt % MKS * TB;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int kr = 32 * b + l32;
+            frag kf[KS];
+#pragma unroll
+            for (int c = 0; c < KS; ++c)
+                kf[c] = *reinterpret_cast<const frag*>(kl + kr * (2 * D) + swz_k<D>(kr, 2 * c + half) * 16);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[b][r] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < KS; ++c) s[b] = T::mma(kf[c], qf[c], s[b]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    uint32_t pk[16];  // P of the current tile: 16-key group g at pk[4 g ..]
+    auto softmax = [&](int kt) {
+        if (kt * MK + MK > wfull) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (kt * MK + 32 * b + 8 * (r >> 2) + 4 * half + (r & 3) >= kmax) s[b][r] = kNegInf;
+        }
+        float mt = s[0][0];
+#pragma unroll
+        for (int r = 1; r < 32; ++r) mt = fmaxf(mt, s[r >> 4][r & 15]);
+        mt = half_max(mt) * a.scale_log2;
+        const bool bump = mt > m + kSlack;
+        const float m_new = bump ? mt : m;
+        if (__ballot(bump)) {
+            const float f = bump ? __builtin_amdgcn_exp2f(m - m_new) : 1.0f;
+            sum *= f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][r] *= f;
+        }
+        m = m_new;
+        const float neg = (m == kNegInf ? 0.0f : -m) + T::kPBias;
+#pragma unroll
+        for (int r = 0; r < 32; r += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r >> 4][r & 15], a.scale_log2, neg));
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r >> 4][(r & 15) + 1], a.scale_log2, neg));
+            pk[r / 2] = T::pack(p0, p1);
+            sum = T::add2(pk[r / 2], sum);
+        }
+    };
+    auto pv = [&](int kt) {
+        const uint8_t* vt = vring + kt % MVS * TB;
+        const bool hidden = kt * MK + MK > wfull;
+        auto group = [&](auto gc) {
+            constexpr int g = decltype(gc)::value;
+            frag vf[DT];
+            read_v<T, D, g>(vt, voff, vf);
+            if (hidden) {
+                bool bad = false;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) bad |= has_nonfinite<T>(vf[d]);
+                if (__ballot(bad)) {
+                    if (nonfinite < 0) nonfinite = kt;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) vf[d] = sanitize<T>(vf[d]);
+                }
+            }
+            const frag pf = __builtin_bit_cast(frag, (v4i){static_cast<int>(pk[4 * g]), static_cast<int>(pk[4 * g + 1]),
+                                                           static_cast<int>(pk[4 * g + 2]), static_cast<int>(pk[4 * g + 3])});
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[d] = T::mma(vf[d], pf, o[d]);
+        };
+        group(std::integral_constant<int, 0>{});
+        group(std::integral_constant<int, 1>{});
+        group(std::integral_constant<int, 2>{});
+        group(std::integral_constant<int, 3>{});
+    };
+    scores(0);
+    const bool lag = wave >= MW / 2;
+    const int wtiles = (wend + MK - 1) / MK;  // tiles that this wave works on
+    for (int kt = 0; kt < nkt; ++kt) {
+        issue(kt + MAHEAD);
+        __builtin_amdgcn_sched_barrier(0);
+        if (lag && kt > 0 && kt <= wtiles) pv(kt - 1);
+        if (kt < wtiles) {
+            softmax(kt);
+            __builtin_amdgcn_sched_barrier(0);
+            scores(kt + 1);
+        }
+        if (!lag && kt < wtiles) pv(kt);
+        // this wave's reads are done and its share of tile kt + 2 has landed
+        __builtin_amdgcn_sched_barrier(0);
+        wait_vmcnt<PER>();
+        wait_lgkmcnt0();
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    if (lag && wtiles == nkt && nkt > 0) pv(nkt - 1);
+    wait_vmcnt<0>();  // the loads past the last tile no longer write the ring
+    if (nonfinite >= 0) add_nonfinite<T, DT>(vbase, a.v_t, nonfinite * MK, kmax, o);
+
+    if (!valid) return;
+    const float tot = half_sum(sum);
+    const float inv = 1.0f / tot;
+    // channels 8 (g + half) .. of block d after the lane halves have exchanged
+    // their four of g and g + 1
+    uint16_t* op = a.out + (static_cast<int64_t>(t.q0) + token) * a.o_t + head * a.o_h + 8 * half;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; g += 2) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t x = T::pack(o[d][4 * g + 2 * i] * inv, o[d][4 * g + 2 * i + 1] * inv);
+                const uint32_t y = T::pack(o[d][4 * g + 4 + 2 * i] * inv, o[d][4 * g + 4 + 2 * i + 1] * inv);
+                const auto sw = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+                w[i] = kmax == 0 ? 0u : sw[0];
+                w[2 + i] = kmax == 0 ? 0u : sw[1];
+            }
+            *reinterpret_cast<u32x4*>(op + 32 * d + 8 * g) = (u32x4){w[0], w[1], w[2], w[3]};
+        }
+}
+
+// upper bound on the tiles of `rows` rows that the sequences have
+int64_t tile_bound(int total_q, int batch, int group, int rows) {
+    const int64_t seqs = batch < total_q ? batch : total_q;
+    return (static_cast<int64_t>(total_q) * group + seqs * (rows - 1)) / rows;
+}
+
+}  // namespace
+
+static bool attn_varlen_many(int total_q, int batch, int hq, int hk) {
+    return tile_bound(total_q, batch, hq / hk, MR) * hk >= 96;
+}
+
+// Key ranges of the few-row kernel: where its tiles leave CUs idle, a
+// sequence's keys are cut into ranges of *split_tiles 32-key tiles (about two
+// workgroups a CU over the whole launch, four tiles a wave at least), at most 32 of them.
+int attn_varlen_splits(int total_q, int total_k, int batch, int hq, int hk, int* split_tiles) {
+    *split_tiles = 1;
+    if (total_q <= 0 || batch <= 0 || total_k <= 0) return 1;
+    const int64_t wgs = tile_bound(total_q, batch, hq / hk, SR) * hk;
+    if (wgs > 128 || attn_varlen_many(total_q, batch, hq, hk)) return 1;
+    const int64_t seqs = batch < total_q ? batch : total_q;
+    const int64_t key_tiles = wgs * ((total_k + seqs - 1) / seqs) / SK;  // of an average sequence
+    int64_t per = (key_tiles + 511) / 512;
+    per = per < 4 * SW ? 4 * SW : per;
+    const int64_t most = (total_k + SK - 1) / SK;
+    *split_tiles = static_cast<int>(per);
+    int64_t s = (most + per - 1) / per;
+    return static_cast<int>(s < 1 ? 1 : s > 32 ? 32 : s);
+}
+
+template <class T, int D>
+static hipError_t launch_few(const AttnVarlenArgs& a, hipStream_t stream) {
+    const int64_t tiles = tile_bound(a.total_q, a.batch, a.group, SR);
+    hipLaunchKernelGGL((attn_few_kernel<T, D>), dim3(static_cast<unsigned>(tiles * a.hk * a.splits)), dim3(SW * 64), 0,
+                       stream, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || a.splits == 1) return e;
+    hipLaunchKernelGGL((attn_join_kernel<T, D>), dim3(static_cast<unsigned>(tiles * a.hk)), dim3(256), 0, stream, a);
+    return hipGetLastError();
+}
+
+template <class T, int D>
+static hipError_t launch_many(const AttnVarlenArgs& a, hipStream_t stream) {
+    const int tiles = static_cast<int>(tile_bound(a.total_q, a.batch, a.group, MR));
+    hipLaunchKernelGGL((attn_many_kernel<T, D>), dim3(tiles * a.hk), dim3(MW * 64), 0, stream, a, tiles);
+    return hipGetLastError();
+}
+
+template <class T, int D>
+static hipError_t launch_attn(const AttnVarlenArgs& a, hipStream_t stream) {
+    return attn_varlen_many(a.total_q, a.batch, a.hq, a.hk) ? launch_many<T, D>(a, stream) : launch_few<T, D>(a, stream);
+}
+
+hipError_t launch_attention_varlen(const AttnVarlenArgs& a, int dtype, int D, hipStream_t stream) {
+    if (dtype == QIMG_BF16)
+        return D == 128 ? launch_attn<Bf16, 128>(a, stream) : launch_attn<Bf16, 64>(a, stream);
+    return D == 128 ? launch_attn<Fp16, 128>(a, stream) : launch_attn<Fp16, 64>(a, stream);
+}
+
+}  // namespace qimg

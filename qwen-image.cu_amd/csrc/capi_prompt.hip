@@ -1,0 +1,90 @@
+// capi_prompt.hip — C entry points of the operators around a prompt: argument
+// checks on the host, then the launches.
+#include <cmath>
+
+#include "qimg_internal.h"
+
+#define QIMG_REQUIRE(cond, ...)                                                     \
+    do {                                                                            \
+        if (!(cond)) return qimg::api_fail(QIMG_ERR_INVALID_ARG, __VA_ARGS__);      \
+    } while (0)
+
+namespace {
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
+
+// strides of one operand of the attention, in elements
+bool good_strides(int64_t t, int64_t h) {
+    return t >= 0 && t <= (int64_t{1} << 24) && h >= 0 && t % 8 == 0 && h % 8 == 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t qimg_attention_varlen_scratch_bytes(int total_q, int total_k, int batch, int n_heads, int n_kv_heads,
+                                            int head_dim) {
+    if (total_q <= 0 || total_k <= 0 || batch <= 0 || n_heads <= 0 || n_kv_heads <= 0 || head_dim <= 0 ||
+        n_heads % n_kv_heads != 0)
+        return 0;
+    int tiles = 0;
+    const int splits = qimg::attn_varlen_splits(total_q, total_k, batch, n_heads, n_kv_heads, &tiles);
+    if (splits == 1) return 0;
+    const int64_t parts = static_cast<int64_t>(total_q) * n_heads * splits;
+    return align256(parts * head_dim * 4) + align256(parts * 8);
+}
+
+int qimg_attention_varlen(const qimg_attn_varlen* args, void* scratch, int64_t scratch_bytes, void* stream) {
+    const char* fn = "qimg_attention_varlen";
+    QIMG_REQUIRE(args, "%s: args is null", fn);
+    const qimg_attn_varlen& p = *args;
+    QIMG_REQUIRE(p.dtype == QIMG_BF16 || p.dtype == QIMG_FP16, "%s: dtype %d must be BF16 or FP16", fn, p.dtype);
+    QIMG_REQUIRE(p.batch >= 0 && p.total_q >= 0 && p.total_k >= 0, "%s: bad sizes batch=%d total_q=%d total_k=%d", fn,
+                 p.batch, p.total_q, p.total_k);
+    QIMG_REQUIRE(p.n_heads > 0 && p.n_kv_heads > 0 && p.n_heads % p.n_kv_heads == 0,
+                 "%s: n_heads %d must be a multiple of n_kv_heads %d", fn, p.n_heads, p.n_kv_heads);
+    if (p.head_dim != 64 && p.head_dim != 128)
+        return qimg::api_fail(QIMG_ERR_UNSUPPORTED, "%s: head_dim %d not supported (64 or 128)", fn, p.head_dim);
+    QIMG_REQUIRE(std::isfinite(p.sm_scale) && p.sm_scale > 0.0f, "%s: sm_scale must be positive and finite", fn);
+    QIMG_REQUIRE(static_cast<int64_t>(p.total_q) * p.n_heads < (int64_t{1} << 30),
+                 "%s: total_q * n_heads must be < 2^30", fn);
+    QIMG_REQUIRE(good_strides(p.q_stride_t, p.q_stride_h) && good_strides(p.k_stride_t, p.k_stride_h) &&
+                     good_strides(p.v_stride_t, p.v_stride_h) && good_strides(p.out_stride_t, p.out_stride_h),
+                 "%s: strides must be non-negative multiples of 8, token strides at most 2^24", fn);
+    if (p.batch == 0 || p.total_q == 0) return QIMG_OK;
+    QIMG_REQUIRE(p.q && p.out && p.cu_seqlens_q && p.cu_seqlens_k, "%s: null pointer", fn);
+    QIMG_REQUIRE(p.total_k == 0 || (p.k && p.v), "%s: null pointer", fn);
+    QIMG_REQUIRE(aligned16(p.q) && aligned16(p.k) && aligned16(p.v) && aligned16(p.out),
+                 "%s: q, k, v and out must be 16-byte aligned", fn);
+    QIMG_REQUIRE(p.out != p.q && p.out != p.k && p.out != p.v, "%s: out must not be q, k or v", fn);
+    QIMG_REQUIRE((p.total_q == 1 || p.out_stride_t >= p.head_dim) && (p.n_heads == 1 || p.out_stride_h >= p.head_dim),
+                 "%s: out strides must be at least head_dim", fn);
+    qimg::AttnVarlenArgs a{};
+    a.q = static_cast<const uint16_t*>(p.q);
+    a.k = static_cast<const uint16_t*>(p.k);
+    a.v = static_cast<const uint16_t*>(p.v);
+    a.out = static_cast<uint16_t*>(p.out);
+    a.q_t = p.q_stride_t, a.q_h = p.q_stride_h, a.k_t = p.k_stride_t, a.k_h = p.k_stride_h;
+    a.v_t = p.v_stride_t, a.v_h = p.v_stride_h, a.o_t = p.out_stride_t, a.o_h = p.out_stride_h;
+    a.cu_q = p.cu_seqlens_q, a.cu_k = p.cu_seqlens_k, a.k_lens = p.k_lens;
+    a.batch = p.batch, a.total_q = p.total_q, a.total_k = p.total_k;
+    a.hq = p.n_heads, a.hk = p.n_kv_heads, a.group = p.n_heads / p.n_kv_heads;
+    a.causal = p.causal != 0;
+    a.scale_log2 = p.sm_scale * 1.4426950408889634f;
+    a.splits = qimg::attn_varlen_splits(p.total_q, p.total_k, p.batch, p.n_heads, p.n_kv_heads, &a.split_tiles);
+    if (a.splits > 1) {
+        const int64_t need = qimg_attention_varlen_scratch_bytes(p.total_q, p.total_k, p.batch, p.n_heads,
+                                                                 p.n_kv_heads, p.head_dim);
+        if (!scratch || scratch_bytes < need)
+            return qimg::api_fail(QIMG_ERR_SCRATCH, "%s: scratch %lld bytes < required %lld", fn,
+                                  static_cast<long long>(scratch_bytes), static_cast<long long>(need));
+        QIMG_REQUIRE(aligned16(scratch), "%s: scratch must be 16-byte aligned", fn);
+        a.part_o = static_cast<float*>(scratch);
+        a.part_ml = a.part_o + align256(static_cast<int64_t>(p.total_q) * p.n_heads * a.splits * p.head_dim * 4) / 4;
+    }
+    return qimg::api_hip_status(
+        qimg::launch_attention_varlen(a, p.dtype, p.head_dim, static_cast<hipStream_t>(stream)), fn);
+}
+
+}  // extern "C"

@@ -323,4 +323,25 @@ hipError_t run_mmdit_block(const qimg_mmdit_block& b, float* img, float* txt, co
                            bool t_ready = false, int mods_set = 0, bool mods_ready = false,
                            const qimg_mmdit_block* next = nullptr, bool* next_ready = nullptr);
 
+// attention_varlen.hip: attention over packed sequences (qimg_attention_varlen),
+// strides in elements
+struct AttnVarlenArgs {
+    const uint16_t* q;
+    const uint16_t* k;
+    const uint16_t* v;
+    uint16_t* out;
+    int64_t q_t, q_h, k_t, k_h, v_t, v_h, o_t, o_h;
+    const int* cu_q;
+    const int* cu_k;
+    const int* k_lens;  // or null: every key of a sequence's slot
+    int batch, total_q, total_k, hq, hk, group;
+    int causal;
+    float scale_log2;  // sm_scale * log2(e)
+    int splits, split_tiles;  // key ranges of the few-row kernel, 32-key tiles a range
+    float* part_o;   // [total_q, hq, splits, D] with splits > 1
+    float* part_ml;  // [total_q, hq, splits, 2]: running maximum, sum
+};
+int attn_varlen_splits(int total_q, int total_k, int batch, int hq, int hk, int* split_tiles);
+hipError_t launch_attention_varlen(const AttnVarlenArgs& a, int dtype, int D, hipStream_t stream);
+
 }  // namespace qimg

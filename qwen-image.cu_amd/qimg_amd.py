@@ -67,6 +67,8 @@ _SIGS = {
     "qimg_sage_quant_k": (_I, [_P, _P, _P, _P, _I, _I, _I, _P]),
     "qimg_sage_attn_quantized": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _P, _I64, _P]),
     "qimg_sage_attention": (_I, [_P, _P, _P, _P, _I, _F, _I, _I, _I, _I, _P, _I64, _P]),
+    "qimg_attention_varlen_scratch_bytes": (_I64, [_I, _I, _I, _I, _I, _I]),
+    "qimg_attention_varlen": (_I, [_P, _P, _I64, _P]),
     "qimg_silu": (_I, [_P, _P, _I64, _P]),
     "qimg_layernorm_modulate": (_I, [_P, _P, _P, _P, _I, _I, _F, _P]),
     "qimg_layernorm_modulate_quant": (_I, [_P, _P, _P, _I, _I, _I, _I, _F, _P, _P, _P]),
@@ -610,6 +612,83 @@ def attention_forward_sage_fp16io(q: torch.Tensor, k: torch.Tensor, v: torch.Ten
         scratch = torch.empty((max(sage_scratch_bytes(BH, S, D), 1),), dtype=torch.uint8, device=q.device)
     _check(_lib.qimg_sage_attention(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _DT[out.dtype], float(scale),
                                     BH, S, D, int(bool(causal)), _ptr(scratch), scratch.numel(), _stream()))
+    return out
+
+
+# --------------------------------------------------- prompts: packed attention
+class _AttnVarlen(ctypes.Structure):
+    _fields_ = [("q", _P), ("k", _P), ("v", _P), ("out", _P), ("dtype", _I),
+                ("q_stride_t", _I64), ("q_stride_h", _I64), ("k_stride_t", _I64), ("k_stride_h", _I64),
+                ("v_stride_t", _I64), ("v_stride_h", _I64), ("out_stride_t", _I64), ("out_stride_h", _I64),
+                ("cu_seqlens_q", _P), ("cu_seqlens_k", _P), ("k_lens", _P),
+                ("batch", _I), ("total_q", _I), ("total_k", _I), ("n_heads", _I), ("n_kv_heads", _I),
+                ("head_dim", _I), ("sm_scale", _F), ("causal", _I)]
+
+
+def _require(cond, message: str):
+    if not cond:
+        raise QimgError(QIMG_ERR_INVALID_ARG, message)
+
+
+def _same_device(ref: torch.Tensor, **tensors):
+    for name, t in tensors.items():
+        if t is not None:
+            _require(t.is_cuda and t.device == ref.device, f"{name} must be a tensor on {ref.device}")
+
+
+def _scratch_for(need: int, scratch: torch.Tensor | None, device) -> torch.Tensor | None:
+    """The caller's scratch, or a buffer of `need` bytes; its bytes are counted, not its elements."""
+    if scratch is None:
+        return torch.empty((need,), dtype=torch.uint8, device=device) if need else None
+    _require(scratch.is_cuda and scratch.device == device and scratch.is_contiguous(),
+             f"scratch must be a contiguous tensor on {device}")
+    return scratch
+
+
+def _nbytes(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.numel() * t.element_size()
+
+
+def attention_varlen_scratch_bytes(total_q: int, total_k: int, batch: int, n_heads: int, n_kv_heads: int,
+                                   head_dim: int) -> int:
+    return int(_lib.qimg_attention_varlen_scratch_bytes(total_q, total_k, batch, n_heads, n_kv_heads, head_dim))
+
+
+def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                     cu_seqlens_k: torch.Tensor, sm_scale: float | None = None, causal: bool = True,
+                     k_lens: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                     scratch: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention over packed sequences of different lengths: q [Tq, Hq, D], k
+    and v [Tk, Hk, D] (bf16 or fp16, D 64 or 128, Hq a multiple of Hk; views
+    with any token and head strides that are multiples of 8 elements),
+    cu_seqlens_* int32 [B + 1]. causal: the last query of a sequence sees its
+    last key. k_lens int32 [B]: keys in use of each sequence's slot (a cache
+    with room behind its last key). Queries that see no key give zeros; rows of
+    no sequence are not written. sm_scale defaults to 1 / sqrt(D)."""
+    _require(q.is_cuda and q.dim() == 3 and k.dim() == 3 and v.dim() == 3, "q, k and v must be device tensors [T, H, D]")
+    _same_device(q, k=k, v=v, cu_seqlens_q=cu_seqlens_q, cu_seqlens_k=cu_seqlens_k, k_lens=k_lens, out=out)
+    _require(q.dtype in (torch.bfloat16, torch.float16) and k.dtype == q.dtype and v.dtype == q.dtype,
+             "q, k and v must be all bfloat16 or all float16")
+    tq, hq, d = q.shape
+    tk, hk, dk = k.shape
+    _require(v.shape == k.shape and dk == d, f"k {tuple(k.shape)} and v {tuple(v.shape)} must be [Tk, Hk, {d}]")
+    _require(q.stride(2) == 1 and k.stride(2) == 1 and v.stride(2) == 1, "the last dimension must be contiguous")
+    batch = cu_seqlens_q.numel() - 1
+    _require(batch >= 0 and cu_seqlens_k.numel() == batch + 1, "cu_seqlens_q and cu_seqlens_k must have B + 1 elements")
+    for name, t in (("cu_seqlens_q", cu_seqlens_q), ("cu_seqlens_k", cu_seqlens_k), ("k_lens", k_lens)):
+        _require(t is None or (t.dtype == torch.int32 and t.is_contiguous()), f"{name} must be contiguous int32")
+    _require(k_lens is None or k_lens.numel() == batch, "k_lens must have B elements")
+    if out is None:
+        out = torch.empty((tq, hq, d), dtype=q.dtype, device=q.device)
+    _require(out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1,
+             f"out must be {tuple(q.shape)} of q's type, its last dimension contiguous")
+    with torch.cuda.device(q.device):
+        scratch = _scratch_for(attention_varlen_scratch_bytes(tq, tk, batch, hq, hk, d), scratch, q.device)
+        args = _AttnVarlen(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _DT[q.dtype], q.stride(0), q.stride(1), k.stride(0),
+                           k.stride(1), v.stride(0), v.stride(1), out.stride(0), out.stride(1), _ptr(cu_seqlens_q),
+                           _ptr(cu_seqlens_k), _ptr(k_lens), batch, tq, tk, hq, hk, d,
+                           1.0 / d ** 0.5 if sm_scale is None else float(sm_scale), int(bool(causal)))
+        _check(_lib.qimg_attention_varlen(ctypes.byref(args), _ptr(scratch), _nbytes(scratch), _stream(q.device)))
     return out
 
 
