@@ -117,28 +117,53 @@ __device__ __forceinline__ int swz_v(int row, int c) {
 struct RowTile {
     int q0, lq, k0, lk;  // first query and key row, their numbers
     int row0;            // first (token, head) row of the tile in the sequence
+    int split, splits;   // key range of it, and into how many the sequence's keys are cut
     bool found;
 };
 
-// Tile `idx` of the launch: the sequences' tiles of `rows` rows in order,
-// inside a causal sequence the last (longest) tile first. Offsets outside
-// [0, total] or falling ones are clamped, so no tile reaches past the tensors.
-// Each lane takes one sequence; a wave scans 64 of them at a time.
-__device__ __forceinline__ RowTile find_tile(const AttnVarlenArgs& a, int idx, int rows) {
+// A lane's sequence b: first query and key row, numbers of both. Offsets
+// outside [0, total] or falling ones are clamped, so no tile reaches past the
+// tensors.
+struct Sequence {
+    int q0, lq, k0, lk;
+};
+__device__ __forceinline__ Sequence load_sequence(const AttnVarlenArgs& a, int b) {
+    Sequence s = {0, 0, 0, 0};
+    if (b < a.batch) {
+        s.q0 = min(max(a.cu_q[b], 0), a.total_q);
+        s.lq = min(max(a.cu_q[b + 1], s.q0), a.total_q) - s.q0;
+        s.k0 = min(max(a.cu_k[b], 0), a.total_k);
+        s.lk = min(max(a.cu_k[b + 1], s.k0), a.total_k) - s.k0;
+        if (a.k_lens != nullptr) s.lk = min(s.lk, max(a.k_lens[b], 0));
+    }
+    return s;
+}
+__device__ __forceinline__ int row_tiles(const AttnVarlenArgs& a, int lq, int rows) {
+    return static_cast<int>((static_cast<int64_t>(lq) * a.group + rows - 1) / rows);
+}
+// key ranges of `per` tiles of SK keys that lk keys are cut into (per = 0: one)
+constexpr int SK = 32;
+__device__ __forceinline__ int key_ranges(int lk, int per) {
+    if (per == 0) return 1;
+    const int n = (lk + SK - 1) / SK;
+    return max((n + per - 1) / per, 1);
+}
+
+// Item `idx` of the launch: the sequences in order, each with its tiles of
+// `rows` rows (inside a causal sequence the last, longest one first) times its
+// key ranges of `per` tiles. Each lane takes one sequence; a wave scans 64 of
+// them at a time.
+__device__ __forceinline__ RowTile find_tile(const AttnVarlenArgs& a, int idx, int rows, int per) {
     const int lane = threadIdx.x & 63;
     RowTile t;
     t.found = false;
-    t.q0 = t.lq = t.k0 = t.lk = t.row0 = 0;
+    t.q0 = t.lq = t.k0 = t.lk = t.row0 = t.split = 0;
+    t.splits = 1;
     int before = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
-        const int b = b0 + lane;
-        int qs = 0, qe = 0;
-        if (b < a.batch) {
-            qs = min(max(a.cu_q[b], 0), a.total_q);
-            qe = min(max(a.cu_q[b + 1], qs), a.total_q);
-        }
-        const int n = static_cast<int>((static_cast<int64_t>(qe - qs) * a.group + rows - 1) / rows);
-        int incl = n;
+        const Sequence s = load_sequence(a, b0 + lane);
+        const int n = row_tiles(a, s.lq, rows), parts = key_ranges(s.lk, per);
+        int incl = n * parts;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
             const int v = __shfl_up(incl, off, 64);
@@ -146,20 +171,17 @@ __device__ __forceinline__ RowTile find_tile(const AttnVarlenArgs& a, int idx, i
         }
         const int total = __builtin_amdgcn_readlane(incl, 63);
         if (idx < before + total) {
-            const uint64_t hit = __ballot(before + incl > idx);
-            const int src = __builtin_ctzll(hit);
-            const int sb = b0 + src;
-            t.q0 = __builtin_amdgcn_readlane(qs, src);
-            t.lq = __builtin_amdgcn_readlane(qe, src) - t.q0;
+            const int src = __builtin_ctzll(__ballot(before + incl > idx));
+            t.q0 = __builtin_amdgcn_readlane(s.q0, src);
+            t.lq = __builtin_amdgcn_readlane(s.lq, src);
+            t.k0 = __builtin_amdgcn_readlane(s.k0, src);
+            t.lk = __builtin_amdgcn_readlane(s.lk, src);
+            t.splits = __builtin_amdgcn_readlane(parts, src);
             const int cnt = __builtin_amdgcn_readlane(n, src);
-            const int first = before + __builtin_amdgcn_readlane(incl, src) - cnt;
-            const int ks = min(max(__builtin_amdgcn_readfirstlane(a.cu_k[sb]), 0), a.total_k);
-            const int ke = min(max(__builtin_amdgcn_readfirstlane(a.cu_k[sb + 1]), ks), a.total_k);
-            t.k0 = ks;
-            t.lk = ke - ks;
-            if (a.k_lens != nullptr) t.lk = min(t.lk, max(__builtin_amdgcn_readfirstlane(a.k_lens[sb]), 0));
-            const int i = idx - first;
-            t.row0 = (a.causal ? cnt - 1 - i : i) * rows;
+            const int i = idx - (before + __builtin_amdgcn_readlane(incl, src) - cnt * t.splits);
+            const int tile = i / t.splits;
+            t.split = i % t.splits;
+            t.row0 = (a.causal ? cnt - 1 - tile : tile) * rows;
             t.found = true;
             return t;
         }
@@ -174,24 +196,19 @@ __device__ __forceinline__ int visible(const AttnVarlenArgs& a, const RowTile& t
     return min(max(token + 1 + t.lk - t.lq, 0), t.lk);
 }
 
-// DMA of keys [key, key + ROWS) of one kv head to LDS: instruction j brings
-// 1 KB = 512 / D rows, instructions w, w + nw, .. here. Rows from the
-// sequence's end on are zeros.
+// DMA of keys [key, key + ROWS) of one kv head to LDS by one wave, 1 KB = 512 / D
+// rows an instruction. Rows from the sequence's end on are zeros.
 template <int D, int ROWS, bool VTILE>
-__device__ __forceinline__ void dma_tile(const uint16_t* base, int64_t stride, int key, int lk, uint8_t* lds, int w,
-                                         int nw) {
+__device__ __forceinline__ void dma_tile(const uint16_t* base, int64_t stride, int key, int lk, uint8_t* lds) {
     constexpr int RPI = 512 / D, CPR = D / 8;
     const int lane = threadIdx.x & 63;
     const int left = min(lk - key, ROWS);
     const int bytes = left > 0 ? static_cast<int>(((left - 1) * stride + D) * 2) : 0;
     const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<uint16_t*>(base + static_cast<int64_t>(key) * stride), 0, bytes, kRsrcWord3);
-    const int lr = lane / CPR;
 #pragma unroll
-    for (int i = 0; i < ROWS / RPI; ++i) {
-        if (i * nw >= ROWS / RPI) break;
-        const int j = w + i * nw;
-        const int row = j * RPI + lr;
+    for (int j = 0; j < ROWS / RPI; ++j) {
+        const int row = j * RPI + lane / CPR;
         const int c = VTILE ? swz_v<D>(row, lane % CPR) : swz_k<D>(row, lane % CPR);
         const uint32_t off = static_cast<uint32_t>(row) * static_cast<uint32_t>(stride) * 2u + c * 16;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(
@@ -296,27 +313,31 @@ __device__ __forceinline__ void add_nonfinite(const uint16_t* v, int64_t stride,
 
 // ---- few rows: 32 of them, the keys over the waves --------------------------
 // Four waves share a tile of 32 rows and take its 32-key tiles in turn, each
-// with a ring of two K and two V slots of its own (no barrier in the loop; a
-// slot is refilled as soon as its fragments are in registers, so a wave keeps
-// up to four half tiles in flight). Their (O, m, sum) are joined through LDS
-// in wave order. With splits > 1 a sequence's keys are further cut into that
-// many ranges, one workgroup each, whose partial results attn_join_kernel adds
-// in order.
-constexpr int SR = 32, SK = 32, SW = 4;
+// with K and V slots of its own (no barrier in the loop; a slot is refilled as
+// soon as its fragments are in registers). Their (O, m, sum) are joined through
+// LDS in wave order. Two workgroups a CU (64 KB of tiles each). With a.splits > 1
+// long sequences' keys are further cut into ranges, whose partial results
+// attn_join_kernel adds in order. The launch is at most two workgroups a CU,
+// which walk over the items that the lengths on the device give: a grid sized by
+// the host's bound on them would mostly be workgroups without work, 2.5 us each.
+constexpr int SR = 32, SW = 4;
 
-// Tiles [begin, end) of key range `split`, of `count` ranges in use: a.split_tiles tiles
-// each, more where the launch's a.splits ranges would not reach kend.
-struct KeyRange {
-    int begin, end, count;
-};
-__device__ __forceinline__ KeyRange split_range(const AttnVarlenArgs& a, int kend, int split) {
-    const int n = (kend + SK - 1) / SK;
-    const int per = a.splits == 1 ? n : max(a.split_tiles, (n + a.splits - 1) / a.splits);
-    KeyRange r;
-    r.begin = min(split * per, n);
-    r.end = min(r.begin + per, n);
-    r.count = per > 0 ? (n + per - 1) / per : 0;
-    return r;
+// Key tiles per range: as many as make the launch about one item a workgroup,
+// at least four a wave, and at most a.splits ranges a sequence. 0: no ranges.
+__device__ __forceinline__ int range_tiles(const AttnVarlenArgs& a) {
+    if (a.splits == 1) return 0;
+    const int lane = threadIdx.x & 63;
+    int longest = 0;
+    float work = 0.0f;  // (row tiles x key tiles: a sum that needs no last digit)
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+        const Sequence s = load_sequence(a, b0 + lane);
+        const int kt = (s.lk + SK - 1) / SK;
+        work += wave_sum_dpp(static_cast<float>(row_tiles(a, s.lq, SR)) * static_cast<float>(kt));
+        longest = max(longest, wave_reduce_dpp(kt, [](int x, int y) { return max(x, y); }));
+    }
+    int per = static_cast<int>(work * static_cast<float>(a.hk) / static_cast<float>(a.target_items)) + 1;
+    per = max(per, 4 * SW);
+    return __builtin_amdgcn_readfirstlane(max(per, (longest + a.splits - 1) / a.splits));
 }
 
 // E channels of an output row: acc / tot, zeros where the row sees no key
@@ -332,41 +353,39 @@ __device__ __forceinline__ void store_row(uint16_t* op, const float (&acc)[E], f
     }
 }
 
+// LDS bytes of a wave: its tiles, later its share of O
+template <int D>
+struct Few {
+    static constexpr int TILES = (D == 128 ? 2 : 4) * SK * D * 2, O = SR * (D + 4) * 4;
+    static constexpr int WB = O > TILES ? O : TILES;
+};
+
 template <class T, int D>
-__global__ __launch_bounds__(SW * 64, 1) void attn_few_kernel(AttnVarlenArgs a) {
+__device__ __forceinline__ void few_item(const AttnVarlenArgs& a, const RowTile& t, int hk, int per, uint8_t* ring) {
     using frag = typename T::frag;
     constexpr int KS = D / 16, DT = D / 32;
-    constexpr int TB = SK * D * 2;  // bytes of a K or V tile
-    constexpr int P = TB / 1024;    // DMA instructions per tile
-    constexpr int PITCH = D + 4;    // floats per row of the joined O
-    // One LDS object: with two, the compiler orders every read of this one
-    // behind all DMA in flight.
-    __shared__ __attribute__((aligned(1024))) uint8_t ring[SW * 4 * TB + SW * SR * 8];
-    float(*ml)[SR][2] = reinterpret_cast<float(*)[SR][2]>(ring + SW * 4 * TB);
-    static_assert(4 * TB >= SR * PITCH * 4, "O takes the place of a wave's ring");
+    constexpr int TB = SK * D * 2;       // bytes of a K or V tile
+    constexpr int P = TB / 1024;         // DMA instructions per tile
+    constexpr int NS = D == 128 ? 1 : 2;  // K and V slots of a wave
+    constexpr int PITCH = D + 4;         // floats per row of the joined O
+    constexpr int WB = SR * PITCH * 4 > 2 * NS * TB ? SR * PITCH * 4 : 2 * NS * TB;  // LDS bytes of a wave
+    static_assert(WB == Few<D>::WB, "LDS of the kernel");
+    float(*ml)[SR][2] = reinterpret_cast<float(*)[SR][2]>(ring + SW * WB);
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l32 = lane & 31, half = lane >> 5;
-    const int split = blockIdx.x % a.splits;
-    const int item = blockIdx.x / a.splits;
-    const int hk = item % a.hk;
-    const RowTile t = find_tile(a, item / a.hk, SR);
-    if (!t.found) return;
-
     const int rows = t.lq * a.group;  // < 2^31: the host bounds total_q * Hq
-    const int row = t.row0 + l32;
-    const bool valid = row < rows;
-    const int token = (valid ? row : rows - 1) / a.group;
-    const int head = hk * a.group + (valid ? row : rows - 1) % a.group;
+    const int row = min(t.row0 + l32, rows - 1);
+    const int token = row / a.group;
+    const int head = hk * a.group + row % a.group;
     const int kmax = visible(a, t, token);
-    const int row_last = min(t.row0 + SR, rows) - 1;
-    const int kend = visible(a, t, row_last / a.group);
+    const int kend = visible(a, t, (min(t.row0 + SR, rows) - 1) / a.group);
     const int kfull = visible(a, t, t.row0 / a.group);
-
-    const KeyRange range = split_range(a, kend, split);
-    const int tile0 = range.begin, tile1 = range.end;
-    if (split >= max(range.count, 1)) return;
+    // 32-key tiles of this range
+    const int ntile = (kend + SK - 1) / SK;
+    const int tile0 = min(t.split * per, ntile);
+    const int tile1 = t.splits > 1 ? min(tile0 + per, ntile) : ntile;
 
     frag qf[KS];
     {
@@ -376,8 +395,8 @@ __global__ __launch_bounds__(SW * 64, 1) void attn_few_kernel(AttnVarlenArgs a) 
     }
     const uint16_t* kbase = a.k + static_cast<int64_t>(t.k0) * a.k_t + hk * a.k_h;
     const uint16_t* vbase = a.v + static_cast<int64_t>(t.k0) * a.v_t + hk * a.v_h;
-    uint8_t* kring = ring + wave * 4 * TB;
-    uint8_t* vring = kring + 2 * TB;
+    uint8_t* kring = ring + wave * WB;
+    uint8_t* vring = kring + NS * TB;
 
     v16f o[DT];
 #pragma unroll
@@ -386,30 +405,30 @@ __global__ __launch_bounds__(SW * 64, 1) void attn_few_kernel(AttnVarlenArgs a) 
         for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
     float m = kNegInf, sum = 0.0f;
     int nonfinite = -1;  // first of this wave's tiles whose V was sanitized
-
     int voff[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d) voff[d] = v_lane_off<D>(d);
 
     auto key_of = [&](int i) { return (tile0 + wave + SW * i) * SK; };
-    auto issue_k = [&](int i) { dma_tile<D, SK, false>(kbase, a.k_t, key_of(i), t.lk, kring + (i & 1) * TB, 0, 1); };
-    auto issue_v = [&](int i) { dma_tile<D, SK, true>(vbase, a.v_t, key_of(i), t.lk, vring + (i & 1) * TB, 0, 1); };
+    auto issue_k = [&](int i) { dma_tile<D, SK, false>(kbase, a.k_t, key_of(i), t.lk, kring + i % NS * TB); };
+    auto issue_v = [&](int i) { dma_tile<D, SK, true>(vbase, a.v_t, key_of(i), t.lk, vring + i % NS * TB); };
     const int n = tile1 - tile0 > wave ? (tile1 - tile0 - wave + SW - 1) / SW : 0;
     if (n > 0) {
-        issue_k(0);
-        issue_v(0);
-        issue_k(1);
-        issue_v(1);
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            issue_k(i);
+            issue_v(i);
+        }
     }
     for (int i = 0; i < n; ++i) {
         const int key0 = key_of(i);
         __builtin_amdgcn_sched_barrier(0);
-        wait_vmcnt<3 * P>();  // K of tile i
+        wait_vmcnt<(2 * NS - 1) * P>();  // K of tile i
         __builtin_amdgcn_sched_barrier(0);
         v16f s;
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = 0.0f;
-        const uint8_t* kt = kring + (i & 1) * TB;
+        const uint8_t* kt = kring + i % NS * TB;
         frag kf[KS];
 #pragma unroll
         for (int c = 0; c < KS; ++c)
@@ -419,7 +438,7 @@ __global__ __launch_bounds__(SW * 64, 1) void attn_few_kernel(AttnVarlenArgs a) 
         __builtin_amdgcn_sched_barrier(0);
         wait_lgkmcnt0();  // the slot's fragments are in registers
         __builtin_amdgcn_sched_barrier(0);
-        issue_k(i + 2);
+        issue_k(i + NS);
 
         const bool hidden = key0 + SK > kfull;  // some row does not see some key
         float p[16];
@@ -453,14 +472,14 @@ __global__ __launch_bounds__(SW * 64, 1) void attn_few_kernel(AttnVarlenArgs a) 
             sum = T::add2(pk[r / 2], sum);
         }
         __builtin_amdgcn_sched_barrier(0);
-        wait_vmcnt<3 * P>();  // V of tile i
+        wait_vmcnt<(2 * NS - 1) * P>();  // V of tile i
         __builtin_amdgcn_sched_barrier(0);
-        const uint8_t* vt = vring + (i & 1) * TB;
+        const uint8_t* vt = vring + i % NS * TB;
         frag vf[2][DT];
         read_v<T, D, 0>(vt, voff, vf[0]);
         read_v<T, D, 1>(vt, voff, vf[1]);
         __builtin_amdgcn_sched_barrier(0);
-        issue_v(i + 2);
+        issue_v(i + NS);
         if (hidden) {
             bool bad = false;
 #pragma unroll
@@ -484,14 +503,13 @@ __global__ __launch_bounds__(SW * 64, 1) void attn_few_kernel(AttnVarlenArgs a) 
         }
     }
     wait_vmcnt<0>();  // the loads past the last tile no longer write the ring
-
     if (nonfinite >= 0)
         for (int i = nonfinite; i < n; ++i)
             add_nonfinite<T, DT>(vbase, a.v_t, key_of(i), min(key_of(i) + SK, kmax), o);
 
-    // the waves' shares: O into the wave's own ring, m and sum beside it
+    // the waves' shares: O into the wave's own LDS, m and sum behind all of it
     sum = half_sum(sum);
-    float* osh = reinterpret_cast<float*>(ring + wave * 4 * TB);
+    float* osh = reinterpret_cast<float*>(ring + wave * WB);
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -507,68 +525,83 @@ __global__ __launch_bounds__(SW * 64, 1) void attn_few_kernel(AttnVarlenArgs a) 
     // thread: row tid / 8, channels (tid % 8) * D / 8 ..
     const int jr = threadIdx.x >> 3;
     const int jrow = t.row0 + jr;
-    if (jrow >= rows) return;
-    constexpr int E = D / 8;
-    const int c0 = (threadIdx.x & 7) * E;
-    float mm = ml[0][jr][0];
+    if (jrow < rows) {
+        constexpr int E = D / 8;
+        const int c0 = (threadIdx.x & 7) * E;
+        float mm = ml[0][jr][0];
 #pragma unroll
-    for (int w = 1; w < SW; ++w) mm = fmaxf(mm, ml[w][jr][0]);
-    float tot = 0.0f, acc[E];
+        for (int w = 1; w < SW; ++w) mm = fmaxf(mm, ml[w][jr][0]);
+        float tot = 0.0f, acc[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+        for (int e = 0; e < E; ++e) acc[e] = 0.0f;
 #pragma unroll
-    for (int w = 0; w < SW; ++w) {
-        const float mw = ml[w][jr][0];
-        if (mw == kNegInf) {  // no finite score: a NaN sum still counts
-            tot += ml[w][jr][1];
-            continue;
+        for (int w = 0; w < SW; ++w) {
+            // no finite score: O is zero there, the sum zero or NaN
+            const float mw = ml[w][jr][0];
+            const float f = mw == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(mw - mm);
+            tot += f * ml[w][jr][1];
+            const float* src = reinterpret_cast<const float*>(ring + w * WB) + jr * PITCH + c0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] += f * src[e];
         }
-        const float f = __builtin_amdgcn_exp2f(mw - mm);
-        tot += f * ml[w][jr][1];
-        const float* src = reinterpret_cast<const float*>(ring + w * 4 * TB) + jr * PITCH + c0;
+        const int64_t jtoken = static_cast<int64_t>(t.q0) + jrow / a.group;
+        const int jhead = hk * a.group + jrow % a.group;
+        if (t.splits > 1) {
+            const int64_t at = (jtoken * a.hq + jhead) * a.splits + t.split;
+            float* po = a.part_o + at * D + c0;
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += f * src[e];
-    }
-    const int jtoken = jrow / a.group, jhead = hk * a.group + jrow % a.group;
-    if (a.splits > 1) {
-        const int64_t at = ((static_cast<int64_t>(t.q0) + jtoken) * a.hq + jhead) * a.splits + split;
-        float* po = a.part_o + at * D + c0;
-#pragma unroll
-        for (int e = 0; e < E; e += 4)
-            *reinterpret_cast<v4f*>(po + e) = (v4f){acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
-        if (c0 == 0) {
-            a.part_ml[2 * at] = mm;
-            a.part_ml[2 * at + 1] = tot;
+            for (int e = 0; e < E; e += 4)
+                *reinterpret_cast<v4f*>(po + e) = (v4f){acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
+            if (c0 == 0) {
+                a.part_ml[2 * at] = mm;
+                a.part_ml[2 * at + 1] = tot;
+            }
+        } else {
+            store_row<T, E>(a.out + jtoken * a.o_t + jhead * a.o_h + c0, acc, tot,
+                            visible(a, t, jrow / a.group) == 0);
         }
-        return;
     }
-    store_row<T, E>(a.out + (static_cast<int64_t>(t.q0) + jtoken) * a.o_t + jhead * a.o_h + c0, acc, tot,
-                    visible(a, t, jtoken) == 0);
+    __syncthreads();  // the next item's tiles take the place of O
+}
+
+template <class T, int D>
+__global__ __launch_bounds__(SW * 64, 2) void attn_few_kernel(AttnVarlenArgs a) {
+    // One LDS object: with two, the compiler orders every read of the tiles
+    // behind all DMA in flight.
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[SW * Few<D>::WB + SW * SR * 8];
+    const int per = range_tiles(a);
+    for (int item = blockIdx.x;; item += gridDim.x) {
+        const RowTile t = find_tile(a, item / a.hk, SR, per);
+        if (!t.found) return;
+        few_item<T, D>(a, t, item % a.hk, per, ring);
+    }
 }
 
 // The key ranges' partial results of a tile of 32 rows, added in range order:
-// thread: row tid / 8, channels (tid % 8) * D / 8 ..
+// thread: row tid / 8, channels (tid % 8) * D / 8 .. Sequences of one range
+// are complete already.
 template <class T, int D>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnVarlenArgs a) {
     constexpr int E = D / 8;
+    const int per = range_tiles(a);
     const int hk = blockIdx.x % a.hk;
-    const RowTile t = find_tile(a, blockIdx.x / a.hk, SR);
+    const RowTile t = find_tile(a, blockIdx.x / a.hk, SR, 0);
     if (!t.found) return;
+    const int splits = key_ranges(t.lk, per);
     const int row = t.row0 + (threadIdx.x >> 3);
-    if (row >= t.lq * a.group) return;
+    if (splits == 1 || row >= t.lq * a.group) return;
     const int c0 = (threadIdx.x & 7) * E;
     const int64_t token = static_cast<int64_t>(t.q0) + row / a.group;
     const int head = hk * a.group + row % a.group;
     const int64_t at = (token * a.hq + head) * a.splits;
-    const int kend = visible(a, t, (min(t.row0 + SR, t.lq * a.group) - 1) / a.group);
-    const int used = split_range(a, kend, 0).count;
     float mm = kNegInf, tot = 0.0f, acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-    for (int s = 0; s < used; ++s) mm = fmaxf(mm, a.part_ml[2 * (at + s)]);
-    for (int s = 0; s < used; ++s) {
+    for (int s = 0; s < splits; ++s) mm = fmaxf(mm, a.part_ml[2 * (at + s)]);
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
         const float ms = a.part_ml[2 * (at + s)], ts = a.part_ml[2 * (at + s) + 1];
-        const float f = ms == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(ms - mm);  // -inf: O is zero there
+        const float f = ms == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(ms - mm);
         tot += f * ts;
         const float* po = a.part_o + (at + s) * D + c0;
 #pragma unroll
@@ -581,24 +614,223 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnVarlenArgs a) {
     store_row<T, E>(a.out + token * a.o_t + head * a.o_h + c0, acc, tot, visible(a, t, row / a.group) == 0);
 }
 
-// ---- many rows: 256 of them, eight waves over one ring -----------------------
-// Wave w owns rows 32 w .. of the tile; 64-key tiles of K and V stream through
-// LDS rings (4 K slots, 5 V slots, three tiles ahead) and serve all eight
-// waves, so a tile's bytes are read once for 256 rows. A step is a softmax
-// phase (VALU, then the next tile's scores) and a PV phase (MFMA); waves 0-3
-// run softmax(kt), PV(kt), waves 4-7 PV(kt - 1), softmax(kt), so that a SIMD's
-// two waves use different units. One barrier a step. A wave skips tiles that
-// none of its rows sees.
-constexpr int MR = 256, MK = 64, MW = 8, MKS = 4, MVS = 5, MAHEAD = 3;
+// ---- many rows: 128 of them, four waves over one ring -----------------------
+// Wave w owns rows 32 w .. of the tile; 64-key tiles stream through an LDS ring
+// of two slots and serve all four waves, so a tile's bytes are read once for 128
+// rows. A slot holds what one matrix phase reads: V of tile p - 1 and K of tile
+// p ("pair" p). Work alternates between a vector phase, V(p): the softmax of
+// tile p, and a matrix phase, M(p): O += V P of tile p - 1, then the scores of
+// tile p. Two workgroups share a CU (64 KB of LDS, two waves a SIMD), so one's
+// exponentials run beside the other's MFMAs. V begins with the fragment reads of
+// the next M's first MFMAs, M reads two groups of four fragments ahead (three
+// buffers), so no MFMA waits for its LDS reads' full latency.
+constexpr int MR = 128, MW = 4, MK = 64, MSLOT = 2;
+
+// The K or V tiles of one head in turn: `p` the next tile's first row, `left`
+// the bytes from there to the end of the sequence's last row (not positive
+// behind it). Each tile's descriptor starts at its own row, so offsets stay
+// below a tile's bytes however long the sequence is, and ends with the
+// sequence: rows behind it arrive as zeros.
+template <int D, bool VTILE>
+struct TileStream {
+    const uint8_t* p;
+    int64_t left, step;
+    uint32_t off[MK * D * 2 / 1024 / MW];  // a lane's byte offsets in a tile, one per DMA instruction
+    __device__ __forceinline__ void init(const uint16_t* base, int64_t stride, int lk, int wave) {
+        p = reinterpret_cast<const uint8_t*>(base);
+        step = 2 * MK * stride;
+        left = 2 * ((lk - 1) * stride + D);
+        if (lk == 0) left = 0;
+        constexpr int RPI = 512 / D, CPR = D / 8;
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < MK / RPI / MW; ++i) {
+            const int row = (wave + MW * i) * RPI + lane / CPR;
+            const int c = VTILE ? swz_v<D>(row, lane % CPR) : swz_k<D>(row, lane % CPR);
+            off[i] = static_cast<uint32_t>(row) * static_cast<uint32_t>(stride) * 2u + c * 16;
+        }
+    }
+    __device__ __forceinline__ void issue(uint8_t* dst, int wave) {
+#if defined(__HIP_DEVICE_COMPILE__)  // (the host pass rejects the builtin, and with it the kernels that share this)
+        const int64_t n = left < 0 ? 0 : left > 0x7fffffff ? 0x7fffffff : left;
+        const __amdgpu_buffer_rsrc_t r =
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, static_cast<int>(n), kRsrcWord3);
+#pragma unroll
+        for (int i = 0; i < MK * D * 2 / 1024 / MW; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                r, (__attribute__((address_space(3))) void*)(dst + (wave + MW * i) * 1024), 16, off[i], 0, 0, 0);
+        p += step;
+        left -= step;
+#endif
+    }
+};
 
 template <class T, int D>
-__global__ __launch_bounds__(MW * 64) void attn_many_kernel(AttnVarlenArgs a, int tiles) {
+struct Many {
     using frag = typename T::frag;
-    constexpr int KS = D / 16, DT = D / 32;
-    constexpr int TB = MK * D * 2;
-    constexpr int PER = 2 * TB / 1024 / MW;  // DMA instructions per wave and tile (K and V)
-    __shared__ __attribute__((aligned(1024))) uint8_t ring[(MKS + MVS) * TB];
-    uint8_t* const vring = ring + MKS * TB;
+    static constexpr int KB = MK / 32;
+    static constexpr int KS = D / 16, DT = D / 32;
+    static constexpr int TB = MK * D * 2;           // bytes of a K or V tile
+    static constexpr int PER = 2 * TB / 1024 / MW;  // DMA instructions per wave and pair
+    static constexpr int NPV = 2 * KB * DT / 4, NG = NPV + KB * KS / 4;  // groups of four MFMAs: PV, all
+    v16f o[DT], s[KB];
+    frag qf[KS], buf[3][4];
+    uint32_t pk[8 * KB];  // P: 16-key group g at pk[4 g ..]
+    int voff[DT], koff[KS];  // lane offsets of V reads (channel block), K reads (k-step)
+    float m, sum;
+
+    // fragments of group j: PV units (16-key group u / DT, channel block
+    // u % DT), then score units (k-step u / KB, key block u % KB)
+    template <int j>
+    __device__ __forceinline__ void read_group(const uint8_t* src, frag (&f)[4]) {
+        using as3 = __attribute__((address_space(3))) v4s*;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (j < NPV) {
+                const int u = 4 * j + i;
+                const uint8_t* p = src + voff[u % DT] + 16 * (u / DT) * (2 * D);
+                const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((as3)(p));
+                const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((as3)(p + 8 * (2 * D)));
+                f[i] = __builtin_bit_cast(frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            } else {
+                const int u = 4 * (j - NPV) + i;
+                f[i] = *reinterpret_cast<const frag*>(src + TB + koff[u / KB] + 32 * (u % KB) * (2 * D));
+            }
+        }
+    }
+    __device__ __forceinline__ frag p_frag(int g) const {
+        return __builtin_bit_cast(frag, (v4i){static_cast<int>(pk[4 * g]), static_cast<int>(pk[4 * g + 1]),
+                                              static_cast<int>(pk[4 * g + 2]), static_cast<int>(pk[4 * g + 3])});
+    }
+    template <int j>
+    __device__ __forceinline__ void mma_group(const frag (&f)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (j < NPV) {
+                const int u = 4 * j + i;
+                o[u % DT] = T::mma(f[i], p_frag(u / DT), o[u % DT]);
+            } else {
+                const int u = 4 * (j - NPV) + i;
+                s[u % KB] = T::mma(f[i], qf[u / KB], s[u % KB]);
+            }
+        }
+    }
+    template <int j, bool MASKED>
+    __device__ __forceinline__ void m_groups(const uint8_t* src, bool& bad) {
+        if constexpr (j < NG) {
+            if constexpr (j + 2 < NG) read_group<j + 2>(src, buf[(j + 2) % 3]);
+            if constexpr (MASKED && j < NPV) {
+                bool b = false;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) b |= has_nonfinite<T>(buf[j % 3][i]);
+                if (__ballot(b)) {
+                    bad = true;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) buf[j % 3][i] = sanitize<T>(buf[j % 3][i]);
+                }
+            }
+            if constexpr (j == NPV) {
+#pragma unroll
+                for (int r = 0; r < 16 * KB; ++r) s[r >> 4][r & 15] = 0.0f;
+            }
+            mma_group<j>(buf[j % 3]);
+            __builtin_amdgcn_sched_barrier(0);
+            m_groups<j + 1, MASKED>(src, bad);
+        }
+    }
+    template <int j>
+    __device__ __forceinline__ void first_scores(const uint8_t* src) {
+        if constexpr (j < NG) {
+            read_group<j>(src, buf[j % 3]);
+            mma_group<j>(buf[j % 3]);
+            first_scores<j + 1>(src);
+        }
+    }
+
+    template <bool MASKED>
+    __device__ __forceinline__ void softmax(int key0, int kmax, float c) {
+        const int half = (threadIdx.x & 63) >> 5;
+        if constexpr (MASKED) {
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (key0 + 32 * b + 8 * (r >> 2) + 4 * half + (r & 3) >= kmax) s[b][r] = kNegInf;
+        }
+        float mt = s[0][0];
+#pragma unroll
+        for (int r = 1; r < 16 * KB; ++r) mt = fmaxf(mt, s[r >> 4][r & 15]);
+        mt = half_max(mt) * c;
+        const bool bump = mt > m + kSlack;
+        const float m_new = bump ? mt : m;
+        if (__ballot(bump)) {
+            const float f = bump ? __builtin_amdgcn_exp2f(m - m_new) : 1.0f;
+            sum *= f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][r] *= f;
+        }
+        m = m_new;
+        const float neg = (m == kNegInf ? 0.0f : -m) + T::kPBias;
+#pragma unroll
+        for (int r = 0; r < 16 * KB; r += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r >> 4][r & 15], c, neg));
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r >> 4][(r & 15) + 1], c, neg));
+            pk[r / 2] = T::pack(p0, p1);
+            sum = T::add2(pk[r / 2], sum);
+        }
+    }
+};
+
+// V(p) and M(p + 1) of one wave. Pair p + 1 has landed once every wave has
+// waited for its share (all but the newest pair's, p + 2) and met the barrier; behind the
+// second barrier all waves are done with it and pair p + 3 goes into its slot.
+// The slot comes as two restrict pointers, which tells the compiler that the
+// reads of `src` do not depend on the DMA into `dst`: the waits and barriers
+// see to that.
+__device__ __forceinline__ void phase_barrier() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");  // no LDS read or DMA moves across, whatever the compiler thinks of aliasing
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+template <class T, int D, bool MASKED>
+__device__ __forceinline__ void many_step(Many<T, D>& w, const uint8_t* __restrict src, uint8_t* __restrict dst,
+                                          TileStream<D, false>& ks, TileStream<D, true>& vs, float scale, int p,
+                                          int wave, int kmax, int& nonfinite) {
+    using W = Many<T, D>;
+    wait_vmcnt<W::PER>();
+    phase_barrier();
+    w.template read_group<0>(src, w.buf[0]);
+    w.template read_group<1>(src, w.buf[1]);
+    __builtin_amdgcn_sched_barrier(0);
+    w.template softmax<MASKED>(p * MK, kmax, scale);
+    // P is made in this phase: left to itself the compiler moves the
+    // exponentials next to the MFMAs that read them
+#pragma unroll
+    for (int i = 0; i < 8 * W::KB; ++i) asm volatile("" : "+v"(w.pk[i]));
+    asm volatile("" : "+v"(w.sum));
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
+    bool bad = false;
+    w.template m_groups<0, MASKED>(src, bad);
+    if (MASKED && bad && nonfinite < 0) nonfinite = p;
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(0);
+    phase_barrier();
+    vs.issue(dst, wave);
+    ks.issue(dst + W::TB, wave);
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+template <class T, int D>
+__global__ __launch_bounds__(MW * 64, 2) void attn_many_kernel(AttnVarlenArgs a, int tiles) {
+    using W = Many<T, D>;
+    constexpr int PAIR = 2 * W::TB;
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[MSLOT * PAIR];
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -615,7 +847,7 @@ __global__ __launch_bounds__(MW * 64) void attn_many_kernel(AttnVarlenArgs a, in
         hk = logical / tiles;
         idx = logical % tiles;
     }
-    const RowTile t = find_tile(a, idx, MR);
+    const RowTile t = find_tile(a, idx, MR, 0);
     if (!t.found) return;
 
     const int rows = t.lq * a.group;
@@ -625,162 +857,75 @@ __global__ __launch_bounds__(MW * 64) void attn_many_kernel(AttnVarlenArgs a, in
     const int head = hk * a.group + row % a.group;
     const int kmax = visible(a, t, token);
     const int kend = visible(a, t, (min(t.row0 + MR, rows) - 1) / a.group);  // of the whole tile
-    const int nkt = (kend + MK - 1) / MK;
-    // of this wave's rows: keys that all of them see, and that any of them sees
-    const int wrow0 = t.row0 + 32 * wave;
-    const int wfull = wrow0 < rows ? visible(a, t, wrow0 / a.group) : 0;
-    const int wend = wrow0 < rows ? visible(a, t, (min(wrow0 + 32, rows) - 1) / a.group) : 0;
+    const int n = (kend + MK - 1) / MK;
+    const int nfull = visible(a, t, t.row0 / a.group) / MK;  // tiles that every row sees whole
 
-    frag qf[KS];
+    W w;
     {
         const uint16_t* qp = a.q + (static_cast<int64_t>(t.q0) + token) * a.q_t + head * a.q_h + 8 * half;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const frag*>(qp + 16 * s);
+        for (int i = 0; i < W::KS; ++i) w.qf[i] = *reinterpret_cast<const typename T::frag*>(qp + 16 * i);
     }
     const uint16_t* kbase = a.k + static_cast<int64_t>(t.k0) * a.k_t + hk * a.k_h;
     const uint16_t* vbase = a.v + static_cast<int64_t>(t.k0) * a.v_t + hk * a.v_h;
-    auto issue = [&](int kt) {
-        dma_tile<D, MK, false>(kbase, a.k_t, kt * MK, t.lk, ring + kt % MKS * TB, wave, MW);
-        dma_tile<D, MK, true>(vbase, a.v_t, kt * MK, t.lk, vring + kt % MVS * TB, wave, MW);
-    };
-
-    v16f o[DT];
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
+    for (int d = 0; d < W::DT; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
-    float m = kNegInf, sum = 0.0f;
+        for (int r = 0; r < 16; ++r) w.o[d][r] = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 16 * W::KB; ++r) w.s[r >> 4][r & 15] = 0.0f;
+    w.m = kNegInf;
+    w.sum = 0.0f;
+#pragma unroll
+    for (int d = 0; d < W::DT; ++d) w.voff[d] = v_lane_off<D>(d);
+#pragma unroll
+    for (int c = 0; c < W::KS; ++c) w.koff[c] = l32 * (2 * D) + swz_k<D>(l32, 2 * c + half) * 16;
     int nonfinite = -1;  // first of this wave's tiles whose V was sanitized
-    int voff[DT];
-#pragma unroll
-    for (int d = 0; d < DT; ++d) voff[d] = v_lane_off<D>(d);
 
-#pragma unroll
-    for (int i = 0; i < MAHEAD; ++i) issue(i);
-    wait_vmcnt<PER>();  // tiles 0 and 1
-    __builtin_amdgcn_s_barrier();
-
-    v16f s[2];
-    auto scores = [&](int kt) {
-        const uint8_t* kl = ring + kt % MKS * TB;
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const int kr = 32 * b + l32;
-            frag kf[KS];
-#pragma unroll
-            for (int c = 0; c < KS; ++c)
-                kf[c] = *reinterpret_cast<const frag*>(kl + kr * (2 * D) + swz_k<D>(kr, 2 * c + half) * 16);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[b][r] = 0.0f;
-#pragma unroll
-            for (int c = 0; c < KS; ++c) s[b] = T::mma(kf[c], qf[c], s[b]);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    };
-    uint32_t pk[16];  // P of the current tile: 16-key group g at pk[4 g ..]
-    auto softmax = [&](int kt) {
-        if (kt * MK + MK > wfull) {
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (kt * MK + 32 * b + 8 * (r >> 2) + 4 * half + (r & 3) >= kmax) s[b][r] = kNegInf;
-        }
-        float mt = s[0][0];
-#pragma unroll
-        for (int r = 1; r < 32; ++r) mt = fmaxf(mt, s[r >> 4][r & 15]);
-        mt = half_max(mt) * a.scale_log2;
-        const bool bump = mt > m + kSlack;
-        const float m_new = bump ? mt : m;
-        if (__ballot(bump)) {
-            const float f = bump ? __builtin_amdgcn_exp2f(m - m_new) : 1.0f;
-            sum *= f;
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[d][r] *= f;
-        }
-        m = m_new;
-        const float neg = (m == kNegInf ? 0.0f : -m) + T::kPBias;
-#pragma unroll
-        for (int r = 0; r < 32; r += 2) {
-            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r >> 4][r & 15], a.scale_log2, neg));
-            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r >> 4][(r & 15) + 1], a.scale_log2, neg));
-            pk[r / 2] = T::pack(p0, p1);
-            sum = T::add2(pk[r / 2], sum);
-        }
-    };
-    auto pv = [&](int kt) {
-        const uint8_t* vt = vring + kt % MVS * TB;
-        const bool hidden = kt * MK + MK > wfull;
-        auto group = [&](auto gc) {
-            constexpr int g = decltype(gc)::value;
-            frag vf[DT];
-            read_v<T, D, g>(vt, voff, vf);
-            if (hidden) {
-                bool bad = false;
-#pragma unroll
-                for (int d = 0; d < DT; ++d) bad |= has_nonfinite<T>(vf[d]);
-                if (__ballot(bad)) {
-                    if (nonfinite < 0) nonfinite = kt;
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) vf[d] = sanitize<T>(vf[d]);
-                }
-            }
-            const frag pf = __builtin_bit_cast(frag, (v4i){static_cast<int>(pk[4 * g]), static_cast<int>(pk[4 * g + 1]),
-                                                           static_cast<int>(pk[4 * g + 2]), static_cast<int>(pk[4 * g + 3])});
-#pragma unroll
-            for (int d = 0; d < DT; ++d) o[d] = T::mma(vf[d], pf, o[d]);
-        };
-        group(std::integral_constant<int, 0>{});
-        group(std::integral_constant<int, 1>{});
-        group(std::integral_constant<int, 2>{});
-        group(std::integral_constant<int, 3>{});
-    };
-    scores(0);
-    const bool lag = wave >= MW / 2;
-    const int wtiles = (wend + MK - 1) / MK;  // tiles that this wave works on
-    for (int kt = 0; kt < nkt; ++kt) {
-        issue(kt + MAHEAD);
-        __builtin_amdgcn_sched_barrier(0);
-        if (lag && kt > 0 && kt <= wtiles) pv(kt - 1);
-        if (kt < wtiles) {
-            softmax(kt);
-            __builtin_amdgcn_sched_barrier(0);
-            scores(kt + 1);
-        }
-        if (!lag && kt < wtiles) pv(kt);
-        // this wave's reads are done and its share of tile kt + 2 has landed
-        __builtin_amdgcn_sched_barrier(0);
-        wait_vmcnt<PER>();
-        wait_lgkmcnt0();
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
-    }
-    if (lag && wtiles == nkt && nkt > 0) pv(nkt - 1);
+    TileStream<D, false> ks;
+    TileStream<D, true> vs;
+    ks.init(kbase, a.k_t, t.lk, wave);
+    vs.init(vbase, a.v_t, t.lk, wave);
+    // pairs 0 (no V) and 1, then the scores of tile 0 and pair 2 in its place
+    ks.issue(ring + W::TB, wave);
+    vs.issue(ring + PAIR, wave);
+    ks.issue(ring + PAIR + W::TB, wave);
+    wait_vmcnt<W::PER>();
+    phase_barrier();
+    w.template first_scores<W::NPV>(ring);
+    phase_barrier();
+    vs.issue(ring, wave);
+    ks.issue(ring + W::TB, wave);
+    int p = 0;
+    for (; p < nfull; ++p)
+        many_step<T, D, false>(w, ring + ((p + 1) % MSLOT) * PAIR, ring + ((p + 1) % MSLOT) * PAIR, ks, vs, a.scale_log2, p,
+                               wave, kmax, nonfinite);
+    for (; p < n; ++p)
+        many_step<T, D, true>(w, ring + ((p + 1) % MSLOT) * PAIR, ring + ((p + 1) % MSLOT) * PAIR, ks, vs, a.scale_log2, p,
+                               wave, kmax, nonfinite);
     wait_vmcnt<0>();  // the loads past the last tile no longer write the ring
-    if (nonfinite >= 0) add_nonfinite<T, DT>(vbase, a.v_t, nonfinite * MK, kmax, o);
+    if (nonfinite >= 0) add_nonfinite<T, W::DT>(vbase, a.v_t, nonfinite * MK, kmax, w.o);
 
     if (!valid) return;
-    const float tot = half_sum(sum);
+    const float tot = half_sum(w.sum);
     const float inv = 1.0f / tot;
     // channels 8 (g + half) .. of block d after the lane halves have exchanged
     // their four of g and g + 1
     uint16_t* op = a.out + (static_cast<int64_t>(t.q0) + token) * a.o_t + head * a.o_h + 8 * half;
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
+    for (int d = 0; d < W::DT; ++d)
 #pragma unroll
         for (int g = 0; g < 4; g += 2) {
-            uint32_t w[4];
+            uint32_t v[4];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const uint32_t x = T::pack(o[d][4 * g + 2 * i] * inv, o[d][4 * g + 2 * i + 1] * inv);
-                const uint32_t y = T::pack(o[d][4 * g + 4 + 2 * i] * inv, o[d][4 * g + 4 + 2 * i + 1] * inv);
+                const uint32_t x = T::pack(w.o[d][4 * g + 2 * i] * inv, w.o[d][4 * g + 2 * i + 1] * inv);
+                const uint32_t y = T::pack(w.o[d][4 * g + 4 + 2 * i] * inv, w.o[d][4 * g + 4 + 2 * i + 1] * inv);
                 const auto sw = __builtin_amdgcn_permlane32_swap(x, y, false, false);
-                w[i] = kmax == 0 ? 0u : sw[0];
-                w[2 + i] = kmax == 0 ? 0u : sw[1];
+                v[i] = kmax == 0 ? 0u : sw[0];
+                v[2 + i] = kmax == 0 ? 0u : sw[1];
             }
-            *reinterpret_cast<u32x4*>(op + 32 * d + 8 * g) = (u32x4){w[0], w[1], w[2], w[3]};
+            *reinterpret_cast<u32x4*>(op + 32 * d + 8 * g) = (u32x4){v[0], v[1], v[2], v[3]};
         }
 }
 
@@ -792,36 +937,32 @@ int64_t tile_bound(int total_q, int batch, int group, int rows) {
 
 }  // namespace
 
+constexpr int kManyTiles = 200;
+constexpr int kFewGrid = 512;  // workgroups of the few-row kernel, two a CU
+
+// Tiles of 128 rows, or of 32.
 static bool attn_varlen_many(int total_q, int batch, int hq, int hk) {
-    return tile_bound(total_q, batch, hq / hk, MR) * hk >= 96;
+    return tile_bound(total_q, batch, hq / hk, MR) * hk >= kManyTiles;
 }
 
-// Key ranges of the few-row kernel: where its tiles leave CUs idle, a
-// sequence's keys are cut into ranges of *split_tiles 32-key tiles (about two
-// workgroups a CU over the whole launch, four tiles a wave at least), at most 32 of them.
-int attn_varlen_splits(int total_q, int total_k, int batch, int hq, int hk, int* split_tiles) {
-    *split_tiles = 1;
-    if (total_q <= 0 || batch <= 0 || total_k <= 0) return 1;
-    const int64_t wgs = tile_bound(total_q, batch, hq / hk, SR) * hk;
-    if (wgs > 128 || attn_varlen_many(total_q, batch, hq, hk)) return 1;
-    const int64_t seqs = batch < total_q ? batch : total_q;
-    const int64_t key_tiles = wgs * ((total_k + seqs - 1) / seqs) / SK;  // of an average sequence
-    int64_t per = (key_tiles + 511) / 512;
-    per = per < 4 * SW ? 4 * SW : per;
-    const int64_t most = (total_k + SK - 1) / SK;
-    *split_tiles = static_cast<int>(per);
-    int64_t s = (most + per - 1) / per;
-    return static_cast<int>(s < 1 ? 1 : s > 32 ? 32 : s);
+// Most key ranges a sequence may be cut into: where the tiles of 32 rows alone
+// do not fill two workgroups a CU. The ranges' length is found on the device.
+int attn_varlen_splits(int total_q, int total_k, int batch, int hq, int hk) {
+    if (total_q <= 0 || batch <= 0 || total_k <= 4 * SW * SK || attn_varlen_many(total_q, batch, hq, hk)) return 1;
+    if (tile_bound(total_q, batch, hq / hk, SR) * hk > kFewGrid / 2) return 1;
+    const int64_t most = (total_k + 4 * SW * SK - 1) / (4 * SW * SK);
+    return static_cast<int>(most > 32 ? 32 : most);
 }
 
 template <class T, int D>
 static hipError_t launch_few(const AttnVarlenArgs& a, hipStream_t stream) {
-    const int64_t tiles = tile_bound(a.total_q, a.batch, a.group, SR);
-    hipLaunchKernelGGL((attn_few_kernel<T, D>), dim3(static_cast<unsigned>(tiles * a.hk * a.splits)), dim3(SW * 64), 0,
-                       stream, a);
+    const int64_t tiles = tile_bound(a.total_q, a.batch, a.group, SR) * a.hk;
+    const int64_t items = tiles * a.splits;
+    hipLaunchKernelGGL((attn_few_kernel<T, D>), dim3(static_cast<unsigned>(items < kFewGrid ? items : kFewGrid)),
+                       dim3(SW * 64), 0, stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.splits == 1) return e;
-    hipLaunchKernelGGL((attn_join_kernel<T, D>), dim3(static_cast<unsigned>(tiles * a.hk)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((attn_join_kernel<T, D>), dim3(static_cast<unsigned>(tiles)), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 

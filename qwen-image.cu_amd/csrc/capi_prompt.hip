@@ -28,8 +28,7 @@ int64_t qimg_attention_varlen_scratch_bytes(int total_q, int total_k, int batch,
     if (total_q <= 0 || total_k <= 0 || batch <= 0 || n_heads <= 0 || n_kv_heads <= 0 || head_dim <= 0 ||
         n_heads % n_kv_heads != 0)
         return 0;
-    int tiles = 0;
-    const int splits = qimg::attn_varlen_splits(total_q, total_k, batch, n_heads, n_kv_heads, &tiles);
+    const int splits = qimg::attn_varlen_splits(total_q, total_k, batch, n_heads, n_kv_heads);
     if (splits == 1) return 0;
     const int64_t parts = static_cast<int64_t>(total_q) * n_heads * splits;
     return align256(parts * head_dim * 4) + align256(parts * 8);
@@ -58,6 +57,8 @@ int qimg_attention_varlen(const qimg_attn_varlen* args, void* scratch, int64_t s
     QIMG_REQUIRE(aligned16(p.q) && aligned16(p.k) && aligned16(p.v) && aligned16(p.out),
                  "%s: q, k, v and out must be 16-byte aligned", fn);
     QIMG_REQUIRE(p.out != p.q && p.out != p.k && p.out != p.v, "%s: out must not be q, k or v", fn);
+    QIMG_REQUIRE(p.total_k <= 1 || (p.k_stride_t >= p.head_dim && p.v_stride_t >= p.head_dim),
+                 "%s: k and v token strides must be at least head_dim", fn);
     QIMG_REQUIRE((p.total_q == 1 || p.out_stride_t >= p.head_dim) && (p.n_heads == 1 || p.out_stride_h >= p.head_dim),
                  "%s: out strides must be at least head_dim", fn);
     qimg::AttnVarlenArgs a{};
@@ -72,7 +73,8 @@ int qimg_attention_varlen(const qimg_attn_varlen* args, void* scratch, int64_t s
     a.hq = p.n_heads, a.hk = p.n_kv_heads, a.group = p.n_heads / p.n_kv_heads;
     a.causal = p.causal != 0;
     a.scale_log2 = p.sm_scale * 1.4426950408889634f;
-    a.splits = qimg::attn_varlen_splits(p.total_q, p.total_k, p.batch, p.n_heads, p.n_kv_heads, &a.split_tiles);
+    a.splits = qimg::attn_varlen_splits(p.total_q, p.total_k, p.batch, p.n_heads, p.n_kv_heads);
+    a.target_items = 512;
     if (a.splits > 1) {
         const int64_t need = qimg_attention_varlen_scratch_bytes(p.total_q, p.total_k, p.batch, p.n_heads,
                                                                  p.n_kv_heads, p.head_dim);

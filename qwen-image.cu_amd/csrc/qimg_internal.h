@@ -337,11 +337,12 @@ struct AttnVarlenArgs {
     int batch, total_q, total_k, hq, hk, group;
     int causal;
     float scale_log2;  // sm_scale * log2(e)
-    int splits, split_tiles;  // key ranges of the few-row kernel, 32-key tiles a range
+    int splits;        // most key ranges of a sequence (the few-row kernel)
+    int target_items;  // items that the ranges' length aims at
     float* part_o;   // [total_q, hq, splits, D] with splits > 1
     float* part_ml;  // [total_q, hq, splits, 2]: running maximum, sum
 };
-int attn_varlen_splits(int total_q, int total_k, int batch, int hq, int hk, int* split_tiles);
+int attn_varlen_splits(int total_q, int total_k, int batch, int hq, int hk);
 hipError_t launch_attention_varlen(const AttnVarlenArgs& a, int dtype, int D, hipStream_t stream);
 
 }  // namespace qimg
