@@ -270,6 +270,45 @@ int64_t qimg_attention_varlen_scratch_bytes(int total_q, int total_k, int batch,
                                             int head_dim);
 int qimg_attention_varlen(const qimg_attn_varlen* args, void* scratch, int64_t scratch_bytes, void* stream);
 
+/* ---- prompts: bf16 linear with its epilogue ------------------------------ */
+
+enum { QIMG_ACT_NONE = 0, QIMG_ACT_GELU_TANH = 1, QIMG_ACT_SILU = 2 };
+
+/* linear_forward_bf16 (cuda_kernels.cu:4534-4596) with the operations that
+ * follow it on the accumulators:
+ *   z = bf16(x) w^T + bias
+ *   y = act(z), with w_up: act(z) * (bf16(x) w_up^T + bias_up)
+ *   out = residual + gate[n] * y
+ * x [M,K] QIMG_FP32 (rounded to bf16, nearest even) or QIMG_BF16, rows of ldx
+ * elements; w and w_up bf16 [N,K]; bias and bias_up bf16 [N], gate fp32 [N],
+ * residual [M,N] QIMG_FP32 or QIMG_BF16 with rows of ld_residual: each may be
+ * NULL (bias_up only with w_up). out [M,N] QIMG_FP32 or QIMG_BF16 with rows of
+ * ldo, may be residual itself (same type and ld), else overlaps no operand.
+ * fp32 accumulation and epilogue, one rounding. bf16 rows of x must start at
+ * 16-byte boundaries (ldx a multiple of 8; fp32: of 4) unless K is no multiple of 8, where x and the
+ * weights are copied to scratch first. ld* < 2^22.
+ * scratch: qimg_linear_bf16_fused_scratch_bytes(...) bytes (may be 0: NULL). */
+typedef struct {
+    const void* x;
+    int x_dtype;
+    int64_t ldx;
+    int M, N, K;
+    const uint16_t* w;
+    const uint16_t* w_up;
+    const uint16_t* bias;
+    const uint16_t* bias_up;
+    int act;
+    const float* gate;
+    const void* residual;
+    int residual_dtype;
+    int64_t ld_residual;
+    void* out;
+    int out_dtype;
+    int64_t ldo;
+} qimg_linear_fused;
+int64_t qimg_linear_bf16_fused_scratch_bytes(int x_dtype, int M, int K, int N, int gated);
+int qimg_linear_bf16_fused(const qimg_linear_fused* args, void* scratch, int64_t scratch_bytes, void* stream);
+
 /* ---- MMDiT joint block: the operations around the hot path ------------ */
 
 /* silu_fp32 (cuda_kernels.cu:1881-1893): out[i] = x[i] / (1 + exp(-x[i])). */

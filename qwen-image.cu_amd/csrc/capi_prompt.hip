@@ -89,4 +89,60 @@ int qimg_attention_varlen(const qimg_attn_varlen* args, void* scratch, int64_t s
         qimg::launch_attention_varlen(a, p.dtype, p.head_dim, static_cast<hipStream_t>(stream)), fn);
 }
 
+int64_t qimg_linear_bf16_fused_scratch_bytes(int x_dtype, int M, int K, int N, int gated) {
+    const qimg::LinearFusedScratch s = qimg::linear_fused_scratch(x_dtype, M, K, N, gated != 0);
+    return s.x + s.w + s.w_up + s.part;
+}
+
+int qimg_linear_bf16_fused(const qimg_linear_fused* args, void* scratch, int64_t scratch_bytes, void* stream) {
+    const char* fn = "qimg_linear_bf16_fused";
+    QIMG_REQUIRE(args, "%s: args is null", fn);
+    const qimg_linear_fused& p = *args;
+    const auto float_type = [](int t) { return t == QIMG_FP32 || t == QIMG_BF16; };
+    QIMG_REQUIRE(float_type(p.x_dtype), "%s: x_dtype %d must be FP32 or BF16", fn, p.x_dtype);
+    QIMG_REQUIRE(float_type(p.out_dtype), "%s: out_dtype %d must be FP32 or BF16", fn, p.out_dtype);
+    QIMG_REQUIRE(!p.residual || float_type(p.residual_dtype), "%s: residual_dtype %d must be FP32 or BF16", fn,
+                 p.residual_dtype);
+    QIMG_REQUIRE(p.act >= QIMG_ACT_NONE && p.act <= QIMG_ACT_SILU, "%s: unknown activation %d", fn, p.act);
+    QIMG_REQUIRE(p.M >= 0 && p.N >= 0 && p.K > 0, "%s: bad sizes M=%d N=%d K=%d", fn, p.M, p.N, p.K);
+    if (p.M == 0 || p.N == 0) return QIMG_OK;
+    QIMG_REQUIRE(p.x && p.w && p.out, "%s: null pointer", fn);
+    QIMG_REQUIRE(!p.bias_up || p.w_up, "%s: bias_up without w_up", fn);
+    QIMG_REQUIRE(aligned16(p.x) && aligned16(p.w) && aligned16(p.w_up) && aligned16(p.out) && aligned16(p.residual),
+                 "%s: x, w, w_up, residual and out must be 16-byte aligned", fn);
+    const int64_t most = int64_t{1} << 22;
+    QIMG_REQUIRE(p.K < most && p.N < most && p.M < (1 << 24), "%s: sizes M=%d N=%d K=%d too large", fn, p.M, p.N, p.K);
+    QIMG_REQUIRE(static_cast<int64_t>(p.M / 64 + 1) * (p.N / 64 + 1) < (int64_t{1} << 26), "%s: M=%d N=%d too large", fn,
+                 p.M, p.N);
+    QIMG_REQUIRE(p.ldx >= p.K && p.ldx < most, "%s: ldx %lld must be at least K and below 2^22", fn,
+                 static_cast<long long>(p.ldx));
+    QIMG_REQUIRE(p.ldo >= p.N && p.ldo < most, "%s: ldo %lld must be at least N and below 2^22", fn,
+                 static_cast<long long>(p.ldo));
+    QIMG_REQUIRE(!p.residual || (p.ld_residual >= p.N && p.ld_residual < most),
+                 "%s: ld_residual %lld must be at least N and below 2^22", fn, static_cast<long long>(p.ld_residual));
+    if (p.K % 8 == 0)
+        QIMG_REQUIRE(p.ldx % (p.x_dtype == QIMG_FP32 ? 4 : 8) == 0, "%s: rows of x must be 16-byte aligned (ldx %lld)",
+                     fn, static_cast<long long>(p.ldx));
+    QIMG_REQUIRE(p.out != p.residual || (p.ldo == p.ld_residual && p.out_dtype == p.residual_dtype),
+                 "%s: out in residual's place must have its type and rows", fn);
+    QIMG_REQUIRE(p.out != p.x && p.out != static_cast<const void*>(p.w), "%s: out must not be x or w", fn);
+    const int64_t need =
+        qimg_linear_bf16_fused_scratch_bytes(p.x_dtype, p.M, p.K, p.N, p.w_up != nullptr);
+    if (need > 0) {
+        if (!scratch || scratch_bytes < need)
+            return qimg::api_fail(QIMG_ERR_SCRATCH, "%s: scratch %lld bytes < required %lld", fn,
+                                  static_cast<long long>(scratch_bytes), static_cast<long long>(need));
+        QIMG_REQUIRE(aligned16(scratch), "%s: scratch must be 16-byte aligned", fn);
+    }
+    qimg::LinearFusedArgs a{};
+    a.x = p.x, a.ldx = p.ldx, a.w = p.w, a.w_up = p.w_up;
+    a.M = p.M, a.N = p.N, a.K = p.K;
+    a.bias = p.bias, a.bias_up = p.bias_up, a.gate = p.gate;
+    a.residual = p.residual, a.ldr = p.ld_residual, a.res_dtype = p.residual_dtype;
+    a.out = p.out, a.ldo = p.ldo, a.out_dtype = p.out_dtype;
+    a.act = p.act;
+    a.vec4 = p.ldo % 4 == 0 && (!p.residual || p.ld_residual % 4 == 0);
+    return qimg::api_hip_status(qimg::launch_linear_fused(a, p.x_dtype, scratch, static_cast<hipStream_t>(stream)), fn);
+}
+
 }  // extern "C"

@@ -1,0 +1,626 @@
+// gemm_fused.hip — the bf16 linear with its epilogue:
+//   z[m,n] = sum_k bf16(x[m,k]) w[n,k] + bias[n]
+//   y[m,n] = act(z[m,n]) * (sum_k bf16(x[m,k]) w_up[n,k] + bias_up[n])   (the second factor with w_up only)
+//   out[m,n] = residual[m,n] + gate[n] * y[m,n]                          (each where given)
+// x fp32 (rounded to bf16, nearest even) or bf16, weights bf16 [N, K], fp32
+// accumulation; bias, activation, product, gate and residual in fp32 on the
+// accumulators, one rounding to out's type.
+//
+// Three kernels: linear_rows_kernel (up to 16 rows: bound by reading the
+// weights), linear_tile_kernel (the rest, also with the sum over k split over
+// workgroups where there are few tiles) and linear_join_kernel (adds the parts
+// in order and applies the epilogue). x in fp32 with more than 16 rows, and
+// operands whose rows are not whole 16-byte pieces, first go through
+// pack_rows_kernel into scratch.
+#include <algorithm>
+#include <type_traits>
+
+#include "qimg_device.h"
+#include "qimg_internal.h"
+
+namespace qimg {
+
+namespace {
+
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+
+constexpr int kRsrcWord3 = 0x00020000;  // raw unswizzled buffer (gfx9 family)
+constexpr uint32_t kOob = 0x80000000u;  // offset >= num_records: reads zero
+
+// v / (1 + 2^-t): the sigmoid form of both activations keeps the relative
+// error of small results (no 1 - 1), also far in the negative tail
+__device__ __forceinline__ float activate(float v, int act) {
+    if (act == QIMG_ACT_NONE) return v;
+    float t;  // log2(e) times the sigmoid's argument
+    if (act == QIMG_ACT_SILU)
+        t = v * 1.4426950408889634f;
+    else
+        t = v * __builtin_fmaf(0.10294324f, v * v, 2.3022082f);  // 2 sqrt(2/pi) log2(e) (v + 0.044715 v^3)
+    return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-t));
+}
+
+// The epilogue of four neighbouring outputs of row m, columns n ..; their
+// bias, bias_up and gate are loaded once per column.
+struct Columns {
+    float b[4], bu[4], g[4];
+};
+__device__ __forceinline__ Columns load_columns(const LinearFusedArgs& a, int n) {
+    Columns c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int k = min(n + i, a.N - 1);
+        c.b[i] = a.bias != nullptr ? bf16_to_f32(a.bias[k]) : 0.0f;
+        c.bu[i] = a.bias_up != nullptr ? bf16_to_f32(a.bias_up[k]) : 0.0f;
+        c.g[i] = a.gate != nullptr ? a.gate[k] : 1.0f;
+    }
+    return c;
+}
+template <bool GATED>
+__device__ __forceinline__ void finish4(const LinearFusedArgs& a, const Columns& c, int m, int n, const float (&z)[4],
+                                        const float (&u)[4]) {
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[i] = activate(z[i] + c.b[i], a.act);
+        if (GATED) v[i] *= u[i] + c.bu[i];
+        v[i] *= c.g[i];
+    }
+    const int64_t o = m * a.ldo + n, r = m * a.ldr + n;
+    const bool bf = a.out_dtype == QIMG_BF16;
+    if (a.vec4 && n + 3 < a.N) {
+        if (a.residual != nullptr) {
+            if (a.res_dtype == QIMG_BF16) {
+                const uint2 q = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.residual) + r);
+                v[0] += __uint_as_float(q.x << 16);
+                v[1] += __uint_as_float(q.x & 0xffff0000u);
+                v[2] += __uint_as_float(q.y << 16);
+                v[3] += __uint_as_float(q.y & 0xffff0000u);
+            } else {
+                const v4f q = *reinterpret_cast<const v4f*>(static_cast<const float*>(a.residual) + r);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] += q[i];
+            }
+        }
+        if (bf)
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + o) =
+                make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+        else
+            *reinterpret_cast<v4f*>(static_cast<float*>(a.out) + o) = (v4f){v[0], v[1], v[2], v[3]};
+        return;
+    }
+    for (int i = 0; i < 4 && n + i < a.N; ++i) {
+        if (a.residual != nullptr)
+            v[i] += a.res_dtype == QIMG_BF16 ? bf16_to_f32(static_cast<const uint16_t*>(a.residual)[r + i])
+                                             : static_cast<const float*>(a.residual)[r + i];
+        if (bf)
+            static_cast<uint16_t*>(a.out)[o + i] = f32_to_bf16(v[i]);
+        else
+            static_cast<float*>(a.out)[o + i] = v[i];
+    }
+}
+
+// ---- tiles -------------------------------------------------------------------
+// A workgroup of eight waves owns TM x TN products (TN weight rows; with GATED
+// 16 rows of w and 16 of w_up in turn, so a lane holds both factors of an
+// output), wave (wm, wn) of 2 x 4 its TM/2 x TN/4, as 16x16 blocks
+// (v_mfma_f32_16x16x32_bf16, w as the A operand: a lane holds four neighbouring
+// columns of a row). K advances 64 elements (128-byte rows) a stage through a
+// ring of LDS slots filled by buffer loads: whole lines, 8 rows an instruction,
+// 16-byte chunk c of row r at c ^ ((r >> 1) & 7), so a fragment's 16 rows fall on
+// different banks; rows past M or N and k past K arrive as zeros.
+//
+// A stage is four phases, one quadrant (half of the wave's rows x half of its
+// columns) each: first the fragments that the quadrant still lacks are read, then
+// its MFMAs run. Waves 4-7 are one barrier behind waves 0-3, so on every SIMD
+// one wave's MFMAs run beside the other's LDS reads and DMA issue. A quarter of
+// a slot (A rows or B rows of one half) is refilled two barriers after its last
+// reader, with the stage NS later.
+template <int TM_, int TN_>
+struct Tile {
+    static constexpr int TM = TM_, TN = TN_;
+    static constexpr int MB = TM / 32, NB = TN / 64;               // 16-blocks of a wave
+    static constexpr int MB0 = (MB + 1) / 2, MB1 = MB - MB0;       // rows of phases 0, 1 and of 2, 3
+    static constexpr int NB0 = NB / 2, NB1 = NB - NB0;
+    static constexpr int AB = TM * 128, BB = TN * 128, STAGE = AB + BB;
+    static constexpr int NS = 152 * 1024 / STAGE < 4 ? 152 * 1024 / STAGE : 4;
+    // DMA instructions a wave issues per quarter
+    static constexpr int IA0 = (4 * MB0 + 7) / 8, IA1 = (4 * MB1 + 7) / 8, IB0 = NB0, IB1 = NB1;
+    static constexpr int ALL = IA0 + IB0 + IB1 + IA1;
+    static constexpr int LDS = NS * STAGE + 1024;  // the last KB takes the DMA of waves without a share
+    static_assert(NS >= 2 && LDS <= 160 * 1024 && NB % 2 == 0, "ring");
+    static constexpr int PITCH = TN / 4 + 4;  // floats per row of a wave's output staging
+    static_assert(8 * 16 * PITCH * 4 <= NS * STAGE, "staging takes the ring's place");
+};
+
+template <class T, bool GATED>
+__global__ __launch_bounds__(512) void linear_tile_kernel(LinearFusedArgs a) {
+    constexpr int NS = T::NS, MB = T::MB, NB = T::NB, MB0 = T::MB0, NB0 = T::NB0, MB1 = T::MB1;
+    constexpr int TNO = GATED ? T::TN / 2 : T::TN;  // output columns of the tile
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[T::LDS];
+
+    const int tiles_m = (a.M + T::TM - 1) / T::TM, tiles_n = (a.N + TNO - 1) / TNO;
+    int logical = xcd_remap(blockIdx.x, tiles_m * tiles_n * a.splits);
+    const int m0 = logical % tiles_m * T::TM;
+    logical /= tiles_m;
+    const int n0 = logical % tiles_n * TNO;
+    const int split = logical / tiles_n;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave >> 2, wn = wave & 3;
+    const int st0 = split * a.split_stages;
+    const int nst = min((a.K + 63) / 64 - st0, a.split_stages);
+
+    // DMA: a wave's instructions of quarter A0, A1 (rows wm * 16 MB + 16 MB0 ..),
+    // B0, B1; instruction q = wave + 8 i of a quarter brings 8 rows
+    const int rows_m = min(a.M - m0, T::TM), rows_n = min(a.N - n0, TNO);
+    uint32_t offa[T::IA0 + T::IA1], offb[T::IB0 + T::IB1];
+    int dsta[T::IA0 + T::IA1], dstb[T::IB0 + T::IB1];  // LDS offset in a slot (A rows, then B rows)
+    int ka[T::IA0 + T::IA1], kb[T::IB0 + T::IB1];      // first k of a lane's chunk
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int cnt = h == 0 ? 4 * MB0 : 4 * MB1, per = cnt / 2;  // instructions, of one wm
+#pragma unroll
+        for (int i = 0; i < (h == 0 ? T::IA0 : T::IA1); ++i) {
+            const int q = wave + 8 * i, j = h == 0 ? i : T::IA0 + i;
+            const int r0 = q / per * (16 * MB) + (h == 0 ? 0 : 16 * MB0) + q % per * 8;
+            const int row = r0 + (lane >> 3);
+            const int c = (lane & 7) ^ ((row >> 1) & 7);
+            dsta[j] = q < cnt ? r0 * 128 : -1;
+            ka[j] = c * 8;
+            offa[j] = q < cnt && row < rows_m ? static_cast<uint32_t>(row) * static_cast<uint32_t>(a.ldx) * 2u + c * 16
+                                              : kOob;
+        }
+#pragma unroll
+        for (int i = 0; i < (h == 0 ? T::IB0 : T::IB1); ++i) {
+            const int q = wave + 8 * i, j = h == 0 ? i : T::IB0 + i;
+            const int r0 = q / (2 * NB0) * (16 * NB) + h * 16 * NB0 + q % (2 * NB0) * 8;
+            const int row = r0 + (lane >> 3);
+            const int c = (lane & 7) ^ ((row >> 1) & 7);
+            const int n = GATED ? (row >> 5) * 16 + (row & 15) : row;
+            dstb[j] = T::AB + r0 * 128;
+            kb[j] = c * 8;
+            offb[j] = n < rows_n ? static_cast<uint32_t>(n) * static_cast<uint32_t>(a.ldw) * 2u + c * 16 : kOob;
+        }
+    }
+    // (16-row blocks of w and w_up in turn: with four blocks a wave's columns
+    // instruction q is of block q / 2 % 2 of a half, with two a half is one block)
+    const uint16_t* xb = a.x16 + static_cast<int64_t>(m0) * a.ldx + st0 * 64;
+    const int64_t woff = static_cast<int64_t>(n0) * a.ldw + st0 * 64;
+    const bool up0 = GATED && NB0 == 2 && ((wave >> 1) & 1);
+    const uint16_t* wb[2] = {(up0 ? a.w_up : a.w) + woff,
+                             (GATED && (NB0 == 1 || up0) ? a.w_up : a.w) + woff};
+    const int64_t xbytes = (static_cast<int64_t>(rows_m - 1) * a.ldx + (a.K - st0 * 64)) * 2;
+    const int64_t wbytes = (static_cast<int64_t>(rows_n - 1) * a.ldw + (a.K - st0 * 64)) * 2;
+    const int kleft = a.K - st0 * 64;
+
+    auto issue = [&](const uint16_t* base, int64_t bytes, uint32_t off, int k, int dst, int st) {
+        // past the last stage: nothing is read, zeros are written
+        const int n = st < nst ? static_cast<int>(bytes - st * 128) : 0;
+        const __amdgpu_buffer_rsrc_t r =
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base + st * 64), 0, n, kRsrcWord3);
+        if ((st + 1) * 64 > kleft && k + st * 64 >= kleft) off = kOob;  // past K
+        uint8_t* to = dst >= 0 ? lds + st % NS * T::STAGE + dst : lds + NS * T::STAGE;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)to, 16, off, 0, 0, 0);
+    };
+    auto issue_a = [&](int h, int st) {
+#pragma unroll
+        for (int i = 0; i < T::IA0 + T::IA1; ++i)
+            if ((i >= T::IA0) == (h == 1)) issue(xb, xbytes, offa[i], ka[i], dsta[i], st);
+    };
+    auto issue_b = [&](int h, int st) {
+#pragma unroll
+        for (int i = 0; i < T::IB0 + T::IB1; ++i)
+            if ((i >= T::IB0) == (h == 1)) issue(wb[h], wbytes, offb[i], kb[i], dstb[i], st);
+    };
+
+    v4f acc[MB][NB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[i][j] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+    const int r = lane & 15, kq = lane >> 4;
+    // fragment of 16-row block `row0`, k-step ks: lane (r, kq) has k 32 ks + 8 kq ..
+    const int lane0 = r * 128 + ((kq ^ (r >> 1)) << 4), lane1 = r * 128 + (((kq + 4) ^ (r >> 1)) << 4);
+    auto frag = [&](const uint8_t* slot, int row0, int ks) {
+        return *reinterpret_cast<const v8bf*>(slot + row0 * 128 + (ks ? lane1 : lane0));
+    };
+    v8bf fa[MB0][2], fb[2][NB0][2];
+    auto mma = [&](auto hm, auto hn) {
+        constexpr int HM = decltype(hm)::value, HN = decltype(hn)::value;
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int i = 0; i < (HM ? MB1 : MB0); ++i)
+#pragma unroll
+                for (int j = 0; j < NB0; ++j)
+                    acc[HM * MB0 + i][HN * NB0 + j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        fb[HN][j][ks], fa[i][ks], acc[HM * MB0 + i][HN * NB0 + j], 0, 0, 0);
+        __builtin_amdgcn_s_setprio(0);
+    };
+    auto barrier = [&]() {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    using H0 = std::integral_constant<int, 0>;
+    using H1 = std::integral_constant<int, 1>;
+
+    // A wave issues stage after stage in the order A0 B0, B1, A1. Behind its wait
+    // before a barrier its share of what the next phases read has landed.
+    constexpr int kAhead = (NS - 2) * T::ALL;
+#pragma unroll
+    for (int st = 0; st < NS; ++st) {
+        issue_a(0, st);
+        issue_b(0, st);
+        issue_b(1, st);
+        issue_a(1, st);
+    }
+    wait_vmcnt<T::IB1 + T::IA1 + T::ALL + kAhead>();  // A0, B0 of stage 0
+    barrier();
+    const bool lag = wave >= 4;
+    if (lag) barrier();
+    for (int st = 0; st < nst; ++st) {
+        const uint8_t* slot = lds + st % NS * T::STAGE;
+        const uint8_t* as = slot + wm * (16 * MB) * 128;
+        const uint8_t* bs = slot + T::AB + wn * (16 * NB) * 128;
+        // phase 0: rows 0, columns 0
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+#pragma unroll
+            for (int j = 0; j < NB0; ++j) fb[0][j][ks] = frag(bs, 16 * j, ks);
+#pragma unroll
+            for (int i = 0; i < MB0; ++i) fa[i][ks] = frag(as, 16 * i, ks);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        wait_vmcnt<T::IA1 + T::ALL + kAhead>();  // B1
+        wait_lgkmcnt0();
+        barrier();
+        mma(H0{}, H0{});
+        barrier();
+        // phase 1: rows 0, columns 1
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int j = 0; j < NB0; ++j) fb[1][j][ks] = frag(bs, 16 * (NB0 + j), ks);
+        __builtin_amdgcn_sched_barrier(0);
+        issue_a(0, st + NS);
+        issue_b(0, st + NS);
+        wait_vmcnt<T::ALL + T::IA0 + T::IB0 + kAhead>();  // A1
+        wait_lgkmcnt0();
+        barrier();
+        mma(H0{}, H1{});
+        barrier();
+        // phase 2: rows 1, columns 1
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int i = 0; i < MB1; ++i) fa[i][ks] = frag(as, 16 * (MB0 + i), ks);
+        __builtin_amdgcn_sched_barrier(0);
+        issue_b(1, st + NS);
+        wait_lgkmcnt0();
+        barrier();
+        mma(H1{}, H1{});
+        barrier();
+        // phase 3: rows 1, columns 0
+        issue_a(1, st + NS);
+        __builtin_amdgcn_sched_barrier(0);
+        wait_vmcnt<T::IB1 + T::IA1 + T::ALL + kAhead>();  // A0, B0 of the next stage
+        barrier();
+        mma(H1{}, H0{});
+        barrier();
+    }
+    if (!lag) barrier();
+    wait_vmcnt<0>();
+    __syncthreads();
+
+    // 16 rows of the wave at a time through LDS, so that a store covers whole
+    // lines of a row: lane 4 columns, OL lanes a row
+    constexpr int WN = T::TN / 4, WO = GATED ? WN / 2 : WN, OL = WO / 4, RP = 64 / OL;
+    float* sh = reinterpret_cast<float*>(lds) + wave * 16 * T::PITCH;
+    const int oc = (lane % OL) * 4;  // output column of the wave
+    const int n = n0 + wn * WO + oc;
+    // staged column of it: GATED: block oc / 16 of w at 32 (oc / 16), of w_up 16 further
+    const int sc = GATED ? (oc >> 4) * 32 + (oc & 15) : oc;
+    Columns col;
+    if (a.splits == 1 && n < a.N) col = load_columns(a, n);
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int j = 0; j < NB; ++j) *reinterpret_cast<v4f*>(sh + r * T::PITCH + 16 * j + 4 * kq) = acc[i][j];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int q = 0; q < 16 / RP; ++q) {
+            const int row = q * RP + lane / OL;
+            const int m = m0 + wm * (16 * MB) + 16 * i + row;
+            const v4f z = *reinterpret_cast<const v4f*>(sh + row * T::PITCH + sc);
+            v4f u = {0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (GATED) u = *reinterpret_cast<const v4f*>(sh + row * T::PITCH + sc + 16);
+            if (m >= a.M || n >= a.N) continue;
+            if (a.splits == 1) {
+                const float zz[4] = {z[0], z[1], z[2], z[3]}, uu[4] = {u[0], u[1], u[2], u[3]};
+                finish4<GATED>(a, col, m, n, zz, uu);
+            } else {  // part rows hold the columns padded to four, then w_up's
+                float* p = a.part + (static_cast<int64_t>(split) * a.M + m) * a.part_ld + n;
+                *reinterpret_cast<v4f*>(p) = z;
+                if constexpr (GATED) *reinterpret_cast<v4f*>(p + a.part_ld / 2) = u;
+            }
+        }
+    }
+}
+
+template <bool GATED>
+__global__ __launch_bounds__(256) void linear_join_kernel(LinearFusedArgs a) {
+    const int groups = (a.N + 3) / 4;
+    const int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (idx >= static_cast<int64_t>(groups) * a.M) return;
+    const int m = static_cast<int>(idx / groups), n = static_cast<int>(idx % groups) * 4;
+    const Columns col = load_columns(a, n);
+    float z[4] = {0.0f, 0.0f, 0.0f, 0.0f}, u[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s) {
+        const float* p = a.part + (static_cast<int64_t>(s) * a.M + m) * a.part_ld + n;
+        const v4f q = *reinterpret_cast<const v4f*>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z[i] += q[i];
+        if constexpr (GATED) {
+            const v4f t = *reinterpret_cast<const v4f*>(p + a.part_ld / 2);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u[i] += t[i];
+        }
+    }
+    finish4<GATED>(a, col, m, n, z, u);
+}
+
+// ---- up to 16 rows -------------------------------------------------------------
+// One workgroup of eight waves per 16 output columns; the waves take the 32-k
+// steps of K in turn, eight at a time, and read their weights straight into
+// fragments (64 bytes of each of 16 rows an instruction, the next ones following in the
+// same lines). The partial tiles are added through LDS in wave order. Bound by
+// the weights' bytes: what counts is how many are in flight (8 KB a wave).
+constexpr int RW = 8, RD = 8;
+
+template <bool XF32, bool GATED>
+__global__ __launch_bounds__(RW * 64) void linear_rows_kernel(LinearFusedArgs a) {
+    constexpr int NP = GATED ? 2 : 1;
+    __shared__ v4f red[NP][RW][64];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = blockIdx.x * 16;
+    const int r = lane & 15, kq = lane >> 4;
+    const int rows_n = min(a.N - n0, 16);
+    const int64_t wbytes = (static_cast<int64_t>(rows_n - 1) * a.ldw + a.K) * 2;
+    const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint16_t*>(a.w + static_cast<int64_t>(n0) * a.ldw), 0, static_cast<int>(wbytes), kRsrcWord3);
+    const __amdgpu_buffer_rsrc_t ru = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint16_t*>(GATED ? a.w_up + static_cast<int64_t>(n0) * a.ldw : a.w), 0,
+        GATED ? static_cast<int>(wbytes) : 0, kRsrcWord3);
+    const uint32_t ow = r < rows_n ? static_cast<uint32_t>(r) * static_cast<uint32_t>(a.ldw) * 2u + kq * 16 : kOob;
+    const bool xrow = r < a.M;
+
+    v4f acc[NP];
+#pragma unroll
+    for (int p = 0; p < NP; ++p) acc[p] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+    const int steps = (a.K + 31) / 32;
+    for (int s0 = wave * RD; s0 < steps; s0 += RW * RD) {
+        v4i fw[NP][RD];
+#pragma unroll
+        for (int d = 0; d < RD; ++d) {
+            const int k = (s0 + d) * 32 + 8 * kq;
+            const uint32_t o = k < a.K && ow != kOob ? ow + static_cast<uint32_t>(s0 + d) * 64 : kOob;
+            fw[0][d] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw, o, 0, 0));
+            if constexpr (GATED) fw[1][d] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(ru, o, 0, 0));
+        }
+#pragma unroll
+        for (int d = 0; d < RD; ++d) {
+            const int k = (s0 + d) * 32 + 8 * kq;
+            v8bf fx = __builtin_bit_cast(v8bf, (v4i){0, 0, 0, 0});
+            if (xrow && k < a.K) {
+                if constexpr (XF32) {
+                    const float* xp = static_cast<const float*>(a.x) + r * a.ldx + k;
+                    const v4f lo = *reinterpret_cast<const v4f*>(xp), hi = *reinterpret_cast<const v4f*>(xp + 4);
+                    fx = __builtin_bit_cast(v8bf, (v4i){static_cast<int>(pack_bf16x2(lo[0], lo[1])),
+                                                        static_cast<int>(pack_bf16x2(lo[2], lo[3])),
+                                                        static_cast<int>(pack_bf16x2(hi[0], hi[1])),
+                                                        static_cast<int>(pack_bf16x2(hi[2], hi[3]))});
+                } else {
+                    fx = *reinterpret_cast<const v8bf*>(a.x16 + r * a.ldx + k);
+                }
+            }
+#pragma unroll
+            for (int p = 0; p < NP; ++p)
+                acc[p] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, fw[p][d]), fx, acc[p], 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < NP; ++p) red[p][wave][lane] = acc[p];
+    __syncthreads();
+    if (wave != 0) return;
+    // lane: row lane % 16, columns 4 (lane / 16) ..
+    v4f z = red[0][0][lane], u = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 1; w < RW; ++w) z += red[0][w][lane];
+    if constexpr (GATED) {
+        u = red[NP - 1][0][lane];
+#pragma unroll
+        for (int w = 1; w < RW; ++w) u += red[NP - 1][w][lane];
+    }
+    const int n = n0 + 4 * kq;
+    if (r >= a.M || n >= a.N) return;
+    const float zz[4] = {z[0], z[1], z[2], z[3]}, uu[4] = {u[0], u[1], u[2], u[3]};
+    finish4<GATED>(a, load_columns(a, n), r, n, zz, uu);
+}
+
+// rows of K values, fp32 or bf16, to bf16 rows of Kp >= K (a multiple of 8),
+// zeros behind K: eight values a thread
+template <bool F32>
+__global__ __launch_bounds__(256) void pack_rows_kernel(const void* __restrict__ in, int64_t ld, int64_t rows, int K,
+                                                        int Kp, uint16_t* __restrict__ out) {
+    const int per = Kp / 8;
+    const int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (idx >= rows * per) return;
+    const int64_t row = idx / per;
+    const int k = static_cast<int>(idx % per) * 8;
+    const float* f = static_cast<const float*>(in) + row * ld + k;
+    const uint16_t* h = static_cast<const uint16_t*>(in) + row * ld + k;
+    uint32_t w[4];
+    if (F32 && k + 8 <= K && (reinterpret_cast<uintptr_t>(f) & 15) == 0) {
+        const v4f lo = *reinterpret_cast<const v4f*>(f), hi = *reinterpret_cast<const v4f*>(f + 4);
+        w[0] = pack_bf16x2(lo[0], lo[1]);
+        w[1] = pack_bf16x2(lo[2], lo[3]);
+        w[2] = pack_bf16x2(hi[0], hi[1]);
+        w[3] = pack_bf16x2(hi[2], hi[3]);
+    } else {
+        uint16_t v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = k + i < K ? (F32 ? f32_to_bf16(f[i]) : h[i]) : static_cast<uint16_t>(0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = v[2 * i] | (static_cast<uint32_t>(v[2 * i + 1]) << 16);
+    }
+    *reinterpret_cast<u32x4*>(out + row * Kp + k) = (u32x4){w[0], w[1], w[2], w[3]};
+}
+
+hipError_t launch_pack(const void* in, bool f32, int64_t ld, int64_t rows, int K, int Kp, uint16_t* out,
+                       hipStream_t stream) {
+    const int64_t total = rows * (Kp / 8);
+    const unsigned blocks = static_cast<unsigned>((total + 255) / 256);
+    if (f32)
+        hipLaunchKernelGGL(pack_rows_kernel<true>, dim3(blocks), dim3(256), 0, stream, in, ld, rows, K, Kp, out);
+    else
+        hipLaunchKernelGGL(pack_rows_kernel<false>, dim3(blocks), dim3(256), 0, stream, in, ld, rows, K, Kp, out);
+    return hipGetLastError();
+}
+
+template <int TM, int TN, bool GATED>
+hipError_t launch_tile(const LinearFusedArgs& a, hipStream_t stream) {
+    constexpr int TNO = GATED ? TN / 2 : TN;
+    const int tiles = ((a.M + TM - 1) / TM) * ((a.N + TNO - 1) / TNO);
+    hipLaunchKernelGGL((linear_tile_kernel<Tile<TM, TN>, GATED>), dim3(tiles * a.splits), dim3(512), 0, stream, a);
+    return hipGetLastError();
+}
+
+int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
+
+}  // namespace
+
+// Tile and number of K splits: the least estimated time of the launch (us). A
+// workgroup's stage costs its MFMAs or its bytes through the CU's port to L2,
+// whichever is more; the parts of a split sum are written and read once.
+LinearFusedPlan linear_fused_plan(int M, int K, int N, bool gated) {
+    LinearFusedPlan best{};
+    if (M <= kLinearRows) return best;
+    static const int tms[] = {256, 224, 192, 160, 128, 64}, tns[] = {256, 128};
+    const int stages = (K + 63) / 64;
+    double best_t = 1e30;
+    for (int tm : tms)
+        for (int tn : tns) {
+            const int tno = gated ? tn / 2 : tn;
+            const int64_t tiles = static_cast<int64_t>((M + tm - 1) / tm) * ((N + tno - 1) / tno);
+            const double stage = std::max(tm * tn / 65536.0 * 1.7, (tm + tn) * 128 / 80e3) + 0.12;
+            for (int s = 1; s <= 16 && s <= stages; ++s) {
+                const int per = (stages + s - 1) / s;
+                if (per * (s - 1) >= stages) continue;  // the last range would be empty
+                const double rounds = static_cast<double>((tiles * s + 255) / 256);
+                double t = rounds * (per * stage + 4.0);
+                if (s > 1) t += 4.0 + 2.0 * s * M * N * (gated ? 8.0 : 4.0) / 4e6;
+                if (t < best_t) {
+                    best_t = t;
+                    best.tm = tm;
+                    best.tn = tn;
+                    best.splits = s;
+                    best.split_stages = per;
+                }
+            }
+        }
+    return best;
+}
+
+// Scratch: packed x, packed w and w_up, the parts of a split sum.
+LinearFusedScratch linear_fused_scratch(int x_dtype, int M, int K, int N, bool gated) {
+    LinearFusedScratch s{};
+    if (M <= 0 || K <= 0 || N <= 0) return s;
+    const int Kp = (K + 7) / 8 * 8;
+    const bool odd = Kp != K;
+    if (odd || (x_dtype == QIMG_FP32 && M > kLinearRows)) s.x = align256(static_cast<int64_t>(M) * Kp * 2);
+    if (odd) s.w = align256(static_cast<int64_t>(N) * Kp * 2);
+    if (odd && gated) s.w_up = s.w;
+    const LinearFusedPlan p = linear_fused_plan(M, K, N, gated);
+    if (p.splits > 1) s.part = align256(static_cast<int64_t>(p.splits) * M * ((N + 3) / 4 * 4) * (gated ? 8 : 4));
+    return s;
+}
+
+hipError_t launch_linear_fused(LinearFusedArgs a, int x_dtype, void* scratch, hipStream_t stream) {
+    const bool gated = a.w_up != nullptr;
+    const LinearFusedScratch s = linear_fused_scratch(x_dtype, a.M, a.K, a.N, gated);
+    uint8_t* p = static_cast<uint8_t*>(scratch);
+    const int Kp = (a.K + 7) / 8 * 8;
+    bool f32 = x_dtype == QIMG_FP32;
+    hipError_t e = hipSuccess;
+    a.x16 = static_cast<const uint16_t*>(a.x);
+    a.ldw = a.K;
+    if (s.x) {
+        uint16_t* xp = reinterpret_cast<uint16_t*>(p);
+        e = launch_pack(a.x, f32, a.ldx, a.M, a.K, Kp, xp, stream);
+        if (e != hipSuccess) return e;
+        a.x = a.x16 = xp;
+        a.ldx = Kp;
+        f32 = false;
+        p += s.x;
+    }
+    for (int i = 0; i < 2; ++i) {
+        if (!(i ? s.w_up : s.w)) continue;
+        uint16_t* wp = reinterpret_cast<uint16_t*>(p);
+        e = launch_pack(i ? a.w_up : a.w, false, a.K, a.N, a.K, Kp, wp, stream);
+        if (e != hipSuccess) return e;
+        (i ? a.w_up : a.w) = wp;
+        p += i ? s.w_up : s.w;
+    }
+    if (s.w) a.ldw = a.K = Kp;
+    a.part = reinterpret_cast<float*>(p);
+    a.part_ld = static_cast<int64_t>((a.N + 3) / 4 * 4) * (gated ? 2 : 1);
+    if (a.M <= kLinearRows) {
+        a.splits = 1;
+        const dim3 grid((a.N + 15) / 16), block(RW * 64);
+        if (f32 && gated)
+            hipLaunchKernelGGL((linear_rows_kernel<true, true>), grid, block, 0, stream, a);
+        else if (f32)
+            hipLaunchKernelGGL((linear_rows_kernel<true, false>), grid, block, 0, stream, a);
+        else if (gated)
+            hipLaunchKernelGGL((linear_rows_kernel<false, true>), grid, block, 0, stream, a);
+        else
+            hipLaunchKernelGGL((linear_rows_kernel<false, false>), grid, block, 0, stream, a);
+        return hipGetLastError();
+    }
+    const LinearFusedPlan plan = linear_fused_plan(a.M, a.K, a.N, gated);
+    a.splits = plan.splits;
+    a.split_stages = plan.split_stages;
+#define QIMG_TILE(TM, TN)                                                                       \
+    if (plan.tm == TM && plan.tn == TN)                                                         \
+    e = gated ? launch_tile<TM, TN, true>(a, stream) : launch_tile<TM, TN, false>(a, stream)
+    QIMG_TILE(256, 256);
+    QIMG_TILE(224, 256);
+    QIMG_TILE(192, 256);
+    QIMG_TILE(160, 256);
+    QIMG_TILE(128, 256);
+    QIMG_TILE(64, 256);
+    QIMG_TILE(256, 128);
+    QIMG_TILE(224, 128);
+    QIMG_TILE(192, 128);
+    QIMG_TILE(160, 128);
+    QIMG_TILE(128, 128);
+    QIMG_TILE(64, 128);
+#undef QIMG_TILE
+    if (e != hipSuccess || plan.splits == 1) return e;
+    const int64_t groups = static_cast<int64_t>((a.N + 3) / 4) * a.M;
+    const dim3 grid(static_cast<unsigned>((groups + 255) / 256));
+    if (gated)
+        hipLaunchKernelGGL(linear_join_kernel<true>, grid, dim3(256), 0, stream, a);
+    else
+        hipLaunchKernelGGL(linear_join_kernel<false>, grid, dim3(256), 0, stream, a);
+    return hipGetLastError();
+}
+
+}  // namespace qimg

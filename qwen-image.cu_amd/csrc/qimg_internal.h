@@ -345,4 +345,37 @@ struct AttnVarlenArgs {
 int attn_varlen_splits(int total_q, int total_k, int batch, int hq, int hk);
 hipError_t launch_attention_varlen(const AttnVarlenArgs& a, int dtype, int D, hipStream_t stream);
 
+// gemm_fused.hip: the bf16 linear with its epilogue (qimg_linear_bf16_fused)
+struct LinearFusedArgs {
+    const void* x;
+    const uint16_t* x16;  // x as bf16 rows
+    int64_t ldx;
+    const uint16_t* w;
+    const uint16_t* w_up;  // or null
+    int64_t ldw;
+    int M, N, K;
+    const uint16_t* bias;
+    const uint16_t* bias_up;
+    const float* gate;
+    const void* residual;
+    int64_t ldr;
+    void* out;
+    int64_t ldo;
+    int act, res_dtype, out_dtype;
+    int vec4;  // rows of out and residual are whole groups of four values
+    int splits, split_stages;  // ranges of K, 64-k stages a range
+    float* part;               // [splits, M, part_ld] with splits > 1
+    int64_t part_ld;
+};
+constexpr int kLinearRows = 16;  // most rows of the kernel that reads weights straight into fragments
+struct LinearFusedPlan {
+    int tm, tn, splits, split_stages;
+};
+struct LinearFusedScratch {
+    int64_t x, w, w_up, part;
+};
+LinearFusedPlan linear_fused_plan(int M, int K, int N, bool gated);
+LinearFusedScratch linear_fused_scratch(int x_dtype, int M, int K, int N, bool gated);
+hipError_t launch_linear_fused(LinearFusedArgs a, int x_dtype, void* scratch, hipStream_t stream);
+
 }  // namespace qimg

@@ -69,6 +69,8 @@ _SIGS = {
     "qimg_sage_attention": (_I, [_P, _P, _P, _P, _I, _F, _I, _I, _I, _I, _P, _I64, _P]),
     "qimg_attention_varlen_scratch_bytes": (_I64, [_I, _I, _I, _I, _I, _I]),
     "qimg_attention_varlen": (_I, [_P, _P, _I64, _P]),
+    "qimg_linear_bf16_fused_scratch_bytes": (_I64, [_I, _I, _I, _I, _I]),
+    "qimg_linear_bf16_fused": (_I, [_P, _P, _I64, _P]),
     "qimg_silu": (_I, [_P, _P, _I64, _P]),
     "qimg_layernorm_modulate": (_I, [_P, _P, _P, _P, _I, _I, _F, _P]),
     "qimg_layernorm_modulate_quant": (_I, [_P, _P, _P, _I, _I, _I, _I, _F, _P, _P, _P]),
@@ -625,23 +627,48 @@ class _AttnVarlen(ctypes.Structure):
                 ("head_dim", _I), ("sm_scale", _F), ("causal", _I)]
 
 
-def _require(cond, message: str):
-    if not cond:
-        raise QimgError(QIMG_ERR_INVALID_ARG, message)
-
-
 def _same_device(ref: torch.Tensor, **tensors):
     for name, t in tensors.items():
-        if t is not None:
-            _require(t.is_cuda and t.device == ref.device, f"{name} must be a tensor on {ref.device}")
+        if t is not None and t.device != ref.device:
+            raise QimgError(QIMG_ERR_INVALID_ARG, f"{name} must be a tensor on {ref.device}")
+
+
+class _NoSwitch:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NO_SWITCH = _NoSwitch()
+
+
+def _on(device):
+    """The device of a call's tensors made current for it (nothing to do where it is already)."""
+    return _NO_SWITCH if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _raw_stream(device):
+    """The current stream of `device` as the C entry points take it."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _row_stride(t: torch.Tensor, n: int) -> int:
+    """Elements between rows of a [rows, n] tensor (a single row's stride says nothing)."""
+    return t.stride(0) if t.shape[0] > 1 else n
 
 
 def _scratch_for(need: int, scratch: torch.Tensor | None, device) -> torch.Tensor | None:
     """The caller's scratch, or a buffer of `need` bytes; its bytes are counted, not its elements."""
     if scratch is None:
         return torch.empty((need,), dtype=torch.uint8, device=device) if need else None
-    _require(scratch.is_cuda and scratch.device == device and scratch.is_contiguous(),
-             f"scratch must be a contiguous tensor on {device}")
+    if scratch.device != device or not scratch.is_contiguous():
+        raise QimgError(QIMG_ERR_INVALID_ARG, f"scratch must be a contiguous tensor on {device}")
     return scratch
 
 
@@ -665,30 +692,98 @@ def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     last key. k_lens int32 [B]: keys in use of each sequence's slot (a cache
     with room behind its last key). Queries that see no key give zeros; rows of
     no sequence are not written. sm_scale defaults to 1 / sqrt(D)."""
-    _require(q.is_cuda and q.dim() == 3 and k.dim() == 3 and v.dim() == 3, "q, k and v must be device tensors [T, H, D]")
+    if not (q.is_cuda and q.dim() == 3 and k.dim() == 3 and v.dim() == 3):
+        raise QimgError(QIMG_ERR_INVALID_ARG, "q, k and v must be device tensors [T, H, D]")
     _same_device(q, k=k, v=v, cu_seqlens_q=cu_seqlens_q, cu_seqlens_k=cu_seqlens_k, k_lens=k_lens, out=out)
-    _require(q.dtype in (torch.bfloat16, torch.float16) and k.dtype == q.dtype and v.dtype == q.dtype,
-             "q, k and v must be all bfloat16 or all float16")
+    dt = q.dtype
+    if dt not in (torch.bfloat16, torch.float16) or k.dtype != dt or v.dtype != dt:
+        raise QimgError(QIMG_ERR_INVALID_ARG, "q, k and v must be all bfloat16 or all float16")
     tq, hq, d = q.shape
     tk, hk, dk = k.shape
-    _require(v.shape == k.shape and dk == d, f"k {tuple(k.shape)} and v {tuple(v.shape)} must be [Tk, Hk, {d}]")
-    _require(q.stride(2) == 1 and k.stride(2) == 1 and v.stride(2) == 1, "the last dimension must be contiguous")
+    if v.shape != k.shape or dk != d:
+        raise QimgError(QIMG_ERR_INVALID_ARG, f"k {tuple(k.shape)} and v {tuple(v.shape)} must be [Tk, Hk, {d}]")
     batch = cu_seqlens_q.numel() - 1
-    _require(batch >= 0 and cu_seqlens_k.numel() == batch + 1, "cu_seqlens_q and cu_seqlens_k must have B + 1 elements")
-    for name, t in (("cu_seqlens_q", cu_seqlens_q), ("cu_seqlens_k", cu_seqlens_k), ("k_lens", k_lens)):
-        _require(t is None or (t.dtype == torch.int32 and t.is_contiguous()), f"{name} must be contiguous int32")
-    _require(k_lens is None or k_lens.numel() == batch, "k_lens must have B elements")
+    if batch < 0 or cu_seqlens_k.numel() != batch + 1 or (k_lens is not None and k_lens.numel() != batch):
+        raise QimgError(QIMG_ERR_INVALID_ARG, "cu_seqlens_q and cu_seqlens_k must have B + 1 elements, k_lens B")
+    for t in (cu_seqlens_q, cu_seqlens_k, k_lens):
+        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
+            raise QimgError(QIMG_ERR_INVALID_ARG, "cu_seqlens_q, cu_seqlens_k and k_lens must be contiguous int32")
     if out is None:
-        out = torch.empty((tq, hq, d), dtype=q.dtype, device=q.device)
-    _require(out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1,
-             f"out must be {tuple(q.shape)} of q's type, its last dimension contiguous")
-    with torch.cuda.device(q.device):
-        scratch = _scratch_for(attention_varlen_scratch_bytes(tq, tk, batch, hq, hk, d), scratch, q.device)
-        args = _AttnVarlen(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _DT[q.dtype], q.stride(0), q.stride(1), k.stride(0),
-                           k.stride(1), v.stride(0), v.stride(1), out.stride(0), out.stride(1), _ptr(cu_seqlens_q),
-                           _ptr(cu_seqlens_k), _ptr(k_lens), batch, tq, tk, hq, hk, d,
-                           1.0 / d ** 0.5 if sm_scale is None else float(sm_scale), int(bool(causal)))
-        _check(_lib.qimg_attention_varlen(ctypes.byref(args), _ptr(scratch), _nbytes(scratch), _stream(q.device)))
+        out = torch.empty((tq, hq, d), dtype=dt, device=q.device)
+    elif out.shape != q.shape or out.dtype != dt:
+        raise QimgError(QIMG_ERR_INVALID_ARG, f"out must be {tuple(q.shape)} of q's type")
+    sq, sk, sv, so = q.stride(), k.stride(), v.stride(), out.stride()
+    if not (sq[2] == 1 and sk[2] == 1 and sv[2] == 1 and so[2] == 1):
+        raise QimgError(QIMG_ERR_INVALID_ARG, "the last dimension of q, k, v and out must be contiguous")
+    with _on(q.device):
+        scratch = _scratch_for(_lib.qimg_attention_varlen_scratch_bytes(tq, tk, batch, hq, hk, d), scratch, q.device)
+        args = _AttnVarlen(_addr(q), _addr(k), _addr(v), _addr(out), _DT[dt], sq[0], sq[1], sk[0], sk[1], sv[0], sv[1],
+                           so[0], so[1], _addr(cu_seqlens_q), _addr(cu_seqlens_k), _addr(k_lens), batch, tq, tk, hq, hk,
+                           d, 1.0 / d ** 0.5 if sm_scale is None else sm_scale, bool(causal))
+        _check(_lib.qimg_attention_varlen(ctypes.byref(args), _addr(scratch), _nbytes(scratch), _raw_stream(q.device)))
+    return out
+
+
+ACTIVATIONS = {"none": 0, "gelu": 1, "silu": 2}
+
+
+class _LinearFused(ctypes.Structure):
+    _fields_ = [("x", _P), ("x_dtype", _I), ("ldx", _I64), ("M", _I), ("N", _I), ("K", _I), ("w", _P), ("w_up", _P),
+                ("bias", _P), ("bias_up", _P), ("act", _I), ("gate", _P), ("residual", _P), ("residual_dtype", _I),
+                ("ld_residual", _I64), ("out", _P), ("out_dtype", _I), ("ldo", _I64)]
+
+
+def linear_bf16_fused_scratch_bytes(x_dtype, M: int, K: int, N: int, gated: bool = False) -> int:
+    return int(_lib.qimg_linear_bf16_fused_scratch_bytes(_DT[x_dtype], M, K, N, int(bool(gated))))
+
+
+def linear_forward_bf16_fused(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
+                              activation: str = "none", weight_up: torch.Tensor | None = None,
+                              bias_up: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+                              residual: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                              out_dtype=torch.bfloat16, scratch: torch.Tensor | None = None) -> torch.Tensor:
+    """out = residual + gate * act(x weight^T + bias) [* (x weight_up^T + bias_up)]:
+    x [M, K] fp32 (rounded to bf16) or bf16, weights bf16 [N, K], biases bf16
+    [N], gate fp32 [N], residual and out [M, N] fp32 or bf16; x, residual and
+    out may be views with longer rows; out may be residual. activation "none",
+    "gelu" (tanh form) or "silu"."""
+    if not (x.is_cuda and x.dim() == 2 and weight.dim() == 2):
+        raise QimgError(QIMG_ERR_INVALID_ARG, "x and weight must be device tensors of two dimensions")
+    _same_device(x, weight=weight, bias=bias, weight_up=weight_up, bias_up=bias_up, gate=gate, residual=residual,
+                 out=out)
+    M, K = x.shape
+    N = weight.shape[0]
+    if weight.shape[1] != K:
+        raise QimgError(QIMG_ERR_INVALID_ARG, f"weight K {weight.shape[1]} != activation K {K}")
+    if x.dtype not in (torch.float32, torch.bfloat16):
+        raise QimgError(QIMG_ERR_INVALID_ARG, "x must be float32 or bfloat16")
+    if weight.dtype != torch.bfloat16 or not weight.is_contiguous():
+        raise QimgError(QIMG_ERR_INVALID_ARG, "weight must be contiguous bfloat16")
+    if weight_up is not None and (weight_up.shape != weight.shape or weight_up.dtype != torch.bfloat16
+                                  or not weight_up.is_contiguous()):
+        raise QimgError(QIMG_ERR_INVALID_ARG, "weight_up must be as weight")
+    for t, name, dt in ((bias, "bias", torch.bfloat16), (bias_up, "bias_up", torch.bfloat16),
+                        (gate, "gate", torch.float32)):
+        if t is not None and (t.dtype != dt or t.numel() != N or not t.is_contiguous()):
+            raise QimgError(QIMG_ERR_INVALID_ARG, f"{name} must be contiguous {dt} of {N} elements")
+    if activation not in ACTIVATIONS:
+        raise QimgError(QIMG_ERR_INVALID_ARG, f"activation {activation!r} must be one of {sorted(ACTIVATIONS)}")
+    if out is None:
+        out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+    for t, name in ((out, "out"), (residual, "residual")):
+        if t is not None and (t.shape != (M, N) or t.dtype not in (torch.float32, torch.bfloat16)
+                              or (N > 1 and t.stride(1) != 1)):
+            raise QimgError(QIMG_ERR_INVALID_ARG, f"{name} must be float32 or bfloat16 [{M}, {N}] with contiguous rows")
+    if K > 1 and x.stride(1) != 1:
+        raise QimgError(QIMG_ERR_INVALID_ARG, "rows of x must be contiguous")
+    with _on(x.device):
+        scratch = _scratch_for(linear_bf16_fused_scratch_bytes(x.dtype, M, K, N, weight_up is not None), scratch, x.device)
+        args = _LinearFused(_addr(x), _DT[x.dtype], _row_stride(x, K), M, N, K, _addr(weight), _addr(weight_up),
+                            _addr(bias), _addr(bias_up), ACTIVATIONS[activation], _addr(gate), _addr(residual),
+                            FP32 if residual is None else _DT[residual.dtype],
+                            N if residual is None else _row_stride(residual, N), _addr(out), _DT[out.dtype],
+                            _row_stride(out, N))
+        _check(_lib.qimg_linear_bf16_fused(ctypes.byref(args), _addr(scratch), _nbytes(scratch), _raw_stream(x.device)))
     return out
 
 
