@@ -6,8 +6,8 @@
 // accumulation; bias, activation, product, gate and residual in fp32 on the
 // accumulators, one rounding to out's type.
 //
-// Three kernels: linear_rows_kernel (up to 16 rows: bound by reading the
-// weights), linear_tile_kernel (the rest, also with the sum over k split over
+// Four kernels: linear_gemv_kernel (one or two rows) and linear_rows_kernel (up
+// to 16), both bound by reading the weights, linear_tile_kernel (the rest, also with the sum over k split over
 // workgroups where there are few tiles) and linear_join_kernel (adds the parts
 // in order and applies the epilogue). x in fp32 with more than 16 rows, and
 // operands whose rows are not whole 16-byte pieces, first go through
@@ -99,6 +99,22 @@ __device__ __forceinline__ void finish4(const LinearFusedArgs& a, const Columns&
     }
 }
 
+// the epilogue of one output
+template <bool GATED>
+__device__ __forceinline__ void finish1(const LinearFusedArgs& a, int m, int n, float z, float u) {
+    float v = activate(z + (a.bias != nullptr ? bf16_to_f32(a.bias[n]) : 0.0f), a.act);
+    if (GATED) v *= u + (a.bias_up != nullptr ? bf16_to_f32(a.bias_up[n]) : 0.0f);
+    if (a.gate != nullptr) v *= a.gate[n];
+    const int64_t o = m * a.ldo + n, r = m * a.ldr + n;
+    if (a.residual != nullptr)
+        v += a.res_dtype == QIMG_BF16 ? bf16_to_f32(static_cast<const uint16_t*>(a.residual)[r])
+                                      : static_cast<const float*>(a.residual)[r];
+    if (a.out_dtype == QIMG_BF16)
+        static_cast<uint16_t*>(a.out)[o] = f32_to_bf16(v);
+    else
+        static_cast<float*>(a.out)[o] = v;
+}
+
 // ---- tiles -------------------------------------------------------------------
 // A workgroup of eight waves owns TM x TN products (TN weight rows; with GATED
 // 16 rows of w and 16 of w_up in turn, so a lane holds both factors of an
@@ -139,11 +155,16 @@ __global__ __launch_bounds__(512) void linear_tile_kernel(LinearFusedArgs a) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[T::LDS];
 
     const int tiles_m = (a.M + T::TM - 1) / T::TM, tiles_n = (a.N + TNO - 1) / TNO;
-    int logical = xcd_remap(blockIdx.x, tiles_m * tiles_n * a.splits);
-    const int m0 = logical % tiles_m * T::TM;
-    logical /= tiles_m;
-    const int n0 = logical % tiles_n * TNO;
-    const int split = logical / tiles_n;
+    // An XCD's workgroups take neighbouring tiles, eight tile rows by n: the 32 in
+    // flight read about 8 + 4 tiles' operands through its L2.
+    const int logical = xcd_remap(blockIdx.x, tiles_m * tiles_n * a.splits);
+    const int split = logical / (tiles_m * tiles_n);
+    const int in_split = logical - split * (tiles_m * tiles_n);
+    const int band = in_split / (8 * tiles_n);
+    const int high = min(tiles_m - 8 * band, 8);
+    const int in_band = in_split - band * 8 * tiles_n;
+    const int m0 = (8 * band + in_band % high) * T::TM;
+    const int n0 = in_band / high * TNO;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave >> 2, wn = wave & 3;
@@ -184,33 +205,46 @@ __global__ __launch_bounds__(512) void linear_tile_kernel(LinearFusedArgs a) {
     }
     // (16-row blocks of w and w_up in turn: with four blocks a wave's columns
     // instruction q is of block q / 2 % 2 of a half, with two a half is one block)
-    const uint16_t* xb = a.x16 + static_cast<int64_t>(m0) * a.ldx + st0 * 64;
-    const int64_t woff = static_cast<int64_t>(n0) * a.ldw + st0 * 64;
     const bool up0 = GATED && NB0 == 2 && ((wave >> 1) & 1);
-    const uint16_t* wb[2] = {(up0 ? a.w_up : a.w) + woff,
-                             (GATED && (NB0 == 1 || up0) ? a.w_up : a.w) + woff};
-    const int64_t xbytes = (static_cast<int64_t>(rows_m - 1) * a.ldx + (a.K - st0 * 64)) * 2;
-    const int64_t wbytes = (static_cast<int64_t>(rows_n - 1) * a.ldw + (a.K - st0 * 64)) * 2;
+    const int64_t woff = static_cast<int64_t>(n0) * a.ldw + st0 * 64;
     const int kleft = a.K - st0 * 64;
-
-    auto issue = [&](const uint16_t* base, int64_t bytes, uint32_t off, int k, int dst, int st) {
-        // past the last stage: nothing is read, zeros are written
-        const int n = st < nst ? static_cast<int>(bytes - st * 128) : 0;
-        const __amdgpu_buffer_rsrc_t r =
-            __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base + st * 64), 0, n, kRsrcWord3);
-        if ((st + 1) * 64 > kleft && k + st * 64 >= kleft) off = kOob;  // past K
-        uint8_t* to = dst >= 0 ? lds + st % NS * T::STAGE + dst : lds + NS * T::STAGE;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)to, 16, off, 0, 0, 0);
+    // An operand's rows from the next stage to issue on: first byte, and bytes to
+    // the end of the last row (nothing past it is read). 3 scalar operations move it
+    // a stage on.
+    struct Rows {
+        const uint16_t* p;
+        int bytes;
     };
-    auto issue_a = [&](int h, int st) {
+    Rows xr = {a.x16 + static_cast<int64_t>(m0) * a.ldx + st0 * 64,
+               static_cast<int>((static_cast<int64_t>(rows_m - 1) * a.ldx + kleft) * 2)};
+    const int wbytes = static_cast<int>((static_cast<int64_t>(rows_n - 1) * a.ldw + kleft) * 2);
+    Rows wr[2] = {{(up0 ? a.w_up : a.w) + woff, wbytes}, {(GATED && (NB0 == 1 || up0) ? a.w_up : a.w) + woff, wbytes}};
+    const int tail = kleft / 64, tail_k = kleft % 64;  // the stage that K ends inside, and where
+    int fill = 0, fill_at = 0;                         // stage to issue next, its slot's offset
+
+    auto issue = [&](const Rows& w, uint32_t off, int k, int dst) {
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint16_t*>(w.p), 0, fill < nst ? w.bytes : 0, kRsrcWord3);  // past the range: zeros, unread
+        const uint32_t o = k >= (fill == tail ? tail_k : 64) ? kOob : off;
+        uint8_t* to = lds + (dst >= 0 ? fill_at + dst : NS * T::STAGE);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)to, 16, o, 0, 0, 0);
+    };
+    auto issue_a = [&](int h) {
 #pragma unroll
         for (int i = 0; i < T::IA0 + T::IA1; ++i)
-            if ((i >= T::IA0) == (h == 1)) issue(xb, xbytes, offa[i], ka[i], dsta[i], st);
+            if ((i >= T::IA0) == (h == 1)) issue(xr, offa[i], ka[i], dsta[i]);
     };
-    auto issue_b = [&](int h, int st) {
+    auto issue_b = [&](int h) {
 #pragma unroll
         for (int i = 0; i < T::IB0 + T::IB1; ++i)
-            if ((i >= T::IB0) == (h == 1)) issue(wb[h], wbytes, offb[i], kb[i], dstb[i], st);
+            if ((i >= T::IB0) == (h == 1)) issue(wr[h], offb[i], kb[i], dstb[i]);
+    };
+    auto next_fill = [&]() {
+        xr = {xr.p + 64, xr.bytes - 128};
+        wr[0] = {wr[0].p + 64, wr[0].bytes - 128};
+        wr[1] = {wr[1].p + 64, wr[1].bytes - 128};
+        ++fill;
+        fill_at = fill_at + T::STAGE == NS * T::STAGE ? 0 : fill_at + T::STAGE;
     };
 
     v4f acc[MB][NB];
@@ -253,17 +287,18 @@ __global__ __launch_bounds__(512) void linear_tile_kernel(LinearFusedArgs a) {
     constexpr int kAhead = (NS - 2) * T::ALL;
 #pragma unroll
     for (int st = 0; st < NS; ++st) {
-        issue_a(0, st);
-        issue_b(0, st);
-        issue_b(1, st);
-        issue_a(1, st);
+        issue_a(0);
+        issue_b(0);
+        issue_b(1);
+        issue_a(1);
+        next_fill();
     }
     wait_vmcnt<T::IB1 + T::IA1 + T::ALL + kAhead>();  // A0, B0 of stage 0
     barrier();
     const bool lag = wave >= 4;
     if (lag) barrier();
     for (int st = 0; st < nst; ++st) {
-        const uint8_t* slot = lds + st % NS * T::STAGE;
+        const uint8_t* slot = lds + fill_at;  // the slot that is read is the one filled behind the reads
         const uint8_t* as = slot + wm * (16 * MB) * 128;
         const uint8_t* bs = slot + T::AB + wn * (16 * NB) * 128;
         // phase 0: rows 0, columns 0
@@ -286,8 +321,8 @@ __global__ __launch_bounds__(512) void linear_tile_kernel(LinearFusedArgs a) {
 #pragma unroll
             for (int j = 0; j < NB0; ++j) fb[1][j][ks] = frag(bs, 16 * (NB0 + j), ks);
         __builtin_amdgcn_sched_barrier(0);
-        issue_a(0, st + NS);
-        issue_b(0, st + NS);
+        issue_a(0);
+        issue_b(0);
         wait_vmcnt<T::ALL + T::IA0 + T::IB0 + kAhead>();  // A1
         wait_lgkmcnt0();
         barrier();
@@ -299,13 +334,14 @@ __global__ __launch_bounds__(512) void linear_tile_kernel(LinearFusedArgs a) {
 #pragma unroll
             for (int i = 0; i < MB1; ++i) fa[i][ks] = frag(as, 16 * (MB0 + i), ks);
         __builtin_amdgcn_sched_barrier(0);
-        issue_b(1, st + NS);
+        issue_b(1);
         wait_lgkmcnt0();
         barrier();
         mma(H1{}, H1{});
         barrier();
         // phase 3: rows 1, columns 0
-        issue_a(1, st + NS);
+        issue_a(1);
+        next_fill();
         __builtin_amdgcn_sched_barrier(0);
         wait_vmcnt<T::IB1 + T::IA1 + T::ALL + kAhead>();  // A0, B0 of the next stage
         barrier();
@@ -376,16 +412,18 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearFusedArgs a) {
 }
 
 // ---- up to 16 rows -------------------------------------------------------------
-// One workgroup of eight waves per 16 output columns; the waves take the 32-k
-// steps of K in turn, eight at a time, and read their weights straight into
-// fragments (64 bytes of each of 16 rows an instruction, the next ones following in the
-// same lines). The partial tiles are added through LDS in wave order. Bound by
-// the weights' bytes: what counts is how many are in flight (8 KB a wave).
-constexpr int RW = 8, RD = 8;
+// One workgroup of four waves per 16 output columns; the waves take the 32-k
+// steps of K in turn, RD at a time, and read their weights straight into
+// fragments (64 bytes of each of 16 rows an instruction, the next ones following
+// in the same lines), the next RD steps' loads in flight while these are
+// multiplied. The partial tiles are added through LDS in wave order. Bound by
+// the weights' bytes: what counts is how many of them are in flight.
+constexpr int RW = 4;
 
 template <bool XF32, bool GATED>
-__global__ __launch_bounds__(RW * 64) void linear_rows_kernel(LinearFusedArgs a) {
-    constexpr int NP = GATED ? 2 : 1;
+__global__ __launch_bounds__(RW * 64, 4) void linear_rows_kernel(LinearFusedArgs a) {
+    constexpr int NP = GATED ? 2 : 1, XV = XF32 ? 2 : 1;
+    constexpr int RD = NP + XV == 4 ? 2 : 4;  // 128 registers: four workgroups a CU
     __shared__ v4f red[NP][RW][64];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -398,42 +436,57 @@ __global__ __launch_bounds__(RW * 64) void linear_rows_kernel(LinearFusedArgs a)
     const __amdgpu_buffer_rsrc_t ru = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<uint16_t*>(GATED ? a.w_up + static_cast<int64_t>(n0) * a.ldw : a.w), 0,
         GATED ? static_cast<int>(wbytes) : 0, kRsrcWord3);
+    constexpr int XE = XF32 ? 4 : 2;
+    const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<void*>(XF32 ? a.x : static_cast<const void*>(a.x16)), 0,
+        static_cast<int>((static_cast<int64_t>(a.M - 1) * a.ldx + a.K) * XE), kRsrcWord3);
+    // rows past N or M and k past K read as zeros
     const uint32_t ow = r < rows_n ? static_cast<uint32_t>(r) * static_cast<uint32_t>(a.ldw) * 2u + kq * 16 : kOob;
-    const bool xrow = r < a.M;
+    const uint32_t ox = r < a.M ? static_cast<uint32_t>(r) * static_cast<uint32_t>(a.ldx) * XE + kq * 8 * XE : kOob;
 
     v4f acc[NP];
 #pragma unroll
     for (int p = 0; p < NP; ++p) acc[p] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
     const int steps = (a.K + 31) / 32;
-    for (int s0 = wave * RD; s0 < steps; s0 += RW * RD) {
-        v4i fw[NP][RD];
+    v4i fw[2][NP][RD], fx[2][XV][RD];
+    auto load = [&](int b, int s0) {
 #pragma unroll
         for (int d = 0; d < RD; ++d) {
-            const int k = (s0 + d) * 32 + 8 * kq;
-            const uint32_t o = k < a.K && ow != kOob ? ow + static_cast<uint32_t>(s0 + d) * 64 : kOob;
-            fw[0][d] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw, o, 0, 0));
-            if constexpr (GATED) fw[1][d] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(ru, o, 0, 0));
+            const uint32_t bad = (s0 + d) * 32 + 8 * kq < a.K ? 0u : kOob;
+            const uint32_t o = (ow + static_cast<uint32_t>(s0 + d) * 64) | (ow & kOob) | bad;
+            const uint32_t x = (ox + static_cast<uint32_t>(s0 + d) * (32 * XE)) | (ox & kOob) | bad;
+#pragma unroll
+            for (int v = 0; v < XV; ++v)
+                fx[b][v][d] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rx, x + 16 * v, 0, 0));
+            fw[b][0][d] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw, o, 0, 0));
+            if constexpr (GATED)
+                fw[b][NP - 1][d] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(ru, o, 0, 0));
         }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto multiply = [&](int b) {
 #pragma unroll
         for (int d = 0; d < RD; ++d) {
-            const int k = (s0 + d) * 32 + 8 * kq;
-            v8bf fx = __builtin_bit_cast(v8bf, (v4i){0, 0, 0, 0});
-            if (xrow && k < a.K) {
-                if constexpr (XF32) {
-                    const float* xp = static_cast<const float*>(a.x) + r * a.ldx + k;
-                    const v4f lo = *reinterpret_cast<const v4f*>(xp), hi = *reinterpret_cast<const v4f*>(xp + 4);
-                    fx = __builtin_bit_cast(v8bf, (v4i){static_cast<int>(pack_bf16x2(lo[0], lo[1])),
-                                                        static_cast<int>(pack_bf16x2(lo[2], lo[3])),
-                                                        static_cast<int>(pack_bf16x2(hi[0], hi[1])),
-                                                        static_cast<int>(pack_bf16x2(hi[2], hi[3]))});
-                } else {
-                    fx = *reinterpret_cast<const v8bf*>(a.x16 + r * a.ldx + k);
-                }
+            v8bf x = __builtin_bit_cast(v8bf, fx[b][0][d]);
+            if constexpr (XF32) {
+                const v4f lo = __builtin_bit_cast(v4f, fx[b][0][d]), hi = __builtin_bit_cast(v4f, fx[b][XV - 1][d]);
+                x = __builtin_bit_cast(v8bf, (v4i){static_cast<int>(pack_bf16x2(lo[0], lo[1])),
+                                                   static_cast<int>(pack_bf16x2(lo[2], lo[3])),
+                                                   static_cast<int>(pack_bf16x2(hi[0], hi[1])),
+                                                   static_cast<int>(pack_bf16x2(hi[2], hi[3]))});
             }
 #pragma unroll
             for (int p = 0; p < NP; ++p)
-                acc[p] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, fw[p][d]), fx, acc[p], 0, 0, 0);
+                acc[p] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, fw[b][p][d]), x, acc[p], 0, 0, 0);
         }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    load(0, wave * RD);
+    for (int s0 = wave * RD; s0 < steps; s0 += 2 * RW * RD) {
+        load(1, s0 + RW * RD);
+        multiply(0);
+        load(0, s0 + 2 * RW * RD);
+        multiply(1);
     }
 #pragma unroll
     for (int p = 0; p < NP; ++p) red[p][wave][lane] = acc[p];
@@ -452,6 +505,88 @@ __global__ __launch_bounds__(RW * 64) void linear_rows_kernel(LinearFusedArgs a)
     if (r >= a.M || n >= a.N) return;
     const float zz[4] = {z[0], z[1], z[2], z[3]}, uu[4] = {u[0], u[1], u[2], u[3]};
     finish4<GATED>(a, load_columns(a, n), r, n, zz, uu);
+}
+
+// ---- one or two rows -------------------------------------------------------------
+// A wave takes two weight rows (GATED: one of w and one of w_up) and all of K, 512
+// elements an instruction: whole KB reads of one row, eight of them in flight
+// for each, products on the vector unit (x rounded to bf16, fp32 sums per lane,
+// then over the lanes).
+template <bool XF32, bool GATED, int MM>
+__global__ __launch_bounds__(256, 2) void linear_gemv_kernel(LinearFusedArgs a) {
+    constexpr int U = 8, XE = XF32 ? 4 : 2, XV = XF32 ? 2 : 1;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = (blockIdx.x * 4 + wave) * (GATED ? 1 : 2);
+    if (n0 >= a.N) return;
+    const int n1 = min(n0 + 1, a.N - 1);
+    const int64_t row = static_cast<int64_t>(n0) * a.ldw;
+    const __amdgpu_buffer_rsrc_t rw[2] = {
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a.w + row), 0, a.K * 2, kRsrcWord3),
+        __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint16_t*>(GATED ? a.w_up + row : a.w + static_cast<int64_t>(n1) * a.ldw), 0, a.K * 2, kRsrcWord3)};
+    const uint8_t* xb = static_cast<const uint8_t*>(XF32 ? a.x : static_cast<const void*>(a.x16));
+    float s[2][MM];
+#pragma unroll
+    for (int m = 0; m < MM; ++m) s[0][m] = s[1][m] = 0.0f;
+    for (int k0 = 0; k0 < a.K; k0 += 512 * U) {
+        v4i w[2][U], x[MM][XV][U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = k0 + 512 * u + 8 * lane;  // past K: out of the row's range, zeros
+#pragma unroll
+            for (int m = 0; m < MM; ++m) {
+                const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(
+                    const_cast<uint8_t*>(xb + static_cast<int64_t>(m) * a.ldx * XE), 0, a.K * XE, kRsrcWord3);
+#pragma unroll
+                for (int v = 0; v < XV; ++v)
+                    x[m][v][u] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rx, k * XE + 16 * v, 0, 0));
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                w[i][u] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw[i], k * 2, 0, 0));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int m = 0; m < MM; ++m) {
+                uint32_t xp[4];  // eight bf16
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    if constexpr (XF32) {
+                        const v4f f = __builtin_bit_cast(v4f, x[m][c >> 1][u]);
+                        xp[c] = pack_bf16x2(f[2 * (c & 1)], f[2 * (c & 1) + 1]);
+                    } else {
+                        xp[c] = static_cast<uint32_t>(x[m][0][u][c]);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const uint32_t wp = static_cast<uint32_t>(w[i][u][c]);
+                        s[i][m] = __builtin_fmaf(__uint_as_float(xp[c] << 16), __uint_as_float(wp << 16), s[i][m]);
+                        s[i][m] = __builtin_fmaf(__uint_as_float(xp[c] & 0xffff0000u), __uint_as_float(wp & 0xffff0000u),
+                                                 s[i][m]);
+                    }
+            }
+    }
+#pragma unroll
+    for (int m = 0; m < MM; ++m) {
+        s[0][m] = wave_sum_dpp(s[0][m]);
+        s[1][m] = wave_sum_dpp(s[1][m]);
+    }
+    // lane: row lane / 2, column lane % 2 of the wave's
+    const int m = lane >> 1, c = GATED ? 0 : lane & 1;
+    if (m >= MM || n0 + c >= a.N || (GATED && (lane & 1))) return;
+    float z = s[0][0], u = s[1][0];
+    if constexpr (MM == 2) {
+        z = m ? s[0][1] : z;
+        u = m ? s[1][1] : u;
+    }
+    if (!GATED && c) z = u;
+    finish1<GATED>(a, m, n0 + c, z, u);
 }
 
 // rows of K values, fp32 or bf16, to bf16 rows of Kp >= K (a multiple of 8),
@@ -507,8 +642,9 @@ int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 }  // namespace
 
 // Tile and number of K splits: the least estimated time of the launch (us). A
-// workgroup's stage costs its MFMAs or its bytes through the CU's port to L2,
-// whichever is more; the parts of a split sum are written and read once.
+// stage of a tile takes 0.4 us and 1.2 us for each 256x256 of it (measured: 256x256
+// 1.6, 224x256 1.5, 160x256 1.2, 160x128 0.8, 128x128 0.7, 64x128 0.6); the parts
+// of a split sum are written and read once.
 LinearFusedPlan linear_fused_plan(int M, int K, int N, bool gated) {
     LinearFusedPlan best{};
     if (M <= kLinearRows) return best;
@@ -519,13 +655,13 @@ LinearFusedPlan linear_fused_plan(int M, int K, int N, bool gated) {
         for (int tn : tns) {
             const int tno = gated ? tn / 2 : tn;
             const int64_t tiles = static_cast<int64_t>((M + tm - 1) / tm) * ((N + tno - 1) / tno);
-            const double stage = std::max(tm * tn / 65536.0 * 1.7, (tm + tn) * 128 / 80e3) + 0.12;
+            const double stage = 0.4 + 1.2 * tm * tn / 65536.0;
             for (int s = 1; s <= 16 && s <= stages; ++s) {
                 const int per = (stages + s - 1) / s;
                 if (per * (s - 1) >= stages) continue;  // the last range would be empty
                 const double rounds = static_cast<double>((tiles * s + 255) / 256);
-                double t = rounds * (per * stage + 4.0);
-                if (s > 1) t += 4.0 + 2.0 * s * M * N * (gated ? 8.0 : 4.0) / 4e6;
+                double t = 3.0 + rounds * (per * stage + 3.0);
+                if (s > 1) t += 3.0 + 2.0 * s * M * N * (gated ? 8.0 : 4.0) / 5e6;
                 if (t < best_t) {
                     best_t = t;
                     best.tm = tm;
@@ -583,6 +719,22 @@ hipError_t launch_linear_fused(LinearFusedArgs a, int x_dtype, void* scratch, hi
     a.part_ld = static_cast<int64_t>((a.N + 3) / 4 * 4) * (gated ? 2 : 1);
     if (a.M <= kLinearRows) {
         a.splits = 1;
+        if (a.M <= kLinearGemvRows) {
+            const dim3 grid(gated ? (a.N + 3) / 4 : (a.N + 7) / 8), block(256);
+#define QIMG_GEMV(F32, GATED)                                                                        \
+    if (f32 == F32 && gated == GATED) {                                                              \
+        if (a.M == 1)                                                                                \
+            hipLaunchKernelGGL((linear_gemv_kernel<F32, GATED, 1>), grid, block, 0, stream, a);      \
+        else                                                                                         \
+            hipLaunchKernelGGL((linear_gemv_kernel<F32, GATED, 2>), grid, block, 0, stream, a);      \
+    }
+            QIMG_GEMV(true, true)
+            QIMG_GEMV(true, false)
+            QIMG_GEMV(false, true)
+            QIMG_GEMV(false, false)
+#undef QIMG_GEMV
+            return hipGetLastError();
+        }
         const dim3 grid((a.N + 15) / 16), block(RW * 64);
         if (f32 && gated)
             hipLaunchKernelGGL((linear_rows_kernel<true, true>), grid, block, 0, stream, a);

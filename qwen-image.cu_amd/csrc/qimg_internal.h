@@ -367,6 +367,7 @@ struct LinearFusedArgs {
     float* part;               // [splits, M, part_ld] with splits > 1
     int64_t part_ld;
 };
+constexpr int kLinearGemvRows = 2;  // most rows of the vector-unit kernel
 constexpr int kLinearRows = 16;  // most rows of the kernel that reads weights straight into fragments
 struct LinearFusedPlan {
     int tm, tn, splits, split_stages;
