@@ -309,6 +309,35 @@ typedef struct {
 int64_t qimg_linear_bf16_fused_scratch_bytes(int x_dtype, int M, int K, int N, int gated);
 int qimg_linear_bf16_fused(const qimg_linear_fused* args, void* scratch, int64_t scratch_bytes, void* stream);
 
+/* ---- prompts: rotary positions ------------------------------------------- */
+
+/* Rotary positions of packed heads (the joint block's own are in
+ * qimg_joint_heads_f16): of each token's n_heads heads of head_dim values in
+ * x, the first n_rotated are turned in their first rotary_dim values,
+ *   (a, b) -> (a cos - b sin, b cos + a sin),
+ * with a, b the values (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with
+ * interleaved != 0; the others are copied (the v heads of a packed [T, (Hq +
+ * 2 Hk) D] projection). x and out QIMG_FP32, QIMG_BF16 or QIMG_FP16, each with
+ * strides in elements between tokens and heads (multiples of 8, the last
+ * dimension contiguous); fp32 arithmetic, one rounding. cos_sin fp32
+ * [table_rows, rotary_dim / 2, 2] (cos, sin); positions int32 [tokens] on the
+ * device: the token's table row. A token whose position lies outside [0,
+ * table_rows) is not written. head_dim and rotary_dim multiples of 8. out may
+ * be x (same type and strides), else does not overlap it. */
+typedef struct {
+    const void* x;
+    int x_dtype;
+    int64_t x_stride_t, x_stride_h;
+    void* out;
+    int out_dtype;
+    int64_t out_stride_t, out_stride_h;
+    int tokens, n_heads, n_rotated, head_dim, rotary_dim, interleaved;
+    const float* cos_sin;
+    int table_rows;
+    const int32_t* positions;
+} qimg_rope;
+int qimg_rope_packed(const qimg_rope* args, void* stream);
+
 /* ---- MMDiT joint block: the operations around the hot path ------------ */
 
 /* silu_fp32 (cuda_kernels.cu:1881-1893): out[i] = x[i] / (1 + exp(-x[i])). */

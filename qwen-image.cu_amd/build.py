@@ -48,7 +48,8 @@ HIP_FLAGS = [
 
 SOURCES = ["hadamard_quant.hip", "gemm_w8a8.hip", "gemm_small_m.hip", "gemm_bf16.hip", "sage_attention.hip", "block_ops.hip",
            "mmdit_block.hip", "capi.hip", "linear_noalloc.hip", "int4.hip", "capi_int4.hip",
-           "attention_varlen.hip", "gemm_fused.hip", "capi_prompt.hip"]
+           "attention_varlen.hip", "gemm_fused.hip", "rope_packed.hip",
+           "capi_prompt.hip"]
 # MFMA results in vector registers: with the accumulators in AGPRs the compiler
 # copies them back and forth around every rescale of the online softmax.
 SOURCE_FLAGS = {"attention_varlen.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form=1")}

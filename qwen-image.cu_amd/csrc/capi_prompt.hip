@@ -145,4 +145,42 @@ int qimg_linear_bf16_fused(const qimg_linear_fused* args, void* scratch, int64_t
     return qimg::api_hip_status(qimg::launch_linear_fused(a, p.x_dtype, scratch, static_cast<hipStream_t>(stream)), fn);
 }
 
+int qimg_rope_packed(const qimg_rope* args, void* stream) {
+    const char* fn = "qimg_rope_packed";
+    QIMG_REQUIRE(args, "%s: args is null", fn);
+    const qimg_rope& p = *args;
+    const auto float_type = [](int t) { return t == QIMG_FP32 || t == QIMG_BF16 || t == QIMG_FP16; };
+    QIMG_REQUIRE(float_type(p.x_dtype) && float_type(p.out_dtype), "%s: dtypes %d and %d must be FP32, BF16 or FP16", fn,
+                 p.x_dtype, p.out_dtype);
+    QIMG_REQUIRE(p.tokens >= 0 && p.n_heads >= 0 && p.n_rotated >= 0 && p.n_rotated <= p.n_heads && p.table_rows >= 0,
+                 "%s: bad sizes tokens=%d n_heads=%d n_rotated=%d table_rows=%d", fn, p.tokens, p.n_heads, p.n_rotated,
+                 p.table_rows);
+    QIMG_REQUIRE(p.head_dim > 0 && p.rotary_dim > 0 && p.rotary_dim <= p.head_dim,
+                 "%s: need 0 < rotary_dim <= head_dim (rotary_dim=%d head_dim=%d)", fn, p.rotary_dim, p.head_dim);
+    if (p.head_dim % 8 != 0 || p.rotary_dim % 8 != 0)
+        return qimg::api_fail(QIMG_ERR_UNSUPPORTED, "%s: head_dim %d and rotary_dim %d must be multiples of 8", fn,
+                              p.head_dim, p.rotary_dim);
+    QIMG_REQUIRE(good_strides(p.x_stride_t, p.x_stride_h) && good_strides(p.out_stride_t, p.out_stride_h),
+                 "%s: strides must be non-negative multiples of 8, token strides at most 2^24", fn);
+    QIMG_REQUIRE(static_cast<int64_t>(p.tokens) * p.n_heads * (p.head_dim / 8) < (int64_t{1} << 38), "%s: too many values",
+                 fn);
+    if (p.tokens == 0 || p.n_heads == 0) return QIMG_OK;
+    QIMG_REQUIRE(p.x && p.out && p.positions && (p.cos_sin || p.table_rows == 0), "%s: null pointer", fn);
+    QIMG_REQUIRE(aligned16(p.x) && aligned16(p.out) && aligned16(p.cos_sin),
+                 "%s: x, out and cos_sin must be 16-byte aligned", fn);
+    QIMG_REQUIRE((p.tokens == 1 || p.out_stride_t >= p.head_dim) && (p.n_heads == 1 || p.out_stride_h >= p.head_dim),
+                 "%s: out strides must be at least head_dim", fn);
+    QIMG_REQUIRE(p.out != p.x || (p.out_dtype == p.x_dtype && p.out_stride_t == p.x_stride_t &&
+                                  p.out_stride_h == p.x_stride_h),
+                 "%s: out in x's place must have its type and strides", fn);
+    qimg::RopeArgs a{};
+    a.x = p.x, a.out = p.out;
+    a.x_t = p.x_stride_t, a.x_h = p.x_stride_h, a.o_t = p.out_stride_t, a.o_h = p.out_stride_h;
+    a.tokens = p.tokens, a.h = p.n_heads, a.h_rot = p.n_rotated, a.d = p.head_dim, a.r = p.rotary_dim;
+    a.interleaved = p.interleaved != 0;
+    a.table = p.cos_sin, a.table_rows = p.table_rows, a.positions = p.positions;
+    return qimg::api_hip_status(
+        qimg::launch_rope_packed(a, p.x_dtype, p.out_dtype, static_cast<hipStream_t>(stream)), fn);
+}
+
 }  // extern "C"

@@ -643,14 +643,19 @@ int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 
 // Tile and number of K splits: the least estimated time of the launch (us). A
 // stage of a tile takes 0.4 us and 1.2 us for each 256x256 of it (measured: 256x256
-// 1.6, 224x256 1.5, 160x256 1.2, 160x128 0.8, 128x128 0.7, 64x128 0.6); the parts
-// of a split sum are written and read once.
-LinearFusedPlan linear_fused_plan(int M, int K, int N, bool gated) {
-    LinearFusedPlan best{};
-    if (M <= kLinearRows) return best;
+// 1.6, 224x256 1.5, 160x256 1.2, 160x128 0.8, 128x128 0.7, 64x128 0.6), the weights
+// come at 4.8 TB/s at best, the parts of a split sum are written and read once. linear_rows_kernel takes about 4 us and
+// the weights' bytes at 3 TB/s: it is the faster one below some 16 M weights
+// (16 rows, us, rows / tiles: 3584x3584 10.6 / 13.2, 4608x3584 17.1 / 14.7,
+// 3584x14336 34.8 / 26.9, gated 14336x3584 53.4 / 39.2); fp32 rows spare it a
+// packing launch of 3 us.
+LinearFusedPlan linear_fused_plan(int x_dtype, int M, int K, int N, bool gated) {
+    LinearFusedPlan best{};  // tm = 0: linear_gemv_kernel or linear_rows_kernel
+    if (M <= kLinearGemvRows) return best;
     static const int tms[] = {256, 224, 192, 160, 128, 64}, tns[] = {256, 128};
     const int stages = (K + 63) / 64;
-    double best_t = 1e30;
+    const double bytes = 2.0 * N * K * (gated ? 2 : 1);  // of weights
+    double best_t = M <= kLinearRows ? 4.0 + bytes / 3e6 - (x_dtype == QIMG_FP32 ? 3.0 : 0.0) : 1e30;
     for (int tm : tms)
         for (int tn : tns) {
             const int tno = gated ? tn / 2 : tn;
@@ -660,7 +665,7 @@ LinearFusedPlan linear_fused_plan(int M, int K, int N, bool gated) {
                 const int per = (stages + s - 1) / s;
                 if (per * (s - 1) >= stages) continue;  // the last range would be empty
                 const double rounds = static_cast<double>((tiles * s + 255) / 256);
-                double t = 3.0 + rounds * (per * stage + 3.0);
+                double t = 3.0 + std::max(rounds * (per * stage + 3.0), bytes / 4.8e6 + 3.0);
                 if (s > 1) t += 3.0 + 2.0 * s * M * N * (gated ? 8.0 : 4.0) / 5e6;
                 if (t < best_t) {
                     best_t = t;
@@ -680,10 +685,10 @@ LinearFusedScratch linear_fused_scratch(int x_dtype, int M, int K, int N, bool g
     if (M <= 0 || K <= 0 || N <= 0) return s;
     const int Kp = (K + 7) / 8 * 8;
     const bool odd = Kp != K;
-    if (odd || (x_dtype == QIMG_FP32 && M > kLinearRows)) s.x = align256(static_cast<int64_t>(M) * Kp * 2);
+    const LinearFusedPlan p = linear_fused_plan(x_dtype, M, K, N, gated);
+    if (odd || (x_dtype == QIMG_FP32 && p.tm != 0)) s.x = align256(static_cast<int64_t>(M) * Kp * 2);
     if (odd) s.w = align256(static_cast<int64_t>(N) * Kp * 2);
     if (odd && gated) s.w_up = s.w;
-    const LinearFusedPlan p = linear_fused_plan(M, K, N, gated);
     if (p.splits > 1) s.part = align256(static_cast<int64_t>(p.splits) * M * ((N + 3) / 4 * 4) * (gated ? 8 : 4));
     return s;
 }
@@ -691,6 +696,7 @@ LinearFusedScratch linear_fused_scratch(int x_dtype, int M, int K, int N, bool g
 hipError_t launch_linear_fused(LinearFusedArgs a, int x_dtype, void* scratch, hipStream_t stream) {
     const bool gated = a.w_up != nullptr;
     const LinearFusedScratch s = linear_fused_scratch(x_dtype, a.M, a.K, a.N, gated);
+    const LinearFusedPlan plan = linear_fused_plan(x_dtype, a.M, a.K, a.N, gated);
     uint8_t* p = static_cast<uint8_t*>(scratch);
     const int Kp = (a.K + 7) / 8 * 8;
     bool f32 = x_dtype == QIMG_FP32;
@@ -717,7 +723,7 @@ hipError_t launch_linear_fused(LinearFusedArgs a, int x_dtype, void* scratch, hi
     if (s.w) a.ldw = a.K = Kp;
     a.part = reinterpret_cast<float*>(p);
     a.part_ld = static_cast<int64_t>((a.N + 3) / 4 * 4) * (gated ? 2 : 1);
-    if (a.M <= kLinearRows) {
+    if (plan.tm == 0) {
         a.splits = 1;
         if (a.M <= kLinearGemvRows) {
             const dim3 grid(gated ? (a.N + 3) / 4 : (a.N + 7) / 8), block(256);
@@ -746,7 +752,6 @@ hipError_t launch_linear_fused(LinearFusedArgs a, int x_dtype, void* scratch, hi
             hipLaunchKernelGGL((linear_rows_kernel<false, false>), grid, block, 0, stream, a);
         return hipGetLastError();
     }
-    const LinearFusedPlan plan = linear_fused_plan(a.M, a.K, a.N, gated);
     a.splits = plan.splits;
     a.split_stages = plan.split_stages;
 #define QIMG_TILE(TM, TN)                                                                       \

@@ -375,8 +375,20 @@ struct LinearFusedPlan {
 struct LinearFusedScratch {
     int64_t x, w, w_up, part;
 };
-LinearFusedPlan linear_fused_plan(int M, int K, int N, bool gated);
+LinearFusedPlan linear_fused_plan(int x_dtype, int M, int K, int N, bool gated);
 LinearFusedScratch linear_fused_scratch(int x_dtype, int M, int K, int N, bool gated);
 hipError_t launch_linear_fused(LinearFusedArgs a, int x_dtype, void* scratch, hipStream_t stream);
+
+// rope_packed.hip: rotary positions of packed heads (qimg_rope_packed), strides in elements
+struct RopeArgs {
+    const void* x;
+    void* out;
+    int64_t x_t, x_h, o_t, o_h;
+    int tokens, h, h_rot, d, r, interleaved;
+    const float* table;  // [table_rows, r / 2, 2]: cos, sin
+    int table_rows;
+    const int* positions;  // [tokens]
+};
+hipError_t launch_rope_packed(const RopeArgs& a, int x_dtype, int out_dtype, hipStream_t stream);
 
 }  // namespace qimg

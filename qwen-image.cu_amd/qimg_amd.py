@@ -71,6 +71,7 @@ _SIGS = {
     "qimg_attention_varlen": (_I, [_P, _P, _I64, _P]),
     "qimg_linear_bf16_fused_scratch_bytes": (_I64, [_I, _I, _I, _I, _I]),
     "qimg_linear_bf16_fused": (_I, [_P, _P, _I64, _P]),
+    "qimg_rope_packed": (_I, [_P, _P]),
     "qimg_silu": (_I, [_P, _P, _I64, _P]),
     "qimg_layernorm_modulate": (_I, [_P, _P, _P, _P, _I, _I, _F, _P]),
     "qimg_layernorm_modulate_quant": (_I, [_P, _P, _P, _I, _I, _I, _I, _F, _P, _P, _P]),
@@ -724,6 +725,7 @@ def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     return out
 
 
+_HEAD_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 ACTIVATIONS = {"none": 0, "gelu": 1, "silu": 2}
 
 
@@ -784,6 +786,43 @@ def linear_forward_bf16_fused(x: torch.Tensor, weight: torch.Tensor, bias: torch
                             N if residual is None else _row_stride(residual, N), _addr(out), _DT[out.dtype],
                             _row_stride(out, N))
         _check(_lib.qimg_linear_bf16_fused(ctypes.byref(args), _addr(scratch), _nbytes(scratch), _raw_stream(x.device)))
+    return out
+
+
+class _Rope(ctypes.Structure):
+    _fields_ = [("x", _P), ("x_dtype", _I), ("x_stride_t", _I64), ("x_stride_h", _I64), ("out", _P), ("out_dtype", _I),
+                ("out_stride_t", _I64), ("out_stride_h", _I64), ("tokens", _I), ("n_heads", _I), ("n_rotated", _I),
+                ("head_dim", _I), ("rotary_dim", _I), ("interleaved", _I), ("cos_sin", _P), ("table_rows", _I),
+                ("positions", _P)]
+
+
+def rope_packed(x: torch.Tensor, cos_sin: torch.Tensor, positions: torch.Tensor, n_rotated: int,
+                interleaved: bool = False, out: torch.Tensor | None = None, out_dtype=None) -> torch.Tensor:
+    """Rotary positions of packed heads: x [T, H, D] (fp32, bf16 or fp16; any
+    token and head strides that are multiples of 8), the first n_rotated heads
+    turned in their first R values by row positions[t] of cos_sin fp32
+    [P, R / 2, 2], the rest copied. Pairs are (i, i + R / 2), or (2 i, 2 i + 1)
+    interleaved. A token whose position lies outside the table is not written.
+    out may be x; its type defaults to x's."""
+    if not (x.is_cuda and x.dim() == 3 and x.stride(2) == 1):
+        raise QimgError(QIMG_ERR_INVALID_ARG, "x must be a device tensor [T, H, D], its last dimension contiguous")
+    _same_device(x, cos_sin=cos_sin, positions=positions, out=out)
+    T, H, D = x.shape
+    if out is None:
+        out = torch.empty((T, H, D), dtype=out_dtype or x.dtype, device=x.device)
+    elif out.shape != x.shape or out.stride(2) != 1:
+        raise QimgError(QIMG_ERR_INVALID_ARG, f"out must be {tuple(x.shape)}, its last dimension contiguous")
+    if x.dtype not in _HEAD_TYPES or out.dtype not in _HEAD_TYPES:
+        raise QimgError(QIMG_ERR_INVALID_ARG, "x and out must be float32, bfloat16 or float16")
+    if cos_sin.dtype != torch.float32 or cos_sin.dim() != 3 or cos_sin.shape[2] != 2 or not cos_sin.is_contiguous():
+        raise QimgError(QIMG_ERR_INVALID_ARG, "cos_sin must be contiguous float32 [P, R / 2, 2]")
+    if positions.dtype != torch.int32 or positions.numel() != T or not positions.is_contiguous():
+        raise QimgError(QIMG_ERR_INVALID_ARG, f"positions must be contiguous int32 of {T} elements")
+    sx, so = x.stride(), out.stride()
+    with _on(x.device):
+        args = _Rope(_addr(x), _DT[x.dtype], sx[0], sx[1], _addr(out), _DT[out.dtype], so[0], so[1], T, H, n_rotated, D,
+                     2 * cos_sin.shape[1], bool(interleaved), _addr(cos_sin), cos_sin.shape[0], _addr(positions))
+        _check(_lib.qimg_rope_packed(ctypes.byref(args), _raw_stream(x.device)))
     return out
 
 
