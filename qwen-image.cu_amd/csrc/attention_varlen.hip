@@ -622,8 +622,9 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnVarlenArgs a) {
 // tile p, and a matrix phase, M(p): O += V P of tile p - 1, then the scores of
 // tile p. Two workgroups share a CU (64 KB of LDS, two waves a SIMD), so one's
 // exponentials run beside the other's MFMAs. V begins with the fragment reads of
-// the next M's first MFMAs, M reads two groups of four fragments ahead (three
-// buffers), so no MFMA waits for its LDS reads' full latency.
+// the next M's first MFMAs, M reads a group of four fragments ahead. (Two groups
+// ahead, with a third buffer, measured 1-2% slower, without the matrix phase's
+// priority 2 x 24 heads of 4352 took 2% more, 1301 tokens 20% more.)
 constexpr int MR = 128, MW = 4, MK = 64, MSLOT = 2;
 
 // The K or V tiles of one head in turn: `p` the next tile's first row, `left`
@@ -674,7 +675,7 @@ struct Many {
     static constexpr int PER = 2 * TB / 1024 / MW;  // DMA instructions per wave and pair
     static constexpr int NPV = 2 * KB * DT / 4, NG = NPV + KB * KS / 4;  // groups of four MFMAs: PV, all
     v16f o[DT], s[KB];
-    frag qf[KS], buf[3][4];
+    frag qf[KS], buf[2][4];
     uint32_t pk[8 * KB];  // P: 16-key group g at pk[4 g ..]
     int voff[DT], koff[KS];  // lane offsets of V reads (channel block), K reads (k-step)
     float m, sum;
@@ -718,22 +719,22 @@ struct Many {
     template <int j, bool MASKED>
     __device__ __forceinline__ void m_groups(const uint8_t* src, bool& bad) {
         if constexpr (j < NG) {
-            if constexpr (j + 2 < NG) read_group<j + 2>(src, buf[(j + 2) % 3]);
+            if constexpr (j + 1 < NG) read_group<j + 1>(src, buf[(j + 1) % 2]);
             if constexpr (MASKED && j < NPV) {
                 bool b = false;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) b |= has_nonfinite<T>(buf[j % 3][i]);
+                for (int i = 0; i < 4; ++i) b |= has_nonfinite<T>(buf[j % 2][i]);
                 if (__ballot(b)) {
                     bad = true;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) buf[j % 3][i] = sanitize<T>(buf[j % 3][i]);
+                    for (int i = 0; i < 4; ++i) buf[j % 2][i] = sanitize<T>(buf[j % 2][i]);
                 }
             }
             if constexpr (j == NPV) {
 #pragma unroll
                 for (int r = 0; r < 16 * KB; ++r) s[r >> 4][r & 15] = 0.0f;
             }
-            mma_group<j>(buf[j % 3]);
+            mma_group<j>(buf[j % 2]);
             __builtin_amdgcn_sched_barrier(0);
             m_groups<j + 1, MASKED>(src, bad);
         }
@@ -741,8 +742,8 @@ struct Many {
     template <int j>
     __device__ __forceinline__ void first_scores(const uint8_t* src) {
         if constexpr (j < NG) {
-            read_group<j>(src, buf[j % 3]);
-            mma_group<j>(buf[j % 3]);
+            read_group<j>(src, buf[j % 2]);
+            mma_group<j>(buf[j % 2]);
             first_scores<j + 1>(src);
         }
     }
@@ -805,7 +806,6 @@ __device__ __forceinline__ void many_step(Many<T, D>& w, const uint8_t* __restri
     wait_vmcnt<W::PER>();
     phase_barrier();
     w.template read_group<0>(src, w.buf[0]);
-    w.template read_group<1>(src, w.buf[1]);
     __builtin_amdgcn_sched_barrier(0);
     w.template softmax<MASKED>(p * MK, kmax, scale);
     // P is made in this phase: left to itself the compiler moves the
