@@ -170,8 +170,9 @@ __device__ __forceinline__ RowTile find_tile(const AttnVarlenArgs& a, int idx, i
             if (lane >= off) incl += v;
         }
         const int total = __builtin_amdgcn_readlane(incl, 63);
-        if (idx < before + total) {
-            const int src = __builtin_ctzll(__ballot(before + incl > idx));
+        const uint64_t hit = __ballot(before + incl > idx);
+        if (idx < before + total && hit != 0) {
+            const int src = __builtin_ctzll(hit);
             t.q0 = __builtin_amdgcn_readlane(s.q0, src);
             t.lq = __builtin_amdgcn_readlane(s.lq, src);
             t.k0 = __builtin_amdgcn_readlane(s.k0, src);
@@ -179,6 +180,7 @@ __device__ __forceinline__ RowTile find_tile(const AttnVarlenArgs& a, int idx, i
             t.splits = __builtin_amdgcn_readlane(parts, src);
             const int cnt = __builtin_amdgcn_readlane(n, src);
             const int i = idx - (before + __builtin_amdgcn_readlane(incl, src) - cnt * t.splits);
+            if (i < 0 || i >= cnt * t.splits) return t;  // (sums past 2^31: offsets that overlap many times)
             const int tile = i / t.splits;
             t.split = i % t.splits;
             t.row0 = (a.causal ? cnt - 1 - tile : tile) * rows;

@@ -677,6 +677,15 @@ def _nbytes(t: torch.Tensor | None) -> int:
     return 0 if t is None else t.numel() * t.element_size()
 
 
+def _head_strides(t: torch.Tensor):
+    """Token and head strides of [T, H, D] (a dimension of one element has none of its own)."""
+    T, H, D = t.shape
+    st, sh, last = t.stride()
+    if last != 1 and D > 1:
+        raise QimgError(QIMG_ERR_INVALID_ARG, "the last dimension of [T, H, D] tensors must be contiguous")
+    return (st if T > 1 else H * D), (sh if H > 1 else D)
+
+
 def attention_varlen_scratch_bytes(total_q: int, total_k: int, batch: int, n_heads: int, n_kv_heads: int,
                                    head_dim: int) -> int:
     return int(_lib.qimg_attention_varlen_scratch_bytes(total_q, total_k, batch, n_heads, n_kv_heads, head_dim))
@@ -713,13 +722,10 @@ def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         out = torch.empty((tq, hq, d), dtype=dt, device=q.device)
     elif out.shape != q.shape or out.dtype != dt:
         raise QimgError(QIMG_ERR_INVALID_ARG, f"out must be {tuple(q.shape)} of q's type")
-    sq, sk, sv, so = q.stride(), k.stride(), v.stride(), out.stride()
-    if not (sq[2] == 1 and sk[2] == 1 and sv[2] == 1 and so[2] == 1):
-        raise QimgError(QIMG_ERR_INVALID_ARG, "the last dimension of q, k, v and out must be contiguous")
     with _on(q.device):
         scratch = _scratch_for(_lib.qimg_attention_varlen_scratch_bytes(tq, tk, batch, hq, hk, d), scratch, q.device)
-        args = _AttnVarlen(_addr(q), _addr(k), _addr(v), _addr(out), _DT[dt], sq[0], sq[1], sk[0], sk[1], sv[0], sv[1],
-                           so[0], so[1], _addr(cu_seqlens_q), _addr(cu_seqlens_k), _addr(k_lens), batch, tq, tk, hq, hk,
+        args = _AttnVarlen(_addr(q), _addr(k), _addr(v), _addr(out), _DT[dt], *_head_strides(q), *_head_strides(k),
+                           *_head_strides(v), *_head_strides(out), _addr(cu_seqlens_q), _addr(cu_seqlens_k), _addr(k_lens), batch, tq, tk, hq, hk,
                            d, 1.0 / d ** 0.5 if sm_scale is None else sm_scale, bool(causal))
         _check(_lib.qimg_attention_varlen(ctypes.byref(args), _addr(scratch), _nbytes(scratch), _raw_stream(q.device)))
     return out
@@ -804,23 +810,22 @@ def rope_packed(x: torch.Tensor, cos_sin: torch.Tensor, positions: torch.Tensor,
     [P, R / 2, 2], the rest copied. Pairs are (i, i + R / 2), or (2 i, 2 i + 1)
     interleaved. A token whose position lies outside the table is not written.
     out may be x; its type defaults to x's."""
-    if not (x.is_cuda and x.dim() == 3 and x.stride(2) == 1):
-        raise QimgError(QIMG_ERR_INVALID_ARG, "x must be a device tensor [T, H, D], its last dimension contiguous")
+    if not (x.is_cuda and x.dim() == 3):
+        raise QimgError(QIMG_ERR_INVALID_ARG, "x must be a device tensor [T, H, D]")
     _same_device(x, cos_sin=cos_sin, positions=positions, out=out)
     T, H, D = x.shape
     if out is None:
         out = torch.empty((T, H, D), dtype=out_dtype or x.dtype, device=x.device)
-    elif out.shape != x.shape or out.stride(2) != 1:
-        raise QimgError(QIMG_ERR_INVALID_ARG, f"out must be {tuple(x.shape)}, its last dimension contiguous")
+    elif out.shape != x.shape:
+        raise QimgError(QIMG_ERR_INVALID_ARG, f"out must be {tuple(x.shape)}")
     if x.dtype not in _HEAD_TYPES or out.dtype not in _HEAD_TYPES:
         raise QimgError(QIMG_ERR_INVALID_ARG, "x and out must be float32, bfloat16 or float16")
     if cos_sin.dtype != torch.float32 or cos_sin.dim() != 3 or cos_sin.shape[2] != 2 or not cos_sin.is_contiguous():
         raise QimgError(QIMG_ERR_INVALID_ARG, "cos_sin must be contiguous float32 [P, R / 2, 2]")
     if positions.dtype != torch.int32 or positions.numel() != T or not positions.is_contiguous():
         raise QimgError(QIMG_ERR_INVALID_ARG, f"positions must be contiguous int32 of {T} elements")
-    sx, so = x.stride(), out.stride()
     with _on(x.device):
-        args = _Rope(_addr(x), _DT[x.dtype], sx[0], sx[1], _addr(out), _DT[out.dtype], so[0], so[1], T, H, n_rotated, D,
+        args = _Rope(_addr(x), _DT[x.dtype], *_head_strides(x), _addr(out), _DT[out.dtype], *_head_strides(out), T, H, n_rotated, D,
                      2 * cos_sin.shape[1], bool(interleaved), _addr(cos_sin), cos_sin.shape[0], _addr(positions))
         _check(_lib.qimg_rope_packed(ctypes.byref(args), _raw_stream(x.device)))
     return out
