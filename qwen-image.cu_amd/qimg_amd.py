@@ -628,10 +628,10 @@ class _AttnVarlen(ctypes.Structure):
                 ("head_dim", _I), ("sm_scale", _F), ("causal", _I)]
 
 
-def _same_device(ref: torch.Tensor, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != ref.device:
-            raise QimgError(QIMG_ERR_INVALID_ARG, f"{name} must be a tensor on {ref.device}")
+def _same_device(device, *tensors):
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise QimgError(QIMG_ERR_INVALID_ARG, f"every tensor must be on {device}, the first argument's device")
 
 
 class _NoSwitch:
@@ -677,9 +677,8 @@ def _nbytes(t: torch.Tensor | None) -> int:
     return 0 if t is None else t.numel() * t.element_size()
 
 
-def _head_strides(t: torch.Tensor):
+def _head_strides(t: torch.Tensor, T: int, H: int, D: int):
     """Token and head strides of [T, H, D] (a dimension of one element has none of its own)."""
-    T, H, D = t.shape
     st, sh, last = t.stride()
     if last != 1 and D > 1:
         raise QimgError(QIMG_ERR_INVALID_ARG, "the last dimension of [T, H, D] tensors must be contiguous")
@@ -704,8 +703,8 @@ def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     no sequence are not written. sm_scale defaults to 1 / sqrt(D)."""
     if not (q.is_cuda and q.dim() == 3 and k.dim() == 3 and v.dim() == 3):
         raise QimgError(QIMG_ERR_INVALID_ARG, "q, k and v must be device tensors [T, H, D]")
-    _same_device(q, k=k, v=v, cu_seqlens_q=cu_seqlens_q, cu_seqlens_k=cu_seqlens_k, k_lens=k_lens, out=out)
-    dt = q.dtype
+    dev, dt = q.device, q.dtype
+    _same_device(dev, k, v, cu_seqlens_q, cu_seqlens_k, k_lens, out)
     if dt not in (torch.bfloat16, torch.float16) or k.dtype != dt or v.dtype != dt:
         raise QimgError(QIMG_ERR_INVALID_ARG, "q, k and v must be all bfloat16 or all float16")
     tq, hq, d = q.shape
@@ -719,15 +718,16 @@ def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
             raise QimgError(QIMG_ERR_INVALID_ARG, "cu_seqlens_q, cu_seqlens_k and k_lens must be contiguous int32")
     if out is None:
-        out = torch.empty((tq, hq, d), dtype=dt, device=q.device)
+        out = q.new_empty((tq, hq, d))
     elif out.shape != q.shape or out.dtype != dt:
         raise QimgError(QIMG_ERR_INVALID_ARG, f"out must be {tuple(q.shape)} of q's type")
-    with _on(q.device):
-        scratch = _scratch_for(_lib.qimg_attention_varlen_scratch_bytes(tq, tk, batch, hq, hk, d), scratch, q.device)
-        args = _AttnVarlen(_addr(q), _addr(k), _addr(v), _addr(out), _DT[dt], *_head_strides(q), *_head_strides(k),
-                           *_head_strides(v), *_head_strides(out), _addr(cu_seqlens_q), _addr(cu_seqlens_k), _addr(k_lens), batch, tq, tk, hq, hk,
+    with _on(dev):
+        scratch = _scratch_for(_lib.qimg_attention_varlen_scratch_bytes(tq, tk, batch, hq, hk, d), scratch, dev)
+        args = _AttnVarlen(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _DT[dt],
+                           *_head_strides(q, tq, hq, d), *_head_strides(k, tk, hk, d), *_head_strides(v, tk, hk, d),
+                           *_head_strides(out, tq, hq, d), _addr(cu_seqlens_q), _addr(cu_seqlens_k), _addr(k_lens), batch, tq, tk, hq, hk,
                            d, 1.0 / d ** 0.5 if sm_scale is None else sm_scale, bool(causal))
-        _check(_lib.qimg_attention_varlen(ctypes.byref(args), _addr(scratch), _nbytes(scratch), _raw_stream(q.device)))
+        _check(_lib.qimg_attention_varlen(ctypes.byref(args), _addr(scratch), _nbytes(scratch), _raw_stream(dev)))
     return out
 
 
@@ -757,8 +757,8 @@ def linear_forward_bf16_fused(x: torch.Tensor, weight: torch.Tensor, bias: torch
     "gelu" (tanh form) or "silu"."""
     if not (x.is_cuda and x.dim() == 2 and weight.dim() == 2):
         raise QimgError(QIMG_ERR_INVALID_ARG, "x and weight must be device tensors of two dimensions")
-    _same_device(x, weight=weight, bias=bias, weight_up=weight_up, bias_up=bias_up, gate=gate, residual=residual,
-                 out=out)
+    dev = x.device
+    _same_device(dev, weight, bias, weight_up, bias_up, gate, residual, out)
     M, K = x.shape
     N = weight.shape[0]
     if weight.shape[1] != K:
@@ -784,14 +784,15 @@ def linear_forward_bf16_fused(x: torch.Tensor, weight: torch.Tensor, bias: torch
             raise QimgError(QIMG_ERR_INVALID_ARG, f"{name} must be float32 or bfloat16 [{M}, {N}] with contiguous rows")
     if K > 1 and x.stride(1) != 1:
         raise QimgError(QIMG_ERR_INVALID_ARG, "rows of x must be contiguous")
-    with _on(x.device):
-        scratch = _scratch_for(linear_bf16_fused_scratch_bytes(x.dtype, M, K, N, weight_up is not None), scratch, x.device)
+    with _on(dev):
+        scratch = _scratch_for(_lib.qimg_linear_bf16_fused_scratch_bytes(_DT[x.dtype], M, K, N, weight_up is not None),
+                               scratch, dev)
         args = _LinearFused(_addr(x), _DT[x.dtype], _row_stride(x, K), M, N, K, _addr(weight), _addr(weight_up),
                             _addr(bias), _addr(bias_up), ACTIVATIONS[activation], _addr(gate), _addr(residual),
                             FP32 if residual is None else _DT[residual.dtype],
                             N if residual is None else _row_stride(residual, N), _addr(out), _DT[out.dtype],
                             _row_stride(out, N))
-        _check(_lib.qimg_linear_bf16_fused(ctypes.byref(args), _addr(scratch), _nbytes(scratch), _raw_stream(x.device)))
+        _check(_lib.qimg_linear_bf16_fused(ctypes.byref(args), _addr(scratch), _nbytes(scratch), _raw_stream(dev)))
     return out
 
 
@@ -812,10 +813,11 @@ def rope_packed(x: torch.Tensor, cos_sin: torch.Tensor, positions: torch.Tensor,
     out may be x; its type defaults to x's."""
     if not (x.is_cuda and x.dim() == 3):
         raise QimgError(QIMG_ERR_INVALID_ARG, "x must be a device tensor [T, H, D]")
-    _same_device(x, cos_sin=cos_sin, positions=positions, out=out)
+    dev = x.device
+    _same_device(dev, cos_sin, positions, out)
     T, H, D = x.shape
     if out is None:
-        out = torch.empty((T, H, D), dtype=out_dtype or x.dtype, device=x.device)
+        out = torch.empty((T, H, D), dtype=out_dtype or x.dtype, device=dev)
     elif out.shape != x.shape:
         raise QimgError(QIMG_ERR_INVALID_ARG, f"out must be {tuple(x.shape)}")
     if x.dtype not in _HEAD_TYPES or out.dtype not in _HEAD_TYPES:
@@ -824,10 +826,11 @@ def rope_packed(x: torch.Tensor, cos_sin: torch.Tensor, positions: torch.Tensor,
         raise QimgError(QIMG_ERR_INVALID_ARG, "cos_sin must be contiguous float32 [P, R / 2, 2]")
     if positions.dtype != torch.int32 or positions.numel() != T or not positions.is_contiguous():
         raise QimgError(QIMG_ERR_INVALID_ARG, f"positions must be contiguous int32 of {T} elements")
-    with _on(x.device):
-        args = _Rope(_addr(x), _DT[x.dtype], *_head_strides(x), _addr(out), _DT[out.dtype], *_head_strides(out), T, H, n_rotated, D,
+    with _on(dev):
+        args = _Rope(_addr(x), _DT[x.dtype], *_head_strides(x, T, H, D), _addr(out), _DT[out.dtype],
+                     *_head_strides(out, T, H, D), T, H, n_rotated, D,
                      2 * cos_sin.shape[1], bool(interleaved), _addr(cos_sin), cos_sin.shape[0], _addr(positions))
-        _check(_lib.qimg_rope_packed(ctypes.byref(args), _raw_stream(x.device)))
+        _check(_lib.qimg_rope_packed(ctypes.byref(args), _raw_stream(dev)))
     return out
 
 
