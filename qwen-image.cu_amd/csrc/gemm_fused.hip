@@ -6,12 +6,13 @@
 // accumulation; bias, activation, product, gate and residual in fp32 on the
 // accumulators, one rounding to out's type.
 //
-// Four kernels: linear_gemv_kernel (one or two rows) and linear_rows_kernel (up
-// to 16), both bound by reading the weights, linear_tile_kernel (the rest, also with the sum over k split over
-// workgroups where there are few tiles) and linear_join_kernel (adds the parts
-// in order and applies the epilogue). x in fp32 with more than 16 rows, and
-// operands whose rows are not whole 16-byte pieces, first go through
-// pack_rows_kernel into scratch.
+// linear_gemv_kernel (one or two rows) and linear_rows_kernel (up to 16) are bound
+// by reading the weights; linear_small_kernel takes products of few tiles (a
+// prompt of some hundred tokens), linear_tile_kernel the rest, both also with the
+// sum over k split over workgroups; linear_join_kernel then adds the parts in
+// order and applies the epilogue. x in fp32 for the tiles, and operands whose
+// rows are not whole 16-byte pieces, first go through pack_rows_kernel into
+// scratch. linear_fused_plan chooses.
 #include <algorithm>
 #include <type_traits>
 
@@ -388,6 +389,170 @@ __global__ __launch_bounds__(512) void linear_tile_kernel(LinearFusedArgs a) {
     }
 }
 
+// ---- small tiles -----------------------------------------------------------------
+// For products of few tiles the eight barriers of a stage above cost more than its
+// MFMAs. Here a stage is 128 elements of K (256-byte rows, 4 rows a DMA
+// instruction, chunk c of row r at c ^ (r & 15)) with one barrier, and the eight
+// waves are two halves of the tile's rows times four quarters of the stage's K, so a
+// wave reads each operand byte of its quarter once; the four partial tiles are
+// added through LDS in order. A workgroup's time is its operand bytes through
+// the CU's port to L2, with NS - 1 stages in flight.
+template <int TM_, int TN_>
+struct Small {
+    static constexpr int TM = TM_, TN = TN_;
+    static constexpr int AB = TM * 256, STAGE = AB + TN * 256;
+    static constexpr int NS = 152 * 1024 / STAGE < 4 ? 152 * 1024 / STAGE : 4;
+    static constexpr int IA = TM / 32, IB = TN / 32, PER = IA + IB;  // DMA instructions per wave and stage
+    static constexpr int PITCH = TN + 4;
+    static_assert(NS >= 2 && TM % 32 == 0 && TN % 32 == 0, "DMA shares");
+    static_assert(4 * TM * PITCH * 4 <= NS * STAGE, "the partial tiles take the ring's place");
+};
+
+template <class T, bool GATED>
+__global__ __launch_bounds__(512) void linear_small_kernel(LinearFusedArgs a) {
+    constexpr int NS = T::NS, TM = T::TM, TN = T::TN, WB = TM / 32, NB = TN / 16;
+    constexpr int TNO = GATED ? TN / 2 : TN;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[NS * T::STAGE];
+    const int tiles_m = (a.M + TM - 1) / TM, tiles_n = (a.N + TNO - 1) / TNO;
+    const int logical = xcd_remap(blockIdx.x, tiles_m * tiles_n * a.splits);
+    const int m0 = logical % tiles_m * TM;
+    const int n0 = logical / tiles_m % tiles_n * TNO;
+    const int split = logical / (tiles_m * tiles_n);
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ks = wave & 3, mw = (wave >> 2) * (TM / 2);
+    // (split_stages counts stages of 64)
+    const int st0 = split * a.split_stages / 2;
+    const int nst = min((a.K + 127) / 128 - st0, a.split_stages / 2);
+
+    const int rows_m = min(a.M - m0, TM), rows_n = min(a.N - n0, TNO);
+    uint32_t off[T::PER];
+    int kc[T::PER];
+#pragma unroll
+    for (int i = 0; i < T::PER; ++i) {
+        const int row = 4 * (wave + 8 * (i < T::IA ? i : i - T::IA)) + (lane >> 4);
+        const int c = (lane & 15) ^ (row & 15);
+        const int n = GATED ? (row >> 5) * 16 + (row & 15) : row;  // of a weight row: w and w_up, 16 in turn
+        kc[i] = 8 * c;
+        if (i < T::IA)
+            off[i] = row < rows_m ? static_cast<uint32_t>(row) * static_cast<uint32_t>(a.ldx) * 2u + c * 16 : kOob;
+        else
+            off[i] = n < rows_n ? static_cast<uint32_t>(n) * static_cast<uint32_t>(a.ldw) * 2u + c * 16 : kOob;
+    }
+    const int kleft = a.K - st0 * 128;
+    const uint16_t* xp = a.x16 + static_cast<int64_t>(m0) * a.ldx + st0 * 128;
+    const uint16_t* wp = (GATED && wave >= 4 ? a.w_up : a.w) + static_cast<int64_t>(n0) * a.ldw + st0 * 128;
+    int xbytes = static_cast<int>((static_cast<int64_t>(rows_m - 1) * a.ldx + kleft) * 2);
+    int wbytes = static_cast<int>((static_cast<int64_t>(rows_n - 1) * a.ldw + kleft) * 2);
+    const int tail = kleft / 128, tail_k = kleft % 128;
+    int fill = 0, fill_at = 0;
+    auto issue = [&]() {
+        const bool in = fill < nst;  // past the range: zeros, unread
+        const __amdgpu_buffer_rsrc_t rx =
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(xp), 0, in ? xbytes : 0, kRsrcWord3);
+        const __amdgpu_buffer_rsrc_t rw =
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(wp), 0, in ? wbytes : 0, kRsrcWord3);
+        const int klim = fill == tail ? tail_k : 128;
+#pragma unroll
+        for (int i = 0; i < T::PER; ++i) {
+            const uint32_t o = kc[i] >= klim ? kOob : off[i];
+            const int q = wave + 8 * (i < T::IA ? i : i - T::IA);
+            uint8_t* to = lds + fill_at + (i < T::IA ? 0 : T::AB) + q * 1024;
+            if (i < T::IA)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_ptr_t)to, 16, o, 0, 0, 0);
+            else
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_ptr_t)to, 16, o, 0, 0, 0);
+        }
+        xp += 128;
+        wp += 128;
+        xbytes -= 256;
+        wbytes -= 256;
+        ++fill;
+        fill_at = fill_at + T::STAGE == NS * T::STAGE ? 0 : fill_at + T::STAGE;
+    };
+
+    v4f acc[WB][NB];
+#pragma unroll
+    for (int i = 0; i < WB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[i][j] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+    const int r = lane & 15, kq = lane >> 4;
+    const int lane_at = r * 256 + (((4 * ks + kq) ^ r) << 4);
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i) issue();
+    int at = 0;
+    for (int st = 0; st < nst; ++st) {
+        // this stage has landed in every wave, and every wave is done with the one before, whose
+        // slot is filled next
+        __builtin_amdgcn_sched_barrier(0);
+        wait_vmcnt<(NS - 2) * T::PER>();
+        wait_lgkmcnt0();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        issue();
+        __builtin_amdgcn_sched_barrier(0);
+        const uint8_t* as = lds + at + mw * 256 + lane_at;
+        const uint8_t* bs = lds + at + T::AB + lane_at;
+        v8bf fa[WB], fb[NB];
+#pragma unroll
+        for (int j = 0; j < NB; ++j) fb[j] = *reinterpret_cast<const v8bf*>(bs + j * 16 * 256);
+#pragma unroll
+        for (int i = 0; i < WB; ++i) fa[i] = *reinterpret_cast<const v8bf*>(as + i * 16 * 256);
+#pragma unroll
+        for (int i = 0; i < WB; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j], fa[i], acc[i][j], 0, 0, 0);
+        at = at + T::STAGE == NS * T::STAGE ? 0 : at + T::STAGE;
+    }
+    wait_vmcnt<0>();
+    __syncthreads();
+    float* red = reinterpret_cast<float*>(lds);
+#pragma unroll
+    for (int i = 0; i < WB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+            *reinterpret_cast<v4f*>(red + (ks * TM + mw + 16 * i + r) * T::PITCH + 16 * j + 4 * kq) = acc[i][j];
+    __syncthreads();
+    constexpr int GR = TNO / 4;  // groups of four columns a row
+    const int oc = static_cast<int>(threadIdx.x) % GR * 4;
+    const int n = n0 + oc;
+    const int sc = GATED ? (oc >> 4) * 32 + (oc & 15) : oc;
+    if (n >= a.N) return;
+    Columns col;
+    if (a.splits == 1) col = load_columns(a, n);
+#pragma unroll
+    for (int q = 0; q < (TM * GR + 511) / 512; ++q) {
+        const int row = (static_cast<int>(threadIdx.x) + 512 * q) / GR;
+        const int m = m0 + row;
+        if (row >= TM || m >= a.M) continue;
+        float z[4], u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z[i] = u[i] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float* p = red + (w * TM + row) * T::PITCH + sc;
+            const v4f t = *reinterpret_cast<const v4f*>(p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z[i] += t[i];
+            if constexpr (GATED) {
+                const v4f t2 = *reinterpret_cast<const v4f*>(p + 16);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) u[i] += t2[i];
+            }
+        }
+        if (a.splits == 1) {
+            finish4<GATED>(a, col, m, n, z, u);
+        } else {
+            float* p = a.part + (static_cast<int64_t>(split) * a.M + m) * a.part_ld + n;
+            *reinterpret_cast<v4f*>(p) = (v4f){z[0], z[1], z[2], z[3]};
+            if constexpr (GATED) *reinterpret_cast<v4f*>(p + a.part_ld / 2) = (v4f){u[0], u[1], u[2], u[3]};
+        }
+    }
+}
+
 template <bool GATED>
 __global__ __launch_bounds__(256) void linear_join_kernel(LinearFusedArgs a) {
     const int groups = (a.N + 3) / 4;
@@ -637,45 +802,62 @@ hipError_t launch_tile(const LinearFusedArgs& a, hipStream_t stream) {
     return hipGetLastError();
 }
 
+template <int TM, int TN, bool GATED>
+hipError_t launch_small(const LinearFusedArgs& a, hipStream_t stream) {
+    constexpr int TNO = GATED ? TN / 2 : TN;
+    const int tiles = ((a.M + TM - 1) / TM) * ((a.N + TNO - 1) / TNO);
+    hipLaunchKernelGGL((linear_small_kernel<Small<TM, TN>, GATED>), dim3(tiles * a.splits), dim3(512), 0, stream, a);
+    return hipGetLastError();
+}
+
 int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 
 }  // namespace
 
-// Tile and number of K splits: the least estimated time of the launch (us). A
-// stage of a tile takes 0.4 us and 1.2 us for each 256x256 of it (measured: 256x256
-// 1.6, 224x256 1.5, 160x256 1.2, 160x128 0.8, 128x128 0.7, 64x128 0.6), the weights
-// come at 4.8 TB/s at best, the parts of a split sum are written and read once. linear_rows_kernel takes about 4 us and
-// the weights' bytes at 3 TB/s: it is the faster one below some 16 M weights
-// (16 rows, us, rows / tiles: 3584x3584 10.6 / 13.2, 4608x3584 17.1 / 14.7,
-// 3584x14336 34.8 / 26.9, gated 14336x3584 53.4 / 39.2); fp32 rows spare it a
-// packing launch of 3 us.
+// Kernel, tile and number of K splits: the least estimated time of the launch
+// (us). A stage of linear_tile_kernel takes 0.4 us and 1.2 us for each 256x256 of
+// the tile (measured: 256x256 1.6, 224x256 1.5, 160x256 1.2, 128x128 0.7), one of
+// linear_small_kernel its bytes at 75 KB a us; the weights come at 4.8 TB/s at
+// best, the parts of a split sum are written and read once. linear_rows_kernel
+// takes about 4 us and the weights' bytes at 2.5 TB/s; fp32 rows spare it a packing
+// launch of 3 us. Measured (us, bf16 x, weights not resident): 16x3584x3584 rows
+// 10.8, 32x64 tiles 13; 16x4608x3584 17.5 / 11.7; 269x4608x3584 96x64 tiles 20.5,
+// 160x256 split in 4 28; 500x4608x3584 96x64 38, 128x256 split in 2 41;
+// 1000x4608x3584 (fp32 x) 160x256 split in 2 56, 128x256 68; 269x3584x14336 160x256
+// split in 9 45-49, 96x64 split in 4 55; 781x14336x3584 gated 224x256 158, 256x256
+// 162; 64x14336x3584 gated 64x128 43.
 LinearFusedPlan linear_fused_plan(int x_dtype, int M, int K, int N, bool gated) {
     LinearFusedPlan best{};  // tm = 0: linear_gemv_kernel or linear_rows_kernel
     if (M <= kLinearGemvRows) return best;
-    static const int tms[] = {256, 224, 192, 160, 128, 64}, tns[] = {256, 128};
-    const int stages = (K + 63) / 64;
     const double bytes = 2.0 * N * K * (gated ? 2 : 1);  // of weights
-    double best_t = M <= kLinearRows ? 4.0 + bytes / 3e6 - (x_dtype == QIMG_FP32 ? 3.0 : 0.0) : 1e30;
-    for (int tm : tms)
-        for (int tn : tns) {
-            const int tno = gated ? tn / 2 : tn;
-            const int64_t tiles = static_cast<int64_t>((M + tm - 1) / tm) * ((N + tno - 1) / tno);
-            const double stage = 0.4 + 1.2 * tm * tn / 65536.0;
-            for (int s = 1; s <= 16 && s <= stages; ++s) {
-                const int per = (stages + s - 1) / s;
-                if (per * (s - 1) >= stages) continue;  // the last range would be empty
-                const double rounds = static_cast<double>((tiles * s + 255) / 256);
-                double t = 3.0 + std::max(rounds * (per * stage + 3.0), bytes / 4.8e6 + 3.0);
-                if (s > 1) t += 3.0 + 2.0 * s * M * N * (gated ? 8.0 : 4.0) / 5e6;
-                if (t < best_t) {
-                    best_t = t;
-                    best.tm = tm;
-                    best.tn = tn;
-                    best.splits = s;
-                    best.split_stages = per;
-                }
+    double best_t = M <= kLinearRows ? 4.0 + bytes / 2.5e6 - (x_dtype == QIMG_FP32 ? 3.0 : 0.0) : 1e30;
+    static const struct {
+        int tm, tn, k;  // k: elements of K a stage
+    } shapes[] = {{256, 256, 64}, {224, 256, 64}, {192, 256, 64}, {160, 256, 64}, {128, 256, 64}, {128, 128, 64},
+                  {128, 64, 128}, {96, 64, 128},  {64, 128, 128}, {64, 64, 128},  {32, 128, 128}, {32, 64, 128}};
+    for (const auto& c : shapes) {
+        const int tno = gated ? c.tn / 2 : c.tn;
+        const int64_t tiles = static_cast<int64_t>((M + c.tm - 1) / c.tm) * ((N + tno - 1) / tno);
+        const int stages = (K + c.k - 1) / c.k;
+        const double stage =
+            c.k == 64 ? 0.4 + 1.2 * c.tm * c.tn / 65536.0 : (c.tm + c.tn) * 256 / 75e3;
+        for (int s = 1; s <= 16 && s <= stages; ++s) {
+            const int per = (stages + s - 1) / s;
+            if (per * (s - 1) >= stages) continue;  // the last range would be empty
+            const double rounds = static_cast<double>((tiles * s + 255) / 256);
+            const double work = rounds * (per * stage + (c.k == 64 ? 3.0 : 1.5)), read = bytes / 4.8e6 + 3.0;
+            double t = 3.0 + std::max(work, read) + 0.2 * std::min(work, read);
+            if (s > 1) t += 5.0 + 2.0 * s * M * N * (gated ? 8.0 : 4.0) / 5e6;
+            if (t < best_t) {
+                best_t = t;
+                best.tm = c.tm;
+                best.tn = c.tn;
+                best.small = c.k == 128;
+                best.splits = s;
+                best.split_stages = per * (c.k / 64);
             }
         }
+    }
     return best;
 }
 
@@ -755,20 +937,24 @@ hipError_t launch_linear_fused(LinearFusedArgs a, int x_dtype, void* scratch, hi
     a.splits = plan.splits;
     a.split_stages = plan.split_stages;
 #define QIMG_TILE(TM, TN)                                                                       \
-    if (plan.tm == TM && plan.tn == TN)                                                         \
+    if (!plan.small && plan.tm == TM && plan.tn == TN)                                          \
     e = gated ? launch_tile<TM, TN, true>(a, stream) : launch_tile<TM, TN, false>(a, stream)
     QIMG_TILE(256, 256);
     QIMG_TILE(224, 256);
     QIMG_TILE(192, 256);
     QIMG_TILE(160, 256);
     QIMG_TILE(128, 256);
-    QIMG_TILE(64, 256);
-    QIMG_TILE(256, 128);
-    QIMG_TILE(224, 128);
-    QIMG_TILE(192, 128);
-    QIMG_TILE(160, 128);
     QIMG_TILE(128, 128);
+#undef QIMG_TILE
+#define QIMG_TILE(TM, TN)                                                                       \
+    if (plan.small && plan.tm == TM && plan.tn == TN)                                           \
+    e = gated ? launch_small<TM, TN, true>(a, stream) : launch_small<TM, TN, false>(a, stream)
+    QIMG_TILE(128, 64);
+    QIMG_TILE(96, 64);
     QIMG_TILE(64, 128);
+    QIMG_TILE(64, 64);
+    QIMG_TILE(32, 128);
+    QIMG_TILE(32, 64);
 #undef QIMG_TILE
     if (e != hipSuccess || plan.splits == 1) return e;
     const int64_t groups = static_cast<int64_t>((a.N + 3) / 4) * a.M;

@@ -370,7 +370,7 @@ struct LinearFusedArgs {
 constexpr int kLinearGemvRows = 2;  // most rows of the vector-unit kernel
 constexpr int kLinearRows = 16;  // most rows of the kernel that reads weights straight into fragments
 struct LinearFusedPlan {
-    int tm, tn, splits, split_stages;
+    int tm, tn, small, splits, split_stages;
 };
 struct LinearFusedScratch {
     int64_t x, w, w_up, part;
