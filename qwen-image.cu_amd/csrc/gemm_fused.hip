@@ -824,7 +824,7 @@ int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 // 10.8, 32x64 tiles 13; 16x4608x3584 17.5 / 11.7; 269x4608x3584 96x64 tiles 20.5,
 // 160x256 split in 4 28; 500x4608x3584 96x64 38, 128x256 split in 2 41;
 // 1000x4608x3584 (fp32 x) 160x256 split in 2 56, 128x256 68; 269x3584x14336 160x256
-// split in 9 45-49, 96x64 split in 4 55; 781x14336x3584 gated 224x256 158, 256x256
+// split in 9 45-49, 96x64 split in 4 72; 781x14336x3584 gated 224x256 158, 256x256
 // 162; 64x14336x3584 gated 64x128 43.
 LinearFusedPlan linear_fused_plan(int x_dtype, int M, int K, int N, bool gated) {
     LinearFusedPlan best{};  // tm = 0: linear_gemv_kernel or linear_rows_kernel

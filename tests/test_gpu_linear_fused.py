@@ -57,6 +57,36 @@ def test_integers_are_exact(qimg, M, N, K, x_dtype):
     assert torch.equal(got, (res.double() + x.double() @ w.double().t()).to(F32).to(BF))
 
 
+# (M, N, K, gated): each kernel's tiles (256 to 128 rows by 256, 128x128; the small ones of
+# 128, 96, 64 and 32 rows), whole K and K split over workgroups; odd sizes, K that ends inside a stage
+TILES = [(196, 11191, 264, 0), (104, 8701, 264, 1), (1675, 2329, 264, 0), (198, 8827, 4024, 0), (198, 8314, 264, 1),
+         (199, 2094, 7992, 1), (98, 8373, 264, 0), (1775, 65, 3896, 0), (107, 4207, 272, 1), (798, 65, 6968, 1),
+         (518, 13478, 272, 0), (137, 10942, 4080, 0), (260, 11553, 280, 1), (130, 2753, 8136, 1), (810, 11318, 264, 0),
+         (728, 2701, 5392, 0), (358, 11089, 264, 1), (367, 2738, 5400, 1), (1951, 5953, 264, 0), (212, 10933, 4112, 0),
+         (408, 11123, 264, 1), (195, 4098, 5784, 1), (1368, 9810, 264, 0), (233, 10927, 4904, 0), (459, 11623, 272, 1),
+         (245, 5473, 5480, 1), (21, 8442, 264, 1), (17, 65, 264, 0), (18, 67, 2472, 0), (19, 65, 264, 1),
+         (17, 67, 2640, 1), (129, 8807, 264, 0), (1192, 65, 4640, 0), (33, 8287, 272, 1), (387, 225, 5432, 1),
+         (2093, 205, 272, 0), (821, 65, 2768, 0), (1683, 131, 264, 1), (385, 66, 3952, 1), (2086, 453, 272, 0),
+         (931, 66, 4104, 0), (2314, 193, 288, 1), (771, 67, 3216, 1)]
+
+
+@pytest.mark.parametrize("M,N,K,gated", TILES, ids=str)
+def test_every_tile_with_integers(qimg, M, N, K, gated):
+    """Exact, as above. K <= 8136 products of at most 4 (2): sums below 2^15, the
+    gated product below 2^24 because its second factor is kept small."""
+    g = _gen(M + N + K)
+    x, w = _ints(g, (M, K), -2, 2), _ints(g, (N, K), -2, 2)
+    z = x.double() @ w.double().t()
+    res = _ints(g, (M, N), -16, 16)
+    if gated:
+        wu = _ints(g, (N, K), -1, 1) * (torch.arange(K, device=DEV) % 37 == 0)
+        z = z * (x.double() @ wu.double().t())
+        assert float(z.abs().max()) + 16 < 2 ** 24
+    got = qimg.linear_forward_bf16_fused(x.to(BF), w.to(BF), weight_up=wu.to(BF) if gated else None, residual=res.to(F32),
+                                         out_dtype=F32)
+    assert torch.equal(got.double(), res + z)
+
+
 def _definition(x, w, b, act, wu, bu, gate, res):
     """The result in 64 bits and the bound on an fp32 evaluation's error."""
     K = x.shape[1]
