@@ -149,11 +149,24 @@ __device__ __forceinline__ int key_ranges(int lk, int per) {
     return max((n + per - 1) / per, 1);
 }
 
+// inclusive sum over the wave's lanes: shifts by 1, 2, 4 and 8 inside rows of
+// 16, then the rows' last lanes broadcast to the rows behind them
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+
 // Item `idx` of the launch: the sequences in order, each with its tiles of
 // `rows` rows (inside a causal sequence the last, longest one first) times its
 // key ranges of `per` tiles. Each lane takes one sequence; a wave scans 64 of
-// them at a time.
-__device__ __forceinline__ RowTile find_tile(const AttnVarlenArgs& a, int idx, int rows, int per) {
+// them at a time, the first 64 (`first`) loaded once by the caller.
+__device__ __forceinline__ RowTile find_tile(const AttnVarlenArgs& a, const Sequence& first, int idx, int rows,
+                                             int per) {
     const int lane = threadIdx.x & 63;
     RowTile t;
     t.found = false;
@@ -161,14 +174,9 @@ __device__ __forceinline__ RowTile find_tile(const AttnVarlenArgs& a, int idx, i
     t.splits = 1;
     int before = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
-        const Sequence s = load_sequence(a, b0 + lane);
+        const Sequence s = b0 == 0 ? first : load_sequence(a, b0 + lane);
         const int n = row_tiles(a, s.lq, rows), parts = key_ranges(s.lk, per);
-        int incl = n * parts;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int v = __shfl_up(incl, off, 64);
-            if (lane >= off) incl += v;
-        }
+        const int incl = wave_scan(n * parts);
         const int total = __builtin_amdgcn_readlane(incl, 63);
         const uint64_t hit = __ballot(before + incl > idx);
         if (idx < before + total && hit != 0) {
@@ -326,13 +334,13 @@ constexpr int SR = 32, SW = 4;
 
 // Key tiles per range: as many as make the launch about one item a workgroup,
 // at least four a wave, and at most a.splits ranges a sequence. 0: no ranges.
-__device__ __forceinline__ int range_tiles(const AttnVarlenArgs& a) {
+__device__ __forceinline__ int range_tiles(const AttnVarlenArgs& a, const Sequence& first) {
     if (a.splits == 1) return 0;
     const int lane = threadIdx.x & 63;
     int longest = 0;
     float work = 0.0f;  // (row tiles x key tiles: a sum that needs no last digit)
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
-        const Sequence s = load_sequence(a, b0 + lane);
+        const Sequence s = b0 == 0 ? first : load_sequence(a, b0 + lane);
         const int kt = (s.lk + SK - 1) / SK;
         work += wave_sum_dpp(static_cast<float>(row_tiles(a, s.lq, SR)) * static_cast<float>(kt));
         longest = max(longest, wave_reduce_dpp(kt, [](int x, int y) { return max(x, y); }));
@@ -571,9 +579,10 @@ __global__ __launch_bounds__(SW * 64, 2) void attn_few_kernel(AttnVarlenArgs a) 
     // One LDS object: with two, the compiler orders every read of the tiles
     // behind all DMA in flight.
     __shared__ __attribute__((aligned(1024))) uint8_t ring[SW * Few<D>::WB + SW * SR * 8];
-    const int per = range_tiles(a);
+    const Sequence first = load_sequence(a, threadIdx.x & 63);
+    const int per = range_tiles(a, first);
     for (int item = blockIdx.x;; item += gridDim.x) {
-        const RowTile t = find_tile(a, item / a.hk, SR, per);
+        const RowTile t = find_tile(a, first, item / a.hk, SR, per);
         if (!t.found) return;
         few_item<T, D>(a, t, item % a.hk, per, ring);
     }
@@ -581,13 +590,15 @@ __global__ __launch_bounds__(SW * 64, 2) void attn_few_kernel(AttnVarlenArgs a) 
 
 // The key ranges' partial results of a tile of 32 rows, added in range order:
 // thread: row tid / 8, channels (tid % 8) * D / 8 .. Sequences of one range
-// are complete already.
+// are complete already. Eight ranges' loads go out together (one after the
+// other, 16 tokens over up to 8192 keys took 7 us here, most of it waiting).
 template <class T, int D>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnVarlenArgs a) {
-    constexpr int E = D / 8;
-    const int per = range_tiles(a);
+    constexpr int E = D / 8, U = 8;
+    const Sequence first = load_sequence(a, threadIdx.x & 63);
+    const int per = range_tiles(a, first);
     const int hk = blockIdx.x % a.hk;
-    const RowTile t = find_tile(a, blockIdx.x / a.hk, SR, 0);
+    const RowTile t = find_tile(a, first, blockIdx.x / a.hk, SR, 0);
     if (!t.found) return;
     const int splits = key_ranges(t.lk, per);
     const int row = t.row0 + (threadIdx.x >> 3);
@@ -596,21 +607,36 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnVarlenArgs a) {
     const int64_t token = static_cast<int64_t>(t.q0) + row / a.group;
     const int head = hk * a.group + row % a.group;
     const int64_t at = (token * a.hq + head) * a.splits;
+    typedef float v2f __attribute__((ext_vector_type(2)));
     float mm = kNegInf, tot = 0.0f, acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-    for (int s = 0; s < splits; ++s) mm = fmaxf(mm, a.part_ml[2 * (at + s)]);
-#pragma unroll 4
-    for (int s = 0; s < splits; ++s) {
-        const float ms = a.part_ml[2 * (at + s)], ts = a.part_ml[2 * (at + s) + 1];
-        const float f = ms == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(ms - mm);
-        tot += f * ts;
-        const float* po = a.part_o + (at + s) * D + c0;
+    for (int s0 = 0; s0 < splits; s0 += U) {
+        v2f ml[U];
+        v4f v[U][E / 4];
 #pragma unroll
-        for (int e = 0; e < E; e += 4) {
-            const v4f v = *reinterpret_cast<const v4f*>(po + e);
+        for (int u = 0; u < U; ++u) {
+            const int64_t p = at + min(s0 + u, splits - 1);
+            ml[u] = *reinterpret_cast<const v2f*>(a.part_ml + 2 * p);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) acc[e + c] += f * v[c];
+            for (int e = 0; e < E / 4; ++e) v[u][e] = *reinterpret_cast<const v4f*>(a.part_o + p * D + c0 + 4 * e);
+        }
+        float top = mm;
+#pragma unroll
+        for (int u = 0; u < U; ++u) top = fmaxf(top, ml[u][0]);
+        const float old = mm == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(mm - top);
+        mm = top;
+        tot *= old;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] *= old;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (s0 + u >= splits) continue;
+            // no finite score: O is zero there, the sum zero or NaN
+            const float f = ml[u][0] == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(ml[u][0] - mm);
+            tot += f * ml[u][1];
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] += f * v[u][e / 4][e % 4];
         }
     }
     store_row<T, E>(a.out + token * a.o_t + head * a.o_h + c0, acc, tot, visible(a, t, row / a.group) == 0);
@@ -849,7 +875,7 @@ __global__ __launch_bounds__(MW * 64, 2) void attn_many_kernel(AttnVarlenArgs a,
         hk = logical / tiles;
         idx = logical % tiles;
     }
-    const RowTile t = find_tile(a, idx, MR, 0);
+    const RowTile t = find_tile(a, load_sequence(a, lane), idx, MR, 0);
     if (!t.found) return;
 
     const int rows = t.lq * a.group;
