@@ -19,9 +19,9 @@
 // element e of lane half h stands for key 16 t + 8 (e / 4) + 4 h + e % 4 of a
 // 16-key group t, and V^T comes from row-major V in LDS through
 // ds_read_b64_tr_b16, whose four values are 4 consecutive keys of one channel.
-// P is rounded to the inputs' type for the second product (relative error at
-// most 2^-8 a term in bf16 as in the result itself; the row sum adds the
-// rounded values, so a constant V is returned exactly). The maximum moves, and
+// P is rounded to the inputs' type for the second product: with u half a step of
+// the type (2^-8 in bf16, 2^-11 in fp16) an error of at most u sum_j p_j |v_j - o|,
+// since the row sum adds the rounded values (a constant V is returned exactly). The maximum moves, and
 // O and the sum are rescaled, only when a tile exceeds it by more than
 // kSlack (log2 units): P then reaches 2^kSlack, which changes no relative
 // rounding. fp16 P carries a further factor 2^kBias16 (at most 2^15 in all),
@@ -60,6 +60,7 @@ struct Bf16 {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
     }
     __device__ static __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
+    __device__ static __forceinline__ uint32_t pack_p(float a, float b) { return pack_bf16x2(a, b); }
     __device__ static __forceinline__ float add2(uint32_t p, float s) {
         typedef __bf16 b2 __attribute__((ext_vector_type(2)));
         return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, p), __builtin_bit_cast(b2, 0x3f803f80u), s,
@@ -78,6 +79,13 @@ struct Fp16 {
         typedef _Float16 h2 __attribute__((ext_vector_type(2)));
         typedef float f2 __attribute__((ext_vector_type(2)));
         return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, h2));
+    }
+    // P towards zero, one instruction for two values (to nearest takes three): off by
+    // up to a whole step downwards, but the row sum adds the same rounded values, so the
+    // half step that all of them lose on average cancels in O / sum, and what is left
+    // is within half a step of the mean, as with rounding to nearest
+    __device__ static __forceinline__ uint32_t pack_p(float a, float b) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
     }
     __device__ static __forceinline__ float add2(uint32_t p, float s) {
         typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -478,7 +486,7 @@ __device__ __forceinline__ void few_item(const AttnVarlenArgs& a, const RowTile&
         uint32_t pk[8];
 #pragma unroll
         for (int r = 0; r < 16; r += 2) {
-            pk[r / 2] = T::pack(__builtin_amdgcn_exp2f(p[r] + neg), __builtin_amdgcn_exp2f(p[r + 1] + neg));
+            pk[r / 2] = T::pack_p(__builtin_amdgcn_exp2f(p[r] + neg), __builtin_amdgcn_exp2f(p[r + 1] + neg));
             sum = T::add2(pk[r / 2], sum);
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -806,7 +814,7 @@ struct Many {
         for (int r = 0; r < 16 * KB; r += 2) {
             const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r >> 4][r & 15], c, neg));
             const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r >> 4][(r & 15) + 1], c, neg));
-            pk[r / 2] = T::pack(p0, p1);
+            pk[r / 2] = T::pack_p(p0, p1);
             sum = T::add2(pk[r / 2], sum);
         }
     }
