@@ -250,8 +250,9 @@ int qimg_sage_attention(const uint16_t* q_f16, const uint16_t* k_f16, const uint
  * What lies behind a sequence's last key or is hidden from a row does not
  * reach that row, NaN and infinities included. sm_scale > 0, finite. out
  * overlaps none of q, k, v.
- * scratch: qimg_attention_varlen_scratch_bytes(...) bytes (may be 0: NULL).
- * One scratch buffer serves one call at a time. */
+ * scratch: qimg_attention_varlen_scratch_bytes(...) bytes (may be 0: NULL) for
+ * this call's sizes; fewer queries can need more (their keys are split). One
+ * scratch buffer serves one call at a time. */
 typedef struct {
     const void* q;
     const void* k;
@@ -287,7 +288,9 @@ enum { QIMG_ACT_NONE = 0, QIMG_ACT_GELU_TANH = 1, QIMG_ACT_SILU = 2 };
  * fp32 accumulation and epilogue, one rounding. bf16 rows of x must start at
  * 16-byte boundaries (ldx a multiple of 8; fp32: of 4) unless K is no multiple of 8, where x and the
  * weights are copied to scratch first. ld* < 2^22.
- * scratch: qimg_linear_bf16_fused_scratch_bytes(...) bytes (may be 0: NULL). */
+ * scratch: qimg_linear_bf16_fused_scratch_bytes(...) bytes (may be 0: NULL) for
+ * this call's sizes; fewer rows can need more (their sum over K is split). One
+ * scratch buffer serves one call at a time. */
 typedef struct {
     const void* x;
     int x_dtype;

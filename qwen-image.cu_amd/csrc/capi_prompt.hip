@@ -90,7 +90,9 @@ int qimg_attention_varlen(const qimg_attn_varlen* args, void* scratch, int64_t s
 }
 
 int64_t qimg_linear_bf16_fused_scratch_bytes(int x_dtype, int M, int K, int N, int gated) {
-    const qimg::LinearFusedScratch s = qimg::linear_fused_scratch(x_dtype, M, K, N, gated != 0);
+    if (M <= 0 || K <= 0 || N <= 0) return 0;
+    const qimg::LinearFusedPlan plan = qimg::linear_fused_plan(x_dtype, M, K, N, gated != 0);
+    const qimg::LinearFusedScratch s = qimg::linear_fused_scratch(plan, x_dtype, M, K, N, gated != 0);
     return s.x + s.w + s.w_up + s.part;
 }
 
@@ -126,8 +128,10 @@ int qimg_linear_bf16_fused(const qimg_linear_fused* args, void* scratch, int64_t
     QIMG_REQUIRE(p.out != p.residual || (p.ldo == p.ld_residual && p.out_dtype == p.residual_dtype),
                  "%s: out in residual's place must have its type and rows", fn);
     QIMG_REQUIRE(p.out != p.x && p.out != static_cast<const void*>(p.w), "%s: out must not be x or w", fn);
-    const int64_t need =
-        qimg_linear_bf16_fused_scratch_bytes(p.x_dtype, p.M, p.K, p.N, p.w_up != nullptr);
+    const qimg::LinearFusedPlan plan = qimg::linear_fused_plan(p.x_dtype, p.M, p.K, p.N, p.w_up != nullptr);
+    const qimg::LinearFusedScratch parts =
+        qimg::linear_fused_scratch(plan, p.x_dtype, p.M, p.K, p.N, p.w_up != nullptr);
+    const int64_t need = parts.x + parts.w + parts.w_up + parts.part;
     if (need > 0) {
         if (!scratch || scratch_bytes < need)
             return qimg::api_fail(QIMG_ERR_SCRATCH, "%s: scratch %lld bytes < required %lld", fn,
@@ -142,7 +146,8 @@ int qimg_linear_bf16_fused(const qimg_linear_fused* args, void* scratch, int64_t
     a.out = p.out, a.ldo = p.ldo, a.out_dtype = p.out_dtype;
     a.act = p.act;
     a.vec4 = p.ldo % 4 == 0 && (!p.residual || p.ld_residual % 4 == 0);
-    return qimg::api_hip_status(qimg::launch_linear_fused(a, p.x_dtype, scratch, static_cast<hipStream_t>(stream)), fn);
+    return qimg::api_hip_status(qimg::launch_linear_fused(a, plan, p.x_dtype, scratch, static_cast<hipStream_t>(stream)),
+                                fn);
 }
 
 int qimg_rope_packed(const qimg_rope* args, void* stream) {

@@ -841,7 +841,7 @@ LinearFusedPlan linear_fused_plan(int x_dtype, int M, int K, int N, bool gated) 
         const int stages = (K + c.k - 1) / c.k;
         const double stage =
             c.k == 64 ? 0.4 + 1.2 * c.tm * c.tn / 65536.0 : (c.tm + c.tn) * 256 / 75e3;
-        for (int s = 1; s <= 16 && s <= stages; ++s) {
+        for (int s = 1; s <= 16 && s <= stages && tiles * (s - 1) < 512; ++s) {  // (past two rounds no split gains)
             const int per = (stages + s - 1) / s;
             if (per * (s - 1) >= stages) continue;  // the last range would be empty
             const double rounds = static_cast<double>((tiles * s + 255) / 256);
@@ -862,12 +862,11 @@ LinearFusedPlan linear_fused_plan(int x_dtype, int M, int K, int N, bool gated) 
 }
 
 // Scratch: packed x, packed w and w_up, the parts of a split sum.
-LinearFusedScratch linear_fused_scratch(int x_dtype, int M, int K, int N, bool gated) {
+LinearFusedScratch linear_fused_scratch(const LinearFusedPlan& p, int x_dtype, int M, int K, int N, bool gated) {
     LinearFusedScratch s{};
     if (M <= 0 || K <= 0 || N <= 0) return s;
     const int Kp = (K + 7) / 8 * 8;
     const bool odd = Kp != K;
-    const LinearFusedPlan p = linear_fused_plan(x_dtype, M, K, N, gated);
     if (odd || (x_dtype == QIMG_FP32 && p.tm != 0)) s.x = align256(static_cast<int64_t>(M) * Kp * 2);
     if (odd) s.w = align256(static_cast<int64_t>(N) * Kp * 2);
     if (odd && gated) s.w_up = s.w;
@@ -875,10 +874,10 @@ LinearFusedScratch linear_fused_scratch(int x_dtype, int M, int K, int N, bool g
     return s;
 }
 
-hipError_t launch_linear_fused(LinearFusedArgs a, int x_dtype, void* scratch, hipStream_t stream) {
+hipError_t launch_linear_fused(LinearFusedArgs a, const LinearFusedPlan& plan, int x_dtype, void* scratch,
+                               hipStream_t stream) {
     const bool gated = a.w_up != nullptr;
-    const LinearFusedScratch s = linear_fused_scratch(x_dtype, a.M, a.K, a.N, gated);
-    const LinearFusedPlan plan = linear_fused_plan(x_dtype, a.M, a.K, a.N, gated);
+    const LinearFusedScratch s = linear_fused_scratch(plan, x_dtype, a.M, a.K, a.N, gated);
     uint8_t* p = static_cast<uint8_t*>(scratch);
     const int Kp = (a.K + 7) / 8 * 8;
     bool f32 = x_dtype == QIMG_FP32;

@@ -370,14 +370,17 @@ struct LinearFusedArgs {
 constexpr int kLinearGemvRows = 2;  // most rows of the vector-unit kernel
 constexpr int kLinearRows = 16;  // most rows of the kernel that reads weights straight into fragments
 struct LinearFusedPlan {
-    int tm, tn, small, splits, split_stages;
+    int tm, tn;  // 0: no tiles (linear_gemv_kernel, linear_rows_kernel)
+    int small;   // linear_small_kernel, else linear_tile_kernel
+    int splits, split_stages;
 };
 struct LinearFusedScratch {
     int64_t x, w, w_up, part;
 };
 LinearFusedPlan linear_fused_plan(int x_dtype, int M, int K, int N, bool gated);
-LinearFusedScratch linear_fused_scratch(int x_dtype, int M, int K, int N, bool gated);
-hipError_t launch_linear_fused(LinearFusedArgs a, int x_dtype, void* scratch, hipStream_t stream);
+LinearFusedScratch linear_fused_scratch(const LinearFusedPlan& plan, int x_dtype, int M, int K, int N, bool gated);
+hipError_t launch_linear_fused(LinearFusedArgs a, const LinearFusedPlan& plan, int x_dtype, void* scratch,
+                               hipStream_t stream);
 
 // rope_packed.hip: rotary positions of packed heads (qimg_rope_packed), strides in elements
 struct RopeArgs {
