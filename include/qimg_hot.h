@@ -249,7 +249,8 @@ int qimg_sage_attention(const uint16_t* q_f16, const uint16_t* k_f16, const uint
  * query that sees no key gives zeros. Rows of no sequence are not written.
  * What lies behind a sequence's last key or is hidden from a row does not
  * reach that row, NaN and infinities included. sm_scale > 0, finite. out
- * overlaps none of q, k, v.
+ * overlaps none of q, k, v. total_q * n_heads and total_k below 2^30; k and v
+ * token strides at least head_dim.
  * scratch: qimg_attention_varlen_scratch_bytes(...) bytes (may be 0: NULL) for
  * this call's sizes; fewer queries can need more (their keys are split). One
  * scratch buffer serves one call at a time. */

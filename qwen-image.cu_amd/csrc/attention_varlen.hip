@@ -66,7 +66,6 @@ struct Bf16 {
         return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, p), __builtin_bit_cast(b2, 0x3f803f80u), s,
                                                false);
     }
-    __device__ static __forceinline__ uint16_t round(float v) { return f32_to_bf16(v); }
 };
 struct Fp16 {
     using frag = v8h;
@@ -91,7 +90,6 @@ struct Fp16 {
         typedef _Float16 h2 __attribute__((ext_vector_type(2)));
         return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, p), __builtin_bit_cast(h2, 0x3c003c00u), s, false);
     }
-    __device__ static __forceinline__ uint16_t round(float v) { return f32_to_f16(v); }
 };
 
 // max of the two lane halves' values (lanes l and l ^ 32)

@@ -45,9 +45,10 @@ int qimg_attention_varlen(const qimg_attn_varlen* args, void* scratch, int64_t s
                  "%s: n_heads %d must be a multiple of n_kv_heads %d", fn, p.n_heads, p.n_kv_heads);
     if (p.head_dim != 64 && p.head_dim != 128)
         return qimg::api_fail(QIMG_ERR_UNSUPPORTED, "%s: head_dim %d not supported (64 or 128)", fn, p.head_dim);
-    QIMG_REQUIRE(std::isfinite(p.sm_scale) && p.sm_scale > 0.0f, "%s: sm_scale must be positive and finite", fn);
-    QIMG_REQUIRE(static_cast<int64_t>(p.total_q) * p.n_heads < (int64_t{1} << 30),
-                 "%s: total_q * n_heads must be < 2^30", fn);
+    const float scale_log2 = p.sm_scale * 1.4426950408889634f;
+    QIMG_REQUIRE(std::isfinite(scale_log2) && scale_log2 > 0.0f, "%s: sm_scale must be positive and finite", fn);
+    QIMG_REQUIRE(static_cast<int64_t>(p.total_q) * p.n_heads < (int64_t{1} << 30) && p.total_k < (1 << 30),
+                 "%s: total_q * n_heads and total_k must be < 2^30", fn);
     QIMG_REQUIRE(good_strides(p.q_stride_t, p.q_stride_h) && good_strides(p.k_stride_t, p.k_stride_h) &&
                      good_strides(p.v_stride_t, p.v_stride_h) && good_strides(p.out_stride_t, p.out_stride_h),
                  "%s: strides must be non-negative multiples of 8, token strides at most 2^24", fn);
@@ -72,7 +73,7 @@ int qimg_attention_varlen(const qimg_attn_varlen* args, void* scratch, int64_t s
     a.batch = p.batch, a.total_q = p.total_q, a.total_k = p.total_k;
     a.hq = p.n_heads, a.hk = p.n_kv_heads, a.group = p.n_heads / p.n_kv_heads;
     a.causal = p.causal != 0;
-    a.scale_log2 = p.sm_scale * 1.4426950408889634f;
+    a.scale_log2 = scale_log2;
     a.splits = qimg::attn_varlen_splits(p.total_q, p.total_k, p.batch, p.n_heads, p.n_kv_heads);
     a.target_items = 512;
     if (a.splits > 1) {
@@ -127,7 +128,8 @@ int qimg_linear_bf16_fused(const qimg_linear_fused* args, void* scratch, int64_t
                      fn, static_cast<long long>(p.ldx));
     QIMG_REQUIRE(p.out != p.residual || (p.ldo == p.ld_residual && p.out_dtype == p.residual_dtype),
                  "%s: out in residual's place must have its type and rows", fn);
-    QIMG_REQUIRE(p.out != p.x && p.out != static_cast<const void*>(p.w), "%s: out must not be x or w", fn);
+    QIMG_REQUIRE(p.out != p.x && p.out != static_cast<const void*>(p.w) && p.out != static_cast<const void*>(p.w_up),
+                 "%s: out must not be x or a weight", fn);
     const qimg::LinearFusedPlan plan = qimg::linear_fused_plan(p.x_dtype, p.M, p.K, p.N, p.w_up != nullptr);
     const qimg::LinearFusedScratch parts =
         qimg::linear_fused_scratch(plan, p.x_dtype, p.M, p.K, p.N, p.w_up != nullptr);
@@ -167,8 +169,6 @@ int qimg_rope_packed(const qimg_rope* args, void* stream) {
                               p.head_dim, p.rotary_dim);
     QIMG_REQUIRE(good_strides(p.x_stride_t, p.x_stride_h) && good_strides(p.out_stride_t, p.out_stride_h),
                  "%s: strides must be non-negative multiples of 8, token strides at most 2^24", fn);
-    QIMG_REQUIRE(static_cast<int64_t>(p.tokens) * p.n_heads * (p.head_dim / 8) < (int64_t{1} << 38), "%s: too many values",
-                 fn);
     if (p.tokens == 0 || p.n_heads == 0) return QIMG_OK;
     QIMG_REQUIRE(p.x && p.out && p.positions && (p.cos_sin || p.table_rows == 0), "%s: null pointer", fn);
     QIMG_REQUIRE(aligned16(p.x) && aligned16(p.out) && aligned16(p.cos_sin),

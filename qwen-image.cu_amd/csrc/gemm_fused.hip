@@ -760,37 +760,38 @@ template <bool F32>
 __global__ __launch_bounds__(256) void pack_rows_kernel(const void* __restrict__ in, int64_t ld, int64_t rows, int K,
                                                         int Kp, uint16_t* __restrict__ out) {
     const int per = Kp / 8;
-    const int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (idx >= rows * per) return;
-    const int64_t row = idx / per;
-    const int k = static_cast<int>(idx % per) * 8;
-    const float* f = static_cast<const float*>(in) + row * ld + k;
-    const uint16_t* h = static_cast<const uint16_t*>(in) + row * ld + k;
-    uint32_t w[4];
-    if (F32 && k + 8 <= K && (reinterpret_cast<uintptr_t>(f) & 15) == 0) {
-        const v4f lo = *reinterpret_cast<const v4f*>(f), hi = *reinterpret_cast<const v4f*>(f + 4);
-        w[0] = pack_bf16x2(lo[0], lo[1]);
-        w[1] = pack_bf16x2(lo[2], lo[3]);
-        w[2] = pack_bf16x2(hi[0], hi[1]);
-        w[3] = pack_bf16x2(hi[2], hi[3]);
-    } else {
-        uint16_t v[8];
+    for (int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; idx < rows * per;
+         idx += static_cast<int64_t>(gridDim.x) * 256) {
+        const int64_t row = idx / per;
+        const int k = static_cast<int>(idx % per) * 8;
+        const float* f = static_cast<const float*>(in) + row * ld + k;
+        const uint16_t* h = static_cast<const uint16_t*>(in) + row * ld + k;
+        uint32_t w[4];
+        if (F32 && k + 8 <= K && (reinterpret_cast<uintptr_t>(f) & 15) == 0) {
+            const v4f lo = *reinterpret_cast<const v4f*>(f), hi = *reinterpret_cast<const v4f*>(f + 4);
+            w[0] = pack_bf16x2(lo[0], lo[1]);
+            w[1] = pack_bf16x2(lo[2], lo[3]);
+            w[2] = pack_bf16x2(hi[0], hi[1]);
+            w[3] = pack_bf16x2(hi[2], hi[3]);
+        } else {
+            uint16_t v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = k + i < K ? (F32 ? f32_to_bf16(f[i]) : h[i]) : static_cast<uint16_t>(0);
+            for (int i = 0; i < 8; ++i) v[i] = k + i < K ? (F32 ? f32_to_bf16(f[i]) : h[i]) : static_cast<uint16_t>(0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = v[2 * i] | (static_cast<uint32_t>(v[2 * i + 1]) << 16);
+            for (int i = 0; i < 4; ++i) w[i] = v[2 * i] | (static_cast<uint32_t>(v[2 * i + 1]) << 16);
+        }
+        *reinterpret_cast<u32x4*>(out + row * Kp + k) = (u32x4){w[0], w[1], w[2], w[3]};
     }
-    *reinterpret_cast<u32x4*>(out + row * Kp + k) = (u32x4){w[0], w[1], w[2], w[3]};
 }
 
 hipError_t launch_pack(const void* in, bool f32, int64_t ld, int64_t rows, int K, int Kp, uint16_t* out,
                        hipStream_t stream) {
-    const int64_t total = rows * (Kp / 8);
-    const unsigned blocks = static_cast<unsigned>((total + 255) / 256);
+    const int64_t want = (rows * (Kp / 8) + 255) / 256, most = 1 << 22;  // (a grid has less than 2^32 threads)
+    const dim3 grid(static_cast<unsigned>(want < most ? want : most));
     if (f32)
-        hipLaunchKernelGGL(pack_rows_kernel<true>, dim3(blocks), dim3(256), 0, stream, in, ld, rows, K, Kp, out);
+        hipLaunchKernelGGL(pack_rows_kernel<true>, grid, dim3(256), 0, stream, in, ld, rows, K, Kp, out);
     else
-        hipLaunchKernelGGL(pack_rows_kernel<false>, dim3(blocks), dim3(256), 0, stream, in, ld, rows, K, Kp, out);
+        hipLaunchKernelGGL(pack_rows_kernel<false>, grid, dim3(256), 0, stream, in, ld, rows, K, Kp, out);
     return hipGetLastError();
 }
 

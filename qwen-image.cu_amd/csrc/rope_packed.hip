@@ -52,11 +52,9 @@ __device__ __forceinline__ void store4(void* p, int64_t i, v4f f) {
 // turned head take pairs (halves: values 4 i .. and r / 2 + 4 i ..;
 // interleaved: 8 i ..), the rest copy eight values.
 template <int IN, int OUT>
-__global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
+__device__ __forceinline__ void rope_eight(const RopeArgs& a, int64_t idx) {
     const int per = a.d / 8;
-    const int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     const int64_t th = idx / per;
-    if (th >= static_cast<int64_t>(a.tokens) * a.h) return;
     const int e = static_cast<int>(idx % per);
     const int64_t t = th / a.h;
     const int head = static_cast<int>(th % a.h);
@@ -95,10 +93,21 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
     store4<OUT>(a.out, o + i1, q);
 }
 
+constexpr int64_t kMaxBlocks = 1 << 22;  // (a grid has less than 2^32 threads)
+
+template <int IN, int OUT>
+__global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
+    const int64_t total = static_cast<int64_t>(a.tokens) * a.h * (a.d / 8);
+    for (int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; idx < total;
+         idx += static_cast<int64_t>(gridDim.x) * 256)
+        rope_eight<IN, OUT>(a, idx);
+}
+
 template <int IN>
 hipError_t launch_in(const RopeArgs& a, int out_dtype, hipStream_t stream) {
     const int64_t total = static_cast<int64_t>(a.tokens) * a.h * (a.d / 8);
-    const dim3 grid(static_cast<unsigned>((total + 255) / 256));
+    const int64_t blocks = (total + 255) / 256;
+    const dim3 grid(static_cast<unsigned>(blocks < kMaxBlocks ? blocks : kMaxBlocks));
     switch (out_dtype) {
     case QIMG_FP32: hipLaunchKernelGGL((rope_kernel<IN, QIMG_FP32>), grid, dim3(256), 0, stream, a); break;
     case QIMG_BF16: hipLaunchKernelGGL((rope_kernel<IN, QIMG_BF16>), grid, dim3(256), 0, stream, a); break;

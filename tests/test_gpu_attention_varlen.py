@@ -212,6 +212,25 @@ def test_constant_values_come_back_exactly(qimg, lq, lk):
         assert bool((got == 0.40625).all())
 
 
+def test_subnormal_values_are_kept(qimg):
+    """fp16 below 2^-14: V of one subnormal value comes back, and K of subnormals
+    gives the scores that they are."""
+    for lens in ([50], [1500, 700]):
+        q, k, v = _make(lens, lens, 28, 4, 64, torch.float16, 3)
+        v[:] = 3 * 2.0 ** -22
+        k = (k.float() * 2.0 ** -18).half()
+        q = (q.float() * 2.0 ** 10).half()
+        cu, c = _cu(lens)
+        got = qimg.attention_varlen(q, k, v, cu, cu, sm_scale=30.0)
+        torch.cuda.synchronize()
+        assert bool((got == 3 * 2.0 ** -22).all())
+        v = torch.randn(v.shape, device=DEV).half()
+        got = qimg.attention_varlen(q, k, v, cu, cu, sm_scale=30.0)
+        want, mag = _oracle(q, k, v, c, c, lens, 30.0, True)
+        torch.cuda.synchronize()
+        _check(got, want, mag, torch.float16)
+
+
 def test_growing_scores_rescale(qimg):
     """Scores that rise along the keys move the running maximum in every tile."""
     n, d = 700, 128

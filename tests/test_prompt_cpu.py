@@ -25,7 +25,8 @@ def _attn(qimg, **kw):
     (1, "dtype", dict(dtype=0)), (1, "bad sizes", dict(batch=-1)), (1, "bad sizes", dict(total_k=-1)),
     (1, "multiple", dict(n_heads=27)), (1, "multiple", dict(n_kv_heads=0)), (2, "head_dim", dict(head_dim=96)),
     (1, "sm_scale", dict(sm_scale=0.0)), (1, "sm_scale", dict(sm_scale=float("nan"))),
-    (1, "sm_scale", dict(sm_scale=float("inf"))), (1, "2^30", dict(total_q=1 << 28)),
+    (1, "sm_scale", dict(sm_scale=float("inf"))), (1, "2^30", dict(total_q=1 << 28)), (1, "2^30", dict(total_k=1 << 30)),
+    (1, "sm_scale", dict(sm_scale=3e38)), (1, "at least head_dim", dict(v_stride_t=64)),
     (1, "strides", dict(k_stride_t=516)), (1, "strides", dict(q_stride_h=-128)),
     (1, "strides", dict(v_stride_t=(1 << 24) + 8)), (1, "null", dict(q=None)), (1, "null", dict(v=None)),
     (1, "null", dict(cu_seqlens_k=None)), (1, "aligned", dict(k=FAKE + 8)), (1, "out must not", dict(out=FAKE)),
@@ -71,7 +72,7 @@ def _linear(qimg, scratch=None, scratch_bytes=0, **kw):
     (1, "ldx", dict(ldx=511)), (1, "ldx", dict(ldx=1 << 22)), (1, "ldo", dict(ldo=299)),
     (1, "16-byte aligned", dict(ldx=516)), (1, "ld_residual", dict(residual=FAKE * 3, ld_residual=10)),
     (1, "residual's place", dict(residual=FAKE * 2, ld_residual=300, residual_dtype=0)),
-    (1, "out must not", dict(out=FAKE)), (1, "too large", dict(N=1 << 22, ldo=1 << 22)),
+    (1, "out must not", dict(out=FAKE)), (1, "out must not", dict(out=FAKE * 3, w_up=FAKE * 3)), (1, "too large", dict(N=1 << 22, ldo=1 << 22)),
     (3, "scratch", dict(K=511, ldx=511)), (3, "scratch", dict(x_dtype=0)),
 ])
 def test_linear_fused_refuses(qimg, status, text, change):
