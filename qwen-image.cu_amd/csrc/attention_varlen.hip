@@ -671,11 +671,11 @@ struct TileStream {
     const uint8_t* p;
     int64_t left, step;
     uint32_t off[MK * D * 2 / 1024 / MW];  // a lane's byte offsets in a tile, one per DMA instruction
-    __device__ __forceinline__ void init(const uint16_t* base, int64_t stride, int lk, int wave) {
-        p = reinterpret_cast<const uint8_t*>(base);
-        step = 2 * MK * stride;
-        left = 2 * ((lk - 1) * stride + D);
-        if (lk == 0) left = 0;
+    // every `every`-th tile from tile `first` on
+    __device__ __forceinline__ void init(const uint16_t* base, int64_t stride, int lk, int first, int every, int wave) {
+        p = reinterpret_cast<const uint8_t*>(base + first * MK * stride);
+        step = 2 * MK * stride * every;
+        left = lk > first * MK ? 2 * ((lk - first * MK - 1) * stride + D) : 0;
         constexpr int RPI = 512 / D, CPR = D / 8;
         const int lane = threadIdx.x & 63;
 #pragma unroll
@@ -818,12 +818,6 @@ struct Many {
     }
 };
 
-// V(p) and M(p + 1) of one wave. Pair p + 1 has landed once every wave has
-// waited for its share (all but the newest pair's, p + 2) and met the barrier; behind the
-// second barrier all waves are done with it and pair p + 3 goes into its slot.
-// The slot comes as two restrict pointers, which tells the compiler that the
-// reads of `src` do not depend on the DMA into `dst`: the waits and barriers
-// see to that.
 __device__ __forceinline__ void phase_barrier() {
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("" ::: "memory");  // no LDS read or DMA moves across, whatever the compiler thinks of aliasing
@@ -832,16 +826,22 @@ __device__ __forceinline__ void phase_barrier() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
+// V(p) and M(p + 1) of one wave. Pair p + 1 has landed once every wave has
+// waited for its share (all but the newest pair's, p + 2) and met the barrier;
+// behind the second barrier all waves are done with it and pair p + 3 goes into
+// its slot. The slot comes as two restrict pointers, which tells the compiler
+// that the reads of `src` do not depend on the DMA into `dst`: the waits and
+// barriers see to that.
 template <class T, int D, bool MASKED>
 __device__ __forceinline__ void many_step(Many<T, D>& w, const uint8_t* __restrict src, uint8_t* __restrict dst,
-                                          TileStream<D, false>& ks, TileStream<D, true>& vs, float scale, int p,
-                                          int wave, int kmax, int& nonfinite) {
+                                          TileStream<D, false>& ks, TileStream<D, true>& vs, float scale,
+                                          int tile, int wave, int kmax, int& nonfinite) {
     using W = Many<T, D>;
     wait_vmcnt<W::PER>();
     phase_barrier();
     w.template read_group<0>(src, w.buf[0]);
     __builtin_amdgcn_sched_barrier(0);
-    w.template softmax<MASKED>(p * MK, kmax, scale);
+    w.template softmax<MASKED>(tile * MK, kmax, scale);
     // P is made in this phase: left to itself the compiler moves the
     // exponentials next to the MFMAs that read them
 #pragma unroll
@@ -851,7 +851,7 @@ __device__ __forceinline__ void many_step(Many<T, D>& w, const uint8_t* __restri
     __builtin_amdgcn_s_setprio(1);
     bool bad = false;
     w.template m_groups<0, MASKED>(src, bad);
-    if (MASKED && bad && nonfinite < 0) nonfinite = p;
+    if (MASKED && bad && nonfinite < 0) nonfinite = tile;
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_setprio(0);
     phase_barrier();
@@ -860,14 +860,49 @@ __device__ __forceinline__ void many_step(Many<T, D>& w, const uint8_t* __restri
     __builtin_amdgcn_sched_barrier(0);
 }
 
-template <class T, int D>
-__global__ __launch_bounds__(MW * 64, 2) void attn_many_kernel(AttnVarlenArgs a, int tiles) {
+// The step of two groups half a step apart: pair p + 2 into the slot that M(p) has
+// left, V(p), a barrier, M(p + 1), a barrier. The other group is one barrier
+// behind, so its V runs beside this M and the other way round.
+template <class T, int D, bool MASKED>
+__device__ __forceinline__ void group_step(Many<T, D>& w, const uint8_t* __restrict src, uint8_t* __restrict dst,
+                                           TileStream<D, false>& ks, TileStream<D, true>& vs, float scale, int tile,
+                                           int wave, int kmax, int& nonfinite) {
     using W = Many<T, D>;
-    constexpr int PAIR = 2 * W::TB;
-    __shared__ __attribute__((aligned(1024))) uint8_t ring[MSLOT * PAIR];
+    vs.issue(dst, wave);
+    ks.issue(dst + W::TB, wave);
+    __builtin_amdgcn_sched_barrier(0);
+    w.template softmax<MASKED>(tile * MK, kmax, scale);
+#pragma unroll
+    for (int i = 0; i < 8 * W::KB; ++i) asm volatile("" : "+v"(w.pk[i]));  // as in many_step
+    asm volatile("" : "+v"(w.sum));
+    __builtin_amdgcn_sched_barrier(0);
+    wait_vmcnt<W::PER>();  // this wave's share of pair p + 1
+    phase_barrier();
+    __builtin_amdgcn_s_setprio(1);
+    w.template read_group<0>(src, w.buf[0]);
+    bool bad = false;
+    w.template m_groups<0, MASKED>(src, bad);
+    if (MASKED && bad && nonfinite < 0) nonfinite = tile;
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(0);
+    phase_barrier();
+}
+
+// KG = 1: as above. KG = 2, for launches of few tiles, whose workgroups have a CU
+// each: eight waves, two groups of four that take the 64-key tiles in turn, each
+// with a ring of its own, half a step apart; the groups' (O, m, sum) are joined
+// through LDS (the lanes of waves w and w + 4 hold the same rows and channels).
+template <class T, int D, int KG>
+__global__ __launch_bounds__(KG * MW * 64, 2) void attn_many_kernel(AttnVarlenArgs a, int tiles) {
+    using W = Many<T, D>;
+    constexpr int PAIR = 2 * W::TB, RING = MSLOT * PAIR, CHUNKS = D / 8;
+    constexpr int JOIN = KG == 2 ? MW * 64 * (D / 2 + 2) * 4 : 0;  // a group's O, m and sum
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[KG * RING > JOIN ? KG * RING : JOIN];
 
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = KG == 1 ? wave_all : wave_all % MW, kg = KG == 1 ? 0 : wave_all / MW;
+    uint8_t* const ring = lds + kg * RING;
     const int l32 = lane & 31, half = lane >> 5;
     // Causal: the sequences' last, longest tiles first, the heads of one tile
     // side by side (a head stays on few XCDs as workgroups go round-robin over
@@ -891,8 +926,8 @@ __global__ __launch_bounds__(MW * 64, 2) void attn_many_kernel(AttnVarlenArgs a,
     const int head = hk * a.group + row % a.group;
     const int kmax = visible(a, t, token);
     const int kend = visible(a, t, (min(t.row0 + MR, rows) - 1) / a.group);  // of the whole tile
-    const int n = (kend + MK - 1) / MK;
-    const int nfull = visible(a, t, t.row0 / a.group) / MK;  // tiles that every row sees whole
+    const int n = (kend + MK * KG - 1) / (MK * KG);                          // steps
+    const int nfull = visible(a, t, t.row0 / a.group) / (MK * KG);           // of tiles that every row sees whole
 
     W w;
     {
@@ -918,8 +953,8 @@ __global__ __launch_bounds__(MW * 64, 2) void attn_many_kernel(AttnVarlenArgs a,
 
     TileStream<D, false> ks;
     TileStream<D, true> vs;
-    ks.init(kbase, a.k_t, t.lk, wave);
-    vs.init(vbase, a.v_t, t.lk, wave);
+    ks.init(kbase, a.k_t, t.lk, kg, KG, wave);
+    vs.init(vbase, a.v_t, t.lk, kg, KG, wave);
     // pairs 0 (no V) and 1, then the scores of tile 0 and pair 2 in its place
     ks.issue(ring + W::TB, wave);
     vs.issue(ring + PAIR, wave);
@@ -928,20 +963,62 @@ __global__ __launch_bounds__(MW * 64, 2) void attn_many_kernel(AttnVarlenArgs a,
     phase_barrier();
     w.template first_scores<W::NPV>(ring);
     phase_barrier();
-    vs.issue(ring, wave);
-    ks.issue(ring + W::TB, wave);
     int p = 0;
-    for (; p < nfull; ++p)
-        many_step<T, D, false>(w, ring + ((p + 1) % MSLOT) * PAIR, ring + ((p + 1) % MSLOT) * PAIR, ks, vs, a.scale_log2, p,
-                               wave, kmax, nonfinite);
-    for (; p < n; ++p)
-        many_step<T, D, true>(w, ring + ((p + 1) % MSLOT) * PAIR, ring + ((p + 1) % MSLOT) * PAIR, ks, vs, a.scale_log2, p,
-                               wave, kmax, nonfinite);
+    if constexpr (KG == 1) {
+        vs.issue(ring, wave);
+        ks.issue(ring + W::TB, wave);
+        for (; p < nfull; ++p)
+            many_step<T, D, false>(w, ring + ((p + 1) % MSLOT) * PAIR, ring + ((p + 1) % MSLOT) * PAIR, ks, vs,
+                                   a.scale_log2, p, wave, kmax, nonfinite);
+        for (; p < n; ++p)
+            many_step<T, D, true>(w, ring + ((p + 1) % MSLOT) * PAIR, ring + ((p + 1) % MSLOT) * PAIR, ks, vs,
+                                  a.scale_log2, p, wave, kmax, nonfinite);
+    } else {
+        if (kg == 1) phase_barrier();
+        for (; p < nfull; ++p)
+            group_step<T, D, false>(w, ring + ((p + 1) % MSLOT) * PAIR, ring + (p % MSLOT) * PAIR, ks, vs, a.scale_log2,
+                                    KG * p + kg, wave, kmax, nonfinite);
+        for (; p < n; ++p)
+            group_step<T, D, true>(w, ring + ((p + 1) % MSLOT) * PAIR, ring + (p % MSLOT) * PAIR, ks, vs, a.scale_log2,
+                                   KG * p + kg, wave, kmax, nonfinite);
+        if (kg == 0) phase_barrier();
+    }
     wait_vmcnt<0>();  // the loads past the last tile no longer write the ring
-    if (nonfinite >= 0) add_nonfinite<T, W::DT>(vbase, a.v_t, nonfinite * MK, kmax, w.o);
+    if (nonfinite >= 0)
+        for (int tile = nonfinite; tile * MK < kmax; tile += KG)
+            add_nonfinite<T, W::DT>(vbase, a.v_t, tile * MK, min(tile * MK + MK, kmax), w.o);
+    float tot = half_sum(w.sum);
+
+    if constexpr (KG == 2) {
+        __syncthreads();
+        float* const part = reinterpret_cast<float*>(lds) + wave * 64 * (D / 2 + 2);
+        if (kg == 1) {
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c)
+                *reinterpret_cast<v4f*>(part + (c * 64 + lane) * 4) =
+                    (v4f){w.o[c / 4][c % 4 * 4], w.o[c / 4][c % 4 * 4 + 1], w.o[c / 4][c % 4 * 4 + 2],
+                          w.o[c / 4][c % 4 * 4 + 3]};
+            part[64 * (D / 2) + lane] = w.m;
+            part[64 * (D / 2) + 64 + lane] = tot;
+        }
+        __syncthreads();
+        if (kg == 1) return;
+        const float m1 = part[64 * (D / 2) + lane], t1 = part[64 * (D / 2) + 64 + lane];
+        const float top = fmaxf(w.m, m1);
+        // no finite score in a group: its O is zero, its sum zero or NaN
+        const float f0 = w.m == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(w.m - top);
+        const float f1 = m1 == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m1 - top);
+        tot = tot * f0 + t1 * f1;
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            const v4f x = *reinterpret_cast<const v4f*>(part + (c * 64 + lane) * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                w.o[c / 4][c % 4 * 4 + e] = w.o[c / 4][c % 4 * 4 + e] * f0 + x[e] * f1;
+        }
+    }
 
     if (!valid) return;
-    const float tot = half_sum(w.sum);
     const float inv = 1.0f / tot;
     // channels 8 (g + half) .. of block d after the lane halves have exchanged
     // their four of g and g + 1
@@ -971,10 +1048,13 @@ int64_t tile_bound(int total_q, int batch, int group, int rows) {
 
 }  // namespace
 
-constexpr int kManyTiles = 200;
+constexpr int kGroupTiles = 256;  // workgroups of two groups that run at once, one a CU
 constexpr int kFewGrid = 512;  // workgroups of the few-row kernel, two a CU
 
-// Tiles of 128 rows, or of 32.
+// Tiles of 128 rows, or of 32: from 160 tiles of 128 on (28 heads, causal, us, 32 /
+// 128 rows: 512 tokens, 112 tiles, 12.6 / 17.2; 781, 172, 21.0 / 20.6; 1024, 224, 25.7 /
+// 23.1; 24 heads of 600, 120, 15.7 / 19.2).
+constexpr int kManyTiles = 160;
 static bool attn_varlen_many(int total_q, int batch, int hq, int hk) {
     return tile_bound(total_q, batch, hq / hk, MR) * hk >= kManyTiles;
 }
@@ -1003,7 +1083,14 @@ static hipError_t launch_few(const AttnVarlenArgs& a, hipStream_t stream) {
 template <class T, int D>
 static hipError_t launch_many(const AttnVarlenArgs& a, hipStream_t stream) {
     const int tiles = static_cast<int>(tile_bound(a.total_q, a.batch, a.group, MR));
-    hipLaunchKernelGGL((attn_many_kernel<T, D>), dim3(tiles * a.hk), dim3(MW * 64), 0, stream, a, tiles);
+    // Two groups a tile while that is about one round of workgroups (a causal launch's
+    // tiles have half the keys on average). 28 heads, causal, us, one group / two:
+    // 1024 tokens (224 tiles) 27.6 / 23.1, 1500 39.8 / 33.8, 2048 (448) 51.6 / 46.9,
+    // 3000 (660) 80 / 89; 24 heads, all keys, 1301 tokens (264) 38.4 / 52.4.
+    if (tiles * a.hk <= (a.causal ? 2 * kGroupTiles : kGroupTiles))
+        hipLaunchKernelGGL((attn_many_kernel<T, D, 2>), dim3(tiles * a.hk), dim3(2 * MW * 64), 0, stream, a, tiles);
+    else
+        hipLaunchKernelGGL((attn_many_kernel<T, D, 1>), dim3(tiles * a.hk), dim3(MW * 64), 0, stream, a, tiles);
     return hipGetLastError();
 }
 

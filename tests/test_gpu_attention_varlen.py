@@ -98,7 +98,7 @@ def test_head_groups(qimg, hq, hk, lens):
     _run(qimg, lens, lens, hq=hq, hk=hk, seed=hq)
 
 
-@pytest.mark.parametrize("lens", [[1500, 1], [700, 1301, 64, 257], [2048]], ids=str)
+@pytest.mark.parametrize("lens", [[1500, 1], [700, 1301, 64, 257], [2048], [1000], [2600]], ids=str)
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("causal", [True, False])
 def test_many_rows(qimg, lens, d, causal):
@@ -107,7 +107,7 @@ def test_many_rows(qimg, lens, d, causal):
 
 
 @pytest.mark.parametrize("lq,lk", [([1, 1, 1], [1, 700, 33]), ([1] * 5, [4097, 0, 64, 1, 2000]), ([3, 40], [3000, 41]),
-                                   ([200, 300], [1000, 300]), ([1], [20000])], ids=str)
+                                   ([200, 300], [1000, 300]), ([1], [20000]), ([900], [1700]), ([2000, 700], [2100, 3000])], ids=str)
 @pytest.mark.parametrize("d", [64, 128])
 def test_cached_keys(qimg, lq, lk, d):
     """More keys than queries, a cache with room behind the last key, and few
@@ -117,7 +117,7 @@ def test_cached_keys(qimg, lq, lk, d):
         _run(qimg, lq, lk, d=d, dtype=dtype, slots=[n + 37 for n in lk], seed=sum(lk) + 1)
 
 
-@pytest.mark.parametrize("lq,lk", [([40, 5], [8, 5]), ([600], [100]), ([33], [1]), ([20], [0])], ids=str)
+@pytest.mark.parametrize("lq,lk", [([40, 5], [8, 5]), ([600], [100]), ([33], [1]), ([20], [0]), ([1900], [65]), ([2900], [700])], ids=str)
 def test_rows_that_see_no_key_are_zero(qimg, lq, lk):
     got = _run(qimg, lq, lk)
     if lq[0] > lk[0]:
@@ -147,7 +147,7 @@ def test_strided_views_and_rows_of_no_sequence(qimg, lens):
     assert bool((got[n:] == 7.0).all())
 
 
-@pytest.mark.parametrize("n", [45, 200, 1800])
+@pytest.mark.parametrize("n", [45, 200, 1800, 2600])
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
 def test_values_in_hidden_places_do_not_reach_a_row(qimg, n, value):
     """Row i sees keys 0 .. i: a NaN or infinite K and V row at key j changes
