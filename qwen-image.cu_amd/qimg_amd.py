@@ -647,7 +647,12 @@ _NO_SWITCH = _NoSwitch()
 
 def _on(device):
     """The device of a call's tensors made current for it (nothing to do where it is already)."""
-    return _NO_SWITCH if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _NO_SWITCH if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
+
+
+def _new(rows: int, cols: int, inner: int, dtype, device) -> torch.Tensor:
+    """A contiguous [rows, cols, inner] tensor (with its strides given torch.empty's 1.65 us are 1.3)."""
+    return torch.empty_strided((rows, cols, inner), (cols * inner, inner, 1), dtype=dtype, device=device)
 
 
 def _raw_stream(device):
@@ -718,15 +723,15 @@ def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
             raise QimgError(QIMG_ERR_INVALID_ARG, "cu_seqlens_q, cu_seqlens_k and k_lens must be contiguous int32")
     if out is None:
-        out = q.new_empty((tq, hq, d))
+        out = _new(tq, hq, d, dt, dev)
     elif out.shape != q.shape or out.dtype != dt:
         raise QimgError(QIMG_ERR_INVALID_ARG, f"out must be {tuple(q.shape)} of q's type")
     with _on(dev):
         scratch = _scratch_for(_lib.qimg_attention_varlen_scratch_bytes(tq, tk, batch, hq, hk, d), scratch, dev)
         args = _AttnVarlen(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _DT[dt],
                            *_head_strides(q, tq, hq, d), *_head_strides(k, tk, hk, d), *_head_strides(v, tk, hk, d),
-                           *_head_strides(out, tq, hq, d), _addr(cu_seqlens_q), _addr(cu_seqlens_k), _addr(k_lens), batch, tq, tk, hq, hk,
-                           d, 1.0 / d ** 0.5 if sm_scale is None else sm_scale, bool(causal))
+                           *_head_strides(out, tq, hq, d), cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
+                           _addr(k_lens), batch, tq, tk, hq, hk, d, 1.0 / d ** 0.5 if sm_scale is None else sm_scale, bool(causal))
         _check(_lib.qimg_attention_varlen(ctypes.byref(args), _addr(scratch), _nbytes(scratch), _raw_stream(dev)))
     return out
 
@@ -777,7 +782,7 @@ def linear_forward_bf16_fused(x: torch.Tensor, weight: torch.Tensor, bias: torch
     if activation not in ACTIVATIONS:
         raise QimgError(QIMG_ERR_INVALID_ARG, f"activation {activation!r} must be one of {sorted(ACTIVATIONS)}")
     if out is None:
-        out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+        out = torch.empty_strided((M, N), (N, 1), dtype=out_dtype, device=dev)
     for t, name in ((out, "out"), (residual, "residual")):
         if t is not None and (t.shape != (M, N) or t.dtype not in (torch.float32, torch.bfloat16)
                               or (N > 1 and t.stride(1) != 1)):
@@ -817,7 +822,7 @@ def rope_packed(x: torch.Tensor, cos_sin: torch.Tensor, positions: torch.Tensor,
     _same_device(dev, cos_sin, positions, out)
     T, H, D = x.shape
     if out is None:
-        out = torch.empty((T, H, D), dtype=out_dtype or x.dtype, device=dev)
+        out = _new(T, H, D, out_dtype or x.dtype, dev)
     elif out.shape != x.shape:
         raise QimgError(QIMG_ERR_INVALID_ARG, f"out must be {tuple(x.shape)}")
     if x.dtype not in _HEAD_TYPES or out.dtype not in _HEAD_TYPES:
