@@ -51,7 +51,11 @@ constexpr float kBias16 = 7.0f;  // log2 of the factor on fp16 P
 constexpr int kRsrcWord3 = 0x00020000;  // raw unswizzled buffer (gfx9 family)
 
 // element type: fragment vector, MFMA, P pair packing and its row sum, and
-// the mask of a value's exponent bits (all ones: infinity or NaN)
+// the mask of a value's exponent bits (all ones: infinity or NaN). The row sum is
+// a matrix product as well: with A = 1 an element of 4x4x4's column j is the sum of
+// the four values that lane j of its group of four holds. (16 dot products of pairs a
+// tile, v_dot2, take 107 cycles alone, but 620 beside another wave's MFMAs, which they
+// wait for; eight of these 4x4x4 take 88. Together 1-3% of the kernel's time.)
 struct Bf16 {
     using frag = v8bf;
     static constexpr float kPBias = 0.0f;
@@ -61,10 +65,11 @@ struct Bf16 {
     }
     __device__ static __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
     __device__ static __forceinline__ uint32_t pack_p(float a, float b) { return pack_bf16x2(a, b); }
-    __device__ static __forceinline__ float add2(uint32_t p, float s) {
-        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, p), __builtin_bit_cast(b2, 0x3f803f80u), s,
-                                               false);
+    __device__ static __forceinline__ v4f add4(uint32_t p0, uint32_t p1, v4f s) {
+        constexpr short one = 0x3f80;
+        return __builtin_amdgcn_mfma_f32_4x4x4bf16_1k((v4s){one, one, one, one},
+                                                      __builtin_bit_cast(v4s, static_cast<uint64_t>(p1) << 32 | p0), s,
+                                                      0, 0, 0);
     }
 };
 struct Fp16 {
@@ -86,9 +91,12 @@ struct Fp16 {
     __device__ static __forceinline__ uint32_t pack_p(float a, float b) {
         return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
     }
-    __device__ static __forceinline__ float add2(uint32_t p, float s) {
-        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-        return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, p), __builtin_bit_cast(h2, 0x3c003c00u), s, false);
+    __device__ static __forceinline__ v4f add4(uint32_t p0, uint32_t p1, v4f s) {
+        typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+        constexpr _Float16 one = 1;
+        return __builtin_amdgcn_mfma_f32_4x4x4f16((h4){one, one, one, one},
+                                                  __builtin_bit_cast(h4, static_cast<uint64_t>(p1) << 32 | p0), s, 0, 0,
+                                                  0);
     }
 };
 
@@ -419,7 +427,8 @@ __device__ __forceinline__ void few_item(const AttnVarlenArgs& a, const RowTile&
     for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
-    float m = kNegInf, sum = 0.0f;
+    float m = kNegInf;
+    v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};  // all four the same
     int nonfinite = -1;  // first of this wave's tiles whose V was sanitized
     int voff[DT];
 #pragma unroll
@@ -483,10 +492,8 @@ __device__ __forceinline__ void few_item(const AttnVarlenArgs& a, const RowTile&
         const float neg = (m == kNegInf ? 0.0f : -m) + T::kPBias;
         uint32_t pk[8];
 #pragma unroll
-        for (int r = 0; r < 16; r += 2) {
+        for (int r = 0; r < 16; r += 2)
             pk[r / 2] = T::pack_p(__builtin_amdgcn_exp2f(p[r] + neg), __builtin_amdgcn_exp2f(p[r + 1] + neg));
-            sum = T::add2(pk[r / 2], sum);
-        }
         __builtin_amdgcn_sched_barrier(0);
         wait_vmcnt<(2 * NS - 1) * P>();  // V of tile i
         __builtin_amdgcn_sched_barrier(0);
@@ -516,6 +523,8 @@ __device__ __forceinline__ void few_item(const AttnVarlenArgs& a, const RowTile&
                                                            static_cast<int>(pk[4 * g + 2]), static_cast<int>(pk[4 * g + 3])});
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[d] = T::mma(vf[g][d], pf, o[d]);
+            sum = T::add4(pk[4 * g], pk[4 * g + 1], sum);
+            sum = T::add4(pk[4 * g + 2], pk[4 * g + 3], sum);
         }
     }
     wait_vmcnt<0>();  // the loads past the last tile no longer write the ring
@@ -524,7 +533,7 @@ __device__ __forceinline__ void few_item(const AttnVarlenArgs& a, const RowTile&
             add_nonfinite<T, DT>(vbase, a.v_t, key_of(i), min(key_of(i) + SK, kmax), o);
 
     // the waves' shares: O into the wave's own LDS, m and sum behind all of it
-    sum = half_sum(sum);
+    const float own = half_sum(sum[0]);
     float* osh = reinterpret_cast<float*>(ring + wave * WB);
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -534,7 +543,7 @@ __device__ __forceinline__ void few_item(const AttnVarlenArgs& a, const RowTile&
                 (v4f){o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
     if (half == 0) {
         ml[wave][l32][0] = m;
-        ml[wave][l32][1] = sum;
+        ml[wave][l32][1] = own;
     }
     __syncthreads();
 
@@ -658,7 +667,12 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnVarlenArgs a) {
 // exponentials run beside the other's MFMAs. V begins with the fragment reads of
 // the next M's first MFMAs, M reads a group of four fragments ahead. (Two groups
 // ahead, with a third buffer, measured 1-2% slower, without the matrix phase's
-// priority 2 x 24 heads of 4352 took 2% more, 1301 tokens 20% more.)
+// priority 2 x 24 heads of 4352 took 2% more, 1301 tokens 20% more.) The DMA
+// instructions are spread over V's exponentials: sent in one go a wave's eight
+// took 460 cycles of the step's 3070, 16 each of the CU's address unit (2 x 24
+// heads of 4352 and 4173 tokens, bf16: 462 -> 450 us; one barrier a step instead
+// of two: 441). A tile now takes a wave 1330 cycles of V, 1290 of M (1104 of
+// them MFMA) and 200 at the barrier, two workgroups' together 2890.
 constexpr int MR = 128, MW = 4, MK = 64, MSLOT = 2;
 
 // The K or V tiles of one head in turn: `p` the next tile's first row, `left`
@@ -685,18 +699,24 @@ struct TileStream {
             off[i] = static_cast<uint32_t>(row) * static_cast<uint32_t>(stride) * 2u + c * 16;
         }
     }
-    __device__ __forceinline__ void issue(uint8_t* dst, int wave) {
+    static constexpr int N = MK * D * 2 / 1024 / MW;  // DMA instructions of a wave
+    // instruction i of the next tile; the last one moves on
+    __device__ __forceinline__ void issue_one(int i, uint8_t* dst, int wave) {
 #if defined(__HIP_DEVICE_COMPILE__)  // (the host pass rejects the builtin, and with it the kernels that share this)
         const int64_t n = left < 0 ? 0 : left > 0x7fffffff ? 0x7fffffff : left;
         const __amdgpu_buffer_rsrc_t r =
             __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, static_cast<int>(n), kRsrcWord3);
-#pragma unroll
-        for (int i = 0; i < MK * D * 2 / 1024 / MW; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                r, (__attribute__((address_space(3))) void*)(dst + (wave + MW * i) * 1024), 16, off[i], 0, 0, 0);
-        p += step;
-        left -= step;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            r, (__attribute__((address_space(3))) void*)(dst + (wave + MW * i) * 1024), 16, off[i], 0, 0, 0);
+        if (i == N - 1) {
+            p += step;
+            left -= step;
+        }
 #endif
+    }
+    __device__ __forceinline__ void issue(uint8_t* dst, int wave) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) issue_one(i, dst, wave);
     }
 };
 
@@ -712,7 +732,8 @@ struct Many {
     frag qf[KS], buf[2][4];
     uint32_t pk[8 * KB];  // P: 16-key group g at pk[4 g ..]
     int voff[DT], koff[KS];  // lane offsets of V reads (channel block), K reads (k-step)
-    float m, sum;
+    float m;
+    v4f sum;  // all four the same
 
     // fragments of group j: PV units (16-key group u / DT, channel block
     // u % DT), then score units (k-step u / KB, key block u % KB)
@@ -744,6 +765,10 @@ struct Many {
             if constexpr (j < NPV) {
                 const int u = 4 * j + i;
                 o[u % DT] = T::mma(f[i], p_frag(u / DT), o[u % DT]);
+                if (u % (DT / 2) == 0) {
+                    const int r = 4 * (u / DT) + 2 * (u % DT != 0);
+                    sum = T::add4(pk[r], pk[r + 1], sum);
+                }
             } else {
                 const int u = 4 * (j - NPV) + i;
                 s[u % KB] = T::mma(f[i], qf[u / KB], s[u % KB]);
@@ -782,8 +807,9 @@ struct Many {
         }
     }
 
-    template <bool MASKED>
-    __device__ __forceinline__ void softmax(int key0, int kmax, float c) {
+    // dma(i), i < PER: the next DMA instructions, spread over the exponentials
+    template <bool MASKED, class Dma>
+    __device__ __forceinline__ void softmax(int key0, int kmax, float c, Dma&& dma) {
         const int half = (threadIdx.x & 63) >> 5;
         if constexpr (MASKED) {
 #pragma unroll
@@ -810,10 +836,14 @@ struct Many {
         const float neg = (m == kNegInf ? 0.0f : -m) + T::kPBias;
 #pragma unroll
         for (int r = 0; r < 16 * KB; r += 2) {
+            if (r % (16 * KB / PER) == 0) {
+                __builtin_amdgcn_sched_barrier(0);
+                dma(r / (16 * KB / PER));
+                __builtin_amdgcn_sched_barrier(0);
+            }
             const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r >> 4][r & 15], c, neg));
             const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r >> 4][(r & 15) + 1], c, neg));
             pk[r / 2] = T::pack_p(p0, p1);
-            sum = T::add2(pk[r / 2], sum);
         }
     }
 };
@@ -826,72 +856,44 @@ __device__ __forceinline__ void phase_barrier() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// V(p) and M(p + 1) of one wave. Pair p + 1 has landed once every wave has
-// waited for its share (all but the newest pair's, p + 2) and met the barrier;
-// behind the second barrier all waves are done with it and pair p + 3 goes into
-// its slot. The slot comes as two restrict pointers, which tells the compiler
-// that the reads of `src` do not depend on the DMA into `dst`: the waits and
-// barriers see to that.
-template <class T, int D, bool MASKED>
+// V(p) and M(p + 1) of one wave. Behind the barrier every wave has done M(p),
+// whose slot takes pair p + 2 during V(p), and pair p + 1, sent during V(p - 1),
+// has landed. The slots come as restrict pointers, which tells the compiler that
+// the reads of `src` do not depend on the DMA into `dst`: the waits and barriers
+// see to that. PHASED: a second barrier between V and M.
+template <class T, int D, bool MASKED, bool PHASED>
 __device__ __forceinline__ void many_step(Many<T, D>& w, const uint8_t* __restrict src, uint8_t* __restrict dst,
-                                          TileStream<D, false>& ks, TileStream<D, true>& vs, float scale,
-                                          int tile, int wave, int kmax, int& nonfinite) {
+                                          TileStream<D, false>& ks, TileStream<D, true>& vs, float scale, int tile,
+                                          int wave, int kmax, int& nonfinite) {
     using W = Many<T, D>;
-    wait_vmcnt<W::PER>();
+    wait_vmcnt<0>();
     phase_barrier();
     w.template read_group<0>(src, w.buf[0]);
     __builtin_amdgcn_sched_barrier(0);
-    w.template softmax<MASKED>(tile * MK, kmax, scale);
+    w.template softmax<MASKED>(tile * MK, kmax, scale, [&](int i) {
+        if (i < W::PER / 2)
+            vs.issue_one(i, dst, wave);
+        else
+            ks.issue_one(i - W::PER / 2, dst + W::TB, wave);
+    });
     // P is made in this phase: left to itself the compiler moves the
     // exponentials next to the MFMAs that read them
 #pragma unroll
     for (int i = 0; i < 8 * W::KB; ++i) asm volatile("" : "+v"(w.pk[i]));
-    asm volatile("" : "+v"(w.sum));
     __builtin_amdgcn_sched_barrier(0);
+    if (PHASED) phase_barrier();
     __builtin_amdgcn_s_setprio(1);
     bool bad = false;
     w.template m_groups<0, MASKED>(src, bad);
     if (MASKED && bad && nonfinite < 0) nonfinite = tile;
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_setprio(0);
-    phase_barrier();
-    vs.issue(dst, wave);
-    ks.issue(dst + W::TB, wave);
-    __builtin_amdgcn_sched_barrier(0);
-}
-
-// The step of two groups half a step apart: pair p + 2 into the slot that M(p) has
-// left, V(p), a barrier, M(p + 1), a barrier. The other group is one barrier
-// behind, so its V runs beside this M and the other way round.
-template <class T, int D, bool MASKED>
-__device__ __forceinline__ void group_step(Many<T, D>& w, const uint8_t* __restrict src, uint8_t* __restrict dst,
-                                           TileStream<D, false>& ks, TileStream<D, true>& vs, float scale, int tile,
-                                           int wave, int kmax, int& nonfinite) {
-    using W = Many<T, D>;
-    vs.issue(dst, wave);
-    ks.issue(dst + W::TB, wave);
-    __builtin_amdgcn_sched_barrier(0);
-    w.template softmax<MASKED>(tile * MK, kmax, scale);
-#pragma unroll
-    for (int i = 0; i < 8 * W::KB; ++i) asm volatile("" : "+v"(w.pk[i]));  // as in many_step
-    asm volatile("" : "+v"(w.sum));
-    __builtin_amdgcn_sched_barrier(0);
-    wait_vmcnt<W::PER>();  // this wave's share of pair p + 1
-    phase_barrier();
-    __builtin_amdgcn_s_setprio(1);
-    w.template read_group<0>(src, w.buf[0]);
-    bool bad = false;
-    w.template m_groups<0, MASKED>(src, bad);
-    if (MASKED && bad && nonfinite < 0) nonfinite = tile;
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_setprio(0);
-    phase_barrier();
 }
 
 // KG = 1: as above. KG = 2, for launches of few tiles, whose workgroups have a CU
 // each: eight waves, two groups of four that take the 64-key tiles in turn, each
-// with a ring of its own, half a step apart; the groups' (O, m, sum) are joined
-// through LDS (the lanes of waves w and w + 4 hold the same rows and channels).
+// with a ring of its own, a phase apart: the second barrier keeps one group's V
+// beside the other's M; the groups' (O, m, sum) are joined through LDS (the lanes of waves w and w + 4 hold the same rows and channels).
 template <class T, int D, int KG>
 __global__ __launch_bounds__(KG * MW * 64, 2) void attn_many_kernel(AttnVarlenArgs a, int tiles) {
     using W = Many<T, D>;
@@ -944,7 +946,7 @@ __global__ __launch_bounds__(KG * MW * 64, 2) void attn_many_kernel(AttnVarlenAr
 #pragma unroll
     for (int r = 0; r < 16 * W::KB; ++r) w.s[r >> 4][r & 15] = 0.0f;
     w.m = kNegInf;
-    w.sum = 0.0f;
+    w.sum = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int d = 0; d < W::DT; ++d) w.voff[d] = v_lane_off<D>(d);
 #pragma unroll
@@ -962,32 +964,20 @@ __global__ __launch_bounds__(KG * MW * 64, 2) void attn_many_kernel(AttnVarlenAr
     wait_vmcnt<W::PER>();
     phase_barrier();
     w.template first_scores<W::NPV>(ring);
-    phase_barrier();
     int p = 0;
-    if constexpr (KG == 1) {
-        vs.issue(ring, wave);
-        ks.issue(ring + W::TB, wave);
-        for (; p < nfull; ++p)
-            many_step<T, D, false>(w, ring + ((p + 1) % MSLOT) * PAIR, ring + ((p + 1) % MSLOT) * PAIR, ks, vs,
-                                   a.scale_log2, p, wave, kmax, nonfinite);
-        for (; p < n; ++p)
-            many_step<T, D, true>(w, ring + ((p + 1) % MSLOT) * PAIR, ring + ((p + 1) % MSLOT) * PAIR, ks, vs,
-                                  a.scale_log2, p, wave, kmax, nonfinite);
-    } else {
-        if (kg == 1) phase_barrier();
-        for (; p < nfull; ++p)
-            group_step<T, D, false>(w, ring + ((p + 1) % MSLOT) * PAIR, ring + (p % MSLOT) * PAIR, ks, vs, a.scale_log2,
-                                    KG * p + kg, wave, kmax, nonfinite);
-        for (; p < n; ++p)
-            group_step<T, D, true>(w, ring + ((p + 1) % MSLOT) * PAIR, ring + (p % MSLOT) * PAIR, ks, vs, a.scale_log2,
-                                   KG * p + kg, wave, kmax, nonfinite);
-        if (kg == 0) phase_barrier();
-    }
+    if (KG == 2 && kg == 1) phase_barrier();
+    for (; p < nfull; ++p)
+        many_step<T, D, false, KG == 2>(w, ring + ((p + 1) % MSLOT) * PAIR, ring + (p % MSLOT) * PAIR, ks, vs,
+                                        a.scale_log2, KG * p + kg, wave, kmax, nonfinite);
+    for (; p < n; ++p)
+        many_step<T, D, true, KG == 2>(w, ring + ((p + 1) % MSLOT) * PAIR, ring + (p % MSLOT) * PAIR, ks, vs,
+                                       a.scale_log2, KG * p + kg, wave, kmax, nonfinite);
+    if (KG == 2 && kg == 0) phase_barrier();
     wait_vmcnt<0>();  // the loads past the last tile no longer write the ring
     if (nonfinite >= 0)
         for (int tile = nonfinite; tile * MK < kmax; tile += KG)
             add_nonfinite<T, W::DT>(vbase, a.v_t, tile * MK, min(tile * MK + MK, kmax), w.o);
-    float tot = half_sum(w.sum);
+    float tot = half_sum(w.sum[0]);
 
     if constexpr (KG == 2) {
         __syncthreads();
