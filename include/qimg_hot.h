@@ -252,8 +252,9 @@ int qimg_sage_attention(const uint16_t* q_f16, const uint16_t* k_f16, const uint
  * overlaps none of q, k, v. total_q * n_heads and total_k below 2^30; k and v
  * token strides at least head_dim.
  * scratch: qimg_attention_varlen_scratch_bytes(...) bytes (may be 0: NULL) for
- * this call's sizes; fewer queries can need more (their keys are split). One
- * scratch buffer serves one call at a time. */
+ * this call's sizes; fewer queries can need more (their keys are split), and
+ * so can causal 0 (the last tiles' keys are). One scratch buffer serves one
+ * call at a time. */
 typedef struct {
     const void* q;
     const void* k;
@@ -269,7 +270,7 @@ typedef struct {
     int causal;
 } qimg_attn_varlen;
 int64_t qimg_attention_varlen_scratch_bytes(int total_q, int total_k, int batch, int n_heads, int n_kv_heads,
-                                            int head_dim);
+                                            int head_dim, int causal);
 int qimg_attention_varlen(const qimg_attn_varlen* args, void* scratch, int64_t scratch_bytes, void* stream);
 
 /* ---- prompts: bf16 linear with its epilogue ------------------------------ */

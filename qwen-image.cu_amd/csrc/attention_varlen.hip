@@ -32,6 +32,8 @@
 // there (another sequence, an unused part of a cache) reaches the result, NaN
 // included. Every tile has a descriptor of its own (64-bit base), so offsets
 // inside one stay small however long the cache is.
+#include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "qimg_device.h"
@@ -603,25 +605,14 @@ __global__ __launch_bounds__(SW * 64, 2) void attn_few_kernel(AttnVarlenArgs a) 
     }
 }
 
-// The key ranges' partial results of a tile of 32 rows, added in range order:
-// thread: row tid / 8, channels (tid % 8) * D / 8 .. Sequences of one range
-// are complete already. Eight ranges' loads go out together (one after the
-// other, 16 tokens over up to 8192 keys took 7 us here, most of it waiting).
-template <class T, int D>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnVarlenArgs a) {
-    constexpr int E = D / 8, U = 8;
-    const Sequence first = load_sequence(a, threadIdx.x & 63);
-    const int per = range_tiles(a, first);
-    const int hk = blockIdx.x % a.hk;
-    const RowTile t = find_tile(a, first, blockIdx.x / a.hk, SR, 0);
-    if (!t.found) return;
-    const int splits = key_ranges(t.lk, per);
-    const int row = t.row0 + (threadIdx.x >> 3);
-    if (splits == 1 || row >= t.lq * a.group) return;
-    const int c0 = (threadIdx.x & 7) * E;
-    const int64_t token = static_cast<int64_t>(t.q0) + row / a.group;
-    const int head = hk * a.group + row % a.group;
-    const int64_t at = (token * a.hq + head) * a.splits;
+// Partial results of one row, added in order: those of range u lie at row
+// at + u * step of part_o and part_ml. Eight ranges' loads go out together (one
+// after the other, 16 tokens over up to 8192 keys took 7 us here, most of it
+// waiting).
+template <class T, int E>
+__device__ __forceinline__ void join_row(const AttnVarlenArgs& a, int64_t at, int64_t step, int splits, int c0,
+                                         uint16_t* op, bool none) {
+    constexpr int D = 8 * E, U = 8;
     typedef float v2f __attribute__((ext_vector_type(2)));
     float mm = kNegInf, tot = 0.0f, acc[E];
 #pragma unroll
@@ -631,7 +622,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnVarlenArgs a) {
         v4f v[U][E / 4];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int64_t p = at + min(s0 + u, splits - 1);
+            const int64_t p = at + min(s0 + u, splits - 1) * step;
             ml[u] = *reinterpret_cast<const v2f*>(a.part_ml + 2 * p);
 #pragma unroll
             for (int e = 0; e < E / 4; ++e) v[u][e] = *reinterpret_cast<const v4f*>(a.part_o + p * D + c0 + 4 * e);
@@ -654,7 +645,25 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnVarlenArgs a) {
             for (int e = 0; e < E; ++e) acc[e] += f * v[u][e / 4][e % 4];
         }
     }
-    store_row<T, E>(a.out + token * a.o_t + head * a.o_h + c0, acc, tot, visible(a, t, row / a.group) == 0);
+    store_row<T, E>(op + c0, acc, tot, none);
+}
+
+// The key ranges of a tile of 32 rows: thread: row tid / 8, channels
+// (tid % 8) * D / 8 .. Sequences of one range are complete already.
+template <class T, int D>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnVarlenArgs a) {
+    const Sequence first = load_sequence(a, threadIdx.x & 63);
+    const int per = range_tiles(a, first);
+    const int hk = blockIdx.x % a.hk;
+    const RowTile t = find_tile(a, first, blockIdx.x / a.hk, SR, 0);
+    if (!t.found) return;
+    const int splits = key_ranges(t.lk, per);
+    const int row = t.row0 + (threadIdx.x >> 3);
+    if (splits == 1 || row >= t.lq * a.group) return;
+    const int64_t token = static_cast<int64_t>(t.q0) + row / a.group;
+    const int head = hk * a.group + row % a.group;
+    join_row<T, D / 8>(a, (token * a.hq + head) * a.splits, 1, splits, (threadIdx.x & 7) * (D / 8),
+                       a.out + token * a.o_t + head * a.o_h, visible(a, t, row / a.group) == 0);
 }
 
 // ---- many rows: 128 of them, four waves over one ring -----------------------
@@ -893,7 +902,13 @@ __device__ __forceinline__ void many_step(Many<T, D>& w, const uint8_t* __restri
 // KG = 1: as above. KG = 2, for launches of few tiles, whose workgroups have a CU
 // each: eight waves, two groups of four that take the 64-key tiles in turn, each
 // with a ring of its own, a phase apart: the second barrier keeps one group's V
-// beside the other's M; the groups' (O, m, sum) are joined through LDS (the lanes of waves w and w + 4 hold the same rows and channels).
+// beside the other's M; the groups' (O, m, sum) are joined through LDS (the
+// lanes of waves w and w + 4 hold the same rows and channels).
+//
+// Without a causal mask all tiles take equally long, and a last round of
+// workgroups that fills few of the CUs takes nearly as long as a full one. The
+// tiles from a.tail on are then cut into a.splits key ranges, a workgroup each
+// (KG = 1), and attn_tail_join_kernel adds what these leave in scratch.
 template <class T, int D, int KG>
 __global__ __launch_bounds__(KG * MW * 64, 2) void attn_many_kernel(AttnVarlenArgs a, int tiles) {
     using W = Many<T, D>;
@@ -909,12 +924,13 @@ __global__ __launch_bounds__(KG * MW * 64, 2) void attn_many_kernel(AttnVarlenAr
     // Causal: the sequences' last, longest tiles first, the heads of one tile
     // side by side (a head stays on few XCDs as workgroups go round-robin over
     // them). Otherwise all tiles of a head on one XCD.
+    const int piece = KG == 1 ? static_cast<int>(blockIdx.x) - a.tail : -1;  // not negative: a range of a tile
     int hk, idx;
     if (a.causal) {
         hk = blockIdx.x % a.hk;
         idx = blockIdx.x / a.hk;
     } else {
-        const int logical = xcd_remap(blockIdx.x, tiles * a.hk);
+        const int logical = xcd_remap(piece < 0 ? blockIdx.x : a.tail + piece % a.tail_tiles, tiles * a.hk);
         hk = logical / tiles;
         idx = logical % tiles;
     }
@@ -928,8 +944,17 @@ __global__ __launch_bounds__(KG * MW * 64, 2) void attn_many_kernel(AttnVarlenAr
     const int head = hk * a.group + row % a.group;
     const int kmax = visible(a, t, token);
     const int kend = visible(a, t, (min(t.row0 + MR, rows) - 1) / a.group);  // of the whole tile
-    const int n = (kend + MK * KG - 1) / (MK * KG);                          // steps
-    const int nfull = visible(a, t, t.row0 / a.group) / (MK * KG);           // of tiles that every row sees whole
+    int n = (kend + MK * KG - 1) / (MK * KG);                         // steps
+    int nfull = visible(a, t, t.row0 / a.group) / (MK * KG);          // of tiles that every row sees whole
+    int tile0 = kg;                                                   // the first 64-key tile, one behind the last
+    int tile1 = KG * n;
+    if (piece >= 0) {
+        const int per = (n + a.splits - 1) / a.splits;
+        tile0 = min(piece / a.tail_tiles * per, n);
+        n = min(per, n - tile0);
+        nfull = min(max(nfull - tile0, 0), n);
+        tile1 = tile0 + n;
+    }
 
     W w;
     {
@@ -955,9 +980,9 @@ __global__ __launch_bounds__(KG * MW * 64, 2) void attn_many_kernel(AttnVarlenAr
 
     TileStream<D, false> ks;
     TileStream<D, true> vs;
-    ks.init(kbase, a.k_t, t.lk, kg, KG, wave);
-    vs.init(vbase, a.v_t, t.lk, kg, KG, wave);
-    // pairs 0 (no V) and 1, then the scores of tile 0 and pair 2 in its place
+    ks.init(kbase, a.k_t, t.lk, tile0, KG, wave);
+    vs.init(vbase, a.v_t, t.lk, tile0, KG, wave);
+    // pairs 0 (no V) and 1, then the scores of the first tile
     ks.issue(ring + W::TB, wave);
     vs.issue(ring + PAIR, wave);
     ks.issue(ring + PAIR + W::TB, wave);
@@ -968,14 +993,14 @@ __global__ __launch_bounds__(KG * MW * 64, 2) void attn_many_kernel(AttnVarlenAr
     if (KG == 2 && kg == 1) phase_barrier();
     for (; p < nfull; ++p)
         many_step<T, D, false, KG == 2>(w, ring + ((p + 1) % MSLOT) * PAIR, ring + (p % MSLOT) * PAIR, ks, vs,
-                                        a.scale_log2, KG * p + kg, wave, kmax, nonfinite);
+                                        a.scale_log2, KG * p + tile0, wave, kmax, nonfinite);
     for (; p < n; ++p)
         many_step<T, D, true, KG == 2>(w, ring + ((p + 1) % MSLOT) * PAIR, ring + (p % MSLOT) * PAIR, ks, vs,
-                                       a.scale_log2, KG * p + kg, wave, kmax, nonfinite);
+                                       a.scale_log2, KG * p + tile0, wave, kmax, nonfinite);
     if (KG == 2 && kg == 0) phase_barrier();
     wait_vmcnt<0>();  // the loads past the last tile no longer write the ring
     if (nonfinite >= 0)
-        for (int tile = nonfinite; tile * MK < kmax; tile += KG)
+        for (int tile = nonfinite; tile < tile1 && tile * MK < kmax; tile += KG)
             add_nonfinite<T, W::DT>(vbase, a.v_t, tile * MK, min(tile * MK + MK, kmax), w.o);
     float tot = half_sum(w.sum[0]);
 
@@ -1008,6 +1033,19 @@ __global__ __launch_bounds__(KG * MW * 64, 2) void attn_many_kernel(AttnVarlenAr
         }
     }
 
+    if (piece >= 0) {
+        const int64_t at = static_cast<int64_t>(piece) * MR + 32 * wave + l32;
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c)
+            *reinterpret_cast<v4f*>(a.part_o + at * D + 32 * (c / 4) + 8 * (c % 4) + 4 * half) =
+                (v4f){w.o[c / 4][c % 4 * 4], w.o[c / 4][c % 4 * 4 + 1], w.o[c / 4][c % 4 * 4 + 2],
+                      w.o[c / 4][c % 4 * 4 + 3]};
+        if (half == 0) {
+            a.part_ml[2 * at] = w.m;
+            a.part_ml[2 * at + 1] = tot;
+        }
+        return;
+    }
     if (!valid) return;
     const float inv = 1.0f / tot;
     // channels 8 (g + half) .. of block d after the lane halves have exchanged
@@ -1030,6 +1068,22 @@ __global__ __launch_bounds__(KG * MW * 64, 2) void attn_many_kernel(AttnVarlenAr
         }
 }
 
+// The key ranges of the last tiles: 32 rows of one a workgroup.
+template <class T, int D>
+__global__ __launch_bounds__(256) void attn_tail_join_kernel(AttnVarlenArgs a, int tiles) {
+    const int tile = blockIdx.x / (MR / 32), row0 = blockIdx.x % (MR / 32) * 32 + (threadIdx.x >> 3);
+    const int logical = xcd_remap(a.tail + tile, tiles * a.hk), hk = logical / tiles;
+    const RowTile t = find_tile(a, load_sequence(a, threadIdx.x & 63), logical % tiles, MR, 0);
+    if (!t.found) return;
+    const int row = t.row0 + row0;
+    if (row >= t.lq * a.group) return;
+    const int64_t token = static_cast<int64_t>(t.q0) + row / a.group;
+    const int head = hk * a.group + row % a.group;
+    join_row<T, D / 8>(a, static_cast<int64_t>(tile) * MR + row0, static_cast<int64_t>(a.tail_tiles) * MR, a.splits,
+                       (threadIdx.x & 7) * (D / 8), a.out + token * a.o_t + head * a.o_h,
+                       visible(a, t, row / a.group) == 0);
+}
+
 // upper bound on the tiles of `rows` rows that the sequences have
 int64_t tile_bound(int total_q, int batch, int group, int rows) {
     const int64_t seqs = batch < total_q ? batch : total_q;
@@ -1039,23 +1093,58 @@ int64_t tile_bound(int total_q, int batch, int group, int rows) {
 }  // namespace
 
 constexpr int kGroupTiles = 256;  // workgroups of two groups that run at once, one a CU
-constexpr int kFewGrid = 512;  // workgroups of the few-row kernel, two a CU
+constexpr int kFewGrid = 512;     // workgroups of the few-row kernel, two a CU
 
 // Tiles of 128 rows, or of 32: from 160 tiles of 128 on (28 heads, causal, us, 32 /
 // 128 rows: 512 tokens, 112 tiles, 12.6 / 17.2; 781, 172, 21.0 / 20.6; 1024, 224, 25.7 /
 // 23.1; 24 heads of 600, 120, 15.7 / 19.2).
 constexpr int kManyTiles = 160;
-static bool attn_varlen_many(int total_q, int batch, int hq, int hk) {
-    return tile_bound(total_q, batch, hq / hk, MR) * hk >= kManyTiles;
+
+// The tail of a launch of `tiles` equal tiles of 128 rows without a causal mask:
+// how many tiles its last round has (a multiple of eight where there are as many, so
+// that a tile's ranges run on one XCD), and into how many key ranges they go, one
+// round of them. The gain in us: a round of few workgroups takes a us a step (64
+// keys), ranges c for their start and the join, and for each of their tiles b a step
+// and d for its float results. Fitted to 24 heads over 1500 and 5000 keys with 16 to
+// 208 tiles in the last round (us, whole / in ranges; D 128, 5000 keys: 16 tiles
+// 227 / 169, 64 228 / 187, 160 232 / 218, 208 234 / 238; 1500 keys: 16 81 / 71, 64
+// 80 / 78, 112 81 / 82; D 64, 5000 keys: 16 127 / 111, 160 138 / 129, 208 141 / 149;
+// 1500 keys: 16 equal, 64 46 / 47). In two ranges, or where a tile has a CU
+// (two wave groups), nothing is gained: power then bounds the last round too. Lengths
+// are on the device: the keys' average stands for them here, which decides the time,
+// not the result.
+static void plan_tail(AttnVarlenPlan& p, int tiles, int total_k, int batch, int D) {
+    const int slots = 2 * kGroupTiles, tail = std::min((tiles % slots + 7) / 8 * 8, tiles);
+    if (tiles <= kGroupTiles || tail == 0) return;
+    const double a = D == 128 ? 0.97 : 0.33, b = D == 128 ? 0.0038 : 0.0012, c = D == 128 ? 11.4 : 8.0,
+                 d = D == 128 ? 0.034 : 0.01;
+    const double steps = static_cast<double>(total_k) / batch / MK;
+    const int s = std::min({16, slots / tail, static_cast<int>(steps / 4)});
+    if (s < 3 || steps * a - c <= tail * (steps * b + d)) return;
+    p.splits = s;
+    p.tail_tiles = tail;
+    p.tail = tiles - tail;
 }
 
-// Most key ranges a sequence may be cut into: where the tiles of 32 rows alone
-// do not fill two workgroups a CU. The ranges' length is found on the device.
-int attn_varlen_splits(int total_q, int total_k, int batch, int hq, int hk) {
-    if (total_q <= 0 || batch <= 0 || total_k <= 4 * SW * SK || attn_varlen_many(total_q, batch, hq, hk)) return 1;
-    if (tile_bound(total_q, batch, hq / hk, SR) * hk > kFewGrid / 2) return 1;
+AttnVarlenPlan attn_varlen_plan(int total_q, int total_k, int batch, int hq, int hk, int D, bool causal) {
+    AttnVarlenPlan p{};
+    p.splits = 1;
+    if (total_q <= 0 || batch <= 0 || total_k <= 0) return p;
+    const int64_t many = tile_bound(total_q, batch, hq / hk, MR) * hk;
+    p.many = many >= kManyTiles;
+    p.tail = static_cast<int>(many);  // (< 2^24)
+    if (p.many) {
+        if (!causal) plan_tail(p, p.tail, total_k, batch, D);
+        p.part_rows = p.splits > 1 ? static_cast<int64_t>(p.tail_tiles) * p.splits * MR : 0;
+        return p;
+    }
+    // Most key ranges a sequence may be cut into: where the tiles of 32 rows alone
+    // do not fill two workgroups a CU. The ranges' length is found on the device.
+    if (total_k <= 4 * SW * SK || tile_bound(total_q, batch, hq / hk, SR) * hk > kFewGrid / 2) return p;
     const int64_t most = (total_k + 4 * SW * SK - 1) / (4 * SW * SK);
-    return static_cast<int>(most > 32 ? 32 : most);
+    p.splits = static_cast<int>(most > 32 ? 32 : most);
+    p.part_rows = static_cast<int64_t>(total_q) * hq * p.splits;
+    return p;
 }
 
 template <class T, int D>
@@ -1077,16 +1166,20 @@ static hipError_t launch_many(const AttnVarlenArgs& a, hipStream_t stream) {
     // tiles have half the keys on average). 28 heads, causal, us, one group / two:
     // 1024 tokens (224 tiles) 27.6 / 23.1, 1500 39.8 / 33.8, 2048 (448) 51.6 / 46.9,
     // 3000 (660) 80 / 89; 24 heads, all keys, 1301 tokens (264) 38.4 / 52.4.
+    const unsigned grid = a.tail + a.tail_tiles * a.splits;
     if (tiles * a.hk <= (a.causal ? 2 * kGroupTiles : kGroupTiles))
-        hipLaunchKernelGGL((attn_many_kernel<T, D, 2>), dim3(tiles * a.hk), dim3(2 * MW * 64), 0, stream, a, tiles);
+        hipLaunchKernelGGL((attn_many_kernel<T, D, 2>), dim3(grid), dim3(2 * MW * 64), 0, stream, a, tiles);
     else
-        hipLaunchKernelGGL((attn_many_kernel<T, D, 1>), dim3(tiles * a.hk), dim3(MW * 64), 0, stream, a, tiles);
+        hipLaunchKernelGGL((attn_many_kernel<T, D, 1>), dim3(grid), dim3(MW * 64), 0, stream, a, tiles);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || a.tail_tiles == 0) return e;
+    hipLaunchKernelGGL((attn_tail_join_kernel<T, D>), dim3(a.tail_tiles * (MR / 32)), dim3(256), 0, stream, a, tiles);
     return hipGetLastError();
 }
 
 template <class T, int D>
 static hipError_t launch_attn(const AttnVarlenArgs& a, hipStream_t stream) {
-    return attn_varlen_many(a.total_q, a.batch, a.hq, a.hk) ? launch_many<T, D>(a, stream) : launch_few<T, D>(a, stream);
+    return a.many ? launch_many<T, D>(a, stream) : launch_few<T, D>(a, stream);
 }
 
 hipError_t launch_attention_varlen(const AttnVarlenArgs& a, int dtype, int D, hipStream_t stream) {

@@ -24,14 +24,13 @@ bool good_strides(int64_t t, int64_t h) {
 extern "C" {
 
 int64_t qimg_attention_varlen_scratch_bytes(int total_q, int total_k, int batch, int n_heads, int n_kv_heads,
-                                            int head_dim) {
+                                            int head_dim, int causal) {
     if (total_q <= 0 || total_k <= 0 || batch <= 0 || n_heads <= 0 || n_kv_heads <= 0 || head_dim <= 0 ||
         n_heads % n_kv_heads != 0)
         return 0;
-    const int splits = qimg::attn_varlen_splits(total_q, total_k, batch, n_heads, n_kv_heads);
-    if (splits == 1) return 0;
-    const int64_t parts = static_cast<int64_t>(total_q) * n_heads * splits;
-    return align256(parts * head_dim * 4) + align256(parts * 8);
+    const int64_t rows =
+        qimg::attn_varlen_plan(total_q, total_k, batch, n_heads, n_kv_heads, head_dim, causal != 0).part_rows;
+    return align256(rows * head_dim * 4) + align256(rows * 8);
 }
 
 int qimg_attention_varlen(const qimg_attn_varlen* args, void* scratch, int64_t scratch_bytes, void* stream) {
@@ -74,17 +73,19 @@ int qimg_attention_varlen(const qimg_attn_varlen* args, void* scratch, int64_t s
     a.hq = p.n_heads, a.hk = p.n_kv_heads, a.group = p.n_heads / p.n_kv_heads;
     a.causal = p.causal != 0;
     a.scale_log2 = scale_log2;
-    a.splits = qimg::attn_varlen_splits(p.total_q, p.total_k, p.batch, p.n_heads, p.n_kv_heads);
+    const qimg::AttnVarlenPlan plan =
+        qimg::attn_varlen_plan(p.total_q, p.total_k, p.batch, p.n_heads, p.n_kv_heads, p.head_dim, a.causal);
+    a.many = plan.many, a.splits = plan.splits, a.tail = plan.tail, a.tail_tiles = plan.tail_tiles;
     a.target_items = 512;
     if (a.splits > 1) {
-        const int64_t need = qimg_attention_varlen_scratch_bytes(p.total_q, p.total_k, p.batch, p.n_heads,
-                                                                 p.n_kv_heads, p.head_dim);
+        const int64_t bytes_o = align256(plan.part_rows * p.head_dim * 4);
+        const int64_t need = bytes_o + align256(plan.part_rows * 8);
         if (!scratch || scratch_bytes < need)
             return qimg::api_fail(QIMG_ERR_SCRATCH, "%s: scratch %lld bytes < required %lld", fn,
                                   static_cast<long long>(scratch_bytes), static_cast<long long>(need));
         QIMG_REQUIRE(aligned16(scratch), "%s: scratch must be 16-byte aligned", fn);
         a.part_o = static_cast<float*>(scratch);
-        a.part_ml = a.part_o + align256(static_cast<int64_t>(p.total_q) * p.n_heads * a.splits * p.head_dim * 4) / 4;
+        a.part_ml = a.part_o + bytes_o / 4;
     }
     return qimg::api_hip_status(
         qimg::launch_attention_varlen(a, p.dtype, p.head_dim, static_cast<hipStream_t>(stream)), fn);

@@ -337,12 +337,18 @@ struct AttnVarlenArgs {
     int batch, total_q, total_k, hq, hk, group;
     int causal;
     float scale_log2;  // sm_scale * log2(e)
-    int splits;        // most key ranges of a sequence (the few-row kernel)
-    int target_items;  // items that the ranges' length aims at
-    float* part_o;   // [total_q, hq, splits, D] with splits > 1
-    float* part_ml;  // [total_q, hq, splits, 2]: running maximum, sum
+    int many;              // tiles of 128 rows, not of 32
+    int splits;            // key ranges: most of a sequence (32 rows), of each tile from `tail` on (128 rows)
+    int tail, tail_tiles;  // 128 rows: the first tile in ranges (or the number of tiles), their number
+    int target_items;      // items that the ranges' length aims at
+    float* part_o;   // [total_q, hq, splits, D] or [splits, tail_tiles, 128, D] with splits > 1
+    float* part_ml;  // the same of 2: running maximum, sum
 };
-int attn_varlen_splits(int total_q, int total_k, int batch, int hq, int hk);
+struct AttnVarlenPlan {
+    int many, splits, tail, tail_tiles;
+    int64_t part_rows;  // rows of part_o
+};
+AttnVarlenPlan attn_varlen_plan(int total_q, int total_k, int batch, int hq, int hk, int D, bool causal);
 hipError_t launch_attention_varlen(const AttnVarlenArgs& a, int dtype, int D, hipStream_t stream);
 
 // gemm_fused.hip: the bf16 linear with its epilogue (qimg_linear_bf16_fused)

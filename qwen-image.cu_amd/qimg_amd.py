@@ -67,7 +67,7 @@ _SIGS = {
     "qimg_sage_quant_k": (_I, [_P, _P, _P, _P, _I, _I, _I, _P]),
     "qimg_sage_attn_quantized": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _P, _I64, _P]),
     "qimg_sage_attention": (_I, [_P, _P, _P, _P, _I, _F, _I, _I, _I, _I, _P, _I64, _P]),
-    "qimg_attention_varlen_scratch_bytes": (_I64, [_I, _I, _I, _I, _I, _I]),
+    "qimg_attention_varlen_scratch_bytes": (_I64, [_I, _I, _I, _I, _I, _I, _I]),
     "qimg_attention_varlen": (_I, [_P, _P, _I64, _P]),
     "qimg_linear_bf16_fused_scratch_bytes": (_I64, [_I, _I, _I, _I, _I]),
     "qimg_linear_bf16_fused": (_I, [_P, _P, _I64, _P]),
@@ -691,8 +691,9 @@ def _head_strides(t: torch.Tensor, T: int, H: int, D: int):
 
 
 def attention_varlen_scratch_bytes(total_q: int, total_k: int, batch: int, n_heads: int, n_kv_heads: int,
-                                   head_dim: int) -> int:
-    return int(_lib.qimg_attention_varlen_scratch_bytes(total_q, total_k, batch, n_heads, n_kv_heads, head_dim))
+                                   head_dim: int, causal: bool = True) -> int:
+    return int(_lib.qimg_attention_varlen_scratch_bytes(total_q, total_k, batch, n_heads, n_kv_heads, head_dim,
+                                                        bool(causal)))
 
 
 def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor,
@@ -727,7 +728,8 @@ def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     elif out.shape != q.shape or out.dtype != dt:
         raise QimgError(QIMG_ERR_INVALID_ARG, f"out must be {tuple(q.shape)} of q's type")
     with _on(dev):
-        scratch = _scratch_for(_lib.qimg_attention_varlen_scratch_bytes(tq, tk, batch, hq, hk, d), scratch, dev)
+        scratch = _scratch_for(_lib.qimg_attention_varlen_scratch_bytes(tq, tk, batch, hq, hk, d, bool(causal)),
+                               scratch, dev)
         args = _AttnVarlen(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _DT[dt],
                            *_head_strides(q, tq, hq, d), *_head_strides(k, tk, hk, d), *_head_strides(v, tk, hk, d),
                            *_head_strides(out, tq, hq, d), cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),

@@ -106,6 +106,35 @@ def test_many_rows(qimg, lens, d, causal):
         _run(qimg, lens, lens, hq=28, hk=4, d=d, dtype=dtype, causal=causal, seed=len(lens))
 
 
+# launches whose last round of workgroups is cut into key ranges: several tiles and
+# one, ranges that a short sequence leaves empty, keys behind a slot's last
+TAILS = [([3000], [3000], None, 24, 24, 128, torch.bfloat16), ([3000], [3000], None, 24, 24, 128, torch.float16),
+         ([5600], [4000], None, 24, 24, 64, torch.float16), ([3000], [9000], None, 24, 4, 64, torch.bfloat16),
+         ([2700, 300, 5], [5000, 40, 0], [7000, 100, 10], 24, 24, 128, torch.bfloat16)]
+
+
+@pytest.mark.parametrize("lq,lk,slots,hq,hk,d,dtype", TAILS, ids=lambda x: str(x).replace("torch.", ""))
+def test_last_tiles_in_key_ranges(qimg, lq, lk, slots, hq, hk, d, dtype):
+    slots = slots or lk
+    assert qimg.attention_varlen_scratch_bytes(sum(lq), sum(slots), len(lq), hq, hk, d, False) > 0
+    q, k, v = _make(lq, slots, hq, hk, d, dtype, 21)
+    cuq, cq = _cu(lq)
+    cuk, ck = _cu(slots)
+    for b, n in enumerate(lk):  # what lies behind a sequence's last key
+        k[ck[b] + n:ck[b + 1]] = float("nan")
+        v[ck[b] + n:ck[b + 1]] = float("inf")
+    v[ck[0] + lk[0] - 1, 0, 3] = float("inf")  # a key that every row sees, in the last range
+    kl = torch.tensor(lk, dtype=torch.int32, device=DEV)
+    runs = [qimg.attention_varlen(q, k, v, cuq, cuk, 1.0 / math.sqrt(d), False, k_lens=kl) for _ in range(2)]
+    want, mag = _oracle(q, k, v, cq, ck, lk, 1.0 / math.sqrt(d), False)
+    torch.cuda.synchronize()
+    assert torch.equal(runs[0], runs[1])
+    seen = torch.isinf(want)
+    assert bool(seen[0, 0, 3]) and bool((runs[0].double()[seen] == want[seen]).all())
+    want[seen], mag[seen] = 0.0, 0.0
+    _check(runs[0].masked_fill(seen, 0.0), want, mag, dtype)
+
+
 @pytest.mark.parametrize("lq,lk", [([1, 1, 1], [1, 700, 33]), ([1] * 5, [4097, 0, 64, 1, 2000]), ([3, 40], [3000, 41]),
                                    ([200, 300], [1000, 300]), ([1], [20000]), ([900], [1700]), ([2000, 700], [2100, 3000])], ids=str)
 @pytest.mark.parametrize("d", [64, 128])

@@ -48,6 +48,10 @@ def test_attention_varlen_empty_calls_and_scratch(qimg):
     assert "scratch" in _err(qimg)
     assert qimg.attention_varlen_scratch_bytes(0, 8192, 1, 28, 4, 128) == 0
     assert qimg.attention_varlen_scratch_bytes(1, 8192, 1, 28, 3, 128) == 0
+    # the last tiles of a launch without a causal mask as well
+    assert qimg.attention_varlen_scratch_bytes(3000, 3000, 1, 24, 24, 128, False) > 0
+    assert qimg.attention_varlen_scratch_bytes(3000, 3000, 1, 24, 24, 128, True) == 0
+    assert _attn(qimg, causal=0, total_q=3000, total_k=3000, n_heads=24, n_kv_heads=24, batch=1) == 3
 
 
 def test_attention_varlen_wrapper_refuses(qimg):
