@@ -819,14 +819,17 @@ int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 // (us). A stage of linear_tile_kernel takes 0.4 us and 1.2 us for each 256x256 of
 // the tile (measured: 256x256 1.6, 224x256 1.5, 160x256 1.2, 128x128 0.7), one of
 // linear_small_kernel its bytes at 75 KB a us; the weights come at 4.8 TB/s at
-// best, the parts of a split sum are written and read once. linear_rows_kernel
-// takes about 4 us and the weights' bytes at 2.5 TB/s; fp32 rows spare it a packing
-// launch of 3 us. Measured (us, bf16 x, weights not resident): 16x3584x3584 rows
-// 10.8, 32x64 tiles 13; 16x4608x3584 17.5 / 11.7; 269x4608x3584 96x64 tiles 20.5,
-// 160x256 split in 4 28; 500x4608x3584 96x64 38, 128x256 split in 2 41;
-// 1000x4608x3584 (fp32 x) 160x256 split in 2 56, 128x256 68; 269x3584x14336 160x256
-// split in 9 45-49, 96x64 split in 4 72; 781x14336x3584 gated 224x256 158, 256x256
-// 162; 64x14336x3584 gated 64x128 43.
+// best, the parts of a split sum are written and read once, mostly in the caches.
+// linear_rows_kernel takes about 4 us and the weights' bytes at 2.5 TB/s; fp32 rows
+// spare it a packing launch of 3 us. Measured (us, bf16 x, weights not resident):
+// 16x3584x3584 rows 10.8, 32x64 tiles 13; 16x4608x3584 17.5 / 11.7; 21x3584x14336
+// 32x64 split in 4 25, 32x128 in 9 26; 269x4608x3584 96x64 tiles 20.5, 160x256 split
+// in 4 28; 269x3584x14336 160x256 split in 9 45-49, 96x64 split in 4 72;
+// 281x3584x12288 160x256 split in 9 45, 96x64 split in 3 56; 500x4608x3584 96x64 38,
+// 128x256 split in 2 41; 930x4608x3584 160x256 split in 2 49, 96x64 56;
+// 1672x3584x3584 192x256 split in 2 58, 128x256 65; 781x14336x3584 gated 224x256 158,
+// 256x256 162; 64x14336x3584 gated 64x128 43. Not always the best: 2605x3584x12288
+// 224x256 split in 3 218, 160x256 215.
 LinearFusedPlan linear_fused_plan(int x_dtype, int M, int K, int N, bool gated) {
     LinearFusedPlan best{};  // tm = 0: linear_gemv_kernel or linear_rows_kernel
     if (M <= kLinearGemvRows) return best;
@@ -848,7 +851,7 @@ LinearFusedPlan linear_fused_plan(int x_dtype, int M, int K, int N, bool gated) 
             const double rounds = static_cast<double>((tiles * s + 255) / 256);
             const double work = rounds * (per * stage + (c.k == 64 ? 3.0 : 1.5)), read = bytes / 4.8e6 + 3.0;
             double t = 3.0 + std::max(work, read) + 0.2 * std::min(work, read);
-            if (s > 1) t += 5.0 + 2.0 * s * M * N * (gated ? 8.0 : 4.0) / 5e6;
+            if (s > 1) t += 4.0 + 0.3 * s + 2.0 * s * M * N * (gated ? 8.0 : 4.0) / 10e6;
             if (t < best_t) {
                 best_t = t;
                 best.tm = c.tm;
