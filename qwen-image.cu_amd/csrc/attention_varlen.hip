@@ -784,11 +784,11 @@ struct Many {
             }
         }
     }
-    template <int j, bool MASKED>
+    template <int j, bool CLEAN>
     __device__ __forceinline__ void m_groups(const uint8_t* src, bool& bad) {
         if constexpr (j < NG) {
             if constexpr (j + 1 < NG) read_group<j + 1>(src, buf[(j + 1) % 2]);
-            if constexpr (MASKED && j < NPV) {
+            if constexpr (CLEAN && j < NPV) {
                 bool b = false;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) b |= has_nonfinite<T>(buf[j % 2][i]);
@@ -804,7 +804,7 @@ struct Many {
             }
             mma_group<j>(buf[j % 2]);
             __builtin_amdgcn_sched_barrier(0);
-            m_groups<j + 1, MASKED>(src, bad);
+            m_groups<j + 1, CLEAN>(src, bad);
         }
     }
     template <int j>
@@ -817,10 +817,10 @@ struct Many {
     }
 
     // dma(i), i < PER: the next DMA instructions, spread over the exponentials
-    template <bool MASKED, class Dma>
-    __device__ __forceinline__ void softmax(int key0, int kmax, float c, Dma&& dma) {
+    template <class Dma>
+    __device__ __forceinline__ void softmax(int key0, int kfull, int kmax, float c, Dma&& dma) {
         const int half = (threadIdx.x & 63) >> 5;
-        if constexpr (MASKED) {
+        if (key0 + MK > kfull) {  // some row of the tile does not see some key
 #pragma unroll
             for (int b = 0; b < KB; ++b)
 #pragma unroll
@@ -869,17 +869,18 @@ __device__ __forceinline__ void phase_barrier() {
 // whose slot takes pair p + 2 during V(p), and pair p + 1, sent during V(p - 1),
 // has landed. The slots come as restrict pointers, which tells the compiler that
 // the reads of `src` do not depend on the DMA into `dst`: the waits and barriers
-// see to that. PHASED: a second barrier between V and M.
-template <class T, int D, bool MASKED, bool PHASED>
+// see to that. PHASED: a second barrier between V and M. CLEAN: infinities and
+// NaN of V are taken out and the first tile that had some is noted.
+template <class T, int D, bool CLEAN, bool PHASED>
 __device__ __forceinline__ void many_step(Many<T, D>& w, const uint8_t* __restrict src, uint8_t* __restrict dst,
                                           TileStream<D, false>& ks, TileStream<D, true>& vs, float scale, int tile,
-                                          int wave, int kmax, int& nonfinite) {
+                                          int wave, int kfull, int kmax, int& nonfinite) {
     using W = Many<T, D>;
     wait_vmcnt<0>();
     phase_barrier();
     w.template read_group<0>(src, w.buf[0]);
     __builtin_amdgcn_sched_barrier(0);
-    w.template softmax<MASKED>(tile * MK, kmax, scale, [&](int i) {
+    w.softmax(tile * MK, kfull, kmax, scale, [&](int i) {
         if (i < W::PER / 2)
             vs.issue_one(i, dst, wave);
         else
@@ -893,8 +894,8 @@ __device__ __forceinline__ void many_step(Many<T, D>& w, const uint8_t* __restri
     if (PHASED) phase_barrier();
     __builtin_amdgcn_s_setprio(1);
     bool bad = false;
-    w.template m_groups<0, MASKED>(src, bad);
-    if (MASKED && bad && nonfinite < 0) nonfinite = tile;
+    w.template m_groups<0, CLEAN>(src, bad);
+    if (CLEAN && bad && nonfinite < 0) nonfinite = tile;
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_setprio(0);
 }
@@ -914,7 +915,8 @@ __global__ __launch_bounds__(KG * MW * 64, 2) void attn_many_kernel(AttnVarlenAr
     using W = Many<T, D>;
     constexpr int PAIR = 2 * W::TB, RING = MSLOT * PAIR, CHUNKS = D / 8;
     constexpr int JOIN = KG == 2 ? MW * 64 * (D / 2 + 2) * 4 : 0;  // a group's O, m and sum
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[KG * RING > JOIN ? KG * RING : JOIN];
+    constexpr int RINGS = KG * RING > JOIN ? KG * RING : JOIN;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[RINGS + KG * MW * 4];  // and a flag of every wave
 
     const int lane = threadIdx.x & 63;
     const int wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -945,63 +947,86 @@ __global__ __launch_bounds__(KG * MW * 64, 2) void attn_many_kernel(AttnVarlenAr
     const int kmax = visible(a, t, token);
     const int kend = visible(a, t, (min(t.row0 + MR, rows) - 1) / a.group);  // of the whole tile
     int n = (kend + MK * KG - 1) / (MK * KG);                         // steps
-    int nfull = visible(a, t, t.row0 / a.group) / (MK * KG);          // of tiles that every row sees whole
-    int tile0 = kg;                                                   // the first 64-key tile, one behind the last
-    int tile1 = KG * n;
+    const int kfull = visible(a, t, t.row0 / a.group);                // of every row
+    int tile0 = kg;                                                   // the first 64-key tile
     if (piece >= 0) {
         const int per = (n + a.splits - 1) / a.splits;
         tile0 = min(piece / a.tail_tiles * per, n);
         n = min(per, n - tile0);
-        nfull = min(max(nfull - tile0, 0), n);
-        tile1 = tile0 + n;
     }
 
     W w;
-    {
-        const uint16_t* qp = a.q + (static_cast<int64_t>(t.q0) + token) * a.q_t + head * a.q_h + 8 * half;
-#pragma unroll
-        for (int i = 0; i < W::KS; ++i) w.qf[i] = *reinterpret_cast<const typename T::frag*>(qp + 16 * i);
-    }
     const uint16_t* kbase = a.k + static_cast<int64_t>(t.k0) * a.k_t + hk * a.k_h;
     const uint16_t* vbase = a.v + static_cast<int64_t>(t.k0) * a.v_t + hk * a.v_h;
-#pragma unroll
-    for (int d = 0; d < W::DT; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) w.o[d][r] = 0.0f;
-#pragma unroll
-    for (int r = 0; r < 16 * W::KB; ++r) w.s[r >> 4][r & 15] = 0.0f;
-    w.m = kNegInf;
-    w.sum = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int d = 0; d < W::DT; ++d) w.voff[d] = v_lane_off<D>(d);
-#pragma unroll
-    for (int c = 0; c < W::KS; ++c) w.koff[c] = l32 * (2 * D) + swz_k<D>(l32, 2 * c + half) * 16;
     int nonfinite = -1;  // first of this wave's tiles whose V was sanitized
 
-    TileStream<D, false> ks;
-    TileStream<D, true> vs;
-    ks.init(kbase, a.k_t, t.lk, tile0, KG, wave);
-    vs.init(vbase, a.v_t, t.lk, tile0, KG, wave);
-    // pairs 0 (no V) and 1, then the scores of the first tile
-    ks.issue(ring + W::TB, wave);
-    vs.issue(ring + PAIR, wave);
-    ks.issue(ring + PAIR + W::TB, wave);
-    wait_vmcnt<W::PER>();
-    phase_barrier();
-    w.template first_scores<W::NPV>(ring);
-    int p = 0;
-    if (KG == 2 && kg == 1) phase_barrier();
-    for (; p < nfull; ++p)
-        many_step<T, D, false, KG == 2>(w, ring + ((p + 1) % MSLOT) * PAIR, ring + (p % MSLOT) * PAIR, ks, vs,
-                                        a.scale_log2, KG * p + tile0, wave, kmax, nonfinite);
-    for (; p < n; ++p)
-        many_step<T, D, true, KG == 2>(w, ring + ((p + 1) % MSLOT) * PAIR, ring + (p % MSLOT) * PAIR, ks, vs,
-                                       a.scale_log2, KG * p + tile0, wave, kmax, nonfinite);
-    if (KG == 2 && kg == 0) phase_barrier();
-    wait_vmcnt<0>();  // the loads past the last tile no longer write the ring
-    if (nonfinite >= 0)
-        for (int tile = nonfinite; tile < tile1 && tile * MK < kmax; tile += KG)
-            add_nonfinite<T, W::DT>(vbase, a.v_t, tile * MK, min(tile * MK + MK, kmax), w.o);
+    const auto pass = [&](auto clean) __attribute__((always_inline)) {
+        constexpr bool CLEAN = decltype(clean)::value;
+        // The scores of the first tile need its K and Q: these loads go out first,
+        // the registers are set up beside them, then follows pair 1. (Q, the registers
+        // and then all loads: 1000 cycles more.)
+        TileStream<D, false> ks;
+        TileStream<D, true> vs;
+        ks.init(kbase, a.k_t, t.lk, tile0, KG, wave);
+        ks.issue(ring + W::TB, wave);
+        if constexpr (!CLEAN) {
+            const uint16_t* qp = a.q + (static_cast<int64_t>(t.q0) + token) * a.q_t + head * a.q_h + 8 * half;
+#pragma unroll
+            for (int i = 0; i < W::KS; ++i) w.qf[i] = *reinterpret_cast<const typename T::frag*>(qp + 16 * i);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int d = 0; d < W::DT; ++d) w.voff[d] = v_lane_off<D>(d);
+#pragma unroll
+            for (int c = 0; c < W::KS; ++c) w.koff[c] = l32 * (2 * D) + swz_k<D>(l32, 2 * c + half) * 16;
+        }
+#pragma unroll
+        for (int d = 0; d < W::DT; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) w.o[d][r] = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16 * W::KB; ++r) w.s[r >> 4][r & 15] = 0.0f;
+        w.m = kNegInf;
+        w.sum = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+        vs.init(vbase, a.v_t, t.lk, tile0, KG, wave);
+        __builtin_amdgcn_sched_barrier(0);
+        vs.issue(ring + PAIR, wave);
+        ks.issue(ring + PAIR + W::TB, wave);
+        wait_vmcnt<W::PER>();
+        phase_barrier();
+        w.template first_scores<W::NPV>(ring);
+        if (KG == 2 && kg == 1) phase_barrier();
+        for (int p = 0; p < n; ++p)
+            many_step<T, D, CLEAN, KG == 2>(w, ring + ((p + 1) % MSLOT) * PAIR, ring + (p % MSLOT) * PAIR, ks, vs,
+                                            a.scale_log2, KG * p + tile0, wave, kfull, kmax, nonfinite);
+        if (KG == 2 && kg == 0) phase_barrier();
+        wait_vmcnt<0>();  // the loads past the last tile no longer write the ring
+    };
+    pass(std::false_type{});
+    // An infinity or NaN of V in a place that some row does not see has made that
+    // row's product 0 * inf: if O holds any such value the tile is done again with
+    // them taken out, and added to the rows that see them. (Looking V over in every
+    // masked step took 3600 of its 6700 cycles, and a second copy of the loop.)
+    if (a.causal && n > 0) {
+        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int d = 0; d < W::DT; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[r & 3] = __builtin_fmaf(w.o[d][r], 0.0f, x[r & 3]);
+        const bool bad = __ballot(x[0] + x[1] + x[2] + x[3] != 0.0f) != 0;
+        int* const flags = reinterpret_cast<int*>(lds + RINGS);
+        if (lane == 0) flags[wave_all] = bad;
+        __syncthreads();
+        int any = 0;
+#pragma unroll
+        for (int i = 0; i < KG * MW; ++i) any |= flags[i];
+        if (__builtin_amdgcn_readfirstlane(any)) {
+            __syncthreads();  // (every wave has left the ring)
+            pass(std::true_type{});
+            if (nonfinite >= 0)
+                for (int tile = nonfinite; tile * MK < kmax; tile += KG)
+                    add_nonfinite<T, W::DT>(vbase, a.v_t, tile * MK, min(tile * MK + MK, kmax), w.o);
+        }
+    }
     float tot = half_sum(w.sum[0]);
 
     if constexpr (KG == 2) {
