@@ -1120,10 +1120,12 @@ int64_t tile_bound(int total_q, int batch, int group, int rows) {
 constexpr int kGroupTiles = 256;  // workgroups of two groups that run at once, one a CU
 constexpr int kFewGrid = 512;     // workgroups of the few-row kernel, two a CU
 
-// Tiles of 128 rows, or of 32: from 160 tiles of 128 on (28 heads, causal, us, 32 /
-// 128 rows: 512 tokens, 112 tiles, 12.6 / 17.2; 781, 172, 21.0 / 20.6; 1024, 224, 25.7 /
-// 23.1; 24 heads of 600, 120, 15.7 / 19.2).
-constexpr int kManyTiles = 160;
+// Tiles of 128 rows, or of 32: the latter while they are one round of workgroups
+// (us, 32 / 128 rows; 28 heads, causal: 120 tiles of 128 14.0 / 16.9, 144 19.5 / 18.1,
+// 192 23.2 / 19.8; 4 heads, all of 500 keys: 104 14.6 / 14.9, 136 20.5 / 15.2; of 8000
+// keys: 72 78 / 84, 136 145 / 90. Single tokens, whose tiles hold 7 rows each, take the
+// same time either way from 32 sequences on: bytes.)
+constexpr int kManyTiles = kFewGrid * SR / MR + 1;
 
 // The tail of a launch of `tiles` equal tiles of 128 rows without a causal mask:
 // how many tiles its last round has (a multiple of eight where there are as many, so
@@ -1189,8 +1191,8 @@ static hipError_t launch_many(const AttnVarlenArgs& a, hipStream_t stream) {
     const int tiles = static_cast<int>(tile_bound(a.total_q, a.batch, a.group, MR));
     // Two groups a tile while that is about one round of workgroups (a causal launch's
     // tiles have half the keys on average). 28 heads, causal, us, one group / two:
-    // 1024 tokens (224 tiles) 27.6 / 23.1, 1500 39.8 / 33.8, 2048 (448) 51.6 / 46.9,
-    // 3000 (660) 80 / 89; 24 heads, all keys, 1301 tokens (264) 38.4 / 52.4.
+    // 1024 tokens (224 tiles) 26.0 / 21.5, 1500 36.1 / 31.0, 2048 (448) 47.3 / 43.8,
+    // 3000 (660) 76 / 81; 24 heads, all keys, 1301 tokens (264) 35.6 / 46.9.
     const unsigned grid = a.tail + a.tail_tiles * a.splits;
     if (tiles * a.hk <= (a.causal ? 2 * kGroupTiles : kGroupTiles))
         hipLaunchKernelGGL((attn_many_kernel<T, D, 2>), dim3(grid), dim3(2 * MW * 64), 0, stream, a, tiles);
