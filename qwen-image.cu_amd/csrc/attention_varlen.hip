@@ -66,7 +66,6 @@ struct Bf16 {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
     }
     __device__ static __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
-    __device__ static __forceinline__ uint32_t pack_p(float a, float b) { return pack_bf16x2(a, b); }
     __device__ static __forceinline__ v4f add4(uint32_t p0, uint32_t p1, v4f s) {
         constexpr short one = 0x3f80;
         return __builtin_amdgcn_mfma_f32_4x4x4bf16_1k((v4s){one, one, one, one},
@@ -85,13 +84,6 @@ struct Fp16 {
         typedef _Float16 h2 __attribute__((ext_vector_type(2)));
         typedef float f2 __attribute__((ext_vector_type(2)));
         return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, h2));
-    }
-    // P towards zero, one instruction for two values (to nearest takes three): off by
-    // up to a whole step downwards, but the row sum adds the same rounded values, so the
-    // half step that all of them lose on average cancels in O / sum, and what is left
-    // is within half a step of the mean, as with rounding to nearest
-    __device__ static __forceinline__ uint32_t pack_p(float a, float b) {
-        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
     }
     __device__ static __forceinline__ v4f add4(uint32_t p0, uint32_t p1, v4f s) {
         typedef _Float16 h4 __attribute__((ext_vector_type(4)));
@@ -205,8 +197,8 @@ __device__ __forceinline__ RowTile find_tile(const AttnVarlenArgs& a, const Sequ
             const int cnt = __builtin_amdgcn_readlane(n, src);
             const int i = idx - (before + __builtin_amdgcn_readlane(incl, src) - cnt * t.splits);
             if (i < 0 || i >= cnt * t.splits) return t;  // (sums past 2^31: offsets that overlap many times)
-            const int tile = i / t.splits;
-            t.split = i % t.splits;
+            const int tile = per == 0 ? i : i / t.splits;
+            t.split = i - tile * t.splits;
             t.row0 = (a.causal ? cnt - 1 - tile : tile) * rows;
             t.found = true;
             return t;
@@ -495,7 +487,7 @@ __device__ __forceinline__ void few_item(const AttnVarlenArgs& a, const RowTile&
         uint32_t pk[8];
 #pragma unroll
         for (int r = 0; r < 16; r += 2)
-            pk[r / 2] = T::pack_p(__builtin_amdgcn_exp2f(p[r] + neg), __builtin_amdgcn_exp2f(p[r + 1] + neg));
+            pk[r / 2] = T::pack(__builtin_amdgcn_exp2f(p[r] + neg), __builtin_amdgcn_exp2f(p[r + 1] + neg));
         __builtin_amdgcn_sched_barrier(0);
         wait_vmcnt<(2 * NS - 1) * P>();  // V of tile i
         __builtin_amdgcn_sched_barrier(0);
@@ -852,7 +844,7 @@ struct Many {
             }
             const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r >> 4][r & 15], c, neg));
             const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r >> 4][(r & 15) + 1], c, neg));
-            pk[r / 2] = T::pack_p(p0, p1);
+            pk[r / 2] = T::pack(p0, p1);
         }
     }
 };

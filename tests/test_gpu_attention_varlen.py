@@ -79,7 +79,7 @@ def _run(qimg, lq, lk, hq=28, hk=4, d=128, dtype=torch.bfloat16, causal=True, sl
     return got
 
 
-# lengths around the tiles (32 and 256 rows, 32 and 64 keys), of one token, of zero
+# lengths around the tiles (32 and 128 rows, 32 and 64 keys), of one token, of zero
 LENS = [[1], [1, 1, 1], [31], [32], [33], [64], [65, 0, 3], [0, 0, 7], [127, 128, 129], [257, 13, 1, 0, 40]]
 DTYPES = [torch.bfloat16, torch.float16]
 
