@@ -1150,9 +1150,10 @@ AttnVarlenPlan attn_varlen_plan(int total_q, int total_k, int batch, int hq, int
     p.splits = 1;
     if (total_q <= 0 || batch <= 0 || total_k <= 0) return p;
     const int64_t many = tile_bound(total_q, batch, hq / hk, MR) * hk;
-    p.many = many >= kManyTiles;
-    p.tail = static_cast<int>(many);  // (< 2^24)
+    // (a workgroup a tile, and a grid has less than 2^32 threads: beyond, the kernel that walks)
+    p.many = many >= kManyTiles && many < (1 << 22);
     if (p.many) {
+        p.tail = static_cast<int>(many);
         if (!causal) plan_tail(p, p.tail, total_k, batch, D);
         p.part_rows = p.splits > 1 ? static_cast<int64_t>(p.tail_tiles) * p.splits * MR : 0;
         return p;
