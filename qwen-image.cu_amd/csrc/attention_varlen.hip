@@ -1159,8 +1159,10 @@ AttnVarlenPlan attn_varlen_plan(int total_q, int total_k, int batch, int hq, int
         return p;
     }
     // Most key ranges a sequence may be cut into: where the tiles of 32 rows alone
-    // do not fill two workgroups a CU. The ranges' length is found on the device.
-    if (total_k <= 4 * SW * SK || tile_bound(total_q, batch, hq / hk, SR) * hk > kFewGrid / 2) return p;
+    // do not fill two workgroups a CU, and the keys are more than 1024 (one token of 28
+    // heads over 600 keys, us, whole / in ranges with their join: 11.1 / 13.2; 1000: 13.6
+    // / 13.6; 1500: 17.3 / 13.4; 3000: 28 / 13.8). The ranges' length is found on the device.
+    if (total_k <= 8 * SW * SK || tile_bound(total_q, batch, hq / hk, SR) * hk > kFewGrid / 2) return p;
     const int64_t most = (total_k + 4 * SW * SK - 1) / (4 * SW * SK);
     p.splits = static_cast<int>(most > 32 ? 32 : most);
     p.part_rows = static_cast<int64_t>(total_q) * hq * p.splits;
