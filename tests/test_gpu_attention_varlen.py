@@ -125,10 +125,13 @@ def test_last_tiles_in_key_ranges(qimg, lq, lk, slots, hq, hk, d, dtype):
         v[ck[b] + n:ck[b + 1]] = float("inf")
     v[ck[0] + lk[0] - 1, 0, 3] = float("inf")  # a key that every row sees, in the last range
     kl = torch.tensor(lk, dtype=torch.int32, device=DEV)
-    runs = [qimg.attention_varlen(q, k, v, cuq, cuk, 1.0 / math.sqrt(d), False, k_lens=kl) for _ in range(2)]
+    room = torch.full((sum(lq) + 3, hq + 1, d + 8), 7.0, dtype=dtype, device=DEV)  # out as a view, and on its own
+    runs = [qimg.attention_varlen(q, k, v, cuq, cuk, 1.0 / math.sqrt(d), False, k_lens=kl,
+                                  out=room[:sum(lq), :hq, :d] if i else None) for i in range(2)]
     want, mag = _oracle(q, k, v, cq, ck, lk, 1.0 / math.sqrt(d), False)
     torch.cuda.synchronize()
     assert torch.equal(runs[0], runs[1])
+    assert bool((room[sum(lq):] == 7).all() and (room[:, hq:] == 7).all() and (room[:, :, d:] == 7).all())
     seen = torch.isinf(want)
     assert bool(seen[0, 0, 3]) and bool((runs[0].double()[seen] == want[seen]).all())
     want[seen], mag[seen] = 0.0, 0.0
@@ -301,28 +304,28 @@ def test_broken_offsets_stay_inside(qimg):
 
 def test_graph_replays_follow_lengths_on_the_device(qimg):
     """Lengths are read on the device: one captured call serves other k_lens."""
-    for lq, cap in (([1] * 4, 2100), ([300, 280], 900)):
+    for lq, cap, causal in (([1] * 4, 2100, True), ([300, 280], 900, True), ([3000], 3000, False)):
         q, k, v = _make(lq, [cap] * len(lq), 28, 4, 128, torch.bfloat16, 6)
         cuq, cq = _cu(lq)
         cuk, ck = _cu([cap] * len(lq))
         kl = torch.full((len(lq),), cap, dtype=torch.int32, device=DEV)
         out = torch.empty_like(q)
-        scratch = torch.empty(max(16, qimg.attention_varlen_scratch_bytes(sum(lq), cap * len(lq), len(lq), 28, 4, 128)),
-                              dtype=torch.uint8, device=DEV)
+        scratch = torch.empty(max(16, qimg.attention_varlen_scratch_bytes(sum(lq), cap * len(lq), len(lq), 28, 4, 128,
+                                                                        causal)), dtype=torch.uint8, device=DEV)
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
-            qimg.attention_varlen(q, k, v, cuq, cuk, k_lens=kl, out=out, scratch=scratch)
+            qimg.attention_varlen(q, k, v, cuq, cuk, causal=causal, k_lens=kl, out=out, scratch=scratch)
         torch.cuda.current_stream().wait_stream(side)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
-            qimg.attention_varlen(q, k, v, cuq, cuk, k_lens=kl, out=out, scratch=scratch)
+            qimg.attention_varlen(q, k, v, cuq, cuk, causal=causal, k_lens=kl, out=out, scratch=scratch)
         for n in (cap, 513, 300, cap - 1):
             kl.fill_(n)
             out.zero_()
             graph.replay()
             torch.cuda.synchronize()
-            want = qimg.attention_varlen(q, k, v, cuq, cuk, k_lens=kl)
+            want = qimg.attention_varlen(q, k, v, cuq, cuk, causal=causal, k_lens=kl)
             torch.cuda.synchronize()
             assert torch.equal(out, want)
 

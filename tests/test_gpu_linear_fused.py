@@ -67,12 +67,14 @@ TILES = [(196, 11191, 264, 0), (104, 8701, 264, 1), (1675, 2329, 264, 0), (198, 
          (245, 5473, 5480, 1), (21, 8442, 264, 1), (17, 65, 264, 0), (18, 67, 2472, 0), (19, 65, 264, 1),
          (17, 67, 2640, 1), (129, 8807, 264, 0), (1192, 65, 4640, 0), (33, 8287, 272, 1), (387, 225, 5432, 1),
          (2093, 205, 272, 0), (821, 65, 2768, 0), (1683, 131, 264, 1), (385, 66, 3952, 1), (2086, 453, 272, 0),
-         (931, 66, 4104, 0), (2314, 193, 288, 1), (771, 67, 3216, 1)]
+         (931, 66, 4104, 0), (2314, 193, 288, 1), (771, 67, 3216, 1), (296, 834, 5352, 0), (289, 417, 6336, 1),
+         (2164, 71, 4112, 0), (1396, 65, 4440, 1), (2515, 68, 5240, 0), (215, 531, 5200, 1), (18, 17663, 264, 0),
+         (25, 5618, 16288, 0), (17, 2733, 14416, 1)]
 
 
 @pytest.mark.parametrize("M,N,K,gated", TILES, ids=str)
 def test_every_tile_with_integers(qimg, M, N, K, gated):
-    """Exact, as above. K <= 8136 products of at most 4 (2): sums below 2^15, the
+    """Exact, as above. K <= 16288 products of at most 4 (2): sums below 2^16, the
     gated product below 2^24 because its second factor is kept small."""
     g = _gen(M + N + K)
     x, w = _ints(g, (M, K), -2, 2), _ints(g, (N, K), -2, 2)
