@@ -127,8 +127,11 @@ __device__ __forceinline__ void finish1(const LinearFusedArgs& a, int m, int n, 
 // different banks; rows past M or N and k past K arrive as zeros.
 //
 // A stage is four phases, one quadrant (half of the wave's rows x half of its
-// columns) each: first the fragments that the quadrant still lacks are read, then
-// its MFMAs run. Waves 4-7 are one barrier behind waves 0-3, so on every SIMD
+// columns) each: first fragments are read, then its MFMAs run. Phases 0 and 2 read
+// the rows' halves, 1 the second half of the columns, and 3 the first half of the
+// next stage's, into the registers of this stage's second: every other stage takes
+// the halves in the other order, and no phase reads more than its MFMAs take (LDS
+// gives a CU 128 bytes a cycle: 8 fragments of four waves 256 cycles). Waves 4-7 are one barrier behind waves 0-3, so on every SIMD
 // one wave's MFMAs run beside the other's LDS reads and DMA issue. A quarter of
 // a slot (A rows or B rows of one half) is refilled two barriers after its last
 // reader, with the stage NS later.
@@ -283,9 +286,21 @@ __global__ __launch_bounds__(512) void linear_tile_kernel(LinearFusedArgs a) {
     using H0 = std::integral_constant<int, 0>;
     using H1 = std::integral_constant<int, 1>;
 
-    // A wave issues stage after stage in the order A0 B0, B1, A1. Behind its wait
-    // before a barrier its share of what the next phases read has landed.
+    // A wave issues a stage's four quarters in the order in which its slot's are
+    // free: A0, a B half, the other, A1. Behind its wait before a barrier its share
+    // of what the next phases read has landed.
     constexpr int kAhead = (NS - 2) * T::ALL;
+    const uint8_t *as, *bs;  // the wave's rows in the slot that is read, which is the one filled behind the reads
+    const auto enter = [&]() {
+        as = lds + fill_at + wm * (16 * MB) * 128;
+        bs = lds + fill_at + T::AB + wn * (16 * NB) * 128;
+    };
+    const auto read_b = [&](int h) {
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int j = 0; j < NB0; ++j) fb[h][j][ks] = frag(bs, 16 * (h * NB0 + j), ks);
+    };
 #pragma unroll
     for (int st = 0; st < NS; ++st) {
         issue_a(0);
@@ -294,60 +309,58 @@ __global__ __launch_bounds__(512) void linear_tile_kernel(LinearFusedArgs a) {
         issue_a(1);
         next_fill();
     }
-    wait_vmcnt<T::IB1 + T::IA1 + T::ALL + kAhead>();  // A0, B0 of stage 0
+    wait_vmcnt<T::IA1 + T::ALL + kAhead>();  // A0, B0, B1 of stage 0
     barrier();
     const bool lag = wave >= 4;
     if (lag) barrier();
-    for (int st = 0; st < nst; ++st) {
-        const uint8_t* slot = lds + fill_at;  // the slot that is read is the one filled behind the reads
-        const uint8_t* as = slot + wm * (16 * MB) * 128;
-        const uint8_t* bs = slot + T::AB + wn * (16 * NB) * 128;
-        // phase 0: rows 0, columns 0
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-#pragma unroll
-            for (int j = 0; j < NB0; ++j) fb[0][j][ks] = frag(bs, 16 * j, ks);
-#pragma unroll
-            for (int i = 0; i < MB0; ++i) fa[i][ks] = frag(as, 16 * i, ks);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        wait_vmcnt<T::IA1 + T::ALL + kAhead>();  // B1
-        wait_lgkmcnt0();
-        barrier();
-        mma(H0{}, H0{});
-        barrier();
-        // phase 1: rows 0, columns 1
+    enter();
+    read_b(0);
+    // One stage, column half F first: its fragments are there already
+    const auto stage = [&](auto first, auto second) __attribute__((always_inline)) {
+        constexpr int F = decltype(first)::value, S = decltype(second)::value;
+        // phase 0: rows 0, columns F
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-            for (int j = 0; j < NB0; ++j) fb[1][j][ks] = frag(bs, 16 * (NB0 + j), ks);
+            for (int i = 0; i < MB0; ++i) fa[i][ks] = frag(as, 16 * i, ks);
+        wait_lgkmcnt0();
+        barrier();
+        mma(H0{}, first);
+        barrier();
+        // phase 1: rows 0, columns S
+        read_b(S);
         __builtin_amdgcn_sched_barrier(0);
         issue_a(0);
-        issue_b(0);
+        issue_b(F);
         wait_vmcnt<T::ALL + T::IA0 + T::IB0 + kAhead>();  // A1
         wait_lgkmcnt0();
         barrier();
-        mma(H0{}, H1{});
+        mma(H0{}, second);
         barrier();
-        // phase 2: rows 1, columns 1
+        // phase 2: rows 1, columns S
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
             for (int i = 0; i < MB1; ++i) fa[i][ks] = frag(as, 16 * (MB0 + i), ks);
         __builtin_amdgcn_sched_barrier(0);
-        issue_b(1);
+        issue_b(S);
+        wait_vmcnt<T::ALL + kAhead>();  // A0, B0, B1 of the next stage
         wait_lgkmcnt0();
         barrier();
-        mma(H1{}, H1{});
+        mma(H1{}, second);
         barrier();
-        // phase 3: rows 1, columns 0
+        // phase 3: rows 1, columns F; the fragments of columns S of the next stage
         issue_a(1);
         next_fill();
-        __builtin_amdgcn_sched_barrier(0);
-        wait_vmcnt<T::IB1 + T::IA1 + T::ALL + kAhead>();  // A0, B0 of the next stage
+        enter();
+        read_b(S);
         barrier();
-        mma(H1{}, H0{});
+        mma(H1{}, first);
         barrier();
+    };
+    for (int st = 0; st < nst; st += 2) {
+        stage(H0{}, H1{});
+        if (st + 1 < nst) stage(H1{}, H0{});
     }
     if (!lag) barrier();
     wait_vmcnt<0>();
