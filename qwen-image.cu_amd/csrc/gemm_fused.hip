@@ -56,16 +56,22 @@ __device__ __forceinline__ Columns load_columns(const LinearFusedArgs& a, int n)
     }
     return c;
 }
-template <bool GATED>
-__device__ __forceinline__ void finish4(const LinearFusedArgs& a, const Columns& c, int m, int n, const float (&z)[4],
-                                        const float (&u)[4]) {
-    float v[4];
+// gate * act(z + bias) [* (u + bias_up)]
+template <bool GATED, class V>
+__device__ __forceinline__ void finish_values(const LinearFusedArgs& a, const Columns& c, const V& z, const V& u,
+                                              float (&v)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         v[i] = activate(z[i] + c.b[i], a.act);
         if (GATED) v[i] *= u[i] + c.bu[i];
         v[i] *= c.g[i];
     }
+}
+template <bool GATED>
+__device__ __forceinline__ void finish4(const LinearFusedArgs& a, const Columns& c, int m, int n, const float (&z)[4],
+                                        const float (&u)[4]) {
+    float v[4];
+    finish_values<GATED>(a, c, z, u, v);
     const int64_t o = m * a.ldo + n, r = m * a.ldr + n;
     const bool bf = a.out_dtype == QIMG_BF16;
     if (a.vec4 && n + 3 < a.N) {
@@ -376,6 +382,70 @@ __global__ __launch_bounds__(512) void linear_tile_kernel(LinearFusedArgs a) {
     const int sc = GATED ? (oc >> 4) * 32 + (oc & 15) : oc;
     Columns col;
     if (a.splits == 1 && n < a.N) col = load_columns(a, n);
+    // Whole groups with a residual: its values are loaded 16 rows ahead. (Loaded
+    // beside its use, each waits for the stores before it as well.)
+    const auto residual = [&](auto res_bf, auto out_bf) __attribute__((always_inline)) {
+        constexpr bool RB = decltype(res_bf)::value, OB = decltype(out_bf)::value;
+        using res_t = std::conditional_t<RB, uint2, v4f>;
+        using out_t = std::conditional_t<OB, uint2, v4f>;
+        const int row0 = m0 + wm * (16 * MB) + lane / OL, at = min(n, a.N - 4);
+        const auto load = [&](int i, res_t(&d)[16 / RP]) {
+#pragma unroll
+            for (int q = 0; q < 16 / RP; ++q) {
+                const int64_t m = min(row0 + 16 * i + q * RP, a.M - 1);
+                d[q] = *reinterpret_cast<const res_t*>(static_cast<const uint8_t*>(a.residual) +
+                                                       (m * a.ldr + at) * (RB ? 2 : 4));
+            }
+        };
+        res_t res[2][16 / RP];
+        load(0, res[0]);
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+            if (i + 1 < MB) load(i + 1, res[(i + 1) & 1]);
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int j = 0; j < NB; ++j) *reinterpret_cast<v4f*>(sh + r * T::PITCH + 16 * j + 4 * kq) = acc[i][j];
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int q = 0; q < 16 / RP; ++q) {
+                const int m = row0 + 16 * i + q * RP;
+                const v4f z = *reinterpret_cast<const v4f*>(sh + (q * RP + lane / OL) * T::PITCH + sc);
+                v4f u = {0.0f, 0.0f, 0.0f, 0.0f};
+                if constexpr (GATED) u = *reinterpret_cast<const v4f*>(sh + (q * RP + lane / OL) * T::PITCH + sc + 16);
+                float v[4];
+                finish_values<GATED>(a, col, z, u, v);
+                if constexpr (RB) {
+                    const uint2 t = res[i & 1][q];
+                    v[0] += __uint_as_float(t.x << 16);
+                    v[1] += __uint_as_float(t.x & 0xffff0000u);
+                    v[2] += __uint_as_float(t.y << 16);
+                    v[3] += __uint_as_float(t.y & 0xffff0000u);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] += res[i & 1][q][e];
+                }
+                if (m < a.M && n < a.N) {
+                    out_t* o = reinterpret_cast<out_t*>(static_cast<uint8_t*>(a.out) + (m * a.ldo + n) * (OB ? 2 : 4));
+                    if constexpr (OB)
+                        *o = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+                    else
+                        *o = (v4f){v[0], v[1], v[2], v[3]};
+                }
+            }
+        }
+    };
+    if (a.splits == 1 && a.residual != nullptr && a.vec4 && a.N % 4 == 0) {
+        const bool rb = a.res_dtype == QIMG_BF16, ob = a.out_dtype == QIMG_BF16;
+        if (rb && ob)
+            residual(H1{}, H1{});
+        else if (rb)
+            residual(H1{}, H0{});
+        else if (ob)
+            residual(H0{}, H1{});
+        else
+            residual(H0{}, H0{});
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < MB; ++i) {
         __builtin_amdgcn_wave_barrier();
