@@ -137,10 +137,14 @@ __device__ __forceinline__ void finish1(const LinearFusedArgs& a, int m, int n, 
 // the rows' halves, 1 the second half of the columns, and 3 the first half of the
 // next stage's, into the registers of this stage's second: every other stage takes
 // the halves in the other order, and no phase reads more than its MFMAs take (LDS
-// gives a CU 128 bytes a cycle: 8 fragments of four waves 256 cycles). Waves 4-7 are one barrier behind waves 0-3, so on every SIMD
-// one wave's MFMAs run beside the other's LDS reads and DMA issue. A quarter of
-// a slot (A rows or B rows of one half) is refilled two barriers after its last
-// reader, with the stage NS later.
+// gives a CU 128 bytes a cycle: 8 fragments of four waves 256 cycles). Waves 4-7
+// are one barrier behind waves 0-3, so on every SIMD one wave's MFMAs run beside
+// the other's LDS reads and DMA issue. A quarter of a slot (A rows or B rows of one
+// half) is refilled two barriers after its last reader, with the stage NS later.
+//
+// Measured: 4352x3584x12288 with gate and residual 283 us (1.35 PFLOP/s, the matrix
+// units busy 78% of the time at the clock that power allows), 8192^3 873 us; all
+// waves in step 15% more, the reads not evened out 1%.
 template <int TM_, int TN_>
 struct Tile {
     static constexpr int TM = TM_, TN = TN_;
