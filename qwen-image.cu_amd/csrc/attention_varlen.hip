@@ -1134,7 +1134,7 @@ constexpr int kManyTiles = kFewGrid * SR / MR + 1;
 // not the result.
 static void plan_tail(AttnVarlenPlan& p, int tiles, int total_k, int batch, int D) {
     const int slots = 2 * kGroupTiles, tail = std::min((tiles % slots + 7) / 8 * 8, tiles);
-    if (tiles <= kGroupTiles || tail == 0) return;
+    if (p.groups == 2 || tail == 0) return;
     const double a = D == 128 ? 0.97 : 0.33, b = D == 128 ? 0.0038 : 0.0012, c = D == 128 ? 11.4 : 8.0,
                  d = D == 128 ? 0.034 : 0.01;
     const double steps = static_cast<double>(total_k) / batch / MK;
@@ -1154,6 +1154,14 @@ AttnVarlenPlan attn_varlen_plan(int total_q, int total_k, int batch, int hq, int
     p.many = many >= kManyTiles && many < (1 << 22);
     if (p.many) {
         p.tail = static_cast<int>(many);
+        // Two groups a tile for one round of workgroups, or two with a causal mask (the
+        // tiles have half the keys on average), where the keys repay the join, about 2 us
+        // a round (us, one group / two, 28 heads, causal: 3 x 300 tokens 13.1 / 14.4, 2 x
+        // 400 14.8 / 15.4, 2 x 500 17.1 / 16.4, 1100 28.9 / 24.3, 4 x 500, 452 tiles, 21.8 /
+        // 28.2, 2 x 1000, 444, 30.1 / 31.4, 1200, 264, 30.4 / 25.6, 2048, 448, 47.3 / 43.8,
+        // 3000, 660, 76 / 81; all keys: 1301 tokens of 24 heads, 264, 35.6 / 46.9).
+        const int keys = total_k / batch;
+        p.groups = (many <= kGroupTiles && keys >= 384) || (causal && many <= 2 * kGroupTiles && keys >= 1100) ? 2 : 1;
         if (!causal) plan_tail(p, p.tail, total_k, batch, D);
         p.part_rows = p.splits > 1 ? static_cast<int64_t>(p.tail_tiles) * p.splits * MR : 0;
         return p;
@@ -1184,12 +1192,8 @@ static hipError_t launch_few(const AttnVarlenArgs& a, hipStream_t stream) {
 template <class T, int D>
 static hipError_t launch_many(const AttnVarlenArgs& a, hipStream_t stream) {
     const int tiles = static_cast<int>(tile_bound(a.total_q, a.batch, a.group, MR));
-    // Two groups a tile while that is about one round of workgroups (a causal launch's
-    // tiles have half the keys on average). 28 heads, causal, us, one group / two:
-    // 1024 tokens (224 tiles) 26.0 / 21.5, 1500 36.1 / 31.0, 2048 (448) 47.3 / 43.8,
-    // 3000 (660) 76 / 81; 24 heads, all keys, 1301 tokens (264) 35.6 / 46.9.
     const unsigned grid = a.tail + a.tail_tiles * a.splits;
-    if (tiles * a.hk <= (a.causal ? 2 * kGroupTiles : kGroupTiles))
+    if (a.groups == 2)
         hipLaunchKernelGGL((attn_many_kernel<T, D, 2>), dim3(grid), dim3(2 * MW * 64), 0, stream, a, tiles);
     else
         hipLaunchKernelGGL((attn_many_kernel<T, D, 1>), dim3(grid), dim3(MW * 64), 0, stream, a, tiles);

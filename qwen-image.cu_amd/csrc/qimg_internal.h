@@ -338,6 +338,7 @@ struct AttnVarlenArgs {
     int causal;
     float scale_log2;  // sm_scale * log2(e)
     int many;              // tiles of 128 rows, not of 32
+    int groups;            // wave groups of a tile of 128 rows: 1 or 2
     int splits;            // key ranges: most of a sequence (32 rows), of each tile from `tail` on (128 rows)
     int tail, tail_tiles;  // 128 rows: the first tile in ranges (or the number of tiles), their number
     int target_items;      // items that the ranges' length aims at
@@ -345,7 +346,7 @@ struct AttnVarlenArgs {
     float* part_ml;  // the same of 2: running maximum, sum
 };
 struct AttnVarlenPlan {
-    int many, splits, tail, tail_tiles;
+    int many, groups, splits, tail, tail_tiles;
     int64_t part_rows;  // rows of part_o
 };
 AttnVarlenPlan attn_varlen_plan(int total_q, int total_k, int batch, int hq, int hk, int D, bool causal);

@@ -98,7 +98,8 @@ def test_head_groups(qimg, hq, hk, lens):
     _run(qimg, lens, lens, hq=hq, hk=hk, seed=hq)
 
 
-@pytest.mark.parametrize("lens", [[1500, 1], [700, 1301, 64, 257], [2048], [1000], [2600]], ids=str)
+@pytest.mark.parametrize("lens", [[1500, 1], [700, 1301, 64, 257], [2048], [1000], [2600], [130] * 8, [80] * 20],
+                         ids=str)
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("causal", [True, False])
 def test_many_rows(qimg, lens, d, causal):
