@@ -1,0 +1,53 @@
+"""GPU parity of qimg_linear_bf16_fused on the large tiles: the epilogue with a
+residual that is loaded ahead of its use (a sum that is not split, rows of whole
+groups of four values), in every tile height, type pair and with a gated second
+product. Definition and bounds are those of test_gpu_linear_fused.py."""
+import pytest
+import torch
+
+from planutil import LinearPlan, linear_plan
+from test_gpu_linear_fused import _check, _definition, _operands
+
+DEV = "cuda:0"
+F32, BF = torch.float32, torch.bfloat16
+
+# (M, N, K, gated) and the tile: M odd, M and N end inside a tile, N a multiple of four
+RESIDUAL = [((197, 11116, 264, 0), (128, 128)), ((103, 8848, 264, 1), (128, 128)), ((449, 8380, 264, 0), (128, 256)),
+            ((129, 11184, 272, 1), (128, 256)), ((661, 11316, 264, 0), (160, 256)), ((263, 11600, 272, 1), (160, 256)),
+            ((831, 10960, 264, 0), (192, 256)), ((321, 11160, 280, 1), (192, 256)), ((977, 10792, 264, 0), (224, 256)),
+            ((385, 11048, 272, 1), (224, 256)), ((1361, 9328, 264, 0), (256, 256)), ((463, 11348, 264, 1), (256, 256))]
+
+
+@pytest.mark.parametrize("shape,tile", RESIDUAL, ids=str)
+def test_residual_shapes_run_unsplit_large_tiles(qimg, shape, tile):
+    M, N, K, gated = shape
+    assert linear_plan(qimg, qimg.BF16, M, N, K, gated) == LinearPlan(*tile, False, False)
+    assert M % tile[0] and N % (tile[1] // (2 if gated else 1)) and N % 4 == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,tile", RESIDUAL, ids=str)
+def test_residual_loaded_ahead(qimg, shape, tile):
+    """fp32 and bf16 residual and out, with bias, activation and channel gate; then
+    out in residual's place, rows longer than N, what lies between them kept."""
+    M, N, K, gated = shape
+    o = _operands(M, N, K, BF, M + N)
+    wu, bu = (o["wu"], o["bu"]) if gated else (None, None)
+    for act, res_dtype, out_dtype in (("gelu", F32, F32), ("silu", BF, F32), ("none", F32, BF), ("gelu", BF, BF)):
+        res = o["res"].to(res_dtype)
+        got = qimg.linear_forward_bf16_fused(o["x"], o["w"], bias=o["b"], activation=act, weight_up=wu, bias_up=bu,
+                                             gate=o["gate"], residual=res, out_dtype=out_dtype)
+        want, err = _definition(o["x"], o["w"], o["b"], act, wu, bu, o["gate"], res)
+        torch.cuda.synchronize()
+        _check(got, want, err)
+    for dtype in (F32, BF):
+        store = torch.full((M, N + 12), 5.0, dtype=dtype, device=DEV)
+        out = store[:, :N]
+        out.copy_(o["res"])
+        want, err = _definition(o["x"], o["w"], o["b"], "silu", wu, bu, o["gate"], out)
+        got = qimg.linear_forward_bf16_fused(o["x"], o["w"], bias=o["b"], activation="silu", weight_up=wu, bias_up=bu,
+                                             gate=o["gate"], residual=out, out=out)
+        torch.cuda.synchronize()
+        assert got.data_ptr() == store.data_ptr()
+        _check(got, want, err)
+        assert bool((store[:, N:] == 5.0).all())
