@@ -1,12 +1,13 @@
 """GPU parity of qimg_linear_bf16_fused on the large tiles: the epilogue with a
 residual that is loaded ahead of its use (a sum that is not split, rows of whole
 groups of four values), in every tile height, type pair and with a gated second
-product. Definition and bounds are those of test_gpu_linear_fused.py."""
+product; and the one tile whose split sum needs sizes of its own. Definition and
+bounds are those of test_gpu_linear_fused.py."""
 import pytest
 import torch
 
 from planutil import LinearPlan, linear_plan
-from test_gpu_linear_fused import _check, _definition, _operands
+from test_gpu_linear_fused import TILES, _check, _definition, _gen, _ints, _operands
 
 DEV = "cuda:0"
 F32, BF = torch.float32, torch.bfloat16
@@ -16,6 +17,20 @@ RESIDUAL = [((197, 11116, 264, 0), (128, 128)), ((103, 8848, 264, 1), (128, 128)
             ((129, 11184, 272, 1), (128, 256)), ((661, 11316, 264, 0), (160, 256)), ((263, 11600, 272, 1), (160, 256)),
             ((831, 10960, 264, 0), (192, 256)), ((321, 11160, 280, 1), (192, 256)), ((977, 10792, 264, 0), (224, 256)),
             ((385, 11048, 272, 1), (224, 256)), ((1361, 9328, 264, 0), (256, 256)), ((463, 11348, 264, 1), (256, 256))]
+# 128x128 with the sum split: many rows over 33 to 64 gated columns and a very long K. (No other
+# sizes plan it: the small tiles or taller ones are estimated faster.)
+LONG = (8713, 34, 20792, 1)
+
+
+def test_every_tile_is_reached(qimg):
+    """The shapes of the integer tests, here and in test_gpu_linear_fused.py, run
+    every tile, gated or not, with the whole sum and with a split one."""
+    large = [(t, 256, False) for t in (256, 224, 192, 160, 128)] + [(128, 128, False)]
+    small = [(128, 64, True), (96, 64, True), (64, 128, True), (64, 64, True), (32, 128, True), (32, 64, True)]
+    want = {(LinearPlan(*t, split), bool(g)) for t in large + small for split in (False, True) for g in (0, 1)}
+    want.remove((LinearPlan(128, 128, False, True), False))  # (only gated sums of LONG's kind)
+    got = {(linear_plan(qimg, qimg.BF16, M, N, K, g), bool(g)) for M, N, K, g in TILES + [LONG]}
+    assert got == want
 
 
 @pytest.mark.parametrize("shape,tile", RESIDUAL, ids=str)
@@ -51,3 +66,19 @@ def test_residual_loaded_ahead(qimg, shape, tile):
         assert got.data_ptr() == store.data_ptr()
         _check(got, want, err)
         assert bool((store[:, N:] == 5.0).all())
+
+
+@pytest.mark.gpu
+def test_long_sum_over_128x128_tiles(qimg):
+    """Exact, as test_every_tile_with_integers: sums below 2^17, the second factor
+    of the gated product kept small."""
+    M, N, K, _ = LONG
+    g = _gen(7)
+    x, w = _ints(g, (M, K), -2, 2), _ints(g, (N, K), -2, 2)
+    wu = _ints(g, (N, K), -1, 1) * (torch.arange(K, device=DEV) % 61 == 0)
+    xd, res = x.to(BF), _ints(g, (M, N), -16, 16)
+    z = (x.double() @ w.double().t()) * (x.double() @ wu.double().t())
+    assert float(z.abs().max()) + 16 < 2 ** 24
+    got = qimg.linear_forward_bf16_fused(xd, w.to(BF), weight_up=wu.to(BF), residual=res.to(F32), out_dtype=F32)
+    torch.cuda.synchronize()
+    assert torch.equal(got.double(), res + z)
