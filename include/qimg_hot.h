@@ -250,7 +250,7 @@ int qimg_sage_attention(const uint16_t* q_f16, const uint16_t* k_f16, const uint
  * What lies behind a sequence's last key or is hidden from a row does not
  * reach that row, NaN and infinities included; an infinity of v that a row
  * sees makes that channel of it infinite, or NaN where the weight is less than
- * the type holds (2^-31 of the row's largest in fp16). sm_scale > 0, finite. out
+ * the type holds (2^-31 of the row's largest in fp16, 2^-88 in bf16). sm_scale > 0, finite. out
  * overlaps none of q, k, v. total_q * n_heads and total_k below 2^30; k and v
  * token strides at least head_dim.
  * scratch: qimg_attention_varlen_scratch_bytes(...) bytes (may be 0: NULL) for

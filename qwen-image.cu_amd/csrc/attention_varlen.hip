@@ -25,7 +25,12 @@
 // O and the sum are rescaled, only when a tile exceeds it by more than
 // kSlack (log2 units): P then reaches 2^kSlack, which changes no relative
 // rounding. fp16 P carries a further factor 2^kBias16 (at most 2^15 in all),
-// so that a value leaves the type's range only below 2^-31 of the maximum.
+// so that a value leaves the type's range only below 2^-31 of the maximum. bf16 V
+// reaches as far as the fp32 sums of P V: with a factor 2^kBiasBf fewer than 2^30 keys
+// of the largest V, each weighing 2^kSlack, stay below 2^128 (without it 4 keys of 1e38
+// gave infinity). For that P vanishes below 2^-88 of the maximum, and V whose average is
+// below 2^-79 loses digits; the fp32 exponent's own rounding is 2^-19 of P, a thousandth
+// of what bf16 leaves.
 //
 // K and V tiles go to LDS by buffer loads whose descriptor ends at the
 // sequence's last key: rows behind it arrive as zeros, so nothing that lies
@@ -50,6 +55,7 @@ typedef short v8s __attribute__((ext_vector_type(8)));
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kSlack = 8.0f;   // lazy-rescale threshold of the running maximum (log2 units)
 constexpr float kBias16 = 7.0f;  // log2 of the factor on fp16 P
+constexpr float kBiasBf = -38.0f;  // and on bf16 P
 constexpr int kRsrcWord3 = 0x00020000;  // raw unswizzled buffer (gfx9 family)
 
 // element type: fragment vector, MFMA, P pair packing and its row sum, and
@@ -60,7 +66,7 @@ constexpr int kRsrcWord3 = 0x00020000;  // raw unswizzled buffer (gfx9 family)
 // wait for; eight of these 4x4x4 take 88. Together 1-3% of the kernel's time.)
 struct Bf16 {
     using frag = v8bf;
-    static constexpr float kPBias = 0.0f;
+    static constexpr float kPBias = kBiasBf;
     static constexpr uint32_t kExp = 0x7f80u, kMant = 0x007fu;
     __device__ static __forceinline__ v16f mma(frag a, frag b, v16f c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
