@@ -155,12 +155,14 @@ __device__ __forceinline__ Sequence load_sequence(const AttnVarlenArgs& a, int b
 __device__ __forceinline__ int row_tiles(const AttnVarlenArgs& a, int lq, int rows) {
     return static_cast<int>((static_cast<int64_t>(lq) * a.group + rows - 1) / rows);
 }
-// key ranges of `per` tiles of SK keys that lk keys are cut into (per = 0: one)
+// key ranges of about `per` tiles of SK keys, equally long, that lk keys are cut into
+// (per = 0: one). Rounded to the nearest number: rounded up, 240 tiles of 8192 keys went
+// into 121, 121 and 14 each and took 220 us, in halves 188.
 constexpr int SK = 32;
 __device__ __forceinline__ int key_ranges(int lk, int per) {
     if (per == 0) return 1;
     const int n = (lk + SK - 1) / SK;
-    return max((n + per - 1) / per, 1);
+    return max((2 * n + per) / (2 * per), 1);
 }
 
 // inclusive sum over the wave's lanes: shifts by 1, 2, 4 and 8 inside rows of
@@ -345,23 +347,34 @@ __device__ __forceinline__ void add_nonfinite(const uint16_t* v, int64_t stride,
 // which walk over the items that the lengths on the device give: a grid sized by
 // the host's bound on them would mostly be workgroups without work, 2.5 us each.
 constexpr int SR = 32, SW = 4;
+constexpr int kFewGrid = 512;  // workgroups of the launch at most, two a CU
 
-// Key tiles per range: as many as make the launch about one item a workgroup,
-// at least four a wave, and at most a.splits ranges a sequence. 0: no ranges.
+// Key tiles per range, about; 0: no ranges. As many as make the launch one item a
+// workgroup, or a quarter more items than row tiles; at least four a wave, at most
+// a.splits ranges a sequence. Where row tiles alone take more than a quarter of the
+// workgroups and are about as long, each stays whole: they keep the memory busy by
+// themselves, and ranges only add their join (us, 24 heads, tokens, whole / in ranges: 6
+// of 1000 keys 26 / 29, 8 of 8192 keys 161 / 176; of unlike lengths, 8192 and 5 of 64 100
+// / 34, 10 random ones up to 8192 135 / 114).
 __device__ __forceinline__ int range_tiles(const AttnVarlenArgs& a, const Sequence& first) {
     if (a.splits == 1) return 0;
     const int lane = threadIdx.x & 63;
     int longest = 0;
-    float work = 0.0f;  // (row tiles x key tiles: a sum that needs no last digit)
+    float work = 0.0f, tiles = 0.0f;  // key tiles of all row tiles, row tiles: sums that need no last digit
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
         const Sequence s = b0 == 0 ? first : load_sequence(a, b0 + lane);
         const int kt = (s.lk + SK - 1) / SK;
-        work += wave_sum_dpp(static_cast<float>(row_tiles(a, s.lq, SR)) * static_cast<float>(kt));
+        const float n = static_cast<float>(row_tiles(a, s.lq, SR));
+        work += wave_sum_dpp(n * static_cast<float>(kt));
+        tiles += wave_sum_dpp(n);
         longest = max(longest, wave_reduce_dpp(kt, [](int x, int y) { return max(x, y); }));
     }
-    int per = static_cast<int>(work * static_cast<float>(a.hk) / static_cast<float>(a.target_items)) + 1;
-    per = max(per, 4 * SW);
-    return __builtin_amdgcn_readfirstlane(max(per, (longest + a.splits - 1) / a.splits));
+    tiles *= static_cast<float>(a.hk);
+    work *= static_cast<float>(a.hk);
+    const bool alike = tiles > kFewGrid / 4 && static_cast<float>(longest) * tiles < 1.5f * work;
+    int per = alike ? longest : static_cast<int>(work / fmaxf(kFewGrid, 1.25f * tiles)) + 1;
+    per = max(max(per, 4 * SW), (longest + a.splits - 1) / a.splits);
+    return __builtin_amdgcn_readfirstlane(min(per, max(longest, 1)));
 }
 
 // E channels of an output row: acc / tot, zeros where the row sees no key
@@ -385,7 +398,7 @@ struct Few {
 };
 
 template <class T, int D>
-__device__ __forceinline__ void few_item(const AttnVarlenArgs& a, const RowTile& t, int hk, int per, uint8_t* ring) {
+__device__ __forceinline__ void few_item(const AttnVarlenArgs& a, const RowTile& t, int hk, uint8_t* ring) {
     using frag = typename T::frag;
     constexpr int KS = D / 16, DT = D / 32;
     constexpr int TB = SK * D * 2;       // bytes of a K or V tile
@@ -407,9 +420,9 @@ __device__ __forceinline__ void few_item(const AttnVarlenArgs& a, const RowTile&
     const int kend = visible(a, t, (min(t.row0 + SR, rows) - 1) / a.group);
     const int kfull = visible(a, t, t.row0 / a.group);
     // 32-key tiles of this range
-    const int ntile = (kend + SK - 1) / SK;
-    const int tile0 = min(t.split * per, ntile);
-    const int tile1 = t.splits > 1 ? min(tile0 + per, ntile) : ntile;
+    const int ntile = (kend + SK - 1) / SK, range = ((t.lk + SK - 1) / SK + t.splits - 1) / t.splits;
+    const int tile0 = min(t.split * range, ntile);
+    const int tile1 = min(tile0 + range, ntile);
 
     frag qf[KS];
     {
@@ -599,7 +612,7 @@ __global__ __launch_bounds__(SW * 64, 2) void attn_few_kernel(AttnVarlenArgs a) 
     for (int item = blockIdx.x;; item += gridDim.x) {
         const RowTile t = find_tile(a, first, item / a.hk, SR, per);
         if (!t.found) return;
-        few_item<T, D>(a, t, item % a.hk, per, ring);
+        few_item<T, D>(a, t, item % a.hk, ring);
     }
 }
 
@@ -1116,13 +1129,17 @@ int64_t tile_bound(int total_q, int batch, int group, int rows) {
 }  // namespace
 
 constexpr int kGroupTiles = 256;  // workgroups of two groups that run at once, one a CU
-constexpr int kFewGrid = 512;     // workgroups of the few-row kernel, two a CU
 
 // Tiles of 128 rows, or of 32: the latter while they are one round of workgroups
 // (us, 32 / 128 rows; 28 heads, causal: 120 tiles of 128 14.0 / 16.9, 144 19.5 / 18.1,
 // 192 23.2 / 19.8; 4 heads, all of 500 keys: 104 14.6 / 14.9, 136 20.5 / 15.2; of 8000
-// keys: 72 78 / 84, 136 145 / 90. Single tokens, whose tiles hold 7 rows each, take the
-// same time either way from 32 sequences on: bytes.)
+// keys: 72 78 / 84, 136 145 / 90). A token or a few over caches fill few rows of
+// either tile, and there the keys of a long sequence have to go into ranges, which the
+// tiles of 32 do by the lengths on the device: up to 1024 of those (us, 32 / 128 rows: one
+// of 8192 keys beside 5 of 64, 24 heads, 34 / 101, beside 31, 28 on 4 heads, 17 / 138,
+// 127 24.6 / 142; 32 random lengths up to 8192 55 / 106; all alike, 6 x 8192 139 / 136, 64 x
+// 300 16.3 / 14.7, the launch that joins; 16 on 8 heads of 64, 32 x 8192 114 / 97). More
+// keep every CU busy whatever their lengths (of 2048 tiles, random, 885 / 819).
 constexpr int kManyTiles = kFewGrid * SR / MR + 1;
 
 // The tail of a launch of `tiles` equal tiles of 128 rows without a causal mask:
@@ -1156,8 +1173,11 @@ AttnVarlenPlan attn_varlen_plan(int total_q, int total_k, int batch, int hq, int
     p.splits = 1;
     if (total_q <= 0 || batch <= 0 || total_k <= 0) return p;
     const int64_t many = tile_bound(total_q, batch, hq / hk, MR) * hk;
+    const int64_t few = tile_bound(total_q, batch, hq / hk, SR) * hk;
+    const bool cached = few <= 2 * kFewGrid && total_k / 8 >= total_q &&
+                        static_cast<int64_t>(total_q) * (hq / hk) <= static_cast<int64_t>(SR) * std::min(batch, total_q);
     // (a workgroup a tile, and a grid has less than 2^32 threads: beyond, the kernel that walks)
-    p.many = many >= kManyTiles && many < (1 << 22);
+    p.many = many >= kManyTiles && many < (1 << 22) && !cached;
     if (p.many) {
         p.tail = static_cast<int>(many);
         // Two groups a tile for one round of workgroups, or two with a causal mask (the
@@ -1173,12 +1193,13 @@ AttnVarlenPlan attn_varlen_plan(int total_q, int total_k, int batch, int hq, int
         return p;
     }
     // Most key ranges a sequence may be cut into: where the tiles of 32 rows alone
-    // do not fill two workgroups a CU, and the keys are more than 1024 (one token of 28
-    // heads over 600 keys, us, whole / in ranges with their join: 11.1 / 13.2; 1000: 13.6
-    // / 13.6; 1500: 17.3 / 13.4; 3000: 28 / 13.8). The ranges' length is found on the device.
-    if (total_k <= 8 * SW * SK || tile_bound(total_q, batch, hq / hk, SR) * hk > kFewGrid / 2) return p;
-    const int64_t most = (total_k + 4 * SW * SK - 1) / (4 * SW * SK);
-    p.splits = static_cast<int>(most > 32 ? 32 : most);
+    // do not fill half of the launch's workgroups, or over caches, and the keys are more
+    // than 1024 (one token of 28 heads over 600 keys, us, whole / in ranges with their join:
+    // 11.1 / 13.2; 1000: 13.6 / 13.6; 1500: 17.3 / 13.4; 3000: 28 / 13.8). The ranges'
+    // length is found on the device.
+    if (total_k <= 8 * SW * SK || (few > kFewGrid / 2 && !cached)) return p;
+    const int64_t most = std::min((total_k + 4 * SW * SK - 1) / (4 * SW * SK), 32);
+    p.splits = static_cast<int>(std::min(most, 8192 / few));  // (parts of 140 MB at most)
     p.part_rows = static_cast<int64_t>(total_q) * hq * p.splits;
     return p;
 }

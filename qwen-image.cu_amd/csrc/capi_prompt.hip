@@ -77,7 +77,6 @@ int qimg_attention_varlen(const qimg_attn_varlen* args, void* scratch, int64_t s
         qimg::attn_varlen_plan(p.total_q, p.total_k, p.batch, p.n_heads, p.n_kv_heads, p.head_dim, a.causal);
     a.many = plan.many, a.groups = plan.groups, a.splits = plan.splits;
     a.tail = plan.tail, a.tail_tiles = plan.tail_tiles;
-    a.target_items = 512;
     if (a.splits > 1) {
         const int64_t bytes_o = align256(plan.part_rows * p.head_dim * 4);
         const int64_t need = bytes_o + align256(plan.part_rows * 8);

@@ -341,7 +341,6 @@ struct AttnVarlenArgs {
     int groups;            // wave groups of a tile of 128 rows: 1 or 2
     int splits;            // key ranges: most of a sequence (32 rows), of each tile from `tail` on (128 rows)
     int tail, tail_tiles;  // 128 rows: the first tile in ranges (or the number of tiles), their number
-    int target_items;      // items that the ranges' length aims at
     float* part_o;   // [total_q, hq, splits, D] or [splits, tail_tiles, 128, D] with splits > 1
     float* part_ml;  // the same of 2: running maximum, sum
 };

@@ -1,0 +1,26 @@
+"""Which kernel the prompt operators' calls take, without a GPU."""
+import pytest
+
+from planutil import attn_plan
+
+
+# (tokens, heads, kv heads, head_dim): the first numbers of sequences whose tiles of 128 rows are
+# more than one round of the few-row kernel, and more
+@pytest.mark.parametrize("b,hq,hk,d", [(6, 24, 24, 128), (10, 24, 24, 128), (17, 16, 8, 64), (32, 28, 4, 128),
+                                       (33, 28, 4, 64), (65, 12, 2, 128), (128, 28, 4, 128)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_tokens_over_caches_may_cut_their_keys(qimg, b, hq, hk, d, causal):
+    """One token a sequence over caches of unknown lengths: the keys of a long one
+    among short ones can go into ranges, however many sequences there are."""
+    for lq in (1, max(1, 32 * hk // hq)):  # up to 32 rows a sequence
+        p = attn_plan(qimg, b * lq, b * 8192, b, hq, hk, d, causal)
+        assert not p.many and p.splits >= 8
+        assert qimg.attention_varlen_scratch_bytes(b * lq, b * 8192, b, hq, hk, d, causal) <= 160 << 20
+
+
+def test_prompts_keep_their_tiles(qimg):
+    """As many keys as queries, or more rows a sequence than a small tile has."""
+    assert attn_plan(qimg, 4096, 4096, 1, 28, 4, 128, True).many
+    assert attn_plan(qimg, 400, 400, 20, 24, 24, 128, True).many
+    assert attn_plan(qimg, 640, 9000, 20, 28, 4, 128, True).many
+    assert not attn_plan(qimg, 90, 90, 2, 28, 4, 128, True).many
