@@ -1182,12 +1182,16 @@ AttnVarlenPlan attn_varlen_plan(int total_q, int total_k, int batch, int hq, int
         p.tail = static_cast<int>(many);
         // Two groups a tile for one round of workgroups, or two with a causal mask (the
         // tiles have half the keys on average), where the keys repay the join, about 2 us
-        // a round (us, one group / two, 28 heads, causal: 3 x 300 tokens 13.1 / 14.4, 2 x
-        // 400 14.8 / 15.4, 2 x 500 17.1 / 16.4, 1100 28.9 / 24.3, 4 x 500, 452 tiles, 21.8 /
-        // 28.2, 2 x 1000, 444, 30.1 / 31.4, 1200, 264, 30.4 / 25.6, 2048, 448, 47.3 / 43.8,
-        // 3000, 660, 76 / 81; all keys: 1301 tokens of 24 heads, 264, 35.6 / 46.9).
+        // a round (us, one group / two, 28 heads, causal: 3 x 300 tokens 14.0 / 15.7, 3 x
+        // 350 15.4 / 15.9, 2 x 400 15.4 / 16.3, 2 x 430 15.7 / 16.3, 2 x 450 16.4 / 16.5, 2 x
+        // 480 17.1 / 16.8, 1100 28.9 / 24.3, 4 x 500, 452 tiles, 21.8 / 28.2, 2 x 1000, 444,
+        // 30.1 / 31.4, 1200, 264, 30.4 / 25.6, 2048, 448, 47.3 / 43.8, 3000, 660, 76 / 81; all
+        // keys: 2 x 400 16.2 / 17.1, 2 x 450 17.5 / 16.9, 1301 tokens of 24 heads, 264, 35.6 /
+        // 46.9). Lengths are on the device: the average decides, of the slots with k_lens.
+        // Unlike lengths would have two groups pay from a lower one (512 + 269 tokens 16.5 /
+        // 16.1, 600 + 180 18.5 / 17.3).
         const int keys = total_k / batch;
-        p.groups = (many <= kGroupTiles && keys >= 384) || (causal && many <= 2 * kGroupTiles && keys >= 1100) ? 2 : 1;
+        p.groups = (many <= kGroupTiles && keys >= 448) || (causal && many <= 2 * kGroupTiles && keys >= 1100) ? 2 : 1;
         if (!causal) plan_tail(p, p.tail, total_k, batch, D);
         p.part_rows = p.splits > 1 ? static_cast<int64_t>(p.tail_tiles) * p.splits * MR : 0;
         return p;

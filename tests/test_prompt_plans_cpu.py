@@ -24,3 +24,13 @@ def test_prompts_keep_their_tiles(qimg):
     assert attn_plan(qimg, 400, 400, 20, 24, 24, 128, True).many
     assert attn_plan(qimg, 640, 9000, 20, 28, 4, 128, True).many
     assert not attn_plan(qimg, 90, 90, 2, 28, 4, 128, True).many
+
+
+@pytest.mark.parametrize("lens,causal,groups", [([300] * 3, True, 1), ([350] * 3, True, 1), ([400] * 2, True, 1),
+                                                ([430] * 2, True, 1), ([480] * 2, True, 2), ([700], True, 2),
+                                                ([400] * 2, False, 1), ([480] * 2, False, 2), ([1100], True, 2),
+                                                ([500] * 4, True, 1), ([2048], True, 2), ([3000], True, 1)], ids=str)
+def test_wave_groups_as_measured(qimg, lens, causal, groups):
+    """Two wave groups a tile only where they were the faster form of these calls."""
+    p = attn_plan(qimg, sum(lens), sum(lens), len(lens), 28, 4, 128, causal)
+    assert p.many and p.groups == groups
