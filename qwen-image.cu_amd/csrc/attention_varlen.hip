@@ -19,13 +19,16 @@
 // element e of lane half h stands for key 16 t + 8 (e / 4) + 4 h + e % 4 of a
 // 16-key group t, and V^T comes from row-major V in LDS through
 // ds_read_b64_tr_b16, whose four values are 4 consecutive keys of one channel.
-// P is rounded to the inputs' type for the second product: with u half a step of
-// the type (2^-8 in bf16, 2^-11 in fp16) an error of at most u sum_j p_j |v_j - o|,
-// since the row sum adds the rounded values (a constant V is returned exactly). The maximum moves, and
-// O and the sum are rescaled, only when a tile exceeds it by more than
-// kSlack (log2 units): P then reaches 2^kSlack, which changes no relative
-// rounding. fp16 P carries a further factor 2^kBias16 (at most 2^15 in all),
-// so that a value leaves the type's range only below 2^-31 of the maximum. bf16 V
+// P is rounded to the inputs' type for the second product, as the matrix unit takes
+// no others at its rate (in two parts they would be half as many products again): with u half
+// a step of the type (2^-8 in bf16, 2^-11 in fp16) an error of at most
+// sum_j u p_j |v_j - o|, since the row sum adds the rounded values (a constant V is
+// returned exactly); against 64 bits 1.15 to 1.4 times what rounding the result alone
+// leaves. The maximum moves, and O and the sum are rescaled, only when a tile exceeds
+// it by more than kSlack (log2 units): P then reaches 2^kSlack, which changes no
+// relative rounding. fp16 P carries a further factor 2^kBias16 (at most 2^15 in all):
+// weights below 2^-21 of the maximum are then subnormal, off by up to 2^-32 of it each
+// (the bound above grows by sum_j 2^-32 |v_j - o|), and vanish below 2^-32. bf16 V
 // reaches as far as the fp32 sums of P V: with a factor 2^kBiasBf fewer than 2^30 keys
 // of the largest V, each weighing 2^kSlack, stay below 2^128 (without it 4 keys of 1e38
 // gave infinity). For that P vanishes below 2^-88 of the maximum, and V whose average is

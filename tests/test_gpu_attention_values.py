@@ -60,3 +60,36 @@ def test_largest_values_stay_finite(qimg, path):
     got = qimg.attention_varlen(q, k, v, cuq, cuk, 1.0, causal)
     torch.cuda.synchronize()
     assert bool((got == 2.0 ** -79).all())
+
+
+@pytest.mark.parametrize("path", PATHS)
+def test_light_weights_in_fp16(qimg, path):
+    """fp16 holds P 2^7 with a step of 2^-24 at least, so a weight below 2^-21 of the
+    running maximum is off by up to 2^-32 of it, whatever it is itself: V is zero at
+    the heavy key and large at keys of weight 2^-24 to 2^-30. With u = 2^-11 the error is
+    at most sum_j (u p_j + 2^-32) |v_j - o|, in fp32 2^-18 of P for its exponent (below 32,
+    rounded twice) and 2^-17 of sum p |v| for up to 2^12 terms, and out's own rounding."""
+    lq, lk, hq, hk, causal = _path(qimg, path)
+    dtype, u = torch.float16, 2.0 ** -11
+    q, k, v = _make(lq, lk, hq, hk, 128, dtype, 33)
+    cuq, cq = _cu(lq)
+    cuk, ck = _cu(lk)
+    first = torch.tensor(ck[:-1], device=DEV)
+    q.zero_()
+    q[:, :, 0] = 1
+    k[:, :, 0] = -math.log(2) * (24 + 6 * torch.rand(k.shape[:2], device=DEV))
+    k[first, :, 0] = 0
+    v = (v.float() * 15000).clamp(-60000, 60000).to(dtype)
+    v[first] = 0
+    got = qimg.attention_varlen(q, k, v, cuq, cuk, 1.0, causal)
+    want, mag = _oracle(q, k, v, cq, ck, lk, 1.0, causal)
+    some = torch.zeros_like(want)  # sum of |v_j - o| over the keys that a row sees, at most
+    for b, n in enumerate(lk):
+        rows = slice(cq[b], cq[b + 1])
+        total = v[ck[b]:ck[b] + n].double().abs().cumsum(0).repeat_interleave(hq // hk, 1)
+        last = torch.arange(lq[b], device=DEV) + (n - lq[b]) if causal else torch.full((lq[b],), n - 1, device=DEV)
+        some[rows] = total[last] + (last + 1)[:, None, None] * want[rows].abs()
+    torch.cuda.synchronize()
+    tol = u * (mag + want.abs()) + 2.0 ** -32 * some + (2.0 ** -18 + 2.0 ** -17) * mag + u * want.abs() + 2.0 ** -25
+    err = (got.double() - want).abs()
+    assert bool((err <= tol).all()), f"max excess {float((err - tol).max())}, max err {float(err.max())}"
