@@ -255,8 +255,9 @@ int qimg_sage_attention(const uint16_t* q_f16, const uint16_t* k_f16, const uint
  * reach that row, NaN and infinities included; an infinity of v that a row
  * sees makes that channel of it infinite, or NaN where the weight is less than
  * the type holds (2^-31 of the row's largest in fp16, 2^-88 in bf16). sm_scale > 0, finite. out
- * overlaps none of q, k, v. total_q * n_heads and total_k below 2^30; k and v
- * token strides at least head_dim.
+ * overlaps none of q, k, v, and its strides keep tokens and heads apart (the
+ * rows of one dimension behind all that the other spans). total_q * n_heads and
+ * total_k below 2^30; k and v token strides at least head_dim.
  * scratch: qimg_attention_varlen_scratch_bytes(...) bytes (may be 0: NULL) for
  * this call's sizes; fewer queries can need more (their keys are split), and
  * so can causal 0 (the last tiles' keys are). One scratch buffer serves one
@@ -334,7 +335,8 @@ int qimg_linear_bf16_fused(const qimg_linear_fused* args, void* scratch, int64_t
  * [table_rows, rotary_dim / 2, 2] (cos, sin); positions int32 [tokens] on the
  * device: the token's table row. A token whose position lies outside [0,
  * table_rows) is not written. head_dim and rotary_dim multiples of 8. out may
- * be x (same type and strides), else does not overlap it. */
+ * be x (same type and strides), else does not overlap it; its strides keep
+ * tokens and heads apart. */
 typedef struct {
     const void* x;
     int x_dtype;

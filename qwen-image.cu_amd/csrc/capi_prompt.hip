@@ -19,6 +19,14 @@ bool good_strides(int64_t t, int64_t h) {
     return t >= 0 && t <= (int64_t{1} << 24) && h >= 0 && t % 8 == 0 && h % 8 == 0;
 }
 
+// no two heads of an output [T, H, D] share memory: the rows of one dimension lie
+// behind all that the other spans
+bool apart(int T, int64_t t, int H, int64_t h, int D) {
+    if (T == 1) return H == 1 || h >= D;
+    if (H == 1) return t >= D;
+    return (h >= D && t >= D && h <= (t - D) / (H - 1)) || (t >= D && h >= D && t <= (h - D) / (T - 1));
+}
+
 }  // namespace
 
 extern "C" {
@@ -59,8 +67,8 @@ int qimg_attention_varlen(const qimg_attn_varlen* args, void* scratch, int64_t s
     QIMG_REQUIRE(p.out != p.q && p.out != p.k && p.out != p.v, "%s: out must not be q, k or v", fn);
     QIMG_REQUIRE(p.total_k <= 1 || (p.k_stride_t >= p.head_dim && p.v_stride_t >= p.head_dim),
                  "%s: k and v token strides must be at least head_dim", fn);
-    QIMG_REQUIRE((p.total_q == 1 || p.out_stride_t >= p.head_dim) && (p.n_heads == 1 || p.out_stride_h >= p.head_dim),
-                 "%s: out strides must be at least head_dim", fn);
+    QIMG_REQUIRE(apart(p.total_q, p.out_stride_t, p.n_heads, p.out_stride_h, p.head_dim),
+                 "%s: out strides must keep its tokens and heads apart", fn);
     qimg::AttnVarlenArgs a{};
     a.q = static_cast<const uint16_t*>(p.q);
     a.k = static_cast<const uint16_t*>(p.k);
@@ -174,8 +182,8 @@ int qimg_rope_packed(const qimg_rope* args, void* stream) {
     QIMG_REQUIRE(p.x && p.out && p.positions && (p.cos_sin || p.table_rows == 0), "%s: null pointer", fn);
     QIMG_REQUIRE(aligned16(p.x) && aligned16(p.out) && aligned16(p.cos_sin),
                  "%s: x, out and cos_sin must be 16-byte aligned", fn);
-    QIMG_REQUIRE((p.tokens == 1 || p.out_stride_t >= p.head_dim) && (p.n_heads == 1 || p.out_stride_h >= p.head_dim),
-                 "%s: out strides must be at least head_dim", fn);
+    QIMG_REQUIRE(apart(p.tokens, p.out_stride_t, p.n_heads, p.out_stride_h, p.head_dim),
+                 "%s: out strides must keep its tokens and heads apart", fn);
     QIMG_REQUIRE(p.out != p.x || (p.out_dtype == p.x_dtype && p.out_stride_t == p.x_stride_t &&
                                   p.out_stride_h == p.x_stride_h),
                  "%s: out in x's place must have its type and strides", fn);
