@@ -256,8 +256,8 @@ int qimg_sage_attention(const uint16_t* q_f16, const uint16_t* k_f16, const uint
  * sees makes that channel of it infinite, or NaN where the weight is less than
  * the type holds (2^-31 of the row's largest in fp16, 2^-88 in bf16). sm_scale > 0, finite. out
  * overlaps none of q, k, v, and its strides keep tokens and heads apart (the
- * rows of one dimension behind all that the other spans). total_q * n_heads and
- * total_k below 2^30; k and v token strides at least head_dim.
+ * rows of one dimension behind all that the other spans). total_q * n_heads,
+ * total_k and batch below 2^30; k and v token strides at least head_dim.
  * scratch: qimg_attention_varlen_scratch_bytes(...) bytes (may be 0: NULL) for
  * this call's sizes; fewer queries can need more (their keys are split), and
  * so can causal 0 (the last tiles' keys are). One scratch buffer serves one

@@ -54,8 +54,9 @@ int qimg_attention_varlen(const qimg_attn_varlen* args, void* scratch, int64_t s
         return qimg::api_fail(QIMG_ERR_UNSUPPORTED, "%s: head_dim %d not supported (64 or 128)", fn, p.head_dim);
     const float scale_log2 = p.sm_scale * 1.4426950408889634f;
     QIMG_REQUIRE(std::isfinite(scale_log2) && scale_log2 > 0.0f, "%s: sm_scale must be positive and finite", fn);
-    QIMG_REQUIRE(static_cast<int64_t>(p.total_q) * p.n_heads < (int64_t{1} << 30) && p.total_k < (1 << 30),
-                 "%s: total_q * n_heads and total_k must be < 2^30", fn);
+    QIMG_REQUIRE(static_cast<int64_t>(p.total_q) * p.n_heads < (int64_t{1} << 30) && p.total_k < (1 << 30) &&
+                     p.batch < (1 << 30),
+                 "%s: total_q * n_heads, total_k and batch must be < 2^30", fn);
     QIMG_REQUIRE(good_strides(p.q_stride_t, p.q_stride_h) && good_strides(p.k_stride_t, p.k_stride_h) &&
                      good_strides(p.v_stride_t, p.v_stride_h) && good_strides(p.out_stride_t, p.out_stride_h),
                  "%s: strides must be non-negative multiples of 8, token strides at most 2^24", fn);

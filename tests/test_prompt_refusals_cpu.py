@@ -25,3 +25,11 @@ def test_outputs_of_either_order(qimg, t, h):
     """Rows of a longer projection and head-major outputs go on to the next check."""
     assert _attn(qimg, total_q=10, total_k=9000, batch=1, out_stride_t=t, out_stride_h=h) == 3
     assert "scratch" in _err(qimg)
+
+
+def test_more_sequences_than_the_kernels_count(qimg):
+    """The kernels walk the sequences 64 at a time in 32 bits: near 2^31 of them the
+    walk would pass the type's end and read in front of the offsets."""
+    for batch in (1 << 30, 2 ** 31 - 1):
+        assert _attn(qimg, batch=batch) == 1
+        assert "2^30" in _err(qimg)
