@@ -634,6 +634,12 @@ def _same_device(device, *tensors):
             raise QimgError(QIMG_ERR_INVALID_ARG, f"every tensor must be on {device}, the first argument's device")
 
 
+def _fits32(*sizes):
+    """The C entry points take 32-bit sizes, which ctypes would cut a larger number down to."""
+    if max(sizes) >= 1 << 31:
+        raise QimgError(QIMG_ERR_INVALID_ARG, f"sizes must be below 2^31, not {max(sizes)}")
+
+
 class _NoSwitch:
     def __enter__(self):
         return self
@@ -692,6 +698,7 @@ def _head_strides(t: torch.Tensor, T: int, H: int, D: int):
 
 def attention_varlen_scratch_bytes(total_q: int, total_k: int, batch: int, n_heads: int, n_kv_heads: int,
                                    head_dim: int, causal: bool = True) -> int:
+    _fits32(total_q, total_k, batch, n_heads, n_kv_heads, head_dim)
     return int(_lib.qimg_attention_varlen_scratch_bytes(total_q, total_k, batch, n_heads, n_kv_heads, head_dim,
                                                         bool(causal)))
 
@@ -718,6 +725,7 @@ def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     if v.shape != k.shape or dk != d:
         raise QimgError(QIMG_ERR_INVALID_ARG, f"k {tuple(k.shape)} and v {tuple(v.shape)} must be [Tk, Hk, {d}]")
     batch = cu_seqlens_q.numel() - 1
+    _fits32(tq, hq, tk, hk, batch)
     if batch < 0 or cu_seqlens_k.numel() != batch + 1 or (k_lens is not None and k_lens.numel() != batch):
         raise QimgError(QIMG_ERR_INVALID_ARG, "cu_seqlens_q and cu_seqlens_k must have B + 1 elements, k_lens B")
     for t in (cu_seqlens_q, cu_seqlens_k, k_lens):
@@ -749,6 +757,7 @@ class _LinearFused(ctypes.Structure):
 
 
 def linear_bf16_fused_scratch_bytes(x_dtype, M: int, K: int, N: int, gated: bool = False) -> int:
+    _fits32(M, K, N)
     return int(_lib.qimg_linear_bf16_fused_scratch_bytes(_DT[x_dtype], M, K, N, int(bool(gated))))
 
 
@@ -768,6 +777,7 @@ def linear_forward_bf16_fused(x: torch.Tensor, weight: torch.Tensor, bias: torch
     _same_device(dev, weight, bias, weight_up, bias_up, gate, residual, out)
     M, K = x.shape
     N = weight.shape[0]
+    _fits32(M, K, N)
     if weight.shape[1] != K:
         raise QimgError(QIMG_ERR_INVALID_ARG, f"weight K {weight.shape[1]} != activation K {K}")
     if x.dtype not in (torch.float32, torch.bfloat16):
@@ -833,6 +843,7 @@ def rope_packed(x: torch.Tensor, cos_sin: torch.Tensor, positions: torch.Tensor,
         raise QimgError(QIMG_ERR_INVALID_ARG, "cos_sin must be contiguous float32 [P, R / 2, 2]")
     if positions.dtype != torch.int32 or positions.numel() != T or not positions.is_contiguous():
         raise QimgError(QIMG_ERR_INVALID_ARG, f"positions must be contiguous int32 of {T} elements")
+    _fits32(T, H, D, n_rotated, cos_sin.shape[0], 2 * cos_sin.shape[1])
     with _on(dev):
         args = _Rope(_addr(x), _DT[x.dtype], *_head_strides(x, T, H, D), _addr(out), _DT[out.dtype],
                      *_head_strides(out, T, H, D), T, H, n_rotated, D,

@@ -2,6 +2,7 @@
 answered in one way, or not within the tensors: without a GPU, on addresses that
 are never read."""
 import pytest
+import torch
 
 from test_prompt_cpu import FAKE, _attn, _err, _rope
 
@@ -33,3 +34,10 @@ def test_more_sequences_than_the_kernels_count(qimg):
     for batch in (1 << 30, 2 ** 31 - 1):
         assert _attn(qimg, batch=batch) == 1
         assert "2^30" in _err(qimg)
+
+
+def test_scratch_of_sizes_past_32_bits(qimg):
+    with pytest.raises(qimg.QimgError, match="2\\^31"):
+        qimg.attention_varlen_scratch_bytes(1 << 32, 100, 1, 1, 1, 64)
+    with pytest.raises(qimg.QimgError, match="2\\^31"):
+        qimg.linear_bf16_fused_scratch_bytes(torch.bfloat16, 100, 1 << 32, 100)
