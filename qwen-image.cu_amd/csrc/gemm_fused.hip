@@ -29,7 +29,9 @@ constexpr int kRsrcWord3 = 0x00020000;  // raw unswizzled buffer (gfx9 family)
 constexpr uint32_t kOob = 0x80000000u;  // offset >= num_records: reads zero
 
 // v / (1 + 2^-t): the sigmoid form of both activations keeps the relative
-// error of small results (no 1 - 1), also far in the negative tail
+// error of small results (no 1 - 1), also far in the negative tail: with e = 2^(-|t|/2)
+// it is v / (1 + e^2), for t < 0 times e twice, so that nothing but the result leaves
+// the range of normal numbers (1 / (1 + 2^-t) did from v = -87 on)
 __device__ __forceinline__ float activate(float v, int act) {
     if (act == QIMG_ACT_NONE) return v;
     float t;  // log2(e) times the sigmoid's argument
@@ -37,7 +39,8 @@ __device__ __forceinline__ float activate(float v, int act) {
         t = v * 1.4426950408889634f;
     else
         t = v * __builtin_fmaf(0.10294324f, v * v, 2.3022082f);  // 2 sqrt(2/pi) log2(e) (v + 0.044715 v^3)
-    return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-t));
+    const float e = __builtin_amdgcn_exp2f(-0.5f * fabsf(t)), f = t < 0.0f ? e : 1.0f;
+    return v * f * __builtin_amdgcn_rcpf(__builtin_fmaf(e, e, 1.0f)) * f;
 }
 
 // The epilogue of four neighbouring outputs of row m, columns n ..; their

@@ -3,6 +3,8 @@ residual that is loaded ahead of its use (a sum that is not split, rows of whole
 groups of four values), in every tile height, type pair and with a gated second
 product; and the one tile whose split sum needs sizes of its own. Definition and
 bounds are those of test_gpu_linear_fused.py."""
+import math
+
 import pytest
 import torch
 
@@ -82,3 +84,21 @@ def test_long_sum_over_128x128_tiles(qimg):
     got = qimg.linear_forward_bf16_fused(xd, w.to(BF), weight_up=wu.to(BF), residual=res.to(F32), out_dtype=F32)
     torch.cuda.synchronize()
     assert torch.equal(got.double(), res + z)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 8, 64])
+def test_activations_to_the_least_normal_value(qimg, M):
+    """Far on the negative side SiLU and GELU are products of v and a sigmoid that is
+    no normal number any more, while they are. The product with the identity is
+    exact; what is left are the argument's roundings (two and those of its constants,
+    2^-23 of it each in all) and eight operations' on the result."""
+    eye = torch.eye(64, dtype=BF, device=DEV)
+    for act, lo, hi in (("silu", -104, -70), ("gelu", -14.5, -9), ("silu", 70, 104), ("gelu", 9, 20)):
+        z = torch.linspace(lo, hi, 64 * M, device=DEV).to(BF).reshape(M, 64)
+        got = qimg.linear_forward_bf16_fused(z, eye, activation=act, out_dtype=F32)
+        zd = z.double()
+        s = zd if act == "silu" else 2 * math.sqrt(2 / math.pi) * (zd + 0.044715 * zd ** 3)
+        want = zd / (1 + torch.exp(-s))
+        torch.cuda.synchronize()
+        _check(got, want, want.abs() * 2.0 ** -23 * (8 + 2 * s.abs().clamp(max=150)))
