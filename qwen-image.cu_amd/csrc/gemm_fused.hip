@@ -34,12 +34,12 @@ constexpr uint32_t kOob = 0x80000000u;  // offset >= num_records: reads zero
 // the range of normal numbers (1 / (1 + 2^-t) did from v = -87 on)
 __device__ __forceinline__ float activate(float v, int act) {
     if (act == QIMG_ACT_NONE) return v;
-    float t;  // log2(e) times the sigmoid's argument
+    float h;  // t / 2: log2(e) / 2 times the sigmoid's argument
     if (act == QIMG_ACT_SILU)
-        t = v * 1.4426950408889634f;
+        h = v * 0.72134752044448170f;
     else
-        t = v * __builtin_fmaf(0.10294324f, v * v, 2.3022082f);  // 2 sqrt(2/pi) log2(e) (v + 0.044715 v^3)
-    const float e = __builtin_amdgcn_exp2f(-0.5f * fabsf(t)), f = t < 0.0f ? e : 1.0f;
+        h = v * __builtin_fmaf(0.05147162f, v * v, 1.1511041f);  // sqrt(2/pi) log2(e) (v + 0.044715 v^3)
+    const float e = __builtin_amdgcn_exp2f(-fabsf(h)), f = h < 0.0f ? e : 1.0f;
     return v * f * __builtin_amdgcn_rcpf(__builtin_fmaf(e, e, 1.0f)) * f;
 }
 
