@@ -295,8 +295,16 @@ enum { QIMG_ACT_NONE = 0, QIMG_ACT_GELU_TANH = 1, QIMG_ACT_SILU = 2 };
  * NULL (bias_up only with w_up). out [M,N] QIMG_FP32 or QIMG_BF16 with rows of
  * ldo, may be residual itself (same type and ld), else overlaps no operand.
  * fp32 accumulation and epilogue, one rounding. bf16 rows of x must start at
- * 16-byte boundaries (ldx a multiple of 8; fp32: of 4) unless K is no multiple of 8, where x and the
- * weights are copied to scratch first. ld* < 2^22.
+ * 16-byte boundaries (ldx a multiple of 8; fp32: of 4) unless K is no multiple of 8,
+ * where x and the weights are copied to scratch on every call, two to three times
+ * the call's bytes (4608 columns, K 3583 and 3584: 1 row 33 and 10 us, 781 rows 73
+ * and 46): pad the weights' K once where it matters. ld* < 2^22.
+ * Without gate, second product and residual qimg_linear_bf16 computes the same
+ * to fp32. It is the faster one for 17 to 64 rows of some thousand columns (32 x 3584 x
+ * 3584 11 us, here 17) and 2 to 16 fp32 rows (2 x 12288 x 1536 11, here 18), this one
+ * from about 128 rows on (512 x 3584 x 3584 27, there 38; fp32 rows 1024 x 14336 x 3584
+ * 101, there 331), for one row of up to some thousand columns (1 x 3584 x 3584 7.5, there
+ * 10.4) and wherever K is no multiple of 64 (256 x 1000 x 2056 9, there 2050).
  * scratch: qimg_linear_bf16_fused_scratch_bytes(...) bytes (may be 0: NULL) for
  * this call's sizes; fewer rows can need more (their sum over K is split). One
  * scratch buffer serves one call at a time. */

@@ -915,8 +915,8 @@ int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 // 16x3584x3584 rows 10.8, 32x64 tiles 13; 16x4608x3584 17.5 / 11.7; 21x3584x14336
 // 32x64 split in 4 25, 32x128 in 9 26; 269x4608x3584 96x64 tiles 20.5, 160x256 split
 // in 4 28; 269x3584x14336 160x256 split in 9 45-49, 96x64 split in 4 72;
-// 281x3584x12288 160x256 split in 9 45, 96x64 split in 3 56; 500x4608x3584 96x64 38,
-// 128x256 split in 2 41; 930x4608x3584 160x256 split in 2 49, 96x64 56;
+// 281x3584x12288 160x256 split in 9 45, 96x64 split in 3 56; 500x4608x3584 128x256
+// split in 3 36, 96x64 38; 930x4608x3584 160x256 split in 2 49, 96x64 56;
 // 1672x3584x3584 192x256 split in 2 58, 128x256 65; 781x14336x3584 gated 224x256 158,
 // 256x256 162; 64x14336x3584 gated 64x128 43. Not always the best: 2605x3584x12288
 // 224x256 split in 3 218, 160x256 215.
