@@ -304,7 +304,7 @@ enum { QIMG_ACT_NONE = 0, QIMG_ACT_GELU_TANH = 1, QIMG_ACT_SILU = 2 };
  * 3584 11 us, here 17) and 2 to 16 fp32 rows (2 x 12288 x 1536 11, here 18), this one
  * from about 128 rows on (512 x 3584 x 3584 27, there 38; fp32 rows 1024 x 14336 x 3584
  * 101, there 331), for one row of up to some thousand columns (1 x 3584 x 3584 7.5, there
- * 10.4) and wherever K is no multiple of 64 (256 x 1000 x 2056 9, there 2050).
+ * 10.4) and wherever K is no multiple of 32 (256 x 1000 x 2056 9, there 2050).
  * scratch: qimg_linear_bf16_fused_scratch_bytes(...) bytes (may be 0: NULL) for
  * this call's sizes; fewer rows can need more (their sum over K is split). One
  * scratch buffer serves one call at a time. */
