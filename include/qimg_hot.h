@@ -250,7 +250,7 @@ int qimg_sage_attention(const uint16_t* q_f16, const uint16_t* k_f16, const uint
  * Scores, softmax statistics and sums are fp32; the weights are rounded to dtype
  * for the matrix unit, before they are summed and multiplied by v: out is off by
  * sum_j (u p_ij + w) |v_j - out_i| at most beside its own rounding, u = 2^-8 and w = 0
- * in bf16, u = 2^-11 and w = 2^-32 in fp16.
+ * in bf16 (of which averages below 2^-79 lose digits), u = 2^-11 and w = 2^-32 in fp16.
  * What lies behind a sequence's last key or is hidden from a row does not
  * reach that row, NaN and infinities included; an infinity of v that a row
  * sees makes that channel of it infinite, or NaN where the weight is less than

@@ -375,7 +375,8 @@ __device__ __forceinline__ int range_tiles(const AttnVarlenArgs& a, const Sequen
     tiles *= static_cast<float>(a.hk);
     work *= static_cast<float>(a.hk);
     const bool alike = tiles > kFewGrid / 4 && static_cast<float>(longest) * tiles < 1.5f * work;
-    int per = alike ? longest : static_cast<int>(work / fmaxf(kFewGrid, 1.25f * tiles)) + 1;
+    // (a sequence has at most 2^25 key tiles; offsets that overlap may sum to any number)
+    int per = alike ? longest : static_cast<int>(fminf(work / fmaxf(kFewGrid, 1.25f * tiles), 0x1p25f)) + 1;
     per = max(max(per, 4 * SW), (longest + a.splits - 1) / a.splits);
     return __builtin_amdgcn_readfirstlane(min(per, max(longest, 1)));
 }
@@ -1142,7 +1143,9 @@ constexpr int kGroupTiles = 256;  // workgroups of two groups that run at once, 
 // of 8192 keys beside 5 of 64, 24 heads, 34 / 101, beside 31, 28 on 4 heads, 17 / 138,
 // 127 24.6 / 142; 32 random lengths up to 8192 55 / 106; all alike, 6 x 8192 139 / 136, 64 x
 // 300 16.3 / 14.7, the launch that joins; 16 on 8 heads of 64, 32 x 8192 114 / 97). More
-// keep every CU busy whatever their lengths (of 2048 tiles, random, 885 / 819).
+// keep every CU busy whatever their lengths (of 2048 tiles, random, 885 / 819). A few: at
+// most 8 queries and 32 rows a sequence on average, as a prompt among tokens wants its
+// large tiles (6 heads, 512 tokens and 31 single ones over 4000 keys each 105 / 78).
 constexpr int kManyTiles = kFewGrid * SR / MR + 1;
 
 // The tail of a launch of `tiles` equal tiles of 128 rows without a causal mask:
@@ -1177,8 +1180,8 @@ AttnVarlenPlan attn_varlen_plan(int total_q, int total_k, int batch, int hq, int
     if (total_q <= 0 || batch <= 0 || total_k <= 0) return p;
     const int64_t many = tile_bound(total_q, batch, hq / hk, MR) * hk;
     const int64_t few = tile_bound(total_q, batch, hq / hk, SR) * hk;
-    const bool cached = few <= 2 * kFewGrid && total_k / 8 >= total_q &&
-                        static_cast<int64_t>(total_q) * (hq / hk) <= static_cast<int64_t>(SR) * std::min(batch, total_q);
+    const int64_t seqs = std::min(batch, total_q), rows = static_cast<int64_t>(total_q) * (hq / hk);
+    const bool cached = few <= 2 * kFewGrid && total_k / 8 >= total_q && total_q <= 8 * seqs && rows <= SR * seqs;
     // (a workgroup a tile, and a grid has less than 2^32 threads: beyond, the kernel that walks)
     p.many = many >= kManyTiles && many < (1 << 22) && !cached;
     if (p.many) {

@@ -12,7 +12,7 @@ from planutil import attn_plan
 def test_tokens_over_caches_may_cut_their_keys(qimg, b, hq, hk, d, causal):
     """One token a sequence over caches of unknown lengths: the keys of a long one
     among short ones can go into ranges, however many sequences there are."""
-    for lq in (1, max(1, 32 * hk // hq)):  # up to 32 rows a sequence
+    for lq in (1, max(1, min(8, 32 * hk // hq))):  # up to 8 queries and 32 rows a sequence
         p = attn_plan(qimg, b * lq, b * 8192, b, hq, hk, d, causal)
         assert not p.many and p.splits >= 8
         assert qimg.attention_varlen_scratch_bytes(b * lq, b * 8192, b, hq, hk, d, causal) <= 160 << 20
@@ -23,6 +23,7 @@ def test_prompts_keep_their_tiles(qimg):
     assert attn_plan(qimg, 4096, 4096, 1, 28, 4, 128, True).many
     assert attn_plan(qimg, 400, 400, 20, 24, 24, 128, True).many
     assert attn_plan(qimg, 640, 9000, 20, 28, 4, 128, True).many
+    assert attn_plan(qimg, 512 + 31, 32 * 4000, 32, 6, 6, 128, True).many  # a prompt among tokens
     assert not attn_plan(qimg, 90, 90, 2, 28, 4, 128, True).many
 
 
