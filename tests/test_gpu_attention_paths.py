@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from planutil import attn_plan
-from test_gpu_attention_varlen import _run
+from test_gpu_attention_varlen import DEV, _check, _oracle, _run
 
 pytestmark = pytest.mark.gpu
 F16, BF = torch.float16, torch.bfloat16
@@ -38,3 +38,36 @@ def test_many_sequences_of_many_rows(qimg, causal):
     keys = [n * (30 + 11 * i) for i, n in enumerate(few)]
     assert attn_plan(qimg, sum(few), sum(keys), 130, 8, 2, 64, causal).splits > 1
     _run(qimg, few, keys, hq=8, hk=2, d=64, causal=causal, seed=5)
+
+
+def test_one_graph_for_like_and_unlike_lengths(qimg):
+    """The ranges follow the lengths on the device: a captured call of 40 tokens serves
+    caches that are all alike (whole), of which one is long (in ranges), and empty ones."""
+    b, cap = 40, 6000
+    g = torch.Generator(device=DEV)
+    g.manual_seed(2)
+    q = torch.randn(b, 28, 128, generator=g, device=DEV).to(BF)
+    k, v = (torch.randn(b * cap, 4, 128, generator=g, device=DEV).to(BF) for _ in range(2))
+    cuq = torch.arange(b + 1, dtype=torch.int32, device=DEV)
+    kl = torch.full((b,), cap, dtype=torch.int32, device=DEV)
+    out = torch.empty_like(q)
+    scratch = torch.empty(qimg.attention_varlen_scratch_bytes(b, b * cap, b, 28, 4, 128), dtype=torch.uint8, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        qimg.attention_varlen(q, k, v, cuq, cuq * cap, k_lens=kl, out=out, scratch=scratch)
+    torch.cuda.current_stream().wait_stream(side)
+    cuk = cuq * cap
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        qimg.attention_varlen(q, k, v, cuq, cuk, k_lens=kl, out=out, scratch=scratch)
+    offsets = [i * cap for i in range(b + 1)]
+    for lens in ([cap] * b, [cap] + [40] * (b - 1), [0] * b, [i * 149 for i in range(b)], [0, 1] * (b // 2), [700] * b):
+        kl.copy_(torch.tensor(lens, dtype=torch.int32))
+        out.fill_(7.0)
+        scratch.fill_(255)  # NaN in every part
+        graph.replay()
+        torch.cuda.synchronize()
+        want, mag = _oracle(q, k, v, list(range(b + 1)), offsets, lens, 128 ** -0.5, True)
+        _check(out, want, mag, BF)
+        assert torch.equal(out, qimg.attention_varlen(q, k, v, cuq, cuk, k_lens=kl))
