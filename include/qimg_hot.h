@@ -359,6 +359,119 @@ typedef struct {
 } qimg_rope;
 int qimg_rope_packed(const qimg_rope* args, void* stream);
 
+/* ---- prompts: head norms, and a quantized key/value cache ------------------- */
+
+/* Norm and rotary positions of packed heads in one pass: of each token's n_q_heads q,
+ * n_kv_heads k and n_kv_heads v heads (in this order along x's head stride) the q and k
+ * heads become
+ *   y = x * (mean(x^2) + eps)^(-1/2) * w,   w = q_norm or k_norm, bf16 [head_dim]
+ * (NULL: no norm), then y's first rotary_dim values are turned as qimg_rope_packed turns
+ * them (cos_sin NULL: no rotation, positions are not read); v heads are copied. x and out
+ * QIMG_FP32, QIMG_BF16 or QIMG_FP16, fp32 arithmetic, one rounding; strides as there.
+ * head_dim a multiple of 8 up to 256, rotary_dim a multiple of 8. A token whose position
+ * lies outside [0, table_rows) is not written. A sum of squares past 2^128 gives zeros, as
+ * the norm of values past 1e18 is not computed. out may be x (same type and strides), else
+ * does not overlap it; its strides keep tokens and heads apart. tokens times heads below
+ * 2^30. (qimg_joint_heads_f16 is the joint block's own form: fp32 in, head-major fp16 out.) */
+typedef struct {
+    const void* x;
+    int x_dtype;
+    int64_t x_stride_t, x_stride_h;
+    void* out;
+    int out_dtype;
+    int64_t out_stride_t, out_stride_h;
+    int tokens, n_q_heads, n_kv_heads, head_dim, rotary_dim, interleaved;
+    const uint16_t* q_norm;
+    const uint16_t* k_norm;
+    float eps;
+    const float* cos_sin;
+    int table_rows;
+    const int32_t* positions;
+} qimg_norm_rope;
+int qimg_norm_rope_packed(const qimg_norm_rope* args, void* stream);
+
+/* A key/value cache in codes of eight bits: n_pages pages of page_size tokens (16, 32, 64,
+ * 128 or 256), k and v codes [n_pages, n_kv_heads, page_size, head_dim] (dtype QIMG_INT8 or
+ * QIMG_FP8_E4M3, head_dim 64 or 128) and their exponents k_exp, v_exp uint8 [n_pages,
+ * n_kv_heads, page_size], all on the device, 16-byte aligned. Row (token, kv head) x has
+ * exponent E, the least from 1 to 254 with max|x| <= 127 * 2^(E - 127) (int8) or
+ * 448 * 2^(E - 127) (e4m3), and codes x / 2^(E - 127) rounded half to even; codes times
+ * powers of two are exact in fp32 and bf16, and in fp16 where it has the range. (fp16 rows
+ * of magnitudes above 63488 round towards zero where they would leave fp16.) A token whose k
+ * or v of a head holds an infinity or a NaN has that k stored as NaN (E = 255) and such a v
+ * as zeros: its scores, and the rows that see it, are NaN, and no others.
+ * n_pages * page_size below 2^31. */
+typedef struct {
+    uint8_t* k;
+    uint8_t* v;
+    uint8_t* k_exp;
+    uint8_t* v_exp;
+    int dtype, n_pages, page_size, n_kv_heads, head_dim;
+} qimg_kv_cache;
+
+/* qimg_norm_rope_packed with k and v written into the cache: out receives the q heads
+ * alone, token t's k and v go to slot slots[t] = page * page_size + place in it (int32
+ * [tokens] on the device). Slots outside the cache are not written (the token's q is); a
+ * token without a position neither. The slots of a call are distinct: of two tokens that
+ * share one either's parts may stay. n_kv_heads and head_dim are the cache's. */
+int qimg_norm_rope_cache(const qimg_norm_rope* args, const qimg_kv_cache* cache, const int32_t* slots, void* stream);
+
+/* Rows k and v [tokens, n_kv_heads, head_dim] (QIMG_FP32, QIMG_BF16 or QIMG_FP16, strides
+ * in elements, multiples of 8) into their slots, as they are. */
+int qimg_kv_cache_write(const void* k, const void* v, int dtype, int64_t k_stride_t, int64_t k_stride_h,
+                        int64_t v_stride_t, int64_t v_stride_h, int tokens, const qimg_kv_cache* cache,
+                        const int32_t* slots, void* stream);
+
+/* The first k_lens[b] keys of each sequence read back: key j of sequence b, slot
+ * j % page_size of page block_table[b][j / page_size] (int32 [batch, max_blocks]), goes to
+ * row cu_seqlens_k[b] + j of k and v [total_k, n_kv_heads, head_dim] (dtype QIMG_FP32,
+ * QIMG_BF16 or QIMG_FP16), while that lies in front of cu_seqlens_k[b + 1] (int32 [batch +
+ * 1], rising) and in the table. Keys of a page outside the cache and other rows are not
+ * written. All lists on the device. */
+int qimg_kv_cache_read(const qimg_kv_cache* cache, const int32_t* block_table, int max_blocks, const int32_t* k_lens,
+                       const int32_t* cu_seqlens_k, int batch, void* k, void* v, int dtype, int64_t k_stride_t,
+                       int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h, int total_k, void* stream);
+
+/* Attention of packed queries over the pages of a cache, without and behind a prefix that
+ * all sequences share (qimg_attention_varlen is the form over unquantized rows):
+ *   q and out [total_q, n_heads, head_dim], dtype QIMG_BF16 or QIMG_FP16, strides in
+ *   elements between tokens and heads (multiples of 8, of tokens at most 2^24); n_heads a
+ *   multiple of the cache's n_kv_heads; cu_seqlens_q int32 [batch + 1] on the device.
+ *   Sequence b's own keys: the first k_lens[b] (int32 [batch] on the device) in the pages
+ *   block_table[b] (int32 [batch, max_blocks] on the device), its new ones among them.
+ *   The prefix: the first prefix_len[0] keys (on the device) in the pages prefix_table
+ *   (int32 [prefix_blocks]); prefix_blocks 0: none. It lies in front of every sequence and
+ *   is read once for all.
+ *   causal: own key j is visible to query i when j <= i + keys - queries; the prefix is
+ *   visible to all.
+ * Lengths may be 0 and are cut to what the tables hold; offsets outside q are clamped; keys of
+ * a page outside the cache are not seen. A query that sees no key gives zeros; rows of no
+ * sequence are not written. What lies behind a sequence's last key does not reach it.
+ * Arithmetic and its bounds as qimg_attention_varlen's, on the values that the codes stand
+ * for (which fp16 q needs to be in fp16's range). sm_scale > 0, finite. out overlaps neither q
+ * nor the cache, and its strides keep tokens and heads apart. total_q * n_heads, batch and the
+ * tokens of a table's pages below 2^30.
+ * scratch: qimg_attention_cache_scratch_bytes(...) bytes (may be 0: NULL) for this call's
+ * sizes. One scratch buffer serves one call at a time. */
+typedef struct {
+    const void* q;
+    void* out;
+    int dtype;
+    int64_t q_stride_t, q_stride_h, out_stride_t, out_stride_h;
+    const int32_t* cu_seqlens_q;
+    const int32_t* block_table;
+    const int32_t* k_lens;
+    const int32_t* prefix_table;
+    const int32_t* prefix_len;
+    int batch, total_q, n_heads, max_blocks, prefix_blocks;
+    float sm_scale;
+    int causal;
+} qimg_attn_cache;
+int64_t qimg_attention_cache_scratch_bytes(int total_q, int batch, int n_heads, int n_kv_heads, int head_dim,
+                                           int page_size, int max_blocks, int prefix_blocks);
+int qimg_attention_cache(const qimg_attn_cache* args, const qimg_kv_cache* cache, void* scratch, int64_t scratch_bytes,
+                         void* stream);
+
 /* ---- MMDiT joint block: the operations around the hot path ------------ */
 
 /* silu_fp32 (cuda_kernels.cu:1881-1893): out[i] = x[i] / (1 + exp(-x[i])). */

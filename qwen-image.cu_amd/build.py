@@ -49,10 +49,11 @@ HIP_FLAGS = [
 SOURCES = ["hadamard_quant.hip", "gemm_w8a8.hip", "gemm_small_m.hip", "gemm_bf16.hip", "sage_attention.hip", "block_ops.hip",
            "mmdit_block.hip", "capi.hip", "linear_noalloc.hip", "int4.hip", "capi_int4.hip",
            "attention_varlen.hip", "gemm_fused.hip", "rope_packed.hip",
-           "capi_prompt.hip"]
+           "capi_prompt.hip", "kv_cache.hip", "attention_cache.hip", "capi_cache.hip"]
 # MFMA results in vector registers: with the accumulators in AGPRs the compiler
 # copies them back and forth around every rescale of the online softmax.
-SOURCE_FLAGS = {"attention_varlen.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form=1")}
+SOURCE_FLAGS = {"attention_varlen.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form=1"),
+                "attention_cache.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form=1")}
 HOST_SOURCES = ["kernels.cpp", "checkpoint.cpp"]
 PROBE_SOURCE = "mfma_probe.hip"
 

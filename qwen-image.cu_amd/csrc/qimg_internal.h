@@ -400,4 +400,82 @@ struct RopeArgs {
 };
 hipError_t launch_rope_packed(const RopeArgs& a, int x_dtype, int out_dtype, hipStream_t stream);
 
+// A quantized cache: codes [n_pages, hk, page, D] and their exponents
+// [n_pages, hk, page] (cache_codes.h), pages of 2^page_shift tokens.
+struct CachePages {
+    const uint8_t* k;
+    const uint8_t* v;
+    const uint8_t* ke;
+    const uint8_t* ve;
+    int n_pages, page_shift, hk;
+};
+
+// kv_cache.hip: norm and rotary positions of packed heads, to a packed output
+// (qimg_norm_rope_packed) or k and v into a cache (qimg_norm_rope_cache,
+// qimg_kv_cache_write: no q heads); strides in elements
+struct HeadsArgs {
+    const void* x;  // q heads; without a cache k and v heads behind them
+    void* out;
+    int64_t x_t, x_h, o_t, o_h;
+    int out_dtype;
+    int tokens, nq, nk, d, r, interleaved;
+    const uint16_t* wq;  // or null: no norm
+    const uint16_t* wk;
+    float eps;
+    const float* table;  // [table_rows, r / 2, 2]: cos, sin; or null: no rotation
+    int table_rows;
+    const int* positions;  // [tokens]
+    const void* k;  // with a cache
+    const void* v;
+    int64_t k_t, k_h, v_t, v_h;
+    uint8_t* ck;
+    uint8_t* cv;
+    uint8_t* cke;
+    uint8_t* cve;
+    int page_shift, n_slots;
+    const int* slots;  // [tokens]
+};
+// codes: QIMG_INT8, QIMG_FP8_E4M3, or -1 without a cache
+hipError_t launch_heads(const HeadsArgs& a, int x_dtype, int codes, hipStream_t stream);
+
+struct CacheReadArgs {
+    CachePages c;
+    int d, batch, total, max_blocks;
+    const int* table;   // [batch, max_blocks]
+    const int* k_lens;  // [batch]
+    const int* cu;      // [batch + 1]: rows of the sequences
+    void* k;
+    void* v;
+    int64_t k_t, k_h, v_t, v_h;
+};
+hipError_t launch_cache_read(const CacheReadArgs& a, int codes, int out_dtype, hipStream_t stream);
+
+// attention_cache.hip: attention over the pages of a cache (qimg_attention_cache)
+struct AttnCacheArgs {
+    const uint16_t* q;
+    uint16_t* out;
+    int64_t q_t, q_h, o_t, o_h;
+    CachePages c;
+    const int* cu_q;    // [batch + 1]
+    const int* table;   // [batch, max_blocks]
+    const int* k_lens;  // [batch]
+    const int* prefix_table;  // [prefix_blocks], or null: no prefix
+    const int* prefix_len;    // [1]
+    int max_blocks, prefix_blocks;
+    int batch, total_q, hq, group;
+    int causal;
+    float scale_log2;  // sm_scale * log2(e)
+    int own_splits, prefix_splits;  // key ranges, most of a sequence, of the prefix
+    float* part_o;   // [total_q, hq, own_splits + prefix_splits, D]
+    float* part_ml;  // the same of 2: running maximum, sum
+};
+struct AttnCachePlan {
+    int own_rows, prefix_rows;      // rows of a tile, of a sequence's own keys and of the prefix
+    int own_splits, prefix_splits;
+    int64_t part_rows;  // rows of part_o: 0 where every sequence's keys are one range and there is no prefix
+};
+AttnCachePlan attn_cache_plan(int total_q, int batch, int hq, int hk, int D, int64_t own_keys, int64_t prefix_keys);
+hipError_t launch_attention_cache(const AttnCacheArgs& a, const AttnCachePlan& plan, int dtype, int codes, int D,
+                                  hipStream_t stream);
+
 }  // namespace qimg

@@ -12,6 +12,7 @@ from __future__ import annotations
 import ctypes
 import os
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
@@ -72,6 +73,12 @@ _SIGS = {
     "qimg_linear_bf16_fused_scratch_bytes": (_I64, [_I, _I, _I, _I, _I]),
     "qimg_linear_bf16_fused": (_I, [_P, _P, _I64, _P]),
     "qimg_rope_packed": (_I, [_P, _P]),
+    "qimg_norm_rope_packed": (_I, [_P, _P]),
+    "qimg_norm_rope_cache": (_I, [_P, _P, _P, _P]),
+    "qimg_kv_cache_write": (_I, [_P, _P, _I, _I64, _I64, _I64, _I64, _I, _P, _P, _P]),
+    "qimg_kv_cache_read": (_I, [_P, _P, _I, _P, _P, _I, _P, _P, _I, _I64, _I64, _I64, _I64, _I, _P]),
+    "qimg_attention_cache_scratch_bytes": (_I64, [_I, _I, _I, _I, _I, _I, _I, _I]),
+    "qimg_attention_cache": (_I, [_P, _P, _P, _I64, _P]),
     "qimg_silu": (_I, [_P, _P, _I64, _P]),
     "qimg_layernorm_modulate": (_I, [_P, _P, _P, _P, _I, _I, _F, _P]),
     "qimg_layernorm_modulate_quant": (_I, [_P, _P, _P, _I, _I, _I, _I, _F, _P, _P, _P]),
@@ -849,6 +856,253 @@ def rope_packed(x: torch.Tensor, cos_sin: torch.Tensor, positions: torch.Tensor,
                      *_head_strides(out, T, H, D), T, H, n_rotated, D,
                      2 * cos_sin.shape[1], bool(interleaved), _addr(cos_sin), cos_sin.shape[0], _addr(positions))
         _check(_lib.qimg_rope_packed(ctypes.byref(args), _raw_stream(dev)))
+    return out
+
+
+# ------------------------- prompts: head norms, a quantized key/value cache
+class _NormRope(ctypes.Structure):
+    _fields_ = [("x", _P), ("x_dtype", _I), ("x_stride_t", _I64), ("x_stride_h", _I64), ("out", _P), ("out_dtype", _I),
+                ("out_stride_t", _I64), ("out_stride_h", _I64), ("tokens", _I), ("n_q_heads", _I), ("n_kv_heads", _I),
+                ("head_dim", _I), ("rotary_dim", _I), ("interleaved", _I), ("q_norm", _P), ("k_norm", _P), ("eps", _F),
+                ("cos_sin", _P), ("table_rows", _I), ("positions", _P)]
+
+
+class _KvCache(ctypes.Structure):
+    _fields_ = [("k", _P), ("v", _P), ("k_exp", _P), ("v_exp", _P), ("dtype", _I), ("n_pages", _I), ("page_size", _I),
+                ("n_kv_heads", _I), ("head_dim", _I)]
+
+
+class _AttnCache(ctypes.Structure):
+    _fields_ = [("q", _P), ("out", _P), ("dtype", _I), ("q_stride_t", _I64), ("q_stride_h", _I64), ("out_stride_t", _I64),
+                ("out_stride_h", _I64), ("cu_seqlens_q", _P), ("block_table", _P), ("k_lens", _P), ("prefix_table", _P),
+                ("prefix_len", _P), ("batch", _I), ("total_q", _I), ("n_heads", _I), ("max_blocks", _I),
+                ("prefix_blocks", _I), ("sm_scale", _F), ("causal", _I)]
+
+
+class KvCache(NamedTuple):
+    """A key/value cache in codes of eight bits (qimg_kv_cache): pages of
+    page_size tokens (16 to 256, a power of two), D 64 or 128."""
+    k: torch.Tensor      # [n_pages, Hk, page_size, D] int8 or float8_e4m3fn
+    v: torch.Tensor
+    k_exp: torch.Tensor  # [n_pages, Hk, page_size] uint8: exponent + 127 of each row's power of two
+    v_exp: torch.Tensor
+
+
+def kv_cache(n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dtype=torch.float8_e4m3fn,
+             device="cuda") -> KvCache:
+    """An empty cache (zeros)."""
+    if dtype not in (torch.int8, torch.float8_e4m3fn):
+        raise QimgError(QIMG_ERR_INVALID_ARG, "a cache holds int8 or float8_e4m3fn codes")
+    k, v = (torch.zeros((n_pages, n_kv_heads, page_size, head_dim), dtype=torch.uint8, device=device).view(dtype)
+            for _ in range(2))
+    ke, ve = (torch.full((n_pages, n_kv_heads, page_size), 127, dtype=torch.uint8, device=device) for _ in range(2))
+    return KvCache(k, v, ke, ve)
+
+
+def _cache_struct(cache: KvCache, device) -> _KvCache:
+    k, v, ke, ve = cache
+    if k.device != device or v.device != device or ke.device != device or ve.device != device:
+        raise QimgError(QIMG_ERR_INVALID_ARG, f"the cache must be on {device}, the first argument's device")
+    if k.dtype not in (torch.int8, torch.float8_e4m3fn) or v.dtype != k.dtype:
+        raise QimgError(QIMG_ERR_INVALID_ARG, "the cache's codes must be int8 or float8_e4m3fn")
+    if k.dim() != 4 or v.shape != k.shape or not k.is_contiguous() or not v.is_contiguous():
+        raise QimgError(QIMG_ERR_INVALID_ARG, "the cache's k and v must be contiguous [n_pages, Hk, page_size, D]")
+    if (ke.dtype != torch.uint8 or ve.dtype != torch.uint8 or ke.shape != k.shape[:3] or ve.shape != ke.shape
+            or not ke.is_contiguous() or not ve.is_contiguous()):
+        raise QimgError(QIMG_ERR_INVALID_ARG, "the cache's exponents must be contiguous uint8 [n_pages, Hk, page_size]")
+    n, hk, page, d = k.shape
+    _fits32(n, hk, page, d)
+    return _KvCache(k.data_ptr(), v.data_ptr(), ke.data_ptr(), ve.data_ptr(), INT8 if k.dtype == torch.int8 else FP8_E4M3,
+                    n, page, hk, d)
+
+
+def _list32(t: torch.Tensor, n: int, name: str):
+    if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous():
+        raise QimgError(QIMG_ERR_INVALID_ARG, f"{name} must be contiguous int32 of {n} elements")
+
+
+def _norm_rope(x, n_q, n_kv, q_norm, k_norm, eps, cos_sin, positions, interleaved, out, out_heads, out_dtype):
+    """The checked arguments and the output of norm_rope_packed and norm_rope_cache."""
+    if not (x.is_cuda and x.dim() == 3):
+        raise QimgError(QIMG_ERR_INVALID_ARG, "x must be a device tensor [T, H, D]")
+    dev = x.device
+    T, H, D = x.shape
+    _same_device(dev, q_norm, k_norm, cos_sin, positions, out)
+    _fits32(T, H, D, n_q, n_kv)
+    if n_q < 0 or n_kv < 0 or H != n_q + 2 * n_kv:
+        raise QimgError(QIMG_ERR_INVALID_ARG, f"x has {H} heads, not {n_q} + 2 * {n_kv}")
+    if out is None:
+        out = _new(T, out_heads, D, out_dtype or x.dtype, dev)
+    elif out.shape != (T, out_heads, D):
+        raise QimgError(QIMG_ERR_INVALID_ARG, f"out must be {(T, out_heads, D)}")
+    if x.dtype not in _HEAD_TYPES or out.dtype not in _HEAD_TYPES:
+        raise QimgError(QIMG_ERR_INVALID_ARG, "x and out must be float32, bfloat16 or float16")
+    for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        if w is not None and (w.dtype != torch.bfloat16 or w.numel() != D or not w.is_contiguous()):
+            raise QimgError(QIMG_ERR_INVALID_ARG, f"{name} must be contiguous bfloat16 of {D} elements")
+    rows = r = 0
+    if cos_sin is not None:
+        if (cos_sin.dtype != torch.float32 or cos_sin.dim() != 3 or cos_sin.shape[2] != 2 or not cos_sin.is_contiguous()
+                or cos_sin.numel() == 0):
+            raise QimgError(QIMG_ERR_INVALID_ARG, "cos_sin must be contiguous float32 [P, R / 2, 2], not empty")
+        if positions is None:
+            raise QimgError(QIMG_ERR_INVALID_ARG, "cos_sin needs positions")
+        _list32(positions, T, "positions")
+        rows, r = cos_sin.shape[0], 2 * cos_sin.shape[1]
+        _fits32(rows, r)
+    return out, _NormRope(x.data_ptr(), _DT[x.dtype], *_head_strides(x, T, H, D), out.data_ptr(), _DT[out.dtype],
+                          *_head_strides(out, T, out_heads, D), T, n_q, n_kv, D, r, bool(interleaved), _addr(q_norm),
+                          _addr(k_norm), eps, _addr(cos_sin), rows, _addr(positions))
+
+
+def norm_rope_packed(x: torch.Tensor, n_q_heads: int, n_kv_heads: int, q_norm: torch.Tensor | None = None,
+                     k_norm: torch.Tensor | None = None, eps: float = 1e-6, cos_sin: torch.Tensor | None = None,
+                     positions: torch.Tensor | None = None, interleaved: bool = False, out: torch.Tensor | None = None,
+                     out_dtype=None) -> torch.Tensor:
+    """Norm and rotary positions of packed heads in one pass: x [T, Hq + 2 Hk,
+    D] (fp32, bf16 or fp16; any token and head strides that are multiples of 8),
+    its q and k heads x * rsqrt(mean(x^2) + eps) * weight (bf16 [D]; None: no
+    norm), turned by row positions[t] of cos_sin as rope_packed turns them
+    (None: not at all), its v heads copied. A token whose position lies outside
+    the table is not written. out may be x; its type defaults to x's."""
+    out, args = _norm_rope(x, n_q_heads, n_kv_heads, q_norm, k_norm, eps, cos_sin, positions, interleaved, out,
+                           x.shape[1] if x.dim() == 3 else 0, out_dtype)
+    with _on(x.device):
+        _check(_lib.qimg_norm_rope_packed(ctypes.byref(args), _raw_stream(x.device)))
+    return out
+
+
+def norm_rope_cache(x: torch.Tensor, n_q_heads: int, cache: KvCache, slots: torch.Tensor,
+                    q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, eps: float = 1e-6,
+                    cos_sin: torch.Tensor | None = None, positions: torch.Tensor | None = None,
+                    interleaved: bool = False, out: torch.Tensor | None = None, out_dtype=None) -> torch.Tensor:
+    """norm_rope_packed with k and v written into the cache: returns the q heads
+    [T, Hq, D]; token t's k and v go to slot slots[t] = page * page_size + place
+    (int32 [T], distinct; a slot outside the cache is not written)."""
+    out, args = _norm_rope(x, n_q_heads, cache.k.shape[1], q_norm, k_norm, eps, cos_sin, positions, interleaved, out,
+                           n_q_heads, out_dtype)
+    dev = x.device
+    c = _cache_struct(cache, dev)
+    _same_device(dev, slots)
+    _list32(slots, x.shape[0], "slots")
+    with _on(dev):
+        _check(_lib.qimg_norm_rope_cache(ctypes.byref(args), ctypes.byref(c), slots.data_ptr(), _raw_stream(dev)))
+    return out
+
+
+def kv_cache_write(cache: KvCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+    """Rows k and v [T, Hk, D] (fp32, bf16 or fp16; any token and head strides
+    that are multiples of 8) into slots [T] of the cache, as they are."""
+    if not (k.is_cuda and k.dim() == 3 and v.dim() == 3):
+        raise QimgError(QIMG_ERR_INVALID_ARG, "k and v must be device tensors [T, Hk, D]")
+    dev = k.device
+    c = _cache_struct(cache, dev)
+    _same_device(dev, v, slots)
+    if k.dtype not in _HEAD_TYPES or v.dtype != k.dtype:
+        raise QimgError(QIMG_ERR_INVALID_ARG, "k and v must be float32, bfloat16 or float16, both the same")
+    T, hk, d = k.shape
+    if v.shape != k.shape or (hk, d) != (c.n_kv_heads, c.head_dim):
+        raise QimgError(QIMG_ERR_INVALID_ARG, f"k and v must be [T, {c.n_kv_heads}, {c.head_dim}]")
+    _fits32(T)
+    _list32(slots, T, "slots")
+    with _on(dev):
+        _check(_lib.qimg_kv_cache_write(k.data_ptr(), v.data_ptr(), _DT[k.dtype], *_head_strides(k, T, hk, d),
+                                        *_head_strides(v, T, hk, d), T, ctypes.byref(c), slots.data_ptr(),
+                                        _raw_stream(dev)))
+
+
+def _block_table(t: torch.Tensor, batch: int):
+    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != batch or not t.is_contiguous():
+        raise QimgError(QIMG_ERR_INVALID_ARG, f"block_table must be contiguous int32 [{batch}, n]")
+
+
+def kv_cache_read(cache: KvCache, block_table: torch.Tensor, k_lens: torch.Tensor, cu_seqlens_k: torch.Tensor,
+                  total_k: int, out_dtype=torch.bfloat16, k_out: torch.Tensor | None = None,
+                  v_out: torch.Tensor | None = None):
+    """The first k_lens[b] keys of each sequence, in the pages block_table[b]
+    (int32 [B, n]), as rows cu_seqlens_k[b] .. of k and v [total_k, Hk, D].
+    Rows behind a sequence's last key are not written. k_out and v_out: both or
+    neither, of one type."""
+    if not cache.k.is_cuda:
+        raise QimgError(QIMG_ERR_INVALID_ARG, "the cache must be on a device")
+    dev = cache.k.device
+    c = _cache_struct(cache, dev)
+    _same_device(dev, block_table, k_lens, cu_seqlens_k, k_out, v_out)
+    batch, hk, d = k_lens.numel(), c.n_kv_heads, c.head_dim
+    _block_table(block_table, batch)
+    _list32(k_lens, batch, "k_lens")
+    _list32(cu_seqlens_k, batch + 1, "cu_seqlens_k")
+    _fits32(total_k, batch, block_table.shape[1])
+    if (k_out is None) != (v_out is None):
+        raise QimgError(QIMG_ERR_INVALID_ARG, "k_out and v_out must be given together")
+    if k_out is None:
+        k_out, v_out = _new(total_k, hk, d, out_dtype, dev), _new(total_k, hk, d, out_dtype, dev)
+    if k_out.shape != (total_k, hk, d) or v_out.shape != k_out.shape:
+        raise QimgError(QIMG_ERR_INVALID_ARG, f"k_out and v_out must be {(total_k, hk, d)}")
+    if k_out.dtype not in _HEAD_TYPES or v_out.dtype != k_out.dtype:
+        raise QimgError(QIMG_ERR_INVALID_ARG, "k_out and v_out must be float32, bfloat16 or float16, both the same")
+    with _on(dev):
+        _check(_lib.qimg_kv_cache_read(ctypes.byref(c), block_table.data_ptr(), block_table.shape[1], k_lens.data_ptr(),
+                                       cu_seqlens_k.data_ptr(), batch, k_out.data_ptr(), v_out.data_ptr(),
+                                       _DT[k_out.dtype], *_head_strides(k_out, total_k, hk, d),
+                                       *_head_strides(v_out, total_k, hk, d), total_k, _raw_stream(dev)))
+    return k_out, v_out
+
+
+def attention_cache_scratch_bytes(total_q: int, batch: int, n_heads: int, n_kv_heads: int, head_dim: int,
+                                  page_size: int, max_blocks: int, prefix_blocks: int = 0) -> int:
+    _fits32(total_q, batch, n_heads, n_kv_heads, head_dim, page_size, max_blocks, prefix_blocks)
+    return int(_lib.qimg_attention_cache_scratch_bytes(total_q, batch, n_heads, n_kv_heads, head_dim, page_size,
+                                                       max_blocks, prefix_blocks))
+
+
+def attention_cache(q: torch.Tensor, cache: KvCache, cu_seqlens_q: torch.Tensor, block_table: torch.Tensor,
+                    k_lens: torch.Tensor, sm_scale: float | None = None, causal: bool = True,
+                    prefix_table: torch.Tensor | None = None, prefix_len: torch.Tensor | None = None,
+                    out: torch.Tensor | None = None, scratch: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of packed queries q [Tq, Hq, D] (bf16 or fp16, any token and
+    head strides that are multiples of 8; cu_seqlens_q int32 [B + 1]) over the
+    first k_lens[b] keys in each sequence's pages block_table[b] (int32 [B, n]),
+    new tokens' among them. causal: the last query of a sequence sees its last
+    key. prefix_table int32 [m], prefix_len int32 [1]: pages and keys of a prefix
+    that lies in front of every sequence and is read once for all. Queries that
+    see no key give zeros; rows of no sequence are not written. sm_scale defaults
+    to 1 / sqrt(D)."""
+    if not (q.is_cuda and q.dim() == 3):
+        raise QimgError(QIMG_ERR_INVALID_ARG, "q must be a device tensor [T, H, D]")
+    dev, dt = q.device, q.dtype
+    if dt not in (torch.bfloat16, torch.float16):
+        raise QimgError(QIMG_ERR_INVALID_ARG, "q must be bfloat16 or float16")
+    c = _cache_struct(cache, dev)
+    _same_device(dev, cu_seqlens_q, block_table, k_lens, prefix_table, prefix_len, out)
+    tq, hq, d = q.shape
+    if d != c.head_dim:
+        raise QimgError(QIMG_ERR_INVALID_ARG, f"q has heads of {d} values, the cache of {c.head_dim}")
+    batch = k_lens.numel()
+    _list32(cu_seqlens_q, batch + 1, "cu_seqlens_q")
+    _list32(k_lens, batch, "k_lens")
+    _block_table(block_table, batch)
+    if (prefix_table is None) != (prefix_len is None):
+        raise QimgError(QIMG_ERR_INVALID_ARG, "prefix_table and prefix_len must be given together")
+    blocks, shared = block_table.shape[1], 0
+    if prefix_table is not None:
+        shared = prefix_table.numel()
+        _list32(prefix_table, shared, "prefix_table")
+        _list32(prefix_len, 1, "prefix_len")
+    _fits32(tq, hq, batch, blocks, shared)
+    if out is None:
+        out = _new(tq, hq, d, dt, dev)
+    elif out.shape != q.shape or out.dtype != dt:
+        raise QimgError(QIMG_ERR_INVALID_ARG, f"out must be {tuple(q.shape)} of q's type")
+    with _on(dev):
+        scratch = _scratch_for(_lib.qimg_attention_cache_scratch_bytes(tq, batch, hq, c.n_kv_heads, d, c.page_size,
+                                                                       blocks, shared), scratch, dev)
+        args = _AttnCache(q.data_ptr(), out.data_ptr(), _DT[dt], *_head_strides(q, tq, hq, d),
+                          *_head_strides(out, tq, hq, d), cu_seqlens_q.data_ptr(), block_table.data_ptr(),
+                          k_lens.data_ptr(), _addr(prefix_table), _addr(prefix_len), batch, tq, hq, blocks, shared,
+                          1.0 / d ** 0.5 if sm_scale is None else sm_scale, bool(causal))
+        _check(_lib.qimg_attention_cache(ctypes.byref(args), ctypes.byref(c), _addr(scratch), _nbytes(scratch),
+                                         _raw_stream(dev)))
     return out
 
 
