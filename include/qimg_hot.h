@@ -444,8 +444,8 @@ int qimg_kv_cache_read(const qimg_kv_cache* cache, const int32_t* block_table, i
  *   is read once for all.
  *   causal: own key j is visible to query i when j <= i + keys - queries; the prefix is
  *   visible to all.
- * Lengths may be 0 and are cut to what the tables hold; offsets outside q are clamped; keys of
- * a page outside the cache are not seen. A query that sees no key gives zeros; rows of no
+ * Lengths may be 0 and are cut to what the tables hold; offsets outside q are clamped. A query
+ * that sees a key of a page outside the cache is NaN, one that sees no key gives zeros; rows of no
  * sequence are not written. What lies behind a sequence's last key does not reach it.
  * Arithmetic and its bounds as qimg_attention_varlen's, on the values that the codes stand
  * for (which fp16 q needs to be in fp16's range). sm_scale > 0, finite. out overlaps neither q

@@ -96,29 +96,41 @@ __device__ __forceinline__ Sequence load_sequence(const AttnCacheArgs& a, int b,
 __device__ __forceinline__ int row_tiles(const AttnCacheArgs& a, int lq, int rows) {
     return static_cast<int>((static_cast<int64_t>(lq) * a.group + rows - 1) / rows);
 }
-// key ranges of about `per` tiles of SK keys, equally long, that lk keys are cut into
+// What a launch works on: the sequences [lo, hi) and `heads` kv heads from h0 on, in tiles
+// of `rows` rows, whose keys are taken in steps of `SK` or, in tiles of MR rows, `MK` keys.
+struct Part {
+    int lo, hi, rows, h0, heads;
+};
 constexpr int SK = 32;
-__device__ __forceinline__ int key_ranges(int lk, int per) {
-    if (per == 0) return 1;
-    const int n = (lk + SK - 1) / SK;
-    return max((2 * n + per) / (2 * per), 1);
+__device__ __forceinline__ int steps_of(const Part& part, int lk) {
+    return part.rows == MR ? (lk + MK - 1) / MK : (lk + SK - 1) / SK;
 }
+__device__ __forceinline__ int most_ranges(const AttnCacheArgs& a, int b) {
+    return max(b == a.batch ? a.prefix_splits : a.own_splits, 1);
+}
+// key ranges of about `per` steps, equally long, that n steps are cut into (per = 0: one)
+__device__ __forceinline__ int key_ranges(int n, int per, int most) {
+    return per == 0 ? 1 : min(max((2 * n + per) / (2 * per), 1), most);
+}
+// steps of a range where n steps are cut into `parts`
+__device__ __forceinline__ int range_steps(int n, int parts) { return max((n + parts - 1) / parts, 1); }
 
-// Item `idx` of the sequences [lo, hi): in order, each with its tiles of `rows` rows
-// times its key ranges of about `per` key tiles. A lane takes one sequence, a wave
-// scans 64 at a time, the first 64 (`first`, of which some may lie behind hi) loaded once
-// by the caller.
-__device__ __forceinline__ RowTile find_tile(const AttnCacheArgs& a, const Sequence& first, int lo, int hi, int idx,
-                                             int rows, int per) {
+// Item `idx` of the launch: the sequences in order, each with its row tiles times its key
+// ranges. A lane takes one sequence, a wave scans 64 at a time, the first 64 (`first`, of
+// which some may lie behind hi) loaded once by the caller. Tiles of MR rows are whole, inside
+// a causal sequence the last, longest one first.
+__device__ __forceinline__ RowTile find_tile(const AttnCacheArgs& a, const Sequence& first, const Part& part, int idx,
+                                             int per) {
     const int lane = threadIdx.x & 63;
     RowTile t;
     t.found = false;
     t.b = t.q0 = t.lq = t.lk = t.row0 = t.split = 0;
     t.splits = 1;
     int before = 0;
-    for (int b0 = lo; b0 < hi; b0 += 64) {
-        const Sequence s = b0 == lo ? first : load_sequence(a, b0 + lane, hi);
-        const int n = b0 + lane < hi ? row_tiles(a, s.lq, rows) : 0, parts = key_ranges(s.lk, per);
+    for (int b0 = part.lo; b0 < part.hi; b0 += 64) {
+        const Sequence s = b0 == part.lo ? first : load_sequence(a, b0 + lane, part.hi);
+        const int n = b0 + lane < part.hi ? row_tiles(a, s.lq, part.rows) : 0;
+        const int parts = part.rows == MR ? 1 : key_ranges(steps_of(part, s.lk), per, most_ranges(a, b0 + lane));
         const int incl = wave_scan(n * parts);
         const int total = __builtin_amdgcn_readlane(incl, 63);
         const uint64_t hit = __ballot(before + incl > idx);
@@ -134,14 +146,134 @@ __device__ __forceinline__ RowTile find_tile(const AttnCacheArgs& a, const Seque
             if (i < 0 || i >= cnt * t.splits) return t;  // (sums past 2^31: offsets that overlap many times)
             const int tile = i / t.splits;
             t.split = i - tile * t.splits;
-            // (inside a causal sequence the last, longest tile first)
-            t.row0 = (rows == MR && a.causal && t.b != a.batch ? cnt - 1 - tile : tile) * rows;
+            t.row0 = (part.rows == MR && a.causal && t.b != a.batch ? cnt - 1 - tile : tile) * part.rows;
             t.found = true;
             return t;
         }
         before += total;
     }
     return t;
+}
+// Tiles of MR rows in shares: the steps of all tiles one behind the other, sequence by
+// sequence, head by head, tile by tile (a causal tile with all of its sequence's), of
+// which each workgroup takes the same number, whatever tiles they belong to.
+__device__ __forceinline__ int tile_steps(const AttnCacheArgs& a, const Part& part, const Sequence& s, int b, int hi) {
+    return b < hi ? row_tiles(a, s.lq, part.rows) * steps_of(part, s.lk) * part.heads : 0;
+}
+// steps of the sequences [lo, hi)
+__device__ __forceinline__ int count_steps(const AttnCacheArgs& a, const Sequence& first, const Part& part, int hi) {
+    const int lane = threadIdx.x & 63;
+    int total = 0;
+    for (int b0 = part.lo; b0 < hi; b0 += 64)
+        total += wave_sum_dpp(tile_steps(a, part, b0 == part.lo ? first : load_sequence(a, b0 + lane, hi), b0 + lane, hi));
+    return total;
+}
+// row tiles of all sequences
+__device__ __forceinline__ int count_tiles(const AttnCacheArgs& a, const Sequence& first, const Part& part) {
+    const int lane = threadIdx.x & 63;
+    int total = 0;
+    for (int b0 = part.lo; b0 < part.hi; b0 += 64) {
+        const Sequence s = b0 == part.lo ? first : load_sequence(a, b0 + lane, part.hi);
+        total += wave_sum_dpp(b0 + lane < part.hi ? row_tiles(a, s.lq, part.rows) : 0);
+    }
+    return total;
+}
+// Shares of a tile of n steps that begins at step `start`: the first one and their number.
+struct Shares {
+    int first, count;
+};
+__device__ __forceinline__ Shares tile_shares(int start, int n, int share) {
+    const int first = start / share;
+    return {first, n > 0 ? (start + n - 1) / share - first + 1 : 0};
+}
+// The tile of step x, its head and the step's number in it; t.split, t.splits: which of the
+// tile's shares `of` is.
+__device__ __forceinline__ RowTile find_step(const AttnCacheArgs& a, const Sequence& first, const Part& part, int x, int share,
+                                             int of, int& hk, int& step) {
+    const int lane = threadIdx.x & 63;
+    RowTile t;
+    t.found = false;
+    int before = 0;
+    for (int b0 = part.lo; b0 < part.hi; b0 += 64) {
+        const Sequence s = b0 == part.lo ? first : load_sequence(a, b0 + lane, part.hi);
+        const int v = tile_steps(a, part, s, b0 + lane, part.hi), incl = wave_scan(v);
+        const int total = __builtin_amdgcn_readlane(incl, 63);
+        const uint64_t hit = __ballot(before + incl > x);
+        if (x < before + total && hit != 0) {
+            const int src = __builtin_ctzll(hit);
+            t.b = b0 + src;
+            t.q0 = __builtin_amdgcn_readlane(s.q0, src);
+            t.lq = __builtin_amdgcn_readlane(s.lq, src);
+            t.lk = __builtin_amdgcn_readlane(s.lk, src);
+            const int n = steps_of(part, t.lk), tiles = row_tiles(a, t.lq, part.rows);
+            const int i = x - (before + __builtin_amdgcn_readlane(incl, src) - __builtin_amdgcn_readlane(v, src));
+            const int tile = i / n;
+            step = i - tile * n;
+            hk = tile / tiles;
+            t.row0 = (tile - hk * tiles) * part.rows;
+            const Shares shares = tile_shares(x - step, n, share);
+            t.split = of - shares.first;
+            t.splits = shares.count;
+            t.found = hk < part.heads;
+            hk += part.h0;
+            return t;
+        }
+        before += total;
+    }
+    return t;
+}
+
+// Workgroups of tiles of 16 (NR = 1), 32 (2) and MR rows that run at once, by registers
+constexpr int few_grid(int rows) { return rows == 16 ? 768 : 512; }
+constexpr int kManyGrid = 512;
+
+// Shares of `share` steps against `whole` of the tiles themselves: in steps, what a workgroup
+// has to do, starts and joins (6) and the float results (6 for each workgroup, and tile).
+__host__ __device__ __forceinline__ bool shares_pay(float share, float tiles, float whole) {
+    return 1.05f * share + 6.0f + (kManyGrid + tiles) * (6.0f / kManyGrid) < whole;
+}
+
+// Steps of a range, about, or of a share; 0: tiles are whole. Lengths are known on the
+// device alone, so this and the ranges follow them in a captured graph.
+// Few rows: as many as make the launch one item a workgroup, at least two a wave. MR rows:
+// shares for the workgroups that run at once, where these take less time than whole tiles.
+__device__ __forceinline__ int range_length(const AttnCacheArgs& a, const Sequence& first, const Part& part) {
+    if (a.own_splits <= 1 && a.prefix_splits <= 1) return 0;
+    const int lane = threadIdx.x & 63;
+    int least = 1, longest = 0;
+    float work = 0.0f, all = 0.0f, tiles = 0.0f;  // steps, with those that a causal mask hides; row tiles: no last digit is needed
+    for (int b0 = part.lo; b0 < part.hi; b0 += 64) {
+        const Sequence s = b0 == part.lo ? first : load_sequence(a, b0 + lane, part.hi);
+        const int n = steps_of(part, s.lk);
+        const float t = b0 + lane < part.hi ? static_cast<float>(row_tiles(a, s.lq, part.rows)) : 0.0f;
+        // (a causal sequence's first tile sees lq keys fewer than its last)
+        const int fewer = part.rows == MR && a.causal && b0 + lane != a.batch ? steps_of(part, min(s.lq, s.lk)) : 0;
+        work += wave_sum_dpp(t * (static_cast<float>(n) - 0.5f * static_cast<float>(fewer)));
+        all += wave_sum_dpp(t * static_cast<float>(n));
+        tiles += wave_sum_dpp(t);
+        const int most = max(most_ranges(a, b0 + lane) - (part.rows == MR ? 1 : 0), 1);
+        least = max(least, wave_reduce_dpp((n + most - 1) / most, [](int x, int y) { return max(x, y); }));
+        longest = max(longest, wave_reduce_dpp(n, [](int x, int y) { return max(x, y); }));
+    }
+    const float heads = static_cast<float>(part.heads);
+    work *= heads;
+    all *= heads;
+    tiles *= heads;
+    int per;
+    if (part.rows == MR) {
+        if (most_ranges(a, part.lo) == 1 || all >= 0x1p30f) return 0;
+        const float each = work / kManyGrid, long_ = static_cast<float>(longest), share = all / kManyGrid;
+        // whole tiles: rounds of the longest, or what evens out while the last ones run
+        const float rounds = ceilf(tiles / kManyGrid) * long_, mixed = each + (a.causal ? 0.25f : 1.0f) * long_;
+        const float whole = fmaxf(fminf(rounds, mixed), fmaxf(each, long_));
+        if (!shares_pay(share, tiles, whole)) return 0;
+        per = max(max(static_cast<int>(share) + 1, 4), least);
+    } else {
+        // (offsets that overlap may sum to any number)
+        per = static_cast<int>(fminf(work / fmaxf(few_grid(part.rows), 1.25f * tiles), 0x1p25f)) + 1;
+        per = max(max(per, 2 * 4), least);
+    }
+    return __builtin_amdgcn_readfirstlane(per);
 }
 
 // number of keys that the query of `token` sees
@@ -177,30 +309,6 @@ __device__ __forceinline__ void store_row(uint16_t* op, const float (&acc)[E], f
 // scale) and takes channel and key of pairs crosswise with v_perm_b32. The k index of
 // the first product is a channel, in any order that K and Q share: a lane's 16 codes.
 constexpr int SW = 4;
-constexpr int kFewGrid = 1024;  // workgroups of the launch at most
-
-// Key tiles per range, about: as many as make the launch one item a workgroup, at least
-// two a wave, at most a.own_splits (prefix_splits) ranges a sequence. 0: no ranges.
-__device__ __forceinline__ int range_tiles(const AttnCacheArgs& a, const Sequence& first, int lo, int hi, int rows) {
-    if (a.own_splits <= 1 && a.prefix_splits <= 1) return 0;
-    const int lane = threadIdx.x & 63;
-    int least = 1;
-    float work = 0.0f, tiles = 0.0f;  // key tiles of all row tiles, row tiles: sums that need no last digit
-    for (int b0 = lo; b0 < hi; b0 += 64) {
-        const Sequence s = b0 == lo ? first : load_sequence(a, b0 + lane, hi);
-        const int kt = (s.lk + SK - 1) / SK;
-        const float n = static_cast<float>(row_tiles(a, s.lq, rows));
-        work += wave_sum_dpp(n * static_cast<float>(kt));
-        tiles += wave_sum_dpp(n);
-        const int most = max(b0 + lane == a.batch ? a.prefix_splits : a.own_splits, 1);
-        least = max(least, wave_reduce_dpp((kt + most - 1) / most, [](int x, int y) { return max(x, y); }));
-    }
-    work *= static_cast<float>(a.c.hk);
-    tiles *= static_cast<float>(a.c.hk);
-    // (offsets that overlap may sum to any number)
-    const int per = static_cast<int>(fminf(work / fmaxf(kFewGrid, 1.25f * tiles), 0x1p25f)) + 1;
-    return __builtin_amdgcn_readfirstlane(max(max(per, 2 * SW), least));
-}
 
 // A wave's 32-key tile as it lies in the cache, each half loaded again as soon as it is used up
 template <int D>
@@ -255,7 +363,7 @@ __device__ __forceinline__ void few_item(const AttnCacheArgs& a, const RowTile& 
     }
     const int kend = visible(a, t, (min(t.row0 + 16 * NR, rows) - 1) / a.group);
     const int kfull = visible(a, t, t.row0 / a.group);
-    const int ntile = (kend + SK - 1) / SK, range = ((t.lk + SK - 1) / SK + t.splits - 1) / t.splits;
+    const int ntile = (kend + SK - 1) / SK, range = range_steps((t.lk + SK - 1) / SK, t.splits);
     const int tile0 = min(t.split * range, ntile), tile1 = min(tile0 + range, ntile);
     const int n = tile1 - tile0 > wave ? (tile1 - tile0 - wave + SW - 1) / SW : 0;
 
@@ -362,7 +470,7 @@ __device__ __forceinline__ void few_item(const AttnCacheArgs& a, const RowTile& 
         __builtin_amdgcn_sched_barrier(0);
         if (i + 1 < n) load_k(i + 1);
         __builtin_amdgcn_sched_barrier(0);
-        const bool hidden = key0 + SK > kfull || x.bad != 0;  // some row does not see some key
+        const bool hidden = key0 + SK > kfull || x.bad != 0;  // some row does not see some key, or not as it lies there
         if (hidden) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -370,8 +478,10 @@ __device__ __forceinline__ void few_item(const AttnCacheArgs& a, const RowTile& 
                 for (int j = 0; j < 4; ++j) {
                     const int key = key0 + 16 * h + 4 * g + j;
 #pragma unroll
-                    for (int r = 0; r < NR; ++r)
-                        if (key >= kmax[r] || (x.bad >> h & 1)) s[r][h][j] = kNegInf;
+                    for (int r = 0; r < NR; ++r) {
+                        if (x.bad >> h & 1) s[r][h][j] = __builtin_nanf("");  // keys of a page outside the cache
+                        if (key >= kmax[r]) s[r][h][j] = kNegInf;
+                    }
                     // what lies there is not a number anybody wrote
                     if (key >= t.lk || (x.bad >> h & 1)) {
                         x.v[4 * h + j] = {};
@@ -503,119 +613,97 @@ __device__ __forceinline__ void few_item(const AttnCacheArgs& a, const RowTile& 
     }
 }
 
+template <int D>
+constexpr int kFewLds = SW * 16 * (kPitch<D> + 2);  // floats
+
+// Workgroup `block` of `blocks` walks over the items.
 template <class T, class C, int D, int NR>
-__global__ __launch_bounds__(SW * 64, NR == 1 ? 3 : 2) void attn_cache_few_kernel(AttnCacheArgs a, int lo, int hi) {
-    __shared__ __attribute__((aligned(16))) float lds[SW * 16 * (kPitch<D> + 2)];
-    const Sequence first = load_sequence(a, lo + (threadIdx.x & 63), hi);
-    const int per = range_tiles(a, first, lo, hi, 16 * NR);
-    for (int item = blockIdx.x;; item += gridDim.x) {
-        const RowTile t = find_tile(a, first, lo, hi, item / a.c.hk, 16 * NR, per);
+__device__ __forceinline__ void few_items(const AttnCacheArgs& a, const Part& part, int block, int blocks, float* lds) {
+    const Sequence first = load_sequence(a, part.lo + (threadIdx.x & 63), part.hi);
+    const int per = range_length(a, first, part);
+    for (int item = block;; item += blocks) {
+        const RowTile t = find_tile(a, first, part, item / a.c.hk, per);
         if (!t.found) return;
         few_item<T, C, D, NR>(a, t, item % a.c.hk, lds);
     }
 }
 
+template <class T, class C, int D, int NR>
+__global__ __launch_bounds__(SW * 64, NR == 1 ? 3 : 2) void attn_cache_few_kernel(AttnCacheArgs a, Part part) {
+    __shared__ __attribute__((aligned(16))) float lds[kFewLds<D>];
+    few_items<T, C, D, NR>(a, part, blockIdx.x, gridDim.x, lds);
+}
+
 // ---- many rows: 128 of them, four waves over one ring -----------------------
-// The work of a wave and its phases are attention_varlen.hip's (Many, its 64-key tiles
-// and the ring of two slots that hold V of tile p - 1 beside K of tile p); what differs is
-// how a tile gets there: codes come to registers, a step ahead of their use, and go to
-// LDS as 16-bit values, once for the four waves. Per step and thread that is 64 codes,
-// between the exponentials of the softmax. Page numbers are loaded a further step ahead.
-// Tiles too few for the CUs have their keys cut into ranges, a workgroup each.
-constexpr int kManyGrid = 512;  // workgroups that run at once, two a CU
+// Codes decoded once: attn_cache_decode_kernel writes a part's keys to scratch as 16-bit
+// rows, head by head, and the work on them is attention_varlen.hip's (its tiles, waves
+// and phases, of which attention_tiles.h holds what both share). Decoding on the way into
+// LDS instead, 64 codes a thread and step, took no pass of its own, but each tile of rows
+// does it anew: with seven tiles a head (128 tokens of 28 / 4 heads) over 16000 int8 keys
+// the loop took 52 us, of fifty (1024 over 8192 e4m3 keys and 333) 169.
+//
+// Where the CUs want more than whole tiles (range_length), the tiles' steps are dealt out
+// in equal shares and a tile's parts joined.
 
-// A tile's key ranges of `per` 64-key tiles each, of `n` in all.
-struct TileRanges {
-    int n, per, count;
-};
-__device__ __forceinline__ TileRanges many_ranges(const AttnCacheArgs& a, const RowTile& t, int row0) {
-    const int rows = t.lq * a.group;
-    TileRanges r;
-    r.n = (visible(a, t, (min(row0 + MR, rows) - 1) / a.group) + MK - 1) / MK;
-    const int most = max(t.b < a.batch ? a.own_splits : a.prefix_splits, 1);
-    r.per = most == 1 ? max(r.n, 1) : max((r.n + most - 1) / most, 4);
-    r.count = max((r.n + r.per - 1) / r.per, 1);
-    return r;
+// Rows of a sequence's slot in scratch: whole 64-key tiles of what its table holds.
+__device__ __forceinline__ int64_t slot_rows(const AttnCacheArgs& a, int b) {
+    const int64_t keys = static_cast<int64_t>(b < a.batch ? a.max_blocks : a.prefix_blocks) << a.c.page_shift;
+    return (keys + MK - 1) / MK * MK;
 }
 
-// V tiles in LDS have their 16-byte chunks also swapped in pairs by bit 2 of the row: the
-// stores of 16 lanes then take 256 bytes of banks (they hold chunks of one parity of
-// two rows, or four, that differ in that bit; with swz_v alone every second one waits).
-template <int D>
-__device__ __forceinline__ int swz_vc(int row, int c) {
-    return swz_v<D>(row, c) ^ ((row >> 2) & 1);
-}
-// (v_lane_off with these chunks)
-template <int D>
-__device__ __forceinline__ int vc_lane_off(int dt) {
-    const int lane = threadIdx.x & 63, i = lane & 15;
-    const int row = 4 * (lane >> 5) + (i >> 2);
-    const int chunk = 4 * dt + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
-    return row * (2 * D) + swz_vc<D>(row, chunk) * 16 + (i & 1) * 8;
-}
-
-// The codes of K or V tiles on their way to LDS: a thread holds 16 codes of N rows. A
-// wave's rows of one load lie in one 16-key group, so its page and the address of the
-// load are uniform.
-template <class T, class C, int D, bool VTILE>
-struct CodeStream {
-    static constexpr int N = D / 64, TPR = D / 16, RPW = 64 / TPR;  // loads of a thread a tile; threads a row, rows a load
-    int row, off;  // a lane's row and offset behind the load's first row
-    int dst[2];    // and its two chunks' places in LDS
-    u32x4 raw[N];
-    uint32_t e[N];
-    __device__ __forceinline__ void init(int wave) {
-        const int lane = threadIdx.x & 63, q = lane / TPR, c = lane % TPR;
-        if constexpr (!VTILE) row = q;
-        else if constexpr (D == 128) row = (q & 1) * 4 + (q >> 1);                             // rows r, r + 4 side by side
-        else row = (q & 1) + (q >> 1 & 1) * 4 + (q >> 2 & 1) * 2 + (q >> 3) * 8;  // r, r + 1, r + 4, r + 5
-        off = row * D + 16 * c;
-        const int at = RPW * wave + row;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) dst[j] = at * (2 * D) + (VTILE ? swz_vc<D>(at, 2 * c + j) : swz_k<D>(at, 2 * c + j)) * 16;
-    }
-    // load i of the tile: the wave's rows begin at these addresses
-    __device__ __forceinline__ void load(const uint8_t* codes, const uint8_t* exps, int i) {
-        raw[i] = Buffer(codes, RPW * D).load<u32x4>(off);
-        e[i] = Buffer(exps, RPW).load<uint8_t>(row);
-    }
-    // codes 8 j .. 8 j + 7 of load i as 16-bit values to their place in the tile. `left`: rows of
-    // the load that hold keys in use; V of the others is zeros, whatever lies there.
-    __device__ __forceinline__ void store(int i, int j, uint8_t* tile, int left) {
-        float scale = exp_scale(e[i]);
-        uint32_t x = raw[i][2 * j], y = raw[i][2 * j + 1];
-        if (VTILE && left < RPW) {
-            const bool none = row >= left;
-            scale = none ? 0.0f : scale;
-            x = none ? 0u : x;
-            y = none ? 0u : y;
-        }
-        const uint2 p = decode_pairs<C, T::kBf>(x, scale), q = decode_pairs<C, T::kBf>(y, scale);
-        *reinterpret_cast<u32x4*>(tile + dst[j] + 64 / N * i * (2 * D)) = (u32x4){p.x, p.y, q.x, q.y};
-    }
-};
-
+// One tile of 64 keys of one head a workgroup. Keys of a page outside the cache are NaN.
 template <class T, class C, int D>
-__global__ __launch_bounds__(MW * 64, 2) void attn_cache_many_kernel(AttnCacheArgs a, int lo, int hi, int tiles, int splits) {
+__global__ __launch_bounds__(256) void attn_cache_decode_kernel(AttnCacheArgs a, Part part, int tiles) {
+    const int tile = static_cast<int>(blockIdx.x) % tiles, at = static_cast<int>(blockIdx.x) / tiles;
+    const int head = at % part.heads, slot = at / part.heads, b = part.lo + slot;
+    const Sequence s = load_sequence(a, b, part.hi);
+    if (s.lq == 0 || tile * MK >= s.lk) return;
+    const int* table = b < a.batch ? a.table + static_cast<int64_t>(b) * a.max_blocks : a.prefix_table;
+    const int last = ((s.lk + (1 << a.c.page_shift) - 1) >> a.c.page_shift) - 1;
+    constexpr int TPR = D / 16, N = MK * TPR / 256;
+    int page[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        page[i] = table[min((tile * MK + static_cast<int>(threadIdx.x) / TPR + 256 / TPR * i) >> a.c.page_shift, last)];
+    const int64_t base = (static_cast<int64_t>(slot) * part.heads + head) * slot_rows(a, b) * D;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int key = tile * MK + static_cast<int>(threadIdx.x) / TPR + 256 / TPR * i, c = 16 * (threadIdx.x % TPR);
+        const bool in = page[i] >= 0 && page[i] < a.c.n_pages;
+        const int64_t row = ((static_cast<int64_t>(in ? page[i] : 0) * a.c.hk + part.h0 + head) << a.c.page_shift) +
+                            (key & ((1 << a.c.page_shift) - 1));
+        const u32x4 kw = *reinterpret_cast<const u32x4*>(a.c.k + row * D + c), vw = *reinterpret_cast<const u32x4*>(a.c.v + row * D + c);
+        const float ks = exp_scale(a.c.ke[row]), vs = exp_scale(a.c.ve[row]);
+        u32x4 r[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint2 k = decode_pairs<C, T::kBf>(kw[j], ks), v = decode_pairs<C, T::kBf>(vw[j], vs);
+            r[j / 2][j % 2 * 2] = in ? k.x : T::kNans, r[j / 2][j % 2 * 2 + 1] = in ? k.y : T::kNans;
+            r[2 + j / 2][j % 2 * 2] = in ? v.x : 0u, r[2 + j / 2][j % 2 * 2 + 1] = in ? v.y : 0u;
+        }
+        uint16_t* ko = a.dense_k + base + static_cast<int64_t>(key) * D + c;
+        uint16_t* vo = a.dense_v + base + static_cast<int64_t>(key) * D + c;
+        *reinterpret_cast<u32x4*>(ko) = r[0];
+        *reinterpret_cast<u32x4*>(ko + 8) = r[1];
+        *reinterpret_cast<u32x4*>(vo) = r[2];
+        *reinterpret_cast<u32x4*>(vo + 8) = r[3];
+    }
+}
+
+template <int D>
+constexpr int kManyLds = MSLOT * 2 * MK * D * 2;  // bytes
+
+// Key tiles [tile0, tile0 + n) of a row tile.
+template <class T, int D>
+__device__ __forceinline__ void many_item(const AttnCacheArgs& a, const Part& part, const RowTile& t, int hk, int tile0, int n,
+                                          uint8_t* lds) {
     using W = Many<T, D>;
-    using KStream = CodeStream<T, C, D, false>;
-    using VStream = CodeStream<T, C, D, true>;
-    constexpr int PAIR = 2 * W::TB, N = KStream::N, RPW = KStream::RPW;
-    static_assert(W::PER == 4 * N, "stores of a thread a pair");
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[MSLOT * PAIR];
+    constexpr int PAIR = 2 * W::TB;
+    static_assert(MSLOT * PAIR == kManyLds<D>, "LDS of the kernels");
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l32 = lane & 31, half = lane >> 5;
-    // The row tiles that share a range of a head's keys side by side on one XCD.
-    const int logical = xcd_remap(blockIdx.x, gridDim.x);
-    const int split = logical / tiles % splits, hk = logical / (tiles * splits);
-    const RowTile t = find_tile(a, load_sequence(a, lo + lane, hi), lo, hi, logical % tiles, MR, 0);
-    if (!t.found) return;
-    const TileRanges ranges = many_ranges(a, t, t.row0);
-    if (split >= ranges.count) return;
-    const int tile0 = split * ranges.per, n = min(ranges.per, ranges.n - tile0);
-
     const int rows = t.lq * a.group;
     const int row = min(t.row0 + 32 * wave + l32, rows - 1);
     const bool valid = t.row0 + 32 * wave + l32 < rows;
@@ -631,134 +719,62 @@ __global__ __launch_bounds__(MW * 64, 2) void attn_cache_many_kernel(AttnCacheAr
     w.m = kNegInf;
     w.sum = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
     if (n > 0) {
-        // Where the keys of 16 tiles lie: lane l holds the first cache row of 16-key group l behind
-        // tile `base`, `bad` a bit for each group whose page is outside the cache (row 0 stands for
-        // it). kTurn tiles further on those of the 16 tiles from there take their place, whose
-        // page numbers are loaded by then: a step reaches three tiles ahead. (Rows worked out anew
-        // from the page number for every load took a fifth of the loop: the wave issues nothing
-        // else meanwhile.)
-        constexpr int kTurn = 12;
-        const int* table = own ? a.table + static_cast<int64_t>(t.b) * a.max_blocks : a.prefix_table;
-        const int last = ((t.lk + (1 << a.c.page_shift) - 1) >> a.c.page_shift) - 1;  // page of the last key in use
-        const auto pages_from = [&](int tile) { return table[min((4 * tile + lane) >> (a.c.page_shift - 4), last)]; };
-        int ids_next = pages_from(tile0), base = tile0, row_lo = 0, row_hi = 0;
-        uint64_t bad = 0;
-        const auto turn = [&](int tile) {
-            const bool in = ids_next >= 0 && ids_next < a.c.n_pages;
-            const int64_t first = ((static_cast<int64_t>(in ? ids_next : 0) * a.c.hk + hk) << a.c.page_shift) +
-                                  (16 * (4 * tile + lane) & ((1 << a.c.page_shift) - 1));
-            row_lo = static_cast<int>(first);
-            row_hi = static_cast<int>(first >> 32);
-            bad = __ballot(!in);
-            base = tile;
-            ids_next = pages_from(tile + kTurn);
-        };
-        turn(tile0);
-        KStream ks;
-        VStream vs;
-        ks.init(wave);
-        vs.init(wave);
-        // the wave's rows of load i: group RPW * wave / 16 of four (D 64) or of two of them
-        const int sub = RPW * wave / 16, in_group = RPW * wave % 16;
-        const auto row_of = [&](int i, int tile) __attribute__((always_inline)) {
-            const int g = 4 * (tile - base) + 4 / N * i + sub;
-            return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(row_hi, g))) << 32 |
-                                        static_cast<uint32_t>(__builtin_amdgcn_readlane(row_lo, g)));
-        };
-        const uint8_t *kc = a.c.k + in_group * D, *kx = a.c.ke + in_group, *vc = a.c.v + in_group * D, *vx = a.c.ve + in_group;
-        const auto load_k = [&](int i, int tile) __attribute__((always_inline)) {
-            const int64_t at = row_of(i, tile);
-            ks.load(kc + at * D, kx + at, i);
-        };
-        const auto load_v = [&](int i, int tile) __attribute__((always_inline)) {
-            const int64_t at = row_of(i, tile);
-            vs.load(vc + at * D, vx + at, i);
-        };
-        // rows of load i that hold keys in use: none in a page outside the cache
-        const auto left_of = [&](int i, int tile) __attribute__((always_inline)) {
-            return bad >> (4 * (tile - base) + 4 / N * i + sub) & 1 ? 0 : t.lk - (tile * MK + 64 / N * i + RPW * wave);
-        };
-#pragma unroll
-        for (int i = 0; i < N; ++i) load_k(i, tile0);
+        const int64_t room = slot_rows(a, t.b);
+        const int64_t base = (static_cast<int64_t>(t.b - part.lo) * part.heads + hk - part.h0) * room * D;
+        TileStream<D, false> ks;
+        TileStream<D, true> vs;
+        ks.init(a.dense_k + base, D, t.lk, tile0, 1, wave);
+        ks.issue(lds + W::TB, wave);
         {
             const uint16_t* qp = a.q + (static_cast<int64_t>(t.q0) + token) * a.q_t + head * a.q_h + 8 * half;
 #pragma unroll
             for (int i = 0; i < W::KS; ++i) w.qf[i] = *reinterpret_cast<const typename T::frag*>(qp + 16 * i);
         }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < N; ++i) load_v(i, tile0);
-#pragma unroll
-        for (int d = 0; d < W::DT; ++d) w.voff[d] = vc_lane_off<D>(d);
+        for (int d = 0; d < W::DT; ++d) w.voff[d] = v_lane_off<D>(d);
 #pragma unroll
         for (int c = 0; c < W::KS; ++c) w.koff[c] = l32 * (2 * D) + swz_k<D>(l32, 2 * c + half) * 16;
 #pragma unroll
         for (int r = 0; r < 16 * W::KB; ++r) w.s[r >> 4][r & 15] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) ks.store(i, j, lds + W::TB, 0);
-#pragma unroll
-        for (int i = 0; i < N; ++i) load_k(i, tile0 + 1);
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) vs.store(i, j, lds + PAIR, left_of(i, tile0));
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) ks.store(i, j, lds + PAIR + W::TB, 0);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {  // pair 2: V of tile 1, K of tile 2
-            load_v(i, tile0 + 1);
-            load_k(i, tile0 + 2);
-        }
-        wait_lgkmcnt0();
+        vs.init(a.dense_v + base, D, t.lk, tile0, 1, wave);
+        __builtin_amdgcn_sched_barrier(0);
+        vs.issue(lds + PAIR, wave);
+        ks.issue(lds + PAIR + W::TB, wave);
+        wait_vmcnt<W::PER>();
         phase_barrier();
         w.template first_scores<W::NPV>(lds);
-        for (int p = 0; p < n; ++p) {
-            const uint8_t* src = lds + ((p + 1) % MSLOT) * PAIR;
-            uint8_t* dst = lds + (p % MSLOT) * PAIR;
-            const int tile = tile0 + p;
-            if (tile == base + kTurn) turn(tile);
-            wait_lgkmcnt0();  // pair p + 1 is in LDS, this wave's part of it
+        // V(p) and M(p + 1): behind the barrier every wave has done M(p), whose slot takes pair p + 2
+        // during V(p), and pair p + 1, sent during V(p - 1), has landed
+        const auto step = [&](int p, const uint8_t* __restrict src, uint8_t* __restrict dst) __attribute__((always_inline)) {
+            wait_vmcnt<0>();
             phase_barrier();
             w.template read_group<0>(src, w.buf[0]);
             __builtin_amdgcn_sched_barrier(0);
-            if (const int odd = static_cast<int>(bad >> 4 * (tile - base)) & 15) {  // keys of a page outside the cache are not seen
-#pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    if (odd >> g & 1)
-#pragma unroll
-                        for (int r = 0; r < 8; ++r) w.s[g / 2][8 * (g % 2) + r] = kNegInf;
-            }
-            w.softmax(tile * MK, kfull, kmax, a.scale_log2, [&](int i) {
-                // Two stores of each load, then the next one into its registers (behind the last
-                // tile too: with loads under a condition the compiler waits for all of them).
-                const int l = i % (2 * N) / 2, j = i % 2;
-                if (i < 2 * N) {
-                    vs.store(l, j, dst, left_of(l, tile + 1));
-                    if (j == 1) load_v(l, tile + 2);
-                } else {
-                    ks.store(l, j, dst + W::TB, 0);
-                    if (j == 1) load_k(l, tile + 3);
-                }
+            w.softmax((tile0 + p) * MK, kfull, kmax, a.scale_log2, [&](int i) {
+                if (i < W::PER / 2)
+                    vs.issue_one(i, dst, wave);
+                else
+                    ks.issue_one(i - W::PER / 2, dst + W::TB, wave);
             });
 #pragma unroll
             for (int i = 0; i < 8 * W::KB; ++i) asm volatile("" : "+v"(w.pk[i]));  // P is made in this phase
             __builtin_amdgcn_sched_barrier(0);
             __builtin_amdgcn_s_setprio(1);
-            bool bad = false;
-            w.template m_groups<0, false>(src, bad);
+            bool none = false;
+            w.template m_groups<0, false>(src, none);
             __builtin_amdgcn_sched_barrier(0);
             __builtin_amdgcn_s_setprio(0);
-        }
+        };
+        for (int p = 0; p < n; ++p) step(p, lds + ((p + 1) % MSLOT) * PAIR, lds + (p % MSLOT) * PAIR);
+        wait_vmcnt<0>();  // the loads past the last tile no longer write the ring
     }
     const float tot = half_sum(w.sum[0]);
     constexpr int CHUNKS = D / 8;
-    if (ranges.count > 1 || a.prefix_splits > 0) {
+    if (t.splits > 1 || a.prefix_splits > 0) {
         if (!valid) return;
         const int64_t at = ((static_cast<int64_t>(t.q0) + token) * a.hq + head) * (a.own_splits + a.prefix_splits) +
-                           (own ? 0 : a.own_splits) + split;
+                           (own ? 0 : a.own_splits) + t.split;
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c)
             *reinterpret_cast<v4f*>(a.part_o + at * D + 32 * (c / 4) + 8 * (c % 4) + 4 * half) =
@@ -792,28 +808,67 @@ __global__ __launch_bounds__(MW * 64, 2) void attn_cache_many_kernel(AttnCacheAr
         }
 }
 
+// Workgroup `block`: a tile, or its share of the steps.
+template <class T, int D>
+__device__ __forceinline__ void many_items(const AttnCacheArgs& a, const Part& part, int block, uint8_t* lds) {
+    const Sequence first = load_sequence(a, part.lo + (threadIdx.x & 63), part.hi);
+    const int share = range_length(a, first, part);
+    const int total = share == 0 ? count_tiles(a, first, part) * part.heads : count_steps(a, first, part, part.hi);
+    const int blocks = share == 0 ? total : (total + share - 1) / share;
+    if (block >= blocks) return;
+    // Neighbours, which read the same keys, on one XCD; whole causal tiles, longest first, over
+    // all of them.
+    const bool spread = share == 0 && a.causal && part.lo < a.batch;
+    const int me = spread ? block : xcd_remap(block, blocks);
+    const int end = share == 0 ? 1 : min((me + 1) * share, total);
+    for (int x = share == 0 ? 0 : me * share; x < end;) {
+        int hk = 0, step = 0;
+        RowTile t;
+        if (share == 0) {
+            const int tiles = total / part.heads;
+            hk = part.h0 + (spread ? me % part.heads : me / tiles);
+            t = find_tile(a, first, part, spread ? me / part.heads : me % tiles, 0);
+        } else {
+            t = find_step(a, first, part, x, share, me, hk, step);
+        }
+        if (!t.found) return;
+        const int all = (t.lk + MK - 1) / MK;
+        const int seen = (visible(a, t, (min(t.row0 + MR, t.lq * a.group) - 1) / a.group) + MK - 1) / MK;
+        const int n = share == 0 ? all : min(all - step, end - x);
+        many_item<T, D>(a, part, t, hk, step, min(n, seen - step), lds);
+        if (share == 0) return;
+        x += n;
+        if (x < end) __syncthreads();  // (the next tile's keys take the place of this one's)
+    }
+}
+
+template <class T, int D>
+__global__ __launch_bounds__(MW * 64, 2) void attn_cache_many_kernel(AttnCacheArgs a, Part part) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[kManyLds<D>];
+    many_items<T, D>(a, part, blockIdx.x, lds);
+}
+
+// The prefix in tiles of MR rows and, by the workgroups from `many` on, the sequences' own
+// keys in tiles of few: in one launch these run in what the prefix leaves idle.
+template <class T, class C, int D, int NR>
+__global__ __launch_bounds__(MW * 64, 2) void attn_cache_mixed_kernel(AttnCacheArgs a, Part prefix, Part own, int many) {
+    constexpr int kBytes = kManyLds<D> > kFewLds<D> * 4 ? kManyLds<D> : kFewLds<D> * 4;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[kBytes];
+    if (static_cast<int>(blockIdx.x) < many)
+        many_items<T, D>(a, prefix, blockIdx.x, lds);
+    else
+        few_items<T, C, D, NR>(a, own, static_cast<int>(blockIdx.x) - many, static_cast<int>(gridDim.x) - many,
+                               reinterpret_cast<float*>(lds));
+}
+
 // Partial results of a row, added in order: 16 threads a row, tiles of 16 rows of one
 // sequence and kv head. Eight parts' loads go out together.
 template <class T, int D>
-__device__ __forceinline__ void join_item(const AttnCacheArgs& a, const AttnCachePlan& plan, const RowTile& t, int hk, int per,
-                                          bool together) {
+__device__ __forceinline__ void join_item(const AttnCacheArgs& a, const RowTile& t, int hk, int own, int shared) {
     constexpr int E = D / 16, U = 8;
     typedef float v2f __attribute__((ext_vector_type(2)));
-    const int own = plan.own_rows == MR ? many_ranges(a, t, t.row0 / MR * MR).count : key_ranges(t.lk, per);
-    int shared = 0;
-    if (a.prefix_splits > 0) {
-        const Sequence p = load_sequence(a, a.batch, a.batch + 1);
-        if (plan.prefix_rows == MR) {
-            RowTile pt = t;
-            pt.b = a.batch, pt.q0 = p.q0, pt.lq = p.lq, pt.lk = p.lk;
-            shared = many_ranges(a, pt, 0).count;
-        } else {
-            shared = key_ranges(p.lk, together ? per : range_tiles(a, load_sequence(a, a.batch + (threadIdx.x & 63), a.batch + 1), a.batch,
-                                                                    a.batch + 1, plan.prefix_rows));
-        }
-    }
     const int row = t.row0 + (threadIdx.x >> 4), c0 = (threadIdx.x & 15) * E;
-    if (own + shared == 1 || row >= t.lq * a.group) return;
+    if (row >= t.lq * a.group) return;
     const int64_t token = static_cast<int64_t>(t.q0) + row / a.group;
     const int head = hk * a.group + row % a.group;
     const int64_t at = (token * a.hq + head) * (a.own_splits + a.prefix_splits);
@@ -854,17 +909,42 @@ __device__ __forceinline__ void join_item(const AttnCacheArgs& a, const AttnCach
 }
 
 template <class T, int D>
-__global__ __launch_bounds__(256) void attn_cache_join_kernel(AttnCacheArgs a, AttnCachePlan plan) {
+__global__ __launch_bounds__(256) void attn_cache_join_kernel(AttnCacheArgs a, Part own_part, Part prefix_part) {
     const int lane = threadIdx.x & 63;
-    const bool together = plan.prefix_splits > 0 && plan.prefix_rows == plan.own_rows && plan.own_rows != MR;
-    const int hi = a.batch + (together ? 1 : 0);
-    const Sequence first = load_sequence(a, lane, hi);
-    const int per = plan.own_rows == MR ? 0 : range_tiles(a, first, 0, hi, plan.own_rows);
+    const Sequence first = load_sequence(a, lane, own_part.hi);
+    const int per = range_length(a, first, own_part);
+    Sequence p = {0, 0, 0};
+    int prefix_per = 0;
+    if (a.prefix_splits > 0) {
+        p = load_sequence(a, a.batch, a.batch + 1);
+        // (one launch of both has one length of ranges)
+        prefix_per = own_part.hi > a.batch ? per : range_length(a, load_sequence(a, a.batch + lane, prefix_part.hi), prefix_part);
+    }
+    const Part rows = {0, a.batch, 16, 0, a.c.hk};
     for (int item = blockIdx.x;; item += gridDim.x) {
         const int hk = item % a.c.hk;
-        const RowTile t = find_tile(a, first, 0, a.batch, item / a.c.hk, 16, 0);
+        const RowTile t = find_tile(a, first, rows, item / a.c.hk, 0);
         if (!t.found) return;
-        join_item<T, D>(a, plan, t, hk, per, together);
+        const int n = steps_of(own_part, t.lk);
+        int own = 1, shared = 0;
+        if (own_part.rows != MR) {
+            own = key_ranges(n, per, max(a.own_splits, 1));
+        } else if (per != 0) {
+            const int tiles = row_tiles(a, t.lq, MR), before = count_steps(a, first, own_part, t.b);
+            own = tile_shares(before + (hk * tiles + t.row0 / MR) * n, n, per).count;
+        }
+        if (a.prefix_splits == 0) {
+            if (own == 1) continue;  // complete already
+        } else if (prefix_part.rows != MR) {
+            shared = key_ranges(steps_of(prefix_part, p.lk), prefix_per, a.prefix_splits);
+        } else {
+            // a row's tile of the prefix, whose rows are those of all sequences
+            const int np = steps_of(prefix_part, p.lk), tiles = row_tiles(a, p.lq, MR);
+            const int row = min(t.row0 + static_cast<int>(threadIdx.x >> 4), t.lq * a.group - 1);
+            const int tile = static_cast<int>(((static_cast<int64_t>(t.q0) - p.q0) * a.group + row) / MR);
+            shared = prefix_per == 0 ? 1 : tile_shares((hk * tiles + tile) * np, np, prefix_per).count;
+        }
+        join_item<T, D>(a, t, hk, own, shared);
     }
 }
 
@@ -878,22 +958,7 @@ int64_t tile_bound(int total_q, int batch, int group, int rows) {
 
 constexpr int kMostSplits = 32;
 constexpr int kMostBlocks = 1 << 22;  // of a launch (a grid has less than 2^32 threads)
-
-// Key ranges of each of `tiles` tiles of 128 rows over `steps` key tiles, so that time is
-// least: rounds of workgroups times a range's steps, each with the start of a range, and
-// what the ranges' float results cost. Lengths are on the device: the table's room stands
-// for them here, which decides the time, not the result.
-static int many_splits(int64_t tiles, int64_t steps) {
-    int best = 1;
-    double least = 0.0;
-    for (int s = 1; s <= kMostSplits && (s == 1 || 4 * s <= steps); ++s) {
-        const int64_t items = tiles * s;
-        const double pace = items <= kManyGrid / 2 ? 1.5 : 1.7, rounds = static_cast<double>((items + kManyGrid - 1) / kManyGrid);
-        const double t = rounds * pace * (static_cast<double>(steps) / s + 3.0) + (s > 1 ? 4.0 + 0.026 * static_cast<double>(items) : 0.0);
-        if (s == 1 || t < least) best = s, least = t;
-    }
-    return best;
-}
+constexpr int64_t kMostDense = int64_t{1} << 30;  // bytes of 16-bit rows at a time, of one head of a sequence at least
 
 AttnCachePlan attn_cache_plan(int total_q, int batch, int hq, int hk, int D, int64_t own_keys, int64_t prefix_keys) {
     AttnCachePlan p{};
@@ -905,52 +970,129 @@ AttnCachePlan attn_cache_plan(int total_q, int batch, int hq, int hk, int D, int
     };
     p.own_rows = tile_rows((static_cast<int64_t>(total_q) * group + batch - 1) / batch, batch);
     p.prefix_rows = tile_rows(static_cast<int64_t>(total_q) * group, 1);
-    // most ranges: at least eight key tiles each, and 2^13 row tiles times ranges; of 128
-    // rows as many as run at once
-    const auto splits = [&](int64_t keys, int rows, int seqs) {
+    // Most ranges of a sequence: eight steps each at least, and 2^13 row tiles times ranges; of
+    // MR rows the shares that may meet in a tile, up to 1.5 tiles a workgroup.
+    const auto splits = [&](int64_t keys, int rows, int seqs) -> int {
         const int64_t tiles = std::max<int64_t>(tile_bound(total_q, seqs, group, rows) * hk, 1);
-        if (rows == MR) return many_splits(tiles, (keys + MK - 1) / MK);
+        if (rows == MR) {
+            const int64_t steps = (keys + MK - 1) / MK;
+            const bool pays = shares_pay(static_cast<float>(tiles * steps) / kManyGrid, static_cast<float>(tiles),
+                                         static_cast<float>((tiles + kManyGrid - 1) / kManyGrid * steps));
+            return tiles > kManyGrid * 3 / 2 || !pays
+                       ? 1
+                       : static_cast<int>(std::min<int64_t>({kManyGrid / tiles + 2, (steps + 3) / 4 + 1, kMostSplits}));
+        }
         const int64_t most = std::min<int64_t>((keys + 8 * SK - 1) / (8 * SK), 8192 / tiles);
         return static_cast<int>(std::max<int64_t>(std::min<int64_t>(most, kMostSplits), 1));
     };
     p.own_splits = splits(own_keys, p.own_rows, batch);
     p.prefix_splits = prefix_keys > 0 ? splits(prefix_keys, p.prefix_rows, 1) : 0;
+    // The 16-bit rows of a part in tiles of MR: as many heads, or sequences, at a time as
+    // kMostDense holds. Where that is not all there are no shares.
+    const auto dense = [&](int64_t keys, int rows, int seqs, int& slots, int& heads, int& splits) {
+        slots = seqs, heads = hk;
+        if (rows != MR || keys == 0) return;
+        const int64_t slot = (keys + MK - 1) / MK * MK, each = slot * D * 4, most = std::max<int64_t>(kMostDense / each, 1);
+        if (most < static_cast<int64_t>(seqs) * hk) {
+            splits = std::min(splits, 1);
+            heads = static_cast<int>(std::clamp<int64_t>(most / seqs, 1, hk));
+            slots = static_cast<int>(std::min<int64_t>(most / heads, seqs));
+        }
+        p.dense_rows = std::max(p.dense_rows, slot * slots * heads);
+    };
+    int one = 1;
+    dense(own_keys, p.own_rows, batch, p.own_slots, p.own_heads, p.own_splits);
+    dense(prefix_keys, p.prefix_rows, 1, one, p.prefix_heads, p.prefix_splits);
     if (p.own_splits > 1 || p.prefix_splits > 0)
         p.part_rows = static_cast<int64_t>(total_q) * hq * (p.own_splits + p.prefix_splits);
     return p;
 }
 
-// The sequences [lo, hi) in tiles of `rows` rows.
+AttnCacheScratch attn_cache_scratch(const AttnCachePlan& plan, int D) {
+    const auto align = [](int64_t n) { return (n + 255) / 256 * 256; };
+    return {align(plan.part_rows * D * 4), align(plan.part_rows * 8), align(plan.dense_rows * D * 2)};
+}
+
+// The codes of a part as 16-bit rows in scratch.
 template <class T, class C, int D>
-static hipError_t launch_part(const AttnCacheArgs& a, int rows, int lo, int hi, hipStream_t stream) {
-    const int64_t own = lo < a.batch ? tile_bound(a.total_q, a.batch, a.group, rows) : 0;
-    const int64_t shared = hi > a.batch ? tile_bound(a.total_q, 1, a.group, rows) : 0;
-    if (rows == MR) {
-        const int splits = lo < a.batch ? a.own_splits : a.prefix_splits;
-        const int tiles = static_cast<int>(own + shared);
-        hipLaunchKernelGGL((attn_cache_many_kernel<T, C, D>), dim3(static_cast<unsigned>(tiles) * splits * a.c.hk),
-                           dim3(MW * 64), 0, stream, a, lo, hi, tiles, splits);
-        return hipGetLastError();
-    }
-    const int64_t items = (own * a.own_splits + shared * a.prefix_splits) * a.c.hk;
-    const dim3 grid(static_cast<unsigned>(items < kFewGrid ? items : kFewGrid));
-    if (rows == 16)
-        hipLaunchKernelGGL((attn_cache_few_kernel<T, C, D, 1>), grid, dim3(SW * 64), 0, stream, a, lo, hi);
-    else
-        hipLaunchKernelGGL((attn_cache_few_kernel<T, C, D, 2>), grid, dim3(SW * 64), 0, stream, a, lo, hi);
+static hipError_t launch_decode(const AttnCacheArgs& a, const Part& part, hipStream_t stream) {
+    const int64_t keys = static_cast<int64_t>(part.lo < a.batch ? a.max_blocks : a.prefix_blocks) << a.c.page_shift;
+    const int64_t tiles = (keys + MK - 1) / MK, blocks = tiles * part.heads * (part.hi - part.lo);
+    if (blocks == 0) return hipSuccess;
+    hipLaunchKernelGGL((attn_cache_decode_kernel<T, C, D>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, a, part,
+                       static_cast<int>(tiles));
     return hipGetLastError();
 }
 
 template <class T, class C, int D>
 static hipError_t launch_attn(const AttnCacheArgs& a, const AttnCachePlan& plan, hipStream_t stream) {
     const bool prefix = plan.prefix_splits > 0;
+    // few rows of both: one launch over them all
     const bool together = prefix && plan.prefix_rows == plan.own_rows && plan.own_rows != MR;
-    hipError_t e = launch_part<T, C, D>(a, plan.own_rows, 0, a.batch + (together ? 1 : 0), stream);
-    if (e == hipSuccess && prefix && !together)
-        e = launch_part<T, C, D>(a, plan.prefix_rows, a.batch, a.batch + 1, stream);
+    const Part own = {0, a.batch + (together ? 1 : 0), plan.own_rows, 0, a.c.hk};
+    const Part shared = {a.batch, a.batch + 1, plan.prefix_rows, 0, a.c.hk};
+    const dim3 block(MW * 64);
+    static_assert(MW == SW, "one workgroup for both");
+    // workgroups of MR rows: the tiles, or the shares of those that run at once
+    const auto many = [&](int seqs, int heads, int splits) {
+        const int64_t tiles = tile_bound(a.total_q, seqs, a.group, MR) * heads;
+        return static_cast<unsigned>(splits > 1 ? std::max<int64_t>(tiles, kManyGrid) : tiles);
+    };
+    // of few rows: they walk over the items
+    const auto few = [&](bool with_own, bool with_prefix, int rows) {
+        int64_t items = with_own ? tile_bound(a.total_q, a.batch, a.group, rows) * a.own_splits : 0;
+        if (with_prefix) items += tile_bound(a.total_q, 1, a.group, rows) * a.prefix_splits;
+        return static_cast<unsigned>(std::min<int64_t>(items * a.c.hk, few_grid(rows)));
+    };
+    bool own_done = false;
+    hipError_t e = hipSuccess;
+    if (prefix && shared.rows == MR) {
+        for (int h = 0; h < a.c.hk && e == hipSuccess; h += plan.prefix_heads) {
+            Part part = shared;
+            part.h0 = h, part.heads = std::min(plan.prefix_heads, a.c.hk - h);
+            e = launch_decode<T, C, D>(a, part, stream);
+            if (e != hipSuccess) break;
+            const unsigned grid = many(1, part.heads, a.prefix_splits);
+            if (own_done || own.rows == MR) {
+                hipLaunchKernelGGL((attn_cache_many_kernel<T, D>), dim3(grid), block, 0, stream, a, part);
+            } else {
+                const unsigned more = few(true, false, own.rows);
+                if (own.rows == 16)
+                    hipLaunchKernelGGL((attn_cache_mixed_kernel<T, C, D, 1>), dim3(grid + more), block, 0, stream, a, part, own,
+                                       static_cast<int>(grid));
+                else
+                    hipLaunchKernelGGL((attn_cache_mixed_kernel<T, C, D, 2>), dim3(grid + more), block, 0, stream, a, part, own,
+                                       static_cast<int>(grid));
+                own_done = true;
+            }
+            e = hipGetLastError();
+        }
+    } else if (prefix && !together) {  // of 32 rows, where the sequences' own tiles have 16
+        hipLaunchKernelGGL((attn_cache_few_kernel<T, C, D, 2>), dim3(few(false, true, 32)), block, 0, stream, a, shared);
+        e = hipGetLastError();
+    }
+    if (e == hipSuccess && own.rows == MR) {
+        for (int b = 0; b < a.batch; b += plan.own_slots) {
+            for (int h = 0; h < a.c.hk; h += plan.own_heads) {
+                const Part part = {b, std::min(b + plan.own_slots, a.batch), MR, h, std::min(plan.own_heads, a.c.hk - h)};
+                e = launch_decode<T, C, D>(a, part, stream);
+                if (e != hipSuccess) return e;
+                hipLaunchKernelGGL((attn_cache_many_kernel<T, D>), dim3(many(part.hi - part.lo, part.heads, a.own_splits)),
+                                   block, 0, stream, a, part);
+                e = hipGetLastError();
+                if (e != hipSuccess) return e;
+            }
+        }
+    } else if (e == hipSuccess && !own_done) {
+        if (own.rows == 16)
+            hipLaunchKernelGGL((attn_cache_few_kernel<T, C, D, 1>), dim3(few(true, together, 16)), block, 0, stream, a, own);
+        else
+            hipLaunchKernelGGL((attn_cache_few_kernel<T, C, D, 2>), dim3(few(true, together, 32)), block, 0, stream, a, own);
+        e = hipGetLastError();
+    }
     if (e != hipSuccess || plan.part_rows == 0) return e;
     const int64_t tiles = std::min<int64_t>(tile_bound(a.total_q, a.batch, a.group, 16) * a.c.hk, kMostBlocks);
-    hipLaunchKernelGGL((attn_cache_join_kernel<T, D>), dim3(static_cast<unsigned>(tiles)), dim3(256), 0, stream, a, plan);
+    hipLaunchKernelGGL((attn_cache_join_kernel<T, D>), dim3(static_cast<unsigned>(tiles)), dim3(256), 0, stream, a, own, shared);
     return hipGetLastError();
 }
 

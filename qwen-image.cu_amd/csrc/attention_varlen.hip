@@ -570,51 +570,6 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnVarlenArgs a) {
 // of two: 441). A tile now takes a wave 1330 cycles of V, 1290 of M (1104 of
 // them MFMA) and 200 at the barrier, two workgroups' together 2890.
 
-// The K or V tiles of one head in turn: `p` the next tile's first row, `left`
-// the bytes from there to the end of the sequence's last row (not positive
-// behind it). Each tile's descriptor starts at its own row, so offsets stay
-// below a tile's bytes however long the sequence is, and ends with the
-// sequence: rows behind it arrive as zeros.
-template <int D, bool VTILE>
-struct TileStream {
-    const uint8_t* p;
-    int64_t left, step;
-    uint32_t off[MK * D * 2 / 1024 / MW];  // a lane's byte offsets in a tile, one per DMA instruction
-    // every `every`-th tile from tile `first` on
-    __device__ __forceinline__ void init(const uint16_t* base, int64_t stride, int lk, int first, int every, int wave) {
-        p = reinterpret_cast<const uint8_t*>(base + first * MK * stride);
-        step = 2 * MK * stride * every;
-        left = lk > first * MK ? 2 * ((lk - first * MK - 1) * stride + D) : 0;
-        constexpr int RPI = 512 / D, CPR = D / 8;
-        const int lane = threadIdx.x & 63;
-#pragma unroll
-        for (int i = 0; i < MK / RPI / MW; ++i) {
-            const int row = (wave + MW * i) * RPI + lane / CPR;
-            const int c = VTILE ? swz_v<D>(row, lane % CPR) : swz_k<D>(row, lane % CPR);
-            off[i] = static_cast<uint32_t>(row) * static_cast<uint32_t>(stride) * 2u + c * 16;
-        }
-    }
-    static constexpr int N = MK * D * 2 / 1024 / MW;  // DMA instructions of a wave
-    // instruction i of the next tile; the last one moves on
-    __device__ __forceinline__ void issue_one(int i, uint8_t* dst, int wave) {
-#if defined(__HIP_DEVICE_COMPILE__)  // (the host pass rejects the builtin, and with it the kernels that share this)
-        const int64_t n = left < 0 ? 0 : left > 0x7fffffff ? 0x7fffffff : left;
-        const __amdgpu_buffer_rsrc_t r =
-            __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, static_cast<int>(n), kRsrcWord3);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            r, (__attribute__((address_space(3))) void*)(dst + (wave + MW * i) * 1024), 16, off[i], 0, 0, 0);
-        if (i == N - 1) {
-            p += step;
-            left -= step;
-        }
-#endif
-    }
-    __device__ __forceinline__ void issue(uint8_t* dst, int wave) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) issue_one(i, dst, wave);
-    }
-};
-
 // V(p) and M(p + 1) of one wave. Behind the barrier every wave has done M(p),
 // whose slot takes pair p + 2 during V(p), and pair p + 1, sent during V(p - 1),
 // has landed. The slots come as restrict pointers, which tells the compiler that

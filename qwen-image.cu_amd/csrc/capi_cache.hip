@@ -178,11 +178,11 @@ int64_t qimg_attention_cache_scratch_bytes(int total_q, int batch, int n_heads, 
     if (total_q <= 0 || batch <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0 || head_dim <= 0 ||
         page_size <= 0 || max_blocks < 0 || prefix_blocks < 0)
         return 0;
-    const int64_t rows = qimg::attn_cache_plan(total_q, batch, n_heads, n_kv_heads, head_dim,
-                                               static_cast<int64_t>(max_blocks) * page_size,
-                                               static_cast<int64_t>(prefix_blocks) * page_size)
-                             .part_rows;
-    return align256(rows * head_dim * 4) + align256(rows * 8);
+    const qimg::AttnCacheScratch s = qimg::attn_cache_scratch(
+        qimg::attn_cache_plan(total_q, batch, n_heads, n_kv_heads, head_dim, static_cast<int64_t>(max_blocks) * page_size,
+                              static_cast<int64_t>(prefix_blocks) * page_size),
+        head_dim);
+    return s.part_o + s.part_ml + 2 * s.dense;
 }
 
 int qimg_attention_cache(const qimg_attn_cache* args, const qimg_kv_cache* cache, void* scratch, int64_t scratch_bytes,
@@ -230,15 +230,17 @@ int qimg_attention_cache(const qimg_attn_cache* args, const qimg_kv_cache* cache
         p.total_q, p.batch, p.n_heads, cache->n_kv_heads, cache->head_dim,
         static_cast<int64_t>(p.max_blocks) * cache->page_size, static_cast<int64_t>(p.prefix_blocks) * cache->page_size);
     a.own_splits = plan.own_splits, a.prefix_splits = plan.prefix_splits;
-    if (plan.part_rows > 0) {
-        const int64_t bytes_o = align256(plan.part_rows * cache->head_dim * 4);
-        const int64_t need = bytes_o + align256(plan.part_rows * 8);
+    const qimg::AttnCacheScratch parts = qimg::attn_cache_scratch(plan, cache->head_dim);
+    const int64_t need = parts.part_o + parts.part_ml + 2 * parts.dense;
+    if (need > 0) {
         if (!scratch || scratch_bytes < need)
             return qimg::api_fail(QIMG_ERR_SCRATCH, "%s: scratch %lld bytes < required %lld", fn,
                                   static_cast<long long>(scratch_bytes), static_cast<long long>(need));
         QIMG_REQUIRE(aligned16(scratch), "%s: scratch must be 16-byte aligned", fn);
         a.part_o = static_cast<float*>(scratch);
-        a.part_ml = a.part_o + bytes_o / 4;
+        a.part_ml = a.part_o + parts.part_o / 4;
+        a.dense_k = reinterpret_cast<uint16_t*>(a.part_ml + parts.part_ml / 4);
+        a.dense_v = a.dense_k + parts.dense / 2;
     }
     return qimg::api_hip_status(
         qimg::launch_attention_cache(a, plan, p.dtype, cache->dtype, cache->head_dim, static_cast<hipStream_t>(stream)),

@@ -11,7 +11,7 @@
 namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
+[[maybe_unused]] int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 
 // strides of a tensor [T, H, D], in elements
 bool good_strides(int64_t t, int64_t h) {

@@ -468,12 +468,20 @@ struct AttnCacheArgs {
     int own_splits, prefix_splits;  // key ranges, most of a sequence, of the prefix
     float* part_o;   // [total_q, hq, own_splits + prefix_splits, D]
     float* part_ml;  // the same of 2: running maximum, sum
+    uint16_t* dense_k;  // 16-bit rows of the keys that tiles of many rows work on
+    uint16_t* dense_v;
 };
 struct AttnCachePlan {
     int own_rows, prefix_rows;      // rows of a tile, of a sequence's own keys and of the prefix
     int own_splits, prefix_splits;
+    int own_slots, own_heads, prefix_heads;  // sequences and heads whose 16-bit rows are made at a time
     int64_t part_rows;  // rows of part_o: 0 where every sequence's keys are one range and there is no prefix
+    int64_t dense_rows;  // rows of dense_k and of dense_v
 };
+struct AttnCacheScratch {
+    int64_t part_o, part_ml, dense;  // bytes; dense twice
+};
+AttnCacheScratch attn_cache_scratch(const AttnCachePlan& plan, int D);
 AttnCachePlan attn_cache_plan(int total_q, int batch, int hq, int hk, int D, int64_t own_keys, int64_t prefix_keys);
 hipError_t launch_attention_cache(const AttnCacheArgs& a, const AttnCachePlan& plan, int dtype, int codes, int D,
                                   hipStream_t stream);

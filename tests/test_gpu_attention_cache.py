@@ -59,8 +59,8 @@ class Case:
             kw.update(prefix_table=self.prefix_table, prefix_len=_i32(self.prefix))
         return qimg.attention_cache(self.q, self.cache, self.cu_q, self.table, self.k_lens, causal=causal, **kw)
 
-    def oracle(self, causal=True, scale=None, hide=None):
-        """The definition, sum_j p_j |v_j| and max |v| n beside it. hide(b, j): own keys nobody sees."""
+    def oracle(self, causal=True, scale=None):
+        """The definition, sum_j p_j |v_j| and max |v| n beside it."""
         d = self.q.shape[2]
         scale = 1.0 / math.sqrt(d) if scale is None else scale
         out = torch.zeros(self.q.shape, dtype=torch.float64, device=DEV)
@@ -74,8 +74,6 @@ class Case:
             own = torch.arange(nk, device=DEV)
             if causal:
                 vis[:, pn:] = own[None] <= torch.arange(nq, device=DEV)[:, None] + (nk - nq)
-            if hide is not None:
-                vis[:, pn:] &= ~hide(b, own)[None]
             none = ~vis.any(-1)
             for h in range(self.q.shape[1]):
                 kk, vv = self.k[at, h // group], self.v[at, h // group]
@@ -225,21 +223,22 @@ def test_a_token_that_is_not_finite(qimg, codes, lq, lk):
         assert torch.equal(got[keep], base[keep])
 
 
-@pytest.mark.parametrize("lq,lk", [([1, 1], [300, 3000]), ([100, 40], [300, 200])], ids=str)
-def test_pages_outside_the_cache_are_not_seen(qimg, lq, lk):
+@pytest.mark.parametrize("lq,lk", [([1, 1, 1], [300, 3000, 40]), ([100, 40, 3], [300, 200, 90])], ids=str)
+@pytest.mark.parametrize("codes", CODES, ids=str)
+def test_pages_outside_the_cache(qimg, lq, lk, codes):
+    """Nothing outside the cache is read: rows that see a key there are NaN, the others do not change."""
     for bad in (-1, 2 ** 31 - 1, -2 ** 31, None):
-        c = Case(qimg, lq, lk, page=16, seed=10, prefix=64)
-        bad = c.cache.k.shape[0] if bad is None else bad
-        c.table[0, 3] = c.table[1, 5] = c.table[1, 6] = bad
-
-        def hide(b, j):
-            return (j // 16 == 3) if b == 0 else (j // 16 == 5) | (j // 16 == 6)
+        c = Case(qimg, lq, lk, page=16, seed=10, prefix=64, codes=codes)
+        base = c.run(qimg)
+        key = 240  # of sequence 0: its last 60 queries' keys reach there
+        c.table[0, key // 16] = c.cache.k.shape[0] if bad is None else bad
         got = c.run(qimg)
         torch.cuda.synchronize()
-        _check(got, *c.oracle(hide=hide))
-    c = Case(qimg, [1], [32], page=16, seed=11)
-    c.table.fill_(-3)
-    assert bool((c.run(qimg) == 0).all())
+        seen = torch.arange(lq[0], device=DEV) + lk[0] - lq[0] >= key
+        assert bool(got[:lq[0]][seen].isnan().all())
+        assert torch.equal(got[:lq[0]][~seen], base[:lq[0]][~seen]) and torch.equal(got[lq[0]:], base[lq[0]:])
+        c.prefix_table[1] = -1
+        assert bool(c.run(qimg).isnan().all())
 
 
 @pytest.mark.parametrize("lq,lk,prefix", [([1] * 3, [700, 4000, 9], 0), ([130, 20], [130, 300], 0), ([1] * 30, [40] * 30, 800)])
@@ -309,6 +308,25 @@ def test_replays_other_streams_and_repeats(qimg, lq, lk, prefix):
         assert torch.equal(got, want)
         c.lk, c.prefix = lens, max(0, prefix - 100 * n)
     # (the rows of the sequences' ends and of the prefix are the first of the same pages)
+
+
+def test_tables_with_room_for_a_million_keys(qimg):
+    """Tiles of many rows make their keys' 16-bit rows a few heads and sequences at a time where the
+    tables have room for more than scratch should hold."""
+    for prefix in (0, 300):
+        c = Case(qimg, [100, 300, 7], [130, 1000, 600], prefix, hq=8, hk=2, page=256, codes=CODES[1], seed=16)
+        wide = torch.full((3, 4096), -1, dtype=torch.int32, device=DEV)
+        wide[:, :c.table.shape[1]] = c.table
+        c.table = wide
+        if prefix:
+            more = torch.full((9000,), 2 ** 30, dtype=torch.int32, device=DEV)
+            more[:c.prefix_table.numel()] = c.prefix_table
+            c.prefix_table = more
+        need = qimg.attention_cache_scratch_bytes(407, 3, 8, 2, 128, 256, 4096, 9000 if prefix else 0)
+        assert 1 << 30 <= need < 5 << 30
+        got = c.run(qimg)
+        torch.cuda.synchronize()
+        _check(got, *c.oracle())
 
 
 def test_caches_past_32_bits(qimg):
