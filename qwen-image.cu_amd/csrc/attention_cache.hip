@@ -957,6 +957,8 @@ int64_t tile_bound(int total_q, int batch, int group, int rows) {
 }  // namespace
 
 constexpr int kMostSplits = 32;
+constexpr int kFewTiles = 320;  // of 32 rows that the card works on without those of MR
+constexpr int kWorkTogether = 24000, kWorkOf32 = 60000;  // products of 16 rows and 32 keys behind a prefix
 constexpr int kMostBlocks = 1 << 22;  // of a launch (a grid has less than 2^32 threads)
 constexpr int64_t kMostDense = int64_t{1} << 30;  // bytes of 16-bit rows at a time, of one head of a sequence at least
 
@@ -964,12 +966,26 @@ AttnCachePlan attn_cache_plan(int total_q, int batch, int hq, int hk, int D, int
     AttnCachePlan p{};
     if (total_q <= 0 || batch <= 0) return p;
     const int group = hq / hk;
-    // rows of a tile, by the average number of a sequence
-    const auto tile_rows = [&](int64_t rows, int seqs) {
-        return rows <= 16 ? 16 : rows <= 64 || tile_bound(total_q, seqs, group, MR) * hk >= kMostBlocks ? 32 : MR;
-    };
-    p.own_rows = tile_rows((static_cast<int64_t>(total_q) * group + batch - 1) / batch, batch);
-    p.prefix_rows = tile_rows(static_cast<int64_t>(total_q) * group, 1);
+    // Rows of a tile. Rows of MR have their keys decoded into scratch first, which pays once some
+    // hundred rows use them and there are tiles for the workgroups; 28/4 heads of 128, e4m3, MR
+    // rows to 32, in us: 16 tokens at 4096 keys 29.5 to 16.5, of 32 sequences 162 to 76; 64 tokens
+    // at 4096 of 16 sequences 144 to 128; 300 at 300 keys 18.0 to 15.4, of 4 sequences 22 to 33;
+    // 200 at 2000 of 8 sequences 80 to 102; 512 at 4096 63 to 63.
+    const auto fits = [&](int rows, int seqs) { return tile_bound(total_q, seqs, group, rows) * hk < kMostBlocks; };
+    const int64_t rows = (static_cast<int64_t>(total_q) * group + batch - 1) / batch;  // of a sequence, on average
+    if (rows <= 16)
+        p.own_rows = 16;
+    else if (rows <= 512 || tile_bound(total_q, batch, group, 32) * hk <= kFewTiles || !fits(MR, batch))
+        p.own_rows = 32;
+    else
+        p.own_rows = MR;
+    // Behind a prefix by the products of 16 rows and 32 keys. One launch for both parts is best
+    // while they are few, tiles of 32 rows take half of them, MR rows more than that; 1 key and
+    // more of their own, MR rows, the own part's 16 and 32, in us: 16 tokens behind 4096 keys
+    // 30.6, 16.9, 22.3; 64 behind 4096 35.2, 28.5, 30.1; 128 behind 4096 47.0, 48.7, 39.7; 256
+    // behind 4096 71.6, 81.7, 66.2; 128 behind 16384 74.3, 114.7, 89.2.
+    const int64_t work = (static_cast<int64_t>(total_q) * group + 15) / 16 * ((prefix_keys + 31) / 32) * hk;
+    p.prefix_rows = work <= kWorkTogether && p.own_rows != MR ? p.own_rows : work <= kWorkOf32 || !fits(MR, 1) ? 32 : MR;
     // Most ranges of a sequence: eight steps each at least, and 2^13 row tiles times ranges; of
     // MR rows the shares that may meet in a tile, up to 1.5 tiles a workgroup.
     const auto splits = [&](int64_t keys, int rows, int seqs) -> int {

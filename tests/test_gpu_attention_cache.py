@@ -143,6 +143,14 @@ def test_pieces_of_prompts(qimg, lq, lk, d, causal):
         _run(qimg, lq, lk, causal, d=d, page=(16, 32, 64, 128)[i], dtype=dtype, codes=codes, seed=len(lq) + d)
 
 
+@pytest.mark.parametrize("lq,lk", PIECES[1:] + [([1, 0, 160], [3, 9, 900])], ids=str)
+@pytest.mark.parametrize("d", [64, 128])
+def test_pieces_of_many_rows(qimg, lq, lk, d):
+    """Ten q heads to a kv head and eight of those: tiles of 128 rows."""
+    for i, (dtype, codes) in enumerate([(BF, CODES[0]), (BF, CODES[1]), (HF, CODES[0]), (HF, CODES[1])]):
+        _run(qimg, lq, lk, i != 1, hq=80, hk=8, d=d, page=(256, 16, 32, 64)[i], dtype=dtype, codes=codes, seed=len(lq) + d)
+
+
 PREFIXES = [([1], [1], 1), ([1] * 3, [5, 0, 40], 100), ([1] * 20, [0] * 20, 700), ([2, 0, 3], [40, 3, 0], 33), ([1] * 40, list(range(1, 41)), 2000),
             ([200, 31], [200, 300], 500), ([1] * 5, [1, 2, 3, 4, 5], 0), ([4] * 30, [64 * i for i in range(30)], 3000),
             ([1] * 130, [1 + i % 50 for i in range(130)], 9000)]
@@ -157,6 +165,22 @@ def test_prefix(qimg, lq, lk, prefix, d):
         got = c.run(qimg, i != 2, with_prefix=True)
         torch.cuda.synchronize()
         _check(got, *c.oracle(i != 2))
+
+
+@pytest.mark.parametrize("lq,lk,prefix", PREFIXES[1:], ids=lambda x: str(x)[:40])
+@pytest.mark.parametrize("d", [64, 128])
+def test_prefix_tables_with_room(qimg, lq, lk, prefix, d):
+    """Behind a table of that many keys the prefix takes tiles of 128 rows; its length is the device's."""
+    for i, (dtype, codes) in enumerate([(BF, CODES[0]), (HF, CODES[1])]):
+        page = (32, 256)[i]
+        c = Case(qimg, lq, lk, prefix, d=d, page=page, dtype=dtype, codes=codes, seed=prefix + d, hq=(28, 48)[i], hk=(4, 24)[i])
+        tiles = -(-sum(lq) * c.q.shape[1] // c.hk // 16)
+        wide = torch.full((60001 * 32 // (tiles * c.hk * page) + 2 + c.prefix_table.numel(),), -1, dtype=torch.int32, device=DEV)
+        wide[:c.prefix_table.numel()] = c.prefix_table
+        c.prefix_table = wide
+        got = c.run(qimg, with_prefix=True)
+        torch.cuda.synchronize()
+        _check(got, *c.oracle())
 
 
 def test_prefix_pages_in_the_tables_instead(qimg):
@@ -201,9 +225,10 @@ def test_constant_values_come_back_exactly(qimg):
 
 @pytest.mark.parametrize("codes", CODES, ids=str)
 @pytest.mark.parametrize("lq,lk", [([1, 1, 1], [100, 2000, 31]), ([150, 60, 3], [200, 60, 2000])], ids=str)
-def test_a_token_that_is_not_finite(qimg, codes, lq, lk):
+@pytest.mark.parametrize("hq,hk", [(8, 2), (80, 8)])
+def test_a_token_that_is_not_finite(qimg, codes, lq, lk, hq, hk):
     """Rows that see it are NaN, in its kv head alone; the others do not change."""
-    c = Case(qimg, lq, lk, seed=9, codes=codes, page=32, hq=8, hk=2)
+    c = Case(qimg, lq, lk, seed=9, codes=codes, page=32, hq=hq, hk=hk)
     base = c.run(qimg)
     n, hk, page, d = c.cache.k.shape
     key = lk[0] - 1  # the last key of sequence 0: of a piece its last query alone sees it
@@ -216,8 +241,9 @@ def test_a_token_that_is_not_finite(qimg, codes, lq, lk):
         qimg.kv_cache_write(cache, *both, _i32(slot))
         got = qimg.attention_cache(c.q, cache, c.cu_q, c.table, c.k_lens)
         torch.cuda.synchronize()
-        assert bool(got[lq[0] - 1, 4:].isnan().all())
-        assert not bool(got[lq[0] - 1, :4].isnan().any())
+        seen = torch.arange(hq, device=DEV) // (hq // hk) == 1
+        assert bool(got[lq[0] - 1, seen].isnan().all())
+        assert not bool(got[lq[0] - 1, ~seen].isnan().any())
         keep = torch.ones(sum(lq), dtype=torch.bool, device=DEV)
         keep[lq[0] - 1] = False
         assert torch.equal(got[keep], base[keep])
@@ -225,10 +251,11 @@ def test_a_token_that_is_not_finite(qimg, codes, lq, lk):
 
 @pytest.mark.parametrize("lq,lk", [([1, 1, 1], [300, 3000, 40]), ([100, 40, 3], [300, 200, 90])], ids=str)
 @pytest.mark.parametrize("codes", CODES, ids=str)
-def test_pages_outside_the_cache(qimg, lq, lk, codes):
+@pytest.mark.parametrize("hq,hk", [(28, 4), (96, 8)])
+def test_pages_outside_the_cache(qimg, lq, lk, codes, hq, hk):
     """Nothing outside the cache is read: rows that see a key there are NaN, the others do not change."""
     for bad in (-1, 2 ** 31 - 1, -2 ** 31, None):
-        c = Case(qimg, lq, lk, page=16, seed=10, prefix=64, codes=codes)
+        c = Case(qimg, lq, lk, page=16, seed=10, prefix=64, codes=codes, hq=hq, hk=hk)
         base = c.run(qimg)
         key = 240  # of sequence 0: its last 60 queries' keys reach there
         c.table[0, key // 16] = c.cache.k.shape[0] if bad is None else bad
@@ -241,7 +268,8 @@ def test_pages_outside_the_cache(qimg, lq, lk, codes):
         assert bool(c.run(qimg).isnan().all())
 
 
-@pytest.mark.parametrize("lq,lk,prefix", [([1] * 3, [700, 4000, 9], 0), ([130, 20], [130, 300], 0), ([1] * 30, [40] * 30, 800)])
+@pytest.mark.parametrize("lq,lk,prefix", [([1] * 3, [700, 4000, 9], 0), ([130, 20], [130, 300], 0), ([1] * 30, [40] * 30, 800),
+                                          ([600, 20], [1300, 300], 0), ([1] * 100, [40] * 100, 12000)])
 def test_views_and_rows_of_no_sequence(qimg, lq, lk, prefix):
     c = Case(qimg, lq, lk, prefix, seed=12)
     want = c.run(qimg)
@@ -256,10 +284,12 @@ def test_views_and_rows_of_no_sequence(qimg, lq, lk, prefix):
     assert bool((room[:, t:] == 7).all() and (room[28:] == 7).all() and (room[:, :, 128:] == 7).all())
 
 
-def test_offsets_and_lengths_outside_are_clamped(qimg):
-    c = Case(qimg, [3, 4, 2], [40, 50, 60], prefix=32, page=16, seed=13)
+@pytest.mark.parametrize("m", [1, 100])
+def test_offsets_and_lengths_outside_are_clamped(qimg, m):
+    c = Case(qimg, [3 * m, 4 * m, 2 * m], [40, 50, 60], prefix=32, page=16, seed=13)
     out = torch.empty_like(c.q)
     for cu in ([0, 5, 3, 20], [-7, 3, 7, 2 ** 31 - 1], [9, 6, 3, 0], [-2 ** 31, 0, 0, 9]):
+        cu = [x * m if abs(x) < 100 else x for x in cu]
         for kl in ([2 ** 31 - 1, -5, 1000], [-2 ** 31, 64, 0]):
             for pl in (-1, 10 ** 9):
                 qimg.attention_cache(c.q, c.cache, _i32(*cu), c.table, _i32(*kl), prefix_table=c.prefix_table,
@@ -274,7 +304,8 @@ def test_offsets_and_lengths_outside_are_clamped(qimg):
     assert torch.equal(a.nan_to_num(5.0), b.nan_to_num(5.0))
 
 
-@pytest.mark.parametrize("lq,lk,prefix", [([1] * 3, [700, 4000, 9], 0), ([130, 20], [1300, 300], 0), ([1] * 30, [40] * 30, 800)])
+@pytest.mark.parametrize("lq,lk,prefix", [([1] * 3, [700, 4000, 9], 0), ([130, 20], [1300, 300], 0), ([1] * 30, [40] * 30, 800),
+                                          ([600, 20], [1300, 300], 0), ([1] * 100, [40] * 100, 12000)])
 def test_replays_other_streams_and_repeats(qimg, lq, lk, prefix):
     """A captured call follows the lists on the device; the same call gives the same bits."""
     c = Case(qimg, lq, lk, prefix, seed=14)
@@ -314,7 +345,7 @@ def test_tables_with_room_for_a_million_keys(qimg):
     """Tiles of many rows make their keys' 16-bit rows a few heads and sequences at a time where the
     tables have room for more than scratch should hold."""
     for prefix in (0, 300):
-        c = Case(qimg, [100, 300, 7], [130, 1000, 600], prefix, hq=8, hk=2, page=256, codes=CODES[1], seed=16)
+        c = Case(qimg, [100, 300, 7], [130, 1000, 600], prefix, hq=32, hk=4, page=256, codes=CODES[1], seed=16)
         wide = torch.full((3, 4096), -1, dtype=torch.int32, device=DEV)
         wide[:, :c.table.shape[1]] = c.table
         c.table = wide
@@ -322,7 +353,7 @@ def test_tables_with_room_for_a_million_keys(qimg):
             more = torch.full((9000,), 2 ** 30, dtype=torch.int32, device=DEV)
             more[:c.prefix_table.numel()] = c.prefix_table
             c.prefix_table = more
-        need = qimg.attention_cache_scratch_bytes(407, 3, 8, 2, 128, 256, 4096, 9000 if prefix else 0)
+        need = qimg.attention_cache_scratch_bytes(407, 3, 32, 4, 128, 256, 4096, 9000 if prefix else 0)
         assert 1 << 30 <= need < 5 << 30
         got = c.run(qimg)
         torch.cuda.synchronize()
@@ -336,7 +367,7 @@ def test_caches_past_32_bits(qimg):
     k, v = (torch.empty(n, hk, page, d, dtype=torch.uint8, device=DEV).view(torch.int8) for _ in range(2))
     ke, ve = (torch.empty(n, hk, page, dtype=torch.uint8, device=DEV) for _ in range(2))
     big = qimg.KvCache(k, v, ke, ve)
-    small = Case(qimg, [1, 200], [700, 900], hq=16, hk=hk, d=d, page=page, seed=15, prefix=300)
+    small = Case(qimg, [1, 700], [700, 900], hq=16, hk=hk, d=d, page=page, seed=15, prefix=300)
     m = small.cache.k.shape[0]
     for dst, src in zip(big, small.cache):
         dst[n - m:].copy_(src)
