@@ -899,21 +899,26 @@ def kv_cache(n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dtype
     return KvCache(k, v, ke, ve)
 
 
+_CODES = {torch.int8: INT8, torch.float8_e4m3fn: FP8_E4M3}
+
+
 def _cache_struct(cache: KvCache, device) -> _KvCache:
     k, v, ke, ve = cache
-    if k.device != device or v.device != device or ke.device != device or ve.device != device:
+    if not (device == k.device == v.device == ke.device == ve.device):
         raise QimgError(QIMG_ERR_INVALID_ARG, f"the cache must be on {device}, the first argument's device")
-    if k.dtype not in (torch.int8, torch.float8_e4m3fn) or v.dtype != k.dtype:
+    codes = _CODES.get(k.dtype)
+    if codes is None or v.dtype is not k.dtype:
         raise QimgError(QIMG_ERR_INVALID_ARG, "the cache's codes must be int8 or float8_e4m3fn")
-    if k.dim() != 4 or v.shape != k.shape or not k.is_contiguous() or not v.is_contiguous():
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape or not k.is_contiguous() or not v.is_contiguous():
         raise QimgError(QIMG_ERR_INVALID_ARG, "the cache's k and v must be contiguous [n_pages, Hk, page_size, D]")
-    if (ke.dtype != torch.uint8 or ve.dtype != torch.uint8 or ke.shape != k.shape[:3] or ve.shape != ke.shape
+    n, hk, page, d = shape
+    exps = ke.shape
+    if (exps != (n, hk, page) or ve.shape != exps or ke.dtype is not torch.uint8 or ve.dtype is not torch.uint8
             or not ke.is_contiguous() or not ve.is_contiguous()):
         raise QimgError(QIMG_ERR_INVALID_ARG, "the cache's exponents must be contiguous uint8 [n_pages, Hk, page_size]")
-    n, hk, page, d = k.shape
     _fits32(n, hk, page, d)
-    return _KvCache(k.data_ptr(), v.data_ptr(), ke.data_ptr(), ve.data_ptr(), INT8 if k.dtype == torch.int8 else FP8_E4M3,
-                    n, page, hk, d)
+    return _KvCache(k.data_ptr(), v.data_ptr(), ke.data_ptr(), ve.data_ptr(), codes, n, page, hk, d)
 
 
 def _list32(t: torch.Tensor, n: int, name: str):
