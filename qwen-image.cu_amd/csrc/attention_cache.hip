@@ -653,8 +653,8 @@ __device__ __forceinline__ int64_t slot_rows(const AttnCacheArgs& a, int b) {
 
 // One tile of 64 keys of one head a workgroup. Keys of a page outside the cache are NaN.
 template <class T, class C, int D>
-__global__ __launch_bounds__(256) void attn_cache_decode_kernel(AttnCacheArgs a, Part part, int tiles) {
-    const int tile = static_cast<int>(blockIdx.x) % tiles, at = static_cast<int>(blockIdx.x) / tiles;
+__device__ __forceinline__ void decode_tile(const AttnCacheArgs& a, const Part& part, int tiles, int block) {
+    const int tile = block % tiles, at = block / tiles;
     const int head = at % part.heads, slot = at / part.heads, b = part.lo + slot;
     const Sequence s = load_sequence(a, b, part.hi);
     if (s.lq == 0 || tile * MK >= s.lk) return;
@@ -688,6 +688,23 @@ __global__ __launch_bounds__(256) void attn_cache_decode_kernel(AttnCacheArgs a,
         *reinterpret_cast<u32x4*>(vo) = r[2];
         *reinterpret_cast<u32x4*>(vo + 8) = r[3];
     }
+}
+
+template <class T, class C, int D>
+__global__ __launch_bounds__(256) void attn_cache_decode_kernel(AttnCacheArgs a, Part part, int tiles) {
+    decode_tile<T, C, D>(a, part, tiles, blockIdx.x);
+}
+
+// The first `few` workgroups work on the sequences' own keys in tiles of few rows, the
+// others decode the prefix for its tiles of MR: one waits for memory, one does not.
+template <class T, class C, int D, int NR>
+__global__ __launch_bounds__(SW * 64, NR == 1 ? 3 : 2) void attn_cache_mixed_kernel(AttnCacheArgs a, Part own, int few,
+                                                                                    Part prefix, int tiles) {
+    __shared__ __attribute__((aligned(16))) float lds[kFewLds<D>];
+    if (static_cast<int>(blockIdx.x) < few)
+        few_items<T, C, D, NR>(a, own, blockIdx.x, few, lds);
+    else
+        decode_tile<T, C, D>(a, prefix, tiles, static_cast<int>(blockIdx.x) - few);
 }
 
 template <int D>
@@ -848,26 +865,15 @@ __global__ __launch_bounds__(MW * 64, 2) void attn_cache_many_kernel(AttnCacheAr
     many_items<T, D>(a, part, blockIdx.x, lds);
 }
 
-// The prefix in tiles of MR rows and, by the workgroups from `many` on, the sequences' own
-// keys in tiles of few: in one launch these run in what the prefix leaves idle.
-template <class T, class C, int D, int NR>
-__global__ __launch_bounds__(MW * 64, 2) void attn_cache_mixed_kernel(AttnCacheArgs a, Part prefix, Part own, int many) {
-    constexpr int kBytes = kManyLds<D> > kFewLds<D> * 4 ? kManyLds<D> : kFewLds<D> * 4;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[kBytes];
-    if (static_cast<int>(blockIdx.x) < many)
-        many_items<T, D>(a, prefix, blockIdx.x, lds);
-    else
-        few_items<T, C, D, NR>(a, own, static_cast<int>(blockIdx.x) - many, static_cast<int>(gridDim.x) - many,
-                               reinterpret_cast<float*>(lds));
-}
-
-// Partial results of a row, added in order: 16 threads a row, tiles of 16 rows of one
-// sequence and kv head. Eight parts' loads go out together.
-template <class T, int D>
+// Partial results of a row: 16 threads add every G-th of them in order, eight parts' loads
+// going out together, and the G sums meet in the wave; tiles of 16 / G rows of one sequence
+// and kv head. G = 4 where tiles of 16 rows would leave CUs
+// idle: 16 tokens of 28/4 heads with 32 parts 5.1 us (7.5 with G = 1); 128 tokens 17 (12).
+template <class T, int D, int G>
 __device__ __forceinline__ void join_item(const AttnCacheArgs& a, const RowTile& t, int hk, int own, int shared) {
     constexpr int E = D / 16, U = 8;
     typedef float v2f __attribute__((ext_vector_type(2)));
-    const int row = t.row0 + (threadIdx.x >> 4), c0 = (threadIdx.x & 15) * E;
+    const int row = t.row0 + threadIdx.x / (16 * G), c0 = (threadIdx.x & 15) * E, g = (threadIdx.x >> 4) % G;
     if (row >= t.lq * a.group) return;
     const int64_t token = static_cast<int64_t>(t.q0) + row / a.group;
     const int head = hk * a.group + row % a.group;
@@ -876,12 +882,12 @@ __device__ __forceinline__ void join_item(const AttnCacheArgs& a, const RowTile&
     float mm = kNegInf, tot = 0.0f, acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-    for (int s0 = 0; s0 < n; s0 += U) {
+    for (int s0 = g; s0 < n; s0 += U * G) {
         v2f ml[U];
         v4f v[U][E / 4];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int s = min(s0 + u, n - 1);
+            const int s = min(s0 + u * G, n - 1);
             const int64_t p = at + (s < own ? s : a.own_splits + s - own);
             ml[u] = *reinterpret_cast<const v2f*>(a.part_ml + 2 * p);
 #pragma unroll
@@ -897,7 +903,7 @@ __device__ __forceinline__ void join_item(const AttnCacheArgs& a, const RowTile&
         for (int e = 0; e < E; ++e) acc[e] *= old;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (s0 + u >= n) continue;
+            if (s0 + u * G >= n) continue;
             // no finite score: O is zero there, the sum zero or NaN
             const float f = ml[u][0] == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(ml[u][0] - mm);
             tot += f * ml[u][1];
@@ -905,10 +911,24 @@ __device__ __forceinline__ void join_item(const AttnCacheArgs& a, const RowTile&
             for (int e = 0; e < E; ++e) acc[e] += f * v[u][e / 4][e % 4];
         }
     }
+#pragma unroll
+    for (int step = 16; step < 16 * G; step *= 2) {
+        const float top = fmaxf(mm, __shfl_xor(mm, step));
+        const float f = mm == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(mm - top);
+        mm = top;
+        tot *= f;
+        tot += __shfl_xor(tot, step);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            acc[e] *= f;
+            acc[e] += __shfl_xor(acc[e], step);
+        }
+    }
+    if (g != 0) return;
     store_row<T, E>(a.out + token * a.o_t + head * a.o_h + c0, acc, tot, tot == 0.0f);
 }
 
-template <class T, int D>
+template <class T, int D, int G>
 __global__ __launch_bounds__(256) void attn_cache_join_kernel(AttnCacheArgs a, Part own_part, Part prefix_part) {
     const int lane = threadIdx.x & 63;
     const Sequence first = load_sequence(a, lane, own_part.hi);
@@ -920,7 +940,7 @@ __global__ __launch_bounds__(256) void attn_cache_join_kernel(AttnCacheArgs a, P
         // (one launch of both has one length of ranges)
         prefix_per = own_part.hi > a.batch ? per : range_length(a, load_sequence(a, a.batch + lane, prefix_part.hi), prefix_part);
     }
-    const Part rows = {0, a.batch, 16, 0, a.c.hk};
+    const Part rows = {0, a.batch, 16 / G, 0, a.c.hk};
     for (int item = blockIdx.x;; item += gridDim.x) {
         const int hk = item % a.c.hk;
         const RowTile t = find_tile(a, first, rows, item / a.c.hk, 0);
@@ -940,11 +960,11 @@ __global__ __launch_bounds__(256) void attn_cache_join_kernel(AttnCacheArgs a, P
         } else {
             // a row's tile of the prefix, whose rows are those of all sequences
             const int np = steps_of(prefix_part, p.lk), tiles = row_tiles(a, p.lq, MR);
-            const int row = min(t.row0 + static_cast<int>(threadIdx.x >> 4), t.lq * a.group - 1);
+            const int row = min(t.row0 + static_cast<int>(threadIdx.x / (16 * G)), t.lq * a.group - 1);
             const int tile = static_cast<int>(((static_cast<int64_t>(t.q0) - p.q0) * a.group + row) / MR);
             shared = prefix_per == 0 ? 1 : tile_shares((hk * tiles + tile) * np, np, prefix_per).count;
         }
-        join_item<T, D>(a, t, hk, own, shared);
+        join_item<T, D, G>(a, t, hk, own, shared);
     }
 }
 
@@ -957,6 +977,7 @@ int64_t tile_bound(int total_q, int batch, int group, int rows) {
 }  // namespace
 
 constexpr int kMostSplits = 32;
+constexpr int kCus = 256;
 constexpr int kFewTiles = 320;  // of 32 rows that the card works on without those of MR
 constexpr int kWorkTogether = 24000, kWorkOf32 = 60000;  // products of 16 rows and 32 keys behind a prefix
 constexpr int kMostBlocks = 1 << 22;  // of a launch (a grid has less than 2^32 threads)
@@ -1029,17 +1050,6 @@ AttnCacheScratch attn_cache_scratch(const AttnCachePlan& plan, int D) {
     return {align(plan.part_rows * D * 4), align(plan.part_rows * 8), align(plan.dense_rows * D * 2)};
 }
 
-// The codes of a part as 16-bit rows in scratch.
-template <class T, class C, int D>
-static hipError_t launch_decode(const AttnCacheArgs& a, const Part& part, hipStream_t stream) {
-    const int64_t keys = static_cast<int64_t>(part.lo < a.batch ? a.max_blocks : a.prefix_blocks) << a.c.page_shift;
-    const int64_t tiles = (keys + MK - 1) / MK, blocks = tiles * part.heads * (part.hi - part.lo);
-    if (blocks == 0) return hipSuccess;
-    hipLaunchKernelGGL((attn_cache_decode_kernel<T, C, D>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, a, part,
-                       static_cast<int>(tiles));
-    return hipGetLastError();
-}
-
 template <class T, class C, int D>
 static hipError_t launch_attn(const AttnCacheArgs& a, const AttnCachePlan& plan, hipStream_t stream) {
     const bool prefix = plan.prefix_splits > 0;
@@ -1048,7 +1058,7 @@ static hipError_t launch_attn(const AttnCacheArgs& a, const AttnCachePlan& plan,
     const Part own = {0, a.batch + (together ? 1 : 0), plan.own_rows, 0, a.c.hk};
     const Part shared = {a.batch, a.batch + 1, plan.prefix_rows, 0, a.c.hk};
     const dim3 block(MW * 64);
-    static_assert(MW == SW, "one workgroup for both");
+    static_assert(MW == SW && SW == 4, "workgroups of 256 for all");
     // workgroups of MR rows: the tiles, or the shares of those that run at once
     const auto many = [&](int seqs, int heads, int splits) {
         const int64_t tiles = tile_bound(a.total_q, seqs, a.group, MR) * heads;
@@ -1060,27 +1070,33 @@ static hipError_t launch_attn(const AttnCacheArgs& a, const AttnCachePlan& plan,
         if (with_prefix) items += tile_bound(a.total_q, 1, a.group, rows) * a.prefix_splits;
         return static_cast<unsigned>(std::min<int64_t>(items * a.c.hk, few_grid(rows)));
     };
+    // the codes of a part as 16-bit rows in scratch; with the own part's few rows if they are asked for
+    const auto decode = [&](const Part& part, bool with_own) {
+        const int64_t keys = static_cast<int64_t>(part.lo < a.batch ? a.max_blocks : a.prefix_blocks) << a.c.page_shift;
+        const int tiles = static_cast<int>((keys + MK - 1) / MK);
+        const unsigned blocks = static_cast<unsigned>(static_cast<int64_t>(tiles) * part.heads * (part.hi - part.lo));
+        const unsigned more = with_own ? few(true, false, own.rows) : 0;
+        if (more > 0 && own.rows == 16)
+            hipLaunchKernelGGL((attn_cache_mixed_kernel<T, C, D, 1>), dim3(more + blocks), block, 0, stream, a, own,
+                               static_cast<int>(more), part, tiles);
+        else if (more > 0)
+            hipLaunchKernelGGL((attn_cache_mixed_kernel<T, C, D, 2>), dim3(more + blocks), block, 0, stream, a, own,
+                               static_cast<int>(more), part, tiles);
+        else if (blocks > 0)
+            hipLaunchKernelGGL((attn_cache_decode_kernel<T, C, D>), dim3(blocks), block, 0, stream, a, part, tiles);
+        return hipGetLastError();
+    };
     bool own_done = false;
     hipError_t e = hipSuccess;
     if (prefix && shared.rows == MR) {
         for (int h = 0; h < a.c.hk && e == hipSuccess; h += plan.prefix_heads) {
             Part part = shared;
             part.h0 = h, part.heads = std::min(plan.prefix_heads, a.c.hk - h);
-            e = launch_decode<T, C, D>(a, part, stream);
+            e = decode(part, h == 0 && own.rows != MR);
             if (e != hipSuccess) break;
-            const unsigned grid = many(1, part.heads, a.prefix_splits);
-            if (own_done || own.rows == MR) {
-                hipLaunchKernelGGL((attn_cache_many_kernel<T, D>), dim3(grid), block, 0, stream, a, part);
-            } else {
-                const unsigned more = few(true, false, own.rows);
-                if (own.rows == 16)
-                    hipLaunchKernelGGL((attn_cache_mixed_kernel<T, C, D, 1>), dim3(grid + more), block, 0, stream, a, part, own,
-                                       static_cast<int>(grid));
-                else
-                    hipLaunchKernelGGL((attn_cache_mixed_kernel<T, C, D, 2>), dim3(grid + more), block, 0, stream, a, part, own,
-                                       static_cast<int>(grid));
-                own_done = true;
-            }
+            own_done = own.rows != MR;
+            hipLaunchKernelGGL((attn_cache_many_kernel<T, D>), dim3(many(1, part.heads, a.prefix_splits)), block, 0, stream, a,
+                               part);
             e = hipGetLastError();
         }
     } else if (prefix && !together) {  // of 32 rows, where the sequences' own tiles have 16
@@ -1091,7 +1107,7 @@ static hipError_t launch_attn(const AttnCacheArgs& a, const AttnCachePlan& plan,
         for (int b = 0; b < a.batch; b += plan.own_slots) {
             for (int h = 0; h < a.c.hk; h += plan.own_heads) {
                 const Part part = {b, std::min(b + plan.own_slots, a.batch), MR, h, std::min(plan.own_heads, a.c.hk - h)};
-                e = launch_decode<T, C, D>(a, part, stream);
+                e = decode(part, false);
                 if (e != hipSuccess) return e;
                 hipLaunchKernelGGL((attn_cache_many_kernel<T, D>), dim3(many(part.hi - part.lo, part.heads, a.own_splits)),
                                    block, 0, stream, a, part);
@@ -1107,8 +1123,16 @@ static hipError_t launch_attn(const AttnCacheArgs& a, const AttnCachePlan& plan,
         e = hipGetLastError();
     }
     if (e != hipSuccess || plan.part_rows == 0) return e;
-    const int64_t tiles = std::min<int64_t>(tile_bound(a.total_q, a.batch, a.group, 16) * a.c.hk, kMostBlocks);
-    hipLaunchKernelGGL((attn_cache_join_kernel<T, D>), dim3(static_cast<unsigned>(tiles)), dim3(256), 0, stream, a, own, shared);
+    const auto join = [&](auto g) {
+        constexpr int G = decltype(g)::value;
+        const int64_t tiles = std::min<int64_t>(tile_bound(a.total_q, a.batch, a.group, 16 / G) * a.c.hk, kMostBlocks);
+        hipLaunchKernelGGL((attn_cache_join_kernel<T, D, G>), dim3(static_cast<unsigned>(tiles)), dim3(256), 0, stream, a, own,
+                           shared);
+    };
+    if (tile_bound(a.total_q, a.batch, a.group, 16) * a.c.hk > kCus)
+        join(std::integral_constant<int, 1>{});
+    else
+        join(std::integral_constant<int, 4>{});
     return hipGetLastError();
 }
 
