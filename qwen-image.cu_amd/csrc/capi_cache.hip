@@ -88,6 +88,13 @@ qimg::CachePages pages_of(const qimg_kv_cache& c) {
     return {c.k, c.v, c.k_exp, c.v_exp, c.n_pages, page_shift(c), c.n_kv_heads};
 }
 
+// Sizes of attention over a cache: queries, and tokens of a table's pages.
+bool attn_sizes(int64_t total_q, int n_heads, int batch, int max_blocks, int prefix_blocks, int page_size) {
+    const int64_t most = int64_t{1} << 30;
+    return total_q * n_heads < most && batch < most && static_cast<int64_t>(max_blocks) * page_size < most &&
+           static_cast<int64_t>(prefix_blocks) * page_size < most;
+}
+
 int64_t bytes_of(int elem_dtype) { return elem_dtype == QIMG_FP32 ? 4 : 2; }
 
 }  // namespace
@@ -175,8 +182,9 @@ int qimg_kv_cache_read(const qimg_kv_cache* cache, const int32_t* block_table, i
 
 int64_t qimg_attention_cache_scratch_bytes(int total_q, int batch, int n_heads, int n_kv_heads, int head_dim,
                                            int page_size, int max_blocks, int prefix_blocks) {
-    if (total_q <= 0 || batch <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0 || head_dim <= 0 ||
-        page_size <= 0 || max_blocks < 0 || prefix_blocks < 0)
+    if (total_q <= 0 || batch <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0 ||
+        (head_dim != 64 && head_dim != 128) || page_size < 16 || page_size > 256 || max_blocks < 0 || prefix_blocks < 0 ||
+        !attn_sizes(total_q, n_heads, batch, max_blocks, prefix_blocks, page_size))
         return 0;
     const qimg::AttnCacheScratch s = qimg::attn_cache_scratch(
         qimg::attn_cache_plan(total_q, batch, n_heads, n_kv_heads, head_dim, static_cast<int64_t>(max_blocks) * page_size,
@@ -199,10 +207,7 @@ int qimg_attention_cache(const qimg_attn_cache* args, const qimg_kv_cache* cache
                  "%s: n_heads %d must be a multiple of the cache's n_kv_heads %d", fn, p.n_heads, cache->n_kv_heads);
     const float scale_log2 = p.sm_scale * 1.4426950408889634f;
     QIMG_REQUIRE(std::isfinite(scale_log2) && scale_log2 > 0.0f, "%s: sm_scale must be positive and finite", fn);
-    const int64_t most = int64_t{1} << 30;
-    QIMG_REQUIRE(static_cast<int64_t>(p.total_q) * p.n_heads < most && p.batch < most &&
-                     static_cast<int64_t>(p.max_blocks) * cache->page_size < most &&
-                     static_cast<int64_t>(p.prefix_blocks) * cache->page_size < most,
+    QIMG_REQUIRE(attn_sizes(p.total_q, p.n_heads, p.batch, p.max_blocks, p.prefix_blocks, cache->page_size),
                  "%s: total_q * n_heads, batch and a table's pages times page_size must be < 2^30", fn);
     QIMG_REQUIRE(good_strides(p.q_stride_t, p.q_stride_h) && good_strides(p.out_stride_t, p.out_stride_h),
                  "%s: strides must be non-negative multiples of 8, token strides at most 2^24", fn);

@@ -139,6 +139,11 @@ def test_empty_calls_and_scratch(qimg):
     assert _attn(qimg, c, batch=0, q=None) == 0 and _attn(qimg, c, total_q=0, q=None) == 0
     need = qimg.attention_cache_scratch_bytes
     assert need(0, 1, 28, 4, 128, 64, 100) == 0 and need(1, 1, 28, 3, 128, 64, 100) == 0
+    # sizes that the call refuses
+    top = (1 << 31) - 1
+    assert need(top, top, top, 1, 128, 256, top, top) == 0 and need(1, 1, 1 << 30, 1, 128, 64, 2) == 0
+    assert need(1, 1, 28, 4, 128, 64, 1 << 24) == 0 and need(1, 1, 28, 4, 96, 64, 100) == 0 and need(1, 1, 28, 4, 128, 8, 100) == 0
+    assert need(1, 1 << 30, 28, 4, 128, 64, 100) == 0 and need(1, 1, 28, 4, 128, 64, 1, 1 << 24) == 0
     assert need(16, 16, 28, 4, 128, 64, 2) == 0      # short caches are not cut
     assert need(16, 16, 28, 4, 128, 64, 128) > 16 * 28 * 128 * 4
     assert need(16, 16, 28, 4, 128, 64, 2, 10) > 16 * 28 * 128 * 4  # a prefix is joined with the own keys
