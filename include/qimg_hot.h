@@ -451,8 +451,11 @@ int qimg_kv_cache_read(const qimg_kv_cache* cache, const int32_t* block_table, i
  * for (which fp16 q needs to be in fp16's range). sm_scale > 0, finite. out overlaps neither q
  * nor the cache, and its strides keep tokens and heads apart. total_q * n_heads, batch and the
  * tokens of a table's pages below 2^30.
- * scratch: qimg_attention_cache_scratch_bytes(...) bytes (may be 0: NULL) for this call's
- * sizes. One scratch buffer serves one call at a time. */
+ * scratch: qimg_attention_cache_scratch_bytes(...) bytes (may be 0: NULL, and is 0 for sizes
+ * that the call refuses) for this call's sizes: partial results, and with some hundred rows
+ * (queries times heads of a group) a sequence, or behind a prefix, the keys in 16 bits, about
+ * 1 GiB of them at a time. The sizes of the tables count, not the lengths in use. One scratch
+ * buffer serves one call at a time. */
 typedef struct {
     const void* q;
     void* out;

@@ -308,6 +308,15 @@ __device__ __forceinline__ void store_row(uint16_t* op, const float (&acc)[E], f
 // its eight keys, decodes them (a pair is two channels of one key, with that key's
 // scale) and takes channel and key of pairs crosswise with v_perm_b32. The k index of
 // the first product is a channel, in any order that K and Q share: a lane's 16 codes.
+//
+// Bound by memory where every row tile has keys of its own: one token of 64 sequences of
+// 28/4 heads over 12541 to 16384 int8 keys 172 us, 5.5 TB/s (a large read reaches 6.1). By
+// the vector unit where row tiles share keys, behind a prefix: 385 vector and 190 scalar
+// instructions a wave and tile of 16 rows, mostly the decoding, V's crosswise pairs and
+// the exponentials; 32 rows decode once for both. Small calls by latency: 16 tokens over
+// up to 8192 keys 14.8 us (two or three tiles a wave), of which their 47 MB take 8. Loading
+// K a whole tile earlier changed none of these. A third and fourth 16 rows did not fit the
+// registers.
 constexpr int SW = 4;
 
 // A wave's 32-key tile as it lies in the cache, each half loaded again as soon as it is used up
@@ -639,8 +648,14 @@ __global__ __launch_bounds__(SW * 64, NR == 1 ? 3 : 2) void attn_cache_few_kerne
 // rows, head by head, and the work on them is attention_varlen.hip's (its tiles, waves
 // and phases, of which attention_tiles.h holds what both share). Decoding on the way into
 // LDS instead, 64 codes a thread and step, took no pass of its own, but each tile of rows
-// does it anew: with seven tiles a head (128 tokens of 28 / 4 heads) over 16000 int8 keys
-// the loop took 52 us, of fifty (1024 over 8192 e4m3 keys and 333) 169.
+// does it anew: with seven tiles a head (128 tokens of 28/4 heads over 16000 int8 keys)
+// the loop took 52 us (50 here, and 11 for the decoding, beside the own keys' tiles), with
+// fifty (1024 tokens over 8192 e4m3 keys and 333 over 2381) 169 (155 and 9).
+//
+// Bound by the softmax's vector instructions and the matrix unit in turn, which work half
+// of the time each: 2.3 us a step of two workgroups, 0.8 PFLOP/s (a large product 1.3). A
+// launch in shares also starts, and writes and joins partial results, 64 KB a workgroup:
+// 18 us of the 50, 12 of the joins.
 //
 // Where the CUs want more than whole tiles (range_length), the tiles' steps are dealt out
 // in equal shares and a tile's parts joined.
@@ -652,6 +667,7 @@ __device__ __forceinline__ int64_t slot_rows(const AttnCacheArgs& a, int b) {
 }
 
 // One tile of 64 keys of one head a workgroup. Keys of a page outside the cache are NaN.
+// Bound by memory: 8192 and 2381 e4m3 keys of 4 heads, 54 MB, 9 us.
 template <class T, class C, int D>
 __device__ __forceinline__ void decode_tile(const AttnCacheArgs& a, const Part& part, int tiles, int block) {
     const int tile = block % tiles, at = block / tiles;
@@ -696,7 +712,9 @@ __global__ __launch_bounds__(256) void attn_cache_decode_kernel(AttnCacheArgs a,
 }
 
 // The first `few` workgroups work on the sequences' own keys in tiles of few rows, the
-// others decode the prefix for its tiles of MR: one waits for memory, one does not.
+// others decode the prefix for its tiles of MR: one waits for memory, one does not. 16000
+// int8 keys beside 128 sequences of 1 to 509: 20 us; the decoding first 23, and in the
+// launch of the prefix' tiles instead the own keys took 9 to 10 besides the 11.
 template <class T, class C, int D, int NR>
 __global__ __launch_bounds__(SW * 64, NR == 1 ? 3 : 2) void attn_cache_mixed_kernel(AttnCacheArgs a, Part own, int few,
                                                                                     Part prefix, int tiles) {
@@ -867,8 +885,9 @@ __global__ __launch_bounds__(MW * 64, 2) void attn_cache_many_kernel(AttnCacheAr
 
 // Partial results of a row: 16 threads add every G-th of them in order, eight parts' loads
 // going out together, and the G sums meet in the wave; tiles of 16 / G rows of one sequence
-// and kv head. G = 4 where tiles of 16 rows would leave CUs
-// idle: 16 tokens of 28/4 heads with 32 parts 5.1 us (7.5 with G = 1); 128 tokens 17 (12).
+// and kv head. Bound by latency, or the parts' bytes: 1357 tokens of 28 heads in up to four
+// parts 16.5 us. G = 4 where tiles of 16 rows would leave CUs idle: 16 tokens of 28/4 heads
+// in up to 32 parts 5.0 us (7.5 with G = 1), but 128 tokens 17 (12).
 template <class T, int D, int G>
 __device__ __forceinline__ void join_item(const AttnCacheArgs& a, const RowTile& t, int hk, int own, int shared) {
     constexpr int E = D / 16, U = 8;
@@ -989,8 +1008,8 @@ AttnCachePlan attn_cache_plan(int total_q, int batch, int hq, int hk, int D, int
     const int group = hq / hk;
     // Rows of a tile. Rows of MR have their keys decoded into scratch first, which pays once some
     // hundred rows use them and there are tiles for the workgroups; 28/4 heads of 128, e4m3, MR
-    // rows to 32, in us: 16 tokens at 4096 keys 29.5 to 16.5, of 32 sequences 162 to 76; 64 tokens
-    // at 4096 of 16 sequences 144 to 128; 300 at 300 keys 18.0 to 15.4, of 4 sequences 22 to 33;
+    // rows to 32, in us: 16 tokens at 4096 keys 29.5 to 16.4, of 32 sequences 162 to 69; 64 tokens
+    // at 4096 of 16 sequences 144 to 114; 300 at 300 keys 18.0 to 15.0, of 4 sequences 22 to 33;
     // 200 at 2000 of 8 sequences 80 to 102; 512 at 4096 63 to 63.
     const auto fits = [&](int rows, int seqs) { return tile_bound(total_q, seqs, group, rows) * hk < kMostBlocks; };
     const int64_t rows = (static_cast<int64_t>(total_q) * group + batch - 1) / batch;  // of a sequence, on average
