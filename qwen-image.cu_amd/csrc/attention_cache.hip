@@ -115,34 +115,36 @@ __device__ __forceinline__ int key_ranges(int n, int per, int most) {
 // steps of a range where n steps are cut into `parts`
 __device__ __forceinline__ int range_steps(int n, int parts) { return max((n + parts - 1) / parts, 1); }
 
+// Where a workgroup's walk over rising items is: the 64 sequences from b0 on, of which some
+// may lie behind the last, and the items in front of them.
+struct Walk {
+    int b0, before;
+    Sequence s;
+};
 // Item `idx` of the launch: the sequences in order, each with its row tiles times its key
-// ranges. A lane takes one sequence, a wave scans 64 at a time, the first 64 (`first`, of
-// which some may lie behind hi) loaded once by the caller. Tiles of MR rows are whole, inside
-// a causal sequence the last, longest one first.
-__device__ __forceinline__ RowTile find_tile(const AttnCacheArgs& a, const Sequence& first, const Part& part, int idx,
-                                             int per) {
+// ranges. A lane takes one sequence, a wave scans 64 at a time. Tiles of MR rows are whole,
+// inside a causal sequence the last, longest one first.
+__device__ __forceinline__ RowTile find_tile(const AttnCacheArgs& a, Walk& w, const Part& part, int idx, int per) {
     const int lane = threadIdx.x & 63;
     RowTile t;
     t.found = false;
     t.b = t.q0 = t.lq = t.lk = t.row0 = t.split = 0;
     t.splits = 1;
-    int before = 0;
-    for (int b0 = part.lo; b0 < part.hi; b0 += 64) {
-        const Sequence s = b0 == part.lo ? first : load_sequence(a, b0 + lane, part.hi);
-        const int n = b0 + lane < part.hi ? row_tiles(a, s.lq, part.rows) : 0;
-        const int parts = part.rows == MR ? 1 : key_ranges(steps_of(part, s.lk), per, most_ranges(a, b0 + lane));
+    for (;;) {
+        const int n = w.b0 + lane < part.hi ? row_tiles(a, w.s.lq, part.rows) : 0;
+        const int parts = part.rows == MR ? 1 : key_ranges(steps_of(part, w.s.lk), per, most_ranges(a, w.b0 + lane));
         const int incl = wave_scan(n * parts);
         const int total = __builtin_amdgcn_readlane(incl, 63);
-        const uint64_t hit = __ballot(before + incl > idx);
-        if (idx < before + total && hit != 0) {
+        const uint64_t hit = __ballot(w.before + incl > idx);
+        if (idx < w.before + total && hit != 0) {
             const int src = __builtin_ctzll(hit);
-            t.b = b0 + src;
-            t.q0 = __builtin_amdgcn_readlane(s.q0, src);
-            t.lq = __builtin_amdgcn_readlane(s.lq, src);
-            t.lk = __builtin_amdgcn_readlane(s.lk, src);
+            t.b = w.b0 + src;
+            t.q0 = __builtin_amdgcn_readlane(w.s.q0, src);
+            t.lq = __builtin_amdgcn_readlane(w.s.lq, src);
+            t.lk = __builtin_amdgcn_readlane(w.s.lk, src);
             t.splits = __builtin_amdgcn_readlane(parts, src);
             const int cnt = __builtin_amdgcn_readlane(n, src);
-            const int i = idx - (before + __builtin_amdgcn_readlane(incl, src) - cnt * t.splits);
+            const int i = idx - (w.before + __builtin_amdgcn_readlane(incl, src) - cnt * t.splits);
             if (i < 0 || i >= cnt * t.splits) return t;  // (sums past 2^31: offsets that overlap many times)
             const int tile = i / t.splits;
             t.split = i - tile * t.splits;
@@ -150,9 +152,11 @@ __device__ __forceinline__ RowTile find_tile(const AttnCacheArgs& a, const Seque
             t.found = true;
             return t;
         }
-        before += total;
+        if (w.b0 + 64 >= part.hi) return t;
+        w.before += total;
+        w.b0 += 64;
+        w.s = load_sequence(a, w.b0 + lane, part.hi);
     }
-    return t;
 }
 // Tiles of MR rows in shares: the steps of all tiles one behind the other, sequence by
 // sequence, head by head, tile by tile (a causal tile with all of its sequence's), of
@@ -628,10 +632,10 @@ constexpr int kFewLds = SW * 16 * (kPitch<D> + 2);  // floats
 // Workgroup `block` of `blocks` walks over the items.
 template <class T, class C, int D, int NR>
 __device__ __forceinline__ void few_items(const AttnCacheArgs& a, const Part& part, int block, int blocks, float* lds) {
-    const Sequence first = load_sequence(a, part.lo + (threadIdx.x & 63), part.hi);
-    const int per = range_length(a, first, part);
+    Walk w = {part.lo, 0, load_sequence(a, part.lo + (threadIdx.x & 63), part.hi)};
+    const int per = range_length(a, w.s, part);
     for (int item = block;; item += blocks) {
-        const RowTile t = find_tile(a, first, part, item / a.c.hk, per);
+        const RowTile t = find_tile(a, w, part, item / a.c.hk, per);
         if (!t.found) return;
         few_item<T, C, D, NR>(a, t, item % a.c.hk, lds);
     }
@@ -862,7 +866,8 @@ __device__ __forceinline__ void many_items(const AttnCacheArgs& a, const Part& p
         if (share == 0) {
             const int tiles = total / part.heads;
             hk = part.h0 + (spread ? me % part.heads : me / tiles);
-            t = find_tile(a, first, part, spread ? me / part.heads : me % tiles, 0);
+            Walk w = {part.lo, 0, first};
+            t = find_tile(a, w, part, spread ? me / part.heads : me % tiles, 0);
         } else {
             t = find_step(a, first, part, x, share, me, hk, step);
         }
@@ -960,9 +965,10 @@ __global__ __launch_bounds__(256) void attn_cache_join_kernel(AttnCacheArgs a, P
         prefix_per = own_part.hi > a.batch ? per : range_length(a, load_sequence(a, a.batch + lane, prefix_part.hi), prefix_part);
     }
     const Part rows = {0, a.batch, 16 / G, 0, a.c.hk};
+    Walk w = {0, 0, first};
     for (int item = blockIdx.x;; item += gridDim.x) {
         const int hk = item % a.c.hk;
-        const RowTile t = find_tile(a, first, rows, item / a.c.hk, 0);
+        const RowTile t = find_tile(a, w, rows, item / a.c.hk, 0);
         if (!t.found) return;
         const int n = steps_of(own_part, t.lk);
         int own = 1, shared = 0;
@@ -996,7 +1002,7 @@ int64_t tile_bound(int total_q, int batch, int group, int rows) {
 }  // namespace
 
 constexpr int kMostSplits = 32;
-constexpr int kCus = 256;
+constexpr int kCus = 256, kJoinGrid = 4096;
 constexpr int kFewTiles = 320;  // of 32 rows that the card works on without those of MR
 constexpr int kWorkTogether = 24000, kWorkOf32 = 60000;  // products of 16 rows and 32 keys behind a prefix
 constexpr int kMostBlocks = 1 << 22;  // of a launch (a grid has less than 2^32 threads)
@@ -1144,7 +1150,7 @@ static hipError_t launch_attn(const AttnCacheArgs& a, const AttnCachePlan& plan,
     if (e != hipSuccess || plan.part_rows == 0) return e;
     const auto join = [&](auto g) {
         constexpr int G = decltype(g)::value;
-        const int64_t tiles = std::min<int64_t>(tile_bound(a.total_q, a.batch, a.group, 16 / G) * a.c.hk, kMostBlocks);
+        const int64_t tiles = std::min<int64_t>(tile_bound(a.total_q, a.batch, a.group, 16 / G) * a.c.hk, kJoinGrid);
         hipLaunchKernelGGL((attn_cache_join_kernel<T, D, G>), dim3(static_cast<unsigned>(tiles)), dim3(256), 0, stream, a, own,
                            shared);
     };
