@@ -170,7 +170,7 @@ __device__ __forceinline__ int count_steps(const AttnCacheArgs& a, const Sequenc
     int total = 0;
     for (int b0 = part.lo; b0 < hi; b0 += 64)
         total += wave_sum_dpp(tile_steps(a, part, b0 == part.lo ? first : load_sequence(a, b0 + lane, hi), b0 + lane, hi));
-    return total;
+    return __builtin_amdgcn_readfirstlane(total);
 }
 // row tiles of all sequences
 __device__ __forceinline__ int count_tiles(const AttnCacheArgs& a, const Sequence& first, const Part& part) {
@@ -180,7 +180,7 @@ __device__ __forceinline__ int count_tiles(const AttnCacheArgs& a, const Sequenc
         const Sequence s = b0 == part.lo ? first : load_sequence(a, b0 + lane, part.hi);
         total += wave_sum_dpp(b0 + lane < part.hi ? row_tiles(a, s.lq, part.rows) : 0);
     }
-    return total;
+    return __builtin_amdgcn_readfirstlane(total);
 }
 // Shares of a tile of n steps that begins at step `start`: the first one and their number.
 struct Shares {
@@ -241,7 +241,7 @@ __host__ __device__ __forceinline__ bool shares_pay(float share, float tiles, fl
 // device alone, so this and the ranges follow them in a captured graph.
 // Few rows: as many as make the launch one item a workgroup, at least two a wave. MR rows:
 // shares for the workgroups that run at once, where these take less time than whole tiles.
-__device__ __forceinline__ int range_length(const AttnCacheArgs& a, const Sequence& first, const Part& part) {
+__device__ __forceinline__ int find_range_length(const AttnCacheArgs& a, const Sequence& first, const Part& part) {
     if (a.own_splits <= 1 && a.prefix_splits <= 1) return 0;
     const int lane = threadIdx.x & 63;
     int least = 1, longest = 0;
@@ -277,7 +277,12 @@ __device__ __forceinline__ int range_length(const AttnCacheArgs& a, const Sequen
         per = static_cast<int>(fminf(work / fmaxf(few_grid(part.rows), 1.25f * tiles), 0x1p25f)) + 1;
         per = max(max(per, 2 * 4), least);
     }
-    return __builtin_amdgcn_readfirstlane(per);
+    return per;
+}
+// Uniform for the compiler too, as are the totals above: a tile that it takes for divergent
+// has each of its DMA instructions in a loop over descriptors (8 a step, 15 to 25% of it).
+__device__ __forceinline__ int range_length(const AttnCacheArgs& a, const Sequence& first, const Part& part) {
+    return __builtin_amdgcn_readfirstlane(find_range_length(a, first, part));
 }
 
 // number of keys that the query of `token` sees
