@@ -658,13 +658,13 @@ __global__ __launch_bounds__(SW * 64, NR == 1 ? 3 : 2) void attn_cache_few_kerne
 // and phases, of which attention_tiles.h holds what both share). Decoding on the way into
 // LDS instead, 64 codes a thread and step, took no pass of its own, but each tile of rows
 // does it anew: with seven tiles a head (128 tokens of 28/4 heads over 16000 int8 keys)
-// the loop took 52 us (50 here, and 11 for the decoding, beside the own keys' tiles), with
-// fifty (1024 tokens over 8192 e4m3 keys and 333 over 2381) 169 (155 and 9).
+// the loop took 52 us (45 here, and 11 for the decoding, beside the own keys' tiles), with
+// fifty (1024 tokens over 8192 e4m3 keys and 333 over 2381) 169 (133 and 9).
 //
-// Bound by the softmax's vector instructions and the matrix unit in turn, which work half
-// of the time each: 2.3 us a step of two workgroups, 0.8 PFLOP/s (a large product 1.3). A
-// launch in shares also starts, and writes and joins partial results, 64 KB a workgroup:
-// 18 us of the 50, 12 of the joins.
+// Bound by the softmax's vector instructions and the matrix unit in turn, which work about
+// half of the time each: 2.0 us a step of two workgroups, 1.07 PFLOP/s in the steps (a
+// large product 1.3). A launch in shares also starts, and writes and joins partial
+// results, 64 KB a workgroup: 18 us of the 45 and of the 133, 12 and 16 of the joins.
 //
 // Where the CUs want more than whole tiles (range_length), the tiles' steps are dealt out
 // in equal shares and a tile's parts joined.
@@ -1009,7 +1009,7 @@ int64_t tile_bound(int total_q, int batch, int group, int rows) {
 constexpr int kMostSplits = 32;
 constexpr int kCus = 256, kJoinGrid = 4096;
 constexpr int kFewTiles = 320;  // of 32 rows that the card works on without those of MR
-constexpr int kWorkTogether = 24000, kWorkOf32 = 60000;  // products of 16 rows and 32 keys behind a prefix
+constexpr int kWorkTogether = 24000, kWorkOf32 = 40000;  // products of 16 rows and 32 keys behind a prefix
 constexpr int kMostBlocks = 1 << 22;  // of a launch (a grid has less than 2^32 threads)
 constexpr int64_t kMostDense = int64_t{1} << 30;  // bytes of 16-bit rows at a time, of one head of a sequence at least
 
@@ -1019,9 +1019,9 @@ AttnCachePlan attn_cache_plan(int total_q, int batch, int hq, int hk, int D, int
     const int group = hq / hk;
     // Rows of a tile. Rows of MR have their keys decoded into scratch first, which pays once some
     // hundred rows use them and there are tiles for the workgroups; 28/4 heads of 128, e4m3, MR
-    // rows to 32, in us: 16 tokens at 4096 keys 29.5 to 16.4, of 32 sequences 162 to 69; 64 tokens
-    // at 4096 of 16 sequences 144 to 114; 300 at 300 keys 18.0 to 15.0, of 4 sequences 22 to 33;
-    // 200 at 2000 of 8 sequences 80 to 102; 512 at 4096 63 to 63.
+    // rows and 32, in us: 16 tokens at 4096 keys 27.4, 15.2, of 32 sequences 159, 68; 64 tokens
+    // at 4096 of 16 sequences 135, 116; 300 at 300 keys 15.8, 15.4, of 4 sequences 20.3, 32.9;
+    // 200 at 2000 of 8 sequences 70, 95; 512 at 4096 58.9, 58.5.
     const auto fits = [&](int rows, int seqs) { return tile_bound(total_q, seqs, group, rows) * hk < kMostBlocks; };
     const int64_t rows = (static_cast<int64_t>(total_q) * group + batch - 1) / batch;  // of a sequence, on average
     if (rows <= 16)
@@ -1031,10 +1031,10 @@ AttnCachePlan attn_cache_plan(int total_q, int batch, int hq, int hk, int D, int
     else
         p.own_rows = MR;
     // Behind a prefix by the products of 16 rows and 32 keys. One launch for both parts is best
-    // while they are few, tiles of 32 rows take half of them, MR rows more than that; 1 key and
-    // more of their own, MR rows, the own part's 16 and 32, in us: 16 tokens behind 4096 keys
-    // 30.6, 16.9, 22.3; 64 behind 4096 35.2, 28.5, 30.1; 128 behind 4096 47.0, 48.7, 39.7; 256
-    // behind 4096 71.6, 81.7, 66.2; 128 behind 16384 74.3, 114.7, 89.2.
+    // while they are few, then tiles of 32 rows, then MR; one token each with 40 keys of its
+    // own, MR rows, 32, and the own part's 16, in us: 16 tokens behind 4096 keys 30.8, 21.5,
+    // 15.9; 64 behind 4096 35.1, 30.2, 28.5; 128 behind 4096 43.1, 39.3, 48.7; 256 behind 4096
+    // 61.3, 64.7, 81.7; 128 behind 16384 72.7, 90.6, 114.7; int8 256 behind 4096 62.2, 73.5.
     const int64_t work = (static_cast<int64_t>(total_q) * group + 15) / 16 * ((prefix_keys + 31) / 32) * hk;
     p.prefix_rows = work <= kWorkTogether && p.own_rows != MR ? p.own_rows : work <= kWorkOf32 || !fits(MR, 1) ? 32 : MR;
     // Most ranges of a sequence: eight steps each at least, and 2^13 row tiles times ranges; of
