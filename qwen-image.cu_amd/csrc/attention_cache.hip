@@ -857,13 +857,16 @@ template <class T, int D>
 __device__ __forceinline__ void many_items(const AttnCacheArgs& a, const Part& part, int block, uint8_t* lds) {
     const Sequence first = load_sequence(a, part.lo + (threadIdx.x & 63), part.hi);
     const int share = range_length(a, first, part);
-    const int total = share == 0 ? count_tiles(a, first, part) * part.heads : count_steps(a, first, part, part.hi);
-    const int blocks = share == 0 ? total : (total + share - 1) / share;
-    if (block >= blocks) return;
     // Neighbours, which read the same keys, on one XCD; whole causal tiles, longest first, over
     // all of them.
     const bool spread = share == 0 && a.causal && part.lo < a.batch;
-    const int me = spread ? block : xcd_remap(block, blocks);
+    int total = 0, me = block;
+    if (!spread) {
+        total = share == 0 ? count_tiles(a, first, part) * part.heads : count_steps(a, first, part, part.hi);
+        const int blocks = share == 0 ? total : (total + share - 1) / share;
+        if (block >= blocks) return;
+        me = xcd_remap(block, blocks);
+    }
     const int end = share == 0 ? 1 : min((me + 1) * share, total);
     for (int x = share == 0 ? 0 : me * share; x < end;) {
         int hk = 0, step = 0;
