@@ -900,7 +900,7 @@ __global__ __launch_bounds__(MW * 64, 2) void attn_cache_many_kernel(AttnCacheAr
 // going out together, and the G sums meet in the wave; tiles of 16 / G rows of one sequence
 // and kv head. Bound by latency, or the parts' bytes: 1357 tokens of 28 heads in up to four
 // parts 16.5 us. G = 4 where tiles of 16 rows would leave CUs idle: 16 tokens of 28/4 heads
-// in up to 32 parts 5.0 us (7.5 with G = 1), but 128 tokens 17 (12).
+// in up to 32 parts 5.2 us (7.5 with G = 1), but 128 tokens 17 (12).
 template <class T, int D, int G>
 __device__ __forceinline__ void join_item(const AttnCacheArgs& a, const RowTile& t, int hk, int own, int shared) {
     constexpr int E = D / 16, U = 8;

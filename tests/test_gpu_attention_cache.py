@@ -183,6 +183,18 @@ def test_prefix_tables_with_room(qimg, lq, lk, prefix, d):
         _check(got, *c.oracle())
 
 
+@pytest.mark.parametrize("prefix,longest", [(0, 30), (0, 3000), (100, 30)])
+def test_thousands_of_sequences(qimg, prefix, longest):
+    """More sequences than a wave looks over at once, and more tiles than workgroups: some empty, one long."""
+    lq = [(1, 0, 2, 1, 3)[i % 5] for i in range(5000)]
+    lk = [i % 31 for i in range(5000)]
+    lq[4321], lk[4321] = 2, longest
+    c = Case(qimg, lq, lk, prefix, hq=2, hk=1, d=64, page=16, codes=CODES[1], seed=21)
+    got = c.run(qimg)
+    torch.cuda.synchronize()
+    _check(got, *c.oracle())
+
+
 def test_prefix_pages_in_the_tables_instead(qimg):
     """A prefix in front of every sequence's own table gives the same within the bounds."""
     c = Case(qimg, [1] * 9, [3 + i for i in range(9)], prefix=256, page=16, seed=4)
