@@ -227,7 +227,9 @@ __device__ __forceinline__ RowTile find_step(const AttnCacheArgs& a, const Seque
     return t;
 }
 
-// Workgroups of tiles of 16 (NR = 1), 32 (2) and MR rows that run at once, by registers
+// Workgroups of tiles of 16 (NR = 1), 32 (2) and MR rows that run at once, by registers (512
+// of 16 rows: one token of 64 long int8 caches 180 to 175 us, but 64 tokens of 24/24 heads
+// behind 4096 int8 keys 44 to 50)
 constexpr int few_grid(int rows) { return rows == 16 ? 768 : 512; }
 constexpr int kManyGrid = 512;
 
