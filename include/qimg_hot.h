@@ -396,8 +396,11 @@ int qimg_norm_rope_packed(const qimg_norm_rope* args, void* stream);
  * n_kv_heads, page_size], all on the device, 16-byte aligned. Row (token, kv head) x has
  * exponent E, the least from 1 to 254 with max|x| <= 127 * 2^(E - 127) (int8) or
  * 448 * 2^(E - 127) (e4m3), and codes x / 2^(E - 127) rounded half to even; codes times
- * powers of two are exact in fp32 and bf16, and in fp16 where it has the range. (fp16 rows
- * of magnitudes above 63488 round towards zero where they would leave fp16.) A token whose k
+ * powers of two are exact in fp32 and bf16, and in fp16 where it has the range. (Codes that
+ * would stand for 2^128, from magnitudes of 63.5 * 2^122 (int8) or 248 * 2^120 (e4m3) on, are
+ * the next smaller ones: what is finite comes back finite. So are those of fp16 rows that
+ * would stand for 65536. fp32 and bf16 rows of magnitudes from 65024 (int8) or 63488 (e4m3)
+ * on may stand for 65536 or more, which fp16 does not hold.) A token whose k
  * or v of a head holds an infinity or a NaN has that k stored as NaN (E = 255) and such a v
  * as zeros: its scores, and the rows that see it, are NaN, and no others.
  * n_pages * page_size below 2^31. */

@@ -141,25 +141,25 @@ __device__ __forceinline__ uint32_t head_amax(const Eight& x) {
     return group_reduce<G>(m, [](uint32_t u, uint32_t v) { return u > v ? u : v; });
 }
 
-// Codes of a head with largest magnitude `amax` (bits). Magnitudes that fp16 holds must
-// not come back as 65536, which is infinite there: that happens to fp16 rows whose largest
-// code is the first of the next power of two (256 times 2^8, 64 times 2^10); the code
-// below replaces it.
+// Codes of a head with largest magnitude `amax` (bits). Two kinds of values must not come
+// back as infinities: finite ones as 2^128, and those of fp16 rows as 65536, which is
+// infinite there. That happens to rows whose largest code would be the first of the next
+// power of two (int8 64 times 2^122 and 2^10, e4m3 256 times 2^120 and 2^8); the code below
+// replaces it.
 template <class C, int IN>
 __device__ __forceinline__ void store_codes(uint8_t* codes, uint8_t* exps, int64_t row, int d, int e, int i0, int i1,
                                             const Eight& x, uint32_t amax) {
     const int exp = row_exp<C>(amax);
     const float inv = __uint_as_float(static_cast<uint32_t>(254 - exp) << 23);
     v4f p = x.p * inv, q = x.q * inv;
-    if constexpr (IN == QIMG_FP16) {
-        constexpr int kEdge = C::kDtype == QIMG_INT8 ? 127 + 10 : 127 + 8;
-        constexpr float kMost = C::kDtype == QIMG_INT8 ? 63.0f : 240.0f;
-        if (exp == kEdge && amax <= 0x477fe000u) {  // 65504
+    constexpr bool kInt8 = C::kDtype == QIMG_INT8;
+    constexpr int kTop = kInt8 ? 127 + 122 : 127 + 120, kTop16 = kInt8 ? 127 + 10 : 127 + 8;
+    if (exp == kTop || (IN == QIMG_FP16 && exp == kTop16 && amax <= 0x477fe000u)) {  // 65504
+        constexpr float kMost = kInt8 ? 63.0f : 240.0f;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                p[c] = __builtin_amdgcn_fmed3f(p[c], -kMost, kMost);
-                q[c] = __builtin_amdgcn_fmed3f(q[c], -kMost, kMost);
-            }
+        for (int c = 0; c < 4; ++c) {
+            p[c] = __builtin_amdgcn_fmed3f(p[c], -kMost, kMost);
+            q[c] = __builtin_amdgcn_fmed3f(q[c], -kMost, kMost);
         }
     }
     *reinterpret_cast<uint32_t*>(codes + row * d + i0) = C::encode4(p[0], p[1], p[2], p[3]);
