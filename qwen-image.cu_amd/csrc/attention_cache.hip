@@ -391,8 +391,10 @@ __device__ __forceinline__ void few_item(const AttnCacheArgs& a, const RowTile& 
     const int* table = own ? a.table + static_cast<int64_t>(t.b) * a.max_blocks : a.prefix_table;
     const int blocks = (t.lk + (1 << a.c.page_shift) - 1) >> a.c.page_shift;  // that hold keys in use
 
-    constexpr bool kScores = C::kDtype == QIMG_INT8;             // K's scale is the scores'
-    constexpr bool kWeights = kScores && T::kBf;                 // V's scale is P's (bf16 has fp32's range)
+    // K's scale is the scores'. (V's is not P's: P carries 2^kPBias, and times a small scale, below
+    // 2^-126, would lose its digits or vanish. That took 180.2 to 179.2 us of one token of 64 long
+    // int8 caches, 151 to 145 of 64 tokens over 4096 keys of 16 sequences.)
+    constexpr bool kScores = C::kDtype == QIMG_INT8;
 
     // Pages of the wave's tiles, 32 at a time: lane l holds that of 16-key group l % 2 of
     // tile l / 2.
@@ -535,14 +537,6 @@ __device__ __forceinline__ void few_item(const AttnCacheArgs& a, const RowTile& 
             for (int j = 0; j < 4; ++j) pk[j] = T::pack(p[2 * j], p[2 * j + 1]);
             pf[r] = as_frag<T>(pk[0], pk[1], pk[2], pk[3]);
             sum[r] = T::mma16(ones, pf[r], sum[r]);
-            if constexpr (kWeights) {
-                // the same roundings, as a power of two changes none
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    pk[j] = T::pack(p[2 * j] * exp_scale(x.ve[j / 2] >> 16 * (j & 1) & 0xffu),
-                                    p[2 * j + 1] * exp_scale(x.ve[j / 2] >> (16 * (j & 1) + 8) & 0xffu));
-                pf[r] = as_frag<T>(pk[0], pk[1], pk[2], pk[3]);
-            }
         }
         // four channels at a time: pairs of two channels of the eight keys, crosswise
 #pragma unroll
@@ -553,8 +547,7 @@ __device__ __forceinline__ void few_item(const AttnCacheArgs& a, const RowTile& 
                 uint32_t raw;
                 if constexpr (D == 128) raw = d4 == 0 ? x.v[j].x : x.v[j].y;
                 else raw = x.v[j];
-                if constexpr (kWeights) w[j] = decode_int8_pairs<true>(raw);
-                else w[j] = decode_pairs<C, T::kBf>(raw, exp_scale(x.ve[j / 4] >> 8 * (j & 3) & 0xffu));
+                w[j] = decode_pairs<C, T::kBf>(raw, exp_scale(x.ve[j / 4] >> 8 * (j & 3) & 0xffu));
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {

@@ -80,3 +80,27 @@ def test_the_largest_values_behind_a_mask(qimg, codes, tiles):
     c.k[key] = 0
     c.v[key] = v[0].sign() * (63 * 2.0 ** 122 if codes == torch.int8 else 240 * 2.0 ** 120)
     _check(got, *c.oracle())
+
+
+@pytest.mark.parametrize("codes", CODES, ids=str)
+@pytest.mark.parametrize("tiles", range(3))
+@pytest.mark.parametrize("scale", [-50, -70, -76])
+def test_small_values_of_small_weights(qimg, codes, tiles, scale):
+    """Thousands of keys at 2^-14 of one key's weight, whose v is zeros: averages of 2^-79 keep
+    their digits, whatever the codes and the tiles' rows."""
+    t = TILES[tiles]
+    c = Case(qimg, t["lq"], [8000] + t["lk"][1:], hq=t["hq"], hk=t["hk"], codes=codes, seed=32, scale=2.0 ** scale)
+    page, hk, d = c.cache.k.shape[2], c.hk, c.q.shape[2]
+    c.q.fill_(1)
+    c.cache.k.view(torch.uint8).zero_()
+    c.cache.k_exp.fill_(127)
+    c.k.zero_()
+    heavy = torch.full((len(t["lq"]), hk, d), 0.875, device=DEV)  # a score of 14.3 log 2
+    qimg.kv_cache_write(c.cache, heavy, torch.zeros_like(heavy), (c.table[:, 0] * page).int())
+    at = torch.tensor(c.ck[:len(t["lq"])], device=DEV)
+    c.k[at], c.v[at] = 0.875, 0.0
+    got = c.run(qimg)
+    torch.cuda.synchronize()
+    want, mag, far = c.oracle()
+    assert float(mag[t["lq"][0] - 1].min()) > 2.0 ** -79
+    _check(got, want, mag, far)
