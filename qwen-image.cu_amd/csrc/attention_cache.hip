@@ -711,8 +711,8 @@ __device__ __forceinline__ void decode_tile(const AttnCacheArgs& a, const Part& 
 }
 
 template <class T, class C, int D>
-__global__ __launch_bounds__(256) void attn_cache_decode_kernel(AttnCacheArgs a, Part part, int tiles) {
-    decode_tile<T, C, D>(a, part, tiles, blockIdx.x);
+__global__ __launch_bounds__(256) void attn_cache_decode_kernel(AttnCacheArgs a, Part part, int tiles, int first) {
+    decode_tile<T, C, D>(a, part, tiles, first + blockIdx.x);
 }
 
 // The first `few` workgroups work on the sequences' own keys in tiles of few rows, the
@@ -1102,16 +1102,21 @@ static hipError_t launch_attn(const AttnCacheArgs& a, const AttnCachePlan& plan,
     const auto decode = [&](const Part& part, bool with_own) {
         const int64_t keys = static_cast<int64_t>(part.lo < a.batch ? a.max_blocks : a.prefix_blocks) << a.c.page_shift;
         const int tiles = static_cast<int>((keys + MK - 1) / MK);
-        const unsigned blocks = static_cast<unsigned>(static_cast<int64_t>(tiles) * part.heads * (part.hi - part.lo));
-        const unsigned more = with_own ? few(true, false, own.rows) : 0;
-        if (more > 0 && own.rows == 16)
-            hipLaunchKernelGGL((attn_cache_mixed_kernel<T, C, D, 1>), dim3(more + blocks), block, 0, stream, a, own,
-                               static_cast<int>(more), part, tiles);
-        else if (more > 0)
-            hipLaunchKernelGGL((attn_cache_mixed_kernel<T, C, D, 2>), dim3(more + blocks), block, 0, stream, a, own,
-                               static_cast<int>(more), part, tiles);
-        else if (blocks > 0)
-            hipLaunchKernelGGL((attn_cache_decode_kernel<T, C, D>), dim3(blocks), block, 0, stream, a, part, tiles);
+        // (scratch bounds them: below 2^25)
+        const int blocks = static_cast<int>(static_cast<int64_t>(tiles) * part.heads * (part.hi - part.lo));
+        int first = 0;
+        if (const int more = with_own ? static_cast<int>(few(true, false, own.rows)) : 0; more > 0) {
+            first = std::min(blocks, kMostBlocks);
+            if (own.rows == 16)
+                hipLaunchKernelGGL((attn_cache_mixed_kernel<T, C, D, 1>), dim3(more + first), block, 0, stream, a, own, more,
+                                   part, tiles);
+            else
+                hipLaunchKernelGGL((attn_cache_mixed_kernel<T, C, D, 2>), dim3(more + first), block, 0, stream, a, own, more,
+                                   part, tiles);
+        }
+        for (; first < blocks; first += kMostBlocks)
+            hipLaunchKernelGGL((attn_cache_decode_kernel<T, C, D>), dim3(std::min(blocks - first, kMostBlocks)), block, 0, stream,
+                               a, part, tiles, first);
         return hipGetLastError();
     };
     bool own_done = false;

@@ -14,6 +14,7 @@
 // heads of 128, fp32 to bf16, 57.5 us (5.2 TB/s; a large copy reaches 4.9, part of this
 // stays in the caches); 10751 tokens with k and v into e4m3 pages 65 us (4.4 TB/s); a few
 // tokens 3.5 to 4.5 us, one chain of loads (position, table and x, or slot and x).
+#include <algorithm>
 #include <type_traits>
 
 #include "cache_codes.h"
@@ -228,17 +229,39 @@ __global__ __launch_bounds__(256) void heads_kernel(HeadsArgs a) {
     }
 }
 
+constexpr int kMostBlocks = 1 << 22;  // of a launch (a grid has less than 2^32 threads)
+
+// `a` from token t on
+template <int IN>
+HeadsArgs from_token(HeadsArgs a, int t) {
+    const auto ahead = [](auto p, int64_t bytes) {
+        if (p != nullptr) p = (decltype(p))((uintptr_t)p + bytes);
+        return p;
+    };
+    constexpr int64_t in = IN == QIMG_FP32 ? 4 : 2;
+    a.x = ahead(a.x, in * t * a.x_t), a.k = ahead(a.k, in * t * a.k_t), a.v = ahead(a.v, in * t * a.v_t);
+    a.out = ahead(a.out, (a.out_dtype == QIMG_FP32 ? 4 : 2) * t * a.o_t);
+    a.positions = ahead(a.positions, int64_t{4} * t), a.slots = ahead(a.slots, int64_t{4} * t);
+    a.tokens -= t;
+    return a;
+}
+
 template <int IN, class C>
-void launch_heads_in(const HeadsArgs& a, hipStream_t stream) {
-    const int g = a.d <= 64 ? 8 : a.d <= 128 ? 16 : 32;
-    const int64_t units = static_cast<int64_t>(a.tokens) * (std::is_same_v<C, void> ? a.nq + 2 * a.nk : a.nq + a.nk);
-    const dim3 grid(static_cast<unsigned>((units + 256 / g - 1) / (256 / g)));
-    if (g == 8) {
-        hipLaunchKernelGGL((heads_kernel<IN, 8, C>), grid, dim3(256), 0, stream, a);
-    } else if (g == 16) {
-        hipLaunchKernelGGL((heads_kernel<IN, 16, C>), grid, dim3(256), 0, stream, a);
-    } else if constexpr (std::is_same_v<C, void>) {
-        hipLaunchKernelGGL((heads_kernel<IN, 32, C>), grid, dim3(256), 0, stream, a);
+void launch_heads_in(const HeadsArgs& all, hipStream_t stream) {
+    const int g = all.d <= 64 ? 8 : all.d <= 128 ? 16 : 32;
+    const int64_t units = std::is_same_v<C, void> ? all.nq + 2 * all.nk : all.nq + all.nk;  // of a token, < 2^24
+    const int64_t most = kMostBlocks * (256 / g) / units;                                   // tokens of a launch
+    for (int64_t t = 0; t < all.tokens; t += most) {
+        HeadsArgs a = from_token<IN>(all, static_cast<int>(t));
+        a.tokens = static_cast<int>(std::min<int64_t>(a.tokens, most));
+        const dim3 grid(static_cast<unsigned>((a.tokens * units + 256 / g - 1) / (256 / g)));
+        if (g == 8) {
+            hipLaunchKernelGGL((heads_kernel<IN, 8, C>), grid, dim3(256), 0, stream, a);
+        } else if (g == 16) {
+            hipLaunchKernelGGL((heads_kernel<IN, 16, C>), grid, dim3(256), 0, stream, a);
+        } else if constexpr (std::is_same_v<C, void>) {
+            hipLaunchKernelGGL((heads_kernel<IN, 32, C>), grid, dim3(256), 0, stream, a);
+        }
     }
 }
 
@@ -271,9 +294,9 @@ __device__ __forceinline__ void read16(const uint8_t* codes, uint32_t exp, void*
 }
 
 template <class C, int OUT>
-__global__ __launch_bounds__(256) void cache_read_kernel(CacheReadArgs a) {
+__global__ __launch_bounds__(256) void cache_read_kernel(CacheReadArgs a, int first) {
     __shared__ int64_t src[RR];  // first slot's row of head 0, -1: nothing to read
-    const int row0 = blockIdx.x * RR;
+    const int row0 = first + blockIdx.x * RR;
     if (threadIdx.x < RR) {
         const int row = row0 + threadIdx.x;
         // the last sequence that starts at or before the row, among those of a rising list
@@ -327,11 +350,15 @@ hipError_t launch_heads(const HeadsArgs& a, int x_dtype, int codes, hipStream_t 
 
 template <class C>
 static void launch_read(const CacheReadArgs& a, int out_dtype, hipStream_t stream) {
-    const dim3 grid(static_cast<unsigned>((a.total + RR - 1) / RR));
-    switch (out_dtype) {
-    case QIMG_FP32: hipLaunchKernelGGL((cache_read_kernel<C, QIMG_FP32>), grid, dim3(256), 0, stream, a); break;
-    case QIMG_BF16: hipLaunchKernelGGL((cache_read_kernel<C, QIMG_BF16>), grid, dim3(256), 0, stream, a); break;
-    default: hipLaunchKernelGGL((cache_read_kernel<C, QIMG_FP16>), grid, dim3(256), 0, stream, a); break;
+    const int blocks = (a.total + RR - 1) / RR;
+    for (int b = 0; b < blocks; b += kMostBlocks) {
+        const dim3 grid(std::min(blocks - b, kMostBlocks));
+        const int first = b * RR;
+        switch (out_dtype) {
+        case QIMG_FP32: hipLaunchKernelGGL((cache_read_kernel<C, QIMG_FP32>), grid, dim3(256), 0, stream, a, first); break;
+        case QIMG_BF16: hipLaunchKernelGGL((cache_read_kernel<C, QIMG_BF16>), grid, dim3(256), 0, stream, a, first); break;
+        default: hipLaunchKernelGGL((cache_read_kernel<C, QIMG_FP16>), grid, dim3(256), 0, stream, a, first); break;
+        }
     }
 }
 
