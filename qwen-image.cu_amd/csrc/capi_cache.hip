@@ -6,19 +6,24 @@
 
 namespace {
 
+// what a cache may have
+bool page_sizes(int n) { return n >= 16 && n <= 256 && (n & (n - 1)) == 0; }
+bool head_dims(int d) { return d == 64 || d == 128; }
+bool kv_heads(int n) { return n > 0 && n < (1 << 16); }
+
 int check_cache(const char* fn, const qimg_kv_cache* c, bool data) {
     QIMG_REQUIRE(c, "%s: cache is null", fn);
     QIMG_REQUIRE(c->dtype == QIMG_INT8 || c->dtype == QIMG_FP8_E4M3, "%s: cache dtype %d must be INT8 or FP8_E4M3", fn,
                  c->dtype);
     QIMG_REQUIRE(c->n_pages >= 0 && c->n_kv_heads > 0, "%s: bad cache sizes n_pages=%d n_kv_heads=%d", fn, c->n_pages,
                  c->n_kv_heads);
-    if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1)) != 0)
+    if (!page_sizes(c->page_size))
         return qimg::api_fail(QIMG_ERR_UNSUPPORTED, "%s: page_size %d not supported (16, 32, 64, 128 or 256)", fn,
                               c->page_size);
-    if (c->head_dim != 64 && c->head_dim != 128)
+    if (!head_dims(c->head_dim))
         return qimg::api_fail(QIMG_ERR_UNSUPPORTED, "%s: head_dim %d of a cache not supported (64 or 128)", fn,
                               c->head_dim);
-    QIMG_REQUIRE(static_cast<int64_t>(c->n_pages) * c->page_size < (int64_t{1} << 31) && c->n_kv_heads < (1 << 16),
+    QIMG_REQUIRE(static_cast<int64_t>(c->n_pages) * c->page_size < (int64_t{1} << 31) && kv_heads(c->n_kv_heads),
                  "%s: n_pages * page_size must be < 2^31, n_kv_heads < 2^16", fn);
     if (!data || c->n_pages == 0) return QIMG_OK;
     QIMG_REQUIRE(c->k && c->v && c->k_exp && c->v_exp, "%s: null pointer in the cache", fn);
@@ -182,8 +187,8 @@ int qimg_kv_cache_read(const qimg_kv_cache* cache, const int32_t* block_table, i
 
 int64_t qimg_attention_cache_scratch_bytes(int total_q, int batch, int n_heads, int n_kv_heads, int head_dim,
                                            int page_size, int max_blocks, int prefix_blocks) {
-    if (total_q <= 0 || batch <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0 ||
-        (head_dim != 64 && head_dim != 128) || page_size < 16 || page_size > 256 || max_blocks < 0 || prefix_blocks < 0 ||
+    if (total_q <= 0 || batch <= 0 || n_heads <= 0 || !kv_heads(n_kv_heads) || n_heads % n_kv_heads != 0 ||
+        !head_dims(head_dim) || !page_sizes(page_size) || max_blocks < 0 || prefix_blocks < 0 ||
         !attn_sizes(total_q, n_heads, batch, max_blocks, prefix_blocks, page_size))
         return 0;
     const qimg::AttnCacheScratch s = qimg::attn_cache_scratch(

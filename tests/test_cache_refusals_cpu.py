@@ -168,3 +168,14 @@ def test_wrappers_refuse(qimg):
         qimg.attention_cache(x.bfloat16(), cache, torch.zeros(5, dtype=torch.int32), i.view(4, 1), i)
     with pytest.raises(qimg.QimgError, match="int8 or float8"):
         qimg.kv_cache(2, 16, 1, 64, dtype=torch.float16, device="cpu")
+
+
+@pytest.mark.parametrize("page", [0, 8, 15, 16, 24, 32, 48, 96, 128, 255, 256, 512])
+@pytest.mark.parametrize("hq,hk", [(28, 4), (28, 3), (1 << 16, 1 << 16), (1 << 17, 1 << 16), ((1 << 16) - 1, (1 << 16) - 1)])
+@pytest.mark.parametrize("d", [64, 96, 128])
+def test_no_scratch_for_sizes_that_the_call_refuses(qimg, page, hq, hk, d):
+    c = _c(qimg, n_pages=100, page_size=page, n_kv_heads=hk, head_dim=d)
+    refused = _attn(qimg, c, n_heads=hq, total_q=0, out_stride_t=0, q_stride_t=0) != 0
+    assert refused == (page not in (16, 32, 64, 128, 256) or hq % hk != 0 or hk >= 1 << 16 or d == 96)
+    need = qimg.attention_cache_scratch_bytes(16, 16, hq, hk, d, page, 2, 4)
+    assert (need == 0) == refused  # (a prefix always takes some)
