@@ -25,6 +25,7 @@
 #include <cmath>
 #include <type_traits>
 
+#include "attention_cache_ranges.h"
 #include "attention_tiles.h"
 #include "cache_codes.h"
 
@@ -227,59 +228,28 @@ __device__ __forceinline__ RowTile find_step(const AttnCacheArgs& a, const Seque
     return t;
 }
 
-// Workgroups of tiles of 16 (NR = 1), 32 (2) and MR rows that run at once, by registers (512
-// of 16 rows: one token of 64 long int8 caches 180 to 175 us, but 64 tokens of 24/24 heads
-// behind 4096 int8 keys 44 to 50)
-constexpr int few_grid(int rows) { return rows == 16 ? 768 : 512; }
-constexpr int kManyGrid = 512;
-
-// Shares of `share` steps against `whole` of the tiles themselves: in steps, what a workgroup
-// has to do, starts and joins (6) and the float results (6 for each workgroup, and tile).
-__host__ __device__ __forceinline__ bool shares_pay(float share, float tiles, float whole) {
-    return 1.05f * share + 6.0f + (kManyGrid + tiles) * (6.0f / kManyGrid) < whole;
-}
-
 // Steps of a range, about, or of a share; 0: tiles are whole. Lengths are known on the
 // device alone, so this and the ranges follow them in a captured graph.
-// Few rows: as many as make the launch one item a workgroup, at least two a wave. MR rows:
-// shares for the workgroups that run at once, where these take less time than whole tiles.
 __device__ __forceinline__ int find_range_length(const AttnCacheArgs& a, const Sequence& first, const Part& part) {
     if (a.own_splits <= 1 && a.prefix_splits <= 1) return 0;
     const int lane = threadIdx.x & 63;
-    int least = 1, longest = 0;
-    float work = 0.0f, all = 0.0f, tiles = 0.0f;  // steps, with those that a causal mask hides; row tiles: no last digit is needed
+    RangeSums sums = {0.0f, 0.0f, 0.0f, 1, 0};  // no last digit is needed, but the same one everywhere
     for (int b0 = part.lo; b0 < part.hi; b0 += 64) {
         const Sequence s = b0 == part.lo ? first : load_sequence(a, b0 + lane, part.hi);
         const int n = steps_of(part, s.lk);
         const float t = b0 + lane < part.hi ? static_cast<float>(row_tiles(a, s.lq, part.rows)) : 0.0f;
         // (a causal sequence's first tile sees lq keys fewer than its last)
         const int fewer = part.rows == MR && a.causal && b0 + lane != a.batch ? steps_of(part, min(s.lq, s.lk)) : 0;
-        work += wave_sum_dpp(t * (static_cast<float>(n) - 0.5f * static_cast<float>(fewer)));
-        all += wave_sum_dpp(t * static_cast<float>(n));
-        tiles += wave_sum_dpp(t);
+        sums.work += wave_sum_dpp(seen_steps(t, n, fewer));
+        sums.all += wave_sum_dpp(seen_steps(t, n, 0));
+        sums.tiles += wave_sum_dpp(t);
         const int most = max(most_ranges(a, b0 + lane) - (part.rows == MR ? 1 : 0), 1);
-        least = max(least, wave_reduce_dpp((n + most - 1) / most, [](int x, int y) { return max(x, y); }));
-        longest = max(longest, wave_reduce_dpp(n, [](int x, int y) { return max(x, y); }));
+        sums.least = max(sums.least, wave_reduce_dpp((n + most - 1) / most, [](int x, int y) { return max(x, y); }));
+        sums.longest = max(sums.longest, wave_reduce_dpp(n, [](int x, int y) { return max(x, y); }));
     }
-    const float heads = static_cast<float>(part.heads);
-    work *= heads;
-    all *= heads;
-    tiles *= heads;
-    int per;
-    if (part.rows == MR) {
-        if (most_ranges(a, part.lo) == 1 || all >= 0x1p30f) return 0;
-        const float each = work / kManyGrid, long_ = static_cast<float>(longest), share = all / kManyGrid;
-        // whole tiles: rounds of the longest, or what evens out while the last ones run
-        const float rounds = ceilf(tiles / kManyGrid) * long_, mixed = each + (a.causal ? 0.25f : 1.0f) * long_;
-        const float whole = fmaxf(fminf(rounds, mixed), fmaxf(each, long_));
-        if (!shares_pay(share, tiles, whole)) return 0;
-        per = max(max(static_cast<int>(share) + 1, 4), least);
-    } else {
-        // (offsets that overlap may sum to any number)
-        per = static_cast<int>(fminf(work / fmaxf(few_grid(part.rows), 1.25f * tiles), 0x1p25f)) + 1;
-        per = max(max(per, 2 * 4), least);
-    }
-    return per;
+    times_heads(sums, part.heads);
+    if (part.rows == MR) return most_ranges(a, part.lo) == 1 ? 0 : share_length(sums, a.causal != 0);
+    return few_length(sums, part.rows);
 }
 // Uniform for the compiler too, as are the totals above: a tile that it takes for divergent
 // has each of its DMA instructions in a loop over descriptors (8 a step, 15 to 25% of it).
