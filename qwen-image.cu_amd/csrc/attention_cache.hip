@@ -297,7 +297,7 @@ __device__ __forceinline__ void store_row(uint16_t* op, const float (&acc)[E], f
 // the exponentials; 32 rows decode once for both. Small calls by latency: 16 tokens over
 // up to 8192 keys 14.8 us (two or three tiles a wave), of which their 47 MB take 8. Loading
 // K a whole tile earlier changed none of these. A third and fourth 16 rows did not fit the
-// registers.
+// registers (and gave wrong rows where they spilled most).
 constexpr int SW = 4;
 
 // A wave's 32-key tile as it lies in the cache, each half loaded again as soon as it is used up
@@ -686,9 +686,10 @@ __global__ __launch_bounds__(256) void attn_cache_decode_kernel(AttnCacheArgs a,
 }
 
 // The first `few` workgroups work on the sequences' own keys in tiles of few rows, the
-// others decode the prefix for its tiles of MR: one waits for memory, one does not. 16000
-// int8 keys beside 128 sequences of 1 to 509: 20 us; the decoding first 23, and in the
-// launch of the prefix' tiles instead the own keys took 9 to 10 besides the 11.
+// others decode the prefix for its tiles of MR, mostly behind them where they are as many as
+// run at once: a launch less. 16000 int8 keys beside 128 sequences of 1 to 509: 20 us; in two
+// launches, the decoding first, 23, and in the launch of the prefix' tiles instead the own
+// keys took 9 to 10 besides the 11.
 template <class T, class C, int D, int NR>
 __global__ __launch_bounds__(SW * 64, NR == 1 ? 3 : 2) void attn_cache_mixed_kernel(AttnCacheArgs a, Part own, int few,
                                                                                     Part prefix, int tiles) {
